@@ -1,0 +1,159 @@
+// adapter_api.cu -- C entry points of the low-rank adapter operators
+// (declared in include/fpemu.h).
+#include <cuda_runtime.h>
+
+#include "adapter_kernels.cuh"
+#include "fpemu_host.h"
+
+using namespace fpemu;
+
+namespace {
+
+int element_size(int dtype) {
+    switch (dtype) {
+        case FPEMU_DT_F64: return 8;
+        case FPEMU_DT_F32: return 4;
+        case FPEMU_DT_F16: return 2;
+        case FPEMU_DT_BF16: return 2;
+        default: return 0;
+    }
+}
+
+int check_sizes(const char* what, int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
+    if (element_size(dtype) == 0) return fail(FPEMU_ERR_INVALID, "%s: unknown dtype code %d", what, dtype);
+    if (rows < 0 || rows > FPEMU_ADAPTER_MAX_ROWS || k < 0 || n < 0)
+        return fail(FPEMU_ERR_INVALID, "%s: bad sizes rows=%lld k=%lld n=%lld", what, (long long)rows, (long long)k,
+                    (long long)n);
+    if (rank < 1 || rank > FPEMU_ADAPTER_MAX_RANK)
+        return fail(FPEMU_ERR_UNSUPPORTED, "%s: rank %lld outside [1, %d]", what, (long long)rank,
+                    FPEMU_ADAPTER_MAX_RANK);
+    if (adapters < 1 || adapters > FPEMU_ADAPTER_MAX_COUNT)
+        return fail(FPEMU_ERR_UNSUPPORTED, "%s: %lld adapters outside [1, %d]", what, (long long)adapters,
+                    FPEMU_ADAPTER_MAX_COUNT);
+    return FPEMU_OK;
+}
+
+template <typename T>
+int launch_rows(const AdapterParams& P, bool transposed, cudaStream_t st) {
+    const int64_t units = P.plan ? plan_slots(P.rows, P.adapters) : P.rows;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(units * kAdapterCluster));
+    cfg.blockDim = dim3(kAdapterThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = kAdapterCluster;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    FPEMU_CUDA(cudaLaunchKernelEx(&cfg, transposed ? adapter_rows_kernel<T, true> : adapter_rows_kernel<T, false>, P));
+    return FPEMU_OK;
+}
+
+template <typename T>
+int launch_grad(const AdapterGradParams& P, cudaStream_t st) {
+    if (P.cols == 0) return FPEMU_OK;
+    const dim3 grid((unsigned)((P.cols + 127) / 128), (unsigned)P.adapters, (unsigned)((P.r + kGradJ - 1) / kGradJ));
+    adapter_grad_kernel<T><<<grid, 128, 0, st>>>(P);
+    FPEMU_CUDA(cudaGetLastError());
+    return FPEMU_OK;
+}
+
+template <typename F>
+int with_type(int dtype, F&& f) {
+    switch (dtype) {
+        case FPEMU_DT_F64: return f((double*)nullptr);
+        case FPEMU_DT_F32: return f((float*)nullptr);
+        case FPEMU_DT_F16: return f((__half*)nullptr);
+        default: return f((__nv_bfloat16*)nullptr);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t fpemu_adapter_plan_size(int64_t rows, int64_t adapters) {
+    if (rows < 0 || rows > FPEMU_ADAPTER_MAX_ROWS || adapters < 1 || adapters > FPEMU_ADAPTER_MAX_COUNT) return 0;
+    return plan_words(rows, adapters) * 4;
+}
+
+int fpemu_adapter_plan(const void* index, int index_bytes, int64_t rows, int64_t adapters, void* plan,
+                       size_t plan_bytes, void* stream) {
+    DevInfo d;
+    FPEMU_TRY(check_sizes("adapter_plan", FPEMU_DT_F64, rows, 0, 0, 1, adapters));
+    if (index_bytes != 4 && index_bytes != 8)
+        return fail(FPEMU_ERR_INVALID, "adapter_plan: index of %d-byte elements", index_bytes);
+    if (plan == nullptr || plan_bytes < (size_t)plan_words(rows, adapters) * 4 ||
+        reinterpret_cast<uintptr_t>(plan) % 16 != 0)
+        return fail(FPEMU_ERR_WORKSPACE, "adapter_plan: need %lld bytes, 16-byte aligned",
+                    (long long)plan_words(rows, adapters) * 4);
+    if (rows > 0 && index == nullptr) return fail(FPEMU_ERR_INVALID, "adapter_plan: null index");
+    FPEMU_TRY(device_info(&d));
+    ErrorSink sink;
+    FPEMU_TRY(error_sink(&sink));
+    adapter_plan_kernel<<<(unsigned)(adapters + 2), 1024, 0, static_cast<cudaStream_t>(stream)>>>(
+        index, index_bytes == 8, rows, (int)adapters, static_cast<int32_t*>(plan), sink);
+    FPEMU_CUDA(cudaGetLastError());
+    return FPEMU_OK;
+}
+
+int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters,
+                         const void* x, int64_t x_row, const void* w1, int64_t w1_adapter, int64_t w1_row,
+                         const void* w2, int64_t w2_adapter, int64_t w2_row, int transposed, const void* base,
+                         int64_t base_row, void* y, int64_t y_row, const double* scales, double scale,
+                         const void* index, int index_bytes, const void* plan, void* u, void* stream) {
+    DevInfo d;
+    FPEMU_TRY(check_sizes("adapter_matmul", dtype, rows, k, n, rank, adapters));
+    if (rows == 0) return FPEMU_OK;
+    if ((k > 0 && (x == nullptr || w1 == nullptr)) || (n > 0 && (w2 == nullptr || y == nullptr)))
+        return fail(FPEMU_ERR_INVALID, "adapter_matmul: null matrix pointer");
+    if (x_row < 0 || base_row < 0 || w1_adapter < 0 || w2_adapter < 0 || w1_row < 0 || w2_row < 0 ||
+        (y_row < n && rows > 1))
+        return fail(FPEMU_ERR_INVALID, "adapter_matmul: negative stride or output rows that overlap");
+    if (plan == nullptr && (rows > FPEMU_ADAPTER_FEW_ROWS || index == nullptr || (index_bytes != 4 && index_bytes != 8)))
+        return fail(FPEMU_ERR_INVALID, "adapter_matmul: %lld rows need a plan, fewer an index of 4 or 8 bytes",
+                    (long long)rows);
+    FPEMU_TRY(device_info(&d));
+    AdapterParams P = {};
+    P.rows = rows, P.k = k, P.n = n, P.r = (int)rank, P.adapters = (int)adapters;
+    P.x = x, P.x_row = x_row;
+    P.w1 = w1, P.w1_adapter = w1_adapter, P.w1_row = w1_row;
+    P.w2 = w2, P.w2_adapter = w2_adapter, P.w2_row = w2_row;
+    P.base = base, P.base_row = base_row, P.y = y, P.y_row = y_row;
+    P.scales = scales, P.scale = scale;
+    P.index = index, P.index_wide = index_bytes == 8, P.plan = static_cast<const int32_t*>(plan), P.u = u;
+    FPEMU_TRY(error_sink(&P.sink));
+    return with_type(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        return launch_rows<T>(P, transposed != 0, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int fpemu_adapter_grads(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters,
+                        const void* x, int64_t x_row, const void* dy, int64_t dy_row, const void* u, const void* v,
+                        const void* plan, void* dA, void* dB, void* stream) {
+    DevInfo d;
+    FPEMU_TRY(check_sizes("adapter_grads", dtype, rows, k, n, rank, adapters));
+    if (plan == nullptr || (dA && (!x || !v) && rows * k > 0) || (dB && (!dy || !u) && rows * n > 0))
+        return fail(FPEMU_ERR_INVALID, "adapter_grads: null pointer");
+    if (x_row < 0 || dy_row < 0) return fail(FPEMU_ERR_INVALID, "adapter_grads: negative stride");
+    FPEMU_TRY(device_info(&d));
+    return with_type(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        AdapterGradParams P = {};
+        P.rows = rows, P.r = (int)rank, P.adapters = (int)adapters, P.plan = static_cast<const int32_t*>(plan);
+        if (dA) {
+            P.cols = k, P.p = v, P.q = x, P.q_row = x_row, P.grad = dA, P.grad_j = k, P.grad_c = 1;
+            FPEMU_TRY(launch_grad<T>(P, static_cast<cudaStream_t>(stream)));
+        }
+        if (dB) {
+            P.cols = n, P.p = u, P.q = dy, P.q_row = dy_row, P.grad = dB, P.grad_j = 1, P.grad_c = rank;
+            FPEMU_TRY(launch_grad<T>(P, static_cast<cudaStream_t>(stream)));
+        }
+        return (int)FPEMU_OK;
+    });
+}
+
+}  // extern "C"

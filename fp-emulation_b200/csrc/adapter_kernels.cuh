@@ -1,0 +1,369 @@
+// adapter_kernels.cuh -- low-rank adapters of many requests beside a shared
+// projection: for every row t with adapter i = index[t],
+//
+//     u_t = s_i * A_i x_t        (r values)
+//     y_t = base_t + B_i u_t
+//
+// and the sums of the backward pass over the rows of each adapter.
+#pragma once
+
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "fpemu_error.cuh"
+
+namespace fpemu {
+
+namespace cg = cooperative_groups;
+
+constexpr int kAdapterMaxRank = 128;
+constexpr int kSlotRows = 64;      // rows of one adapter that a slot of the plan holds
+constexpr int kFewRows = 256;      // up to here the kernels group the rows themselves
+constexpr int kAdapterThreads = 256;
+constexpr int kAdapterCluster = 8;
+constexpr int kGroupRows = 8;      // rows that share one read of a weight
+
+// Sums are held in float for 16- and 32-bit data and in double for float64.
+template <typename T>
+struct AccOf {
+    using type = float;
+};
+template <>
+struct AccOf<double> {
+    using type = double;
+};
+
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ double widen(double v) { return v; }
+__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T>
+__device__ __forceinline__ T narrow(typename AccOf<T>::type v);
+template <>
+__device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ double narrow<double>(double v) { return v; }
+template <>
+__device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// One slot of the plan: up to kSlotRows rows of one adapter (class `cls`:
+// an adapter, `adapters` for rows without one, `adapters + 1` for bad ids).
+struct AdapterSlot {
+    int cls, start, count, unused;
+};
+
+// The plan: int32 words [0, adapters + 3) are the first position of each class
+// in `perm` (classes in order; the last word is the number of rows), then the
+// slots (16-byte aligned), then perm, the rows sorted by class and in their own
+// order within one.  A class's slots begin at start/kSlotRows + class: ranges of
+// two classes never meet because ceil(c/S) <= (start + c)/S - start/S + 1.
+__host__ __device__ __forceinline__ int64_t plan_slots(int64_t rows, int64_t adapters) {
+    return rows / kSlotRows + adapters + 2;
+}
+__host__ __device__ __forceinline__ int64_t plan_slot_word(int64_t adapters) { return (adapters + 3 + 3) / 4 * 4; }
+__host__ __device__ __forceinline__ int64_t plan_perm_word(int64_t rows, int64_t adapters) {
+    return plan_slot_word(adapters) + 4 * plan_slots(rows, adapters);
+}
+__host__ __device__ __forceinline__ int64_t plan_words(int64_t rows, int64_t adapters) {
+    return plan_perm_word(rows, adapters) + rows;
+}
+
+__device__ __forceinline__ int row_class(const void* index, int wide, int64_t t, int adapters) {
+    const int64_t id = wide ? static_cast<const int64_t*>(index)[t] : (int64_t) static_cast<const int32_t*>(index)[t];
+    return id == -1 ? adapters : (id < 0 || id >= adapters) ? adapters + 1 : (int)id;
+}
+
+// One block per class.  Each warp counts the class's rows, and those of smaller
+// classes, in its own stretch of the index; a scan over the warps' counts gives
+// every warp its first position, and a second walk writes the rows in order.
+// No atomics: the order is that of the rows.
+__global__ void __launch_bounds__(1024) adapter_plan_kernel(const void* index, int wide, int64_t rows, int adapters,
+                                                            int32_t* plan, ErrorSink sink) {
+    __shared__ int own_count[32], below_count[32];
+    const int cls = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t stretch = ((rows + 31) / 32 + 31) / 32 * 32;
+    const int64_t t0 = warp * stretch, t1 = t0 + stretch < rows ? t0 + stretch : rows;
+    int own = 0, below = 0;
+    for (int64_t t = t0 + lane; t < t1; t += 32) {
+        const int c = row_class(index, wide, t, adapters);
+        own += c == cls;
+        below += c < cls;
+    }
+    own = __reduce_add_sync(0xffffffffu, own);
+    below = __reduce_add_sync(0xffffffffu, below);
+    if (lane == 0) own_count[warp] = own, below_count[warp] = below;
+    __syncthreads();
+    int start = 0, total = 0, at = 0;
+    for (int w = 0; w < 32; ++w) {
+        start += below_count[w];
+        if (w == warp) at = total;
+        total += own_count[w];
+    }
+    int32_t* perm = plan + plan_perm_word(rows, adapters);
+    at += start;
+    for (int64_t b = t0; b < t1; b += 32) {
+        const int64_t t = b + lane;
+        const bool mine = t < t1 && row_class(index, wide, t, adapters) == cls;
+        const unsigned m = __ballot_sync(0xffffffffu, mine);
+        if (mine) perm[at + __popc(m & ((1u << lane) - 1))] = (int32_t)t;
+        at += __popc(m);
+    }
+    const int64_t s0 = start / kSlotRows + cls, s1 = (start + total) / kSlotRows + cls + 1;
+    AdapterSlot* slots = reinterpret_cast<AdapterSlot*>(plan + plan_slot_word(adapters));
+    for (int64_t s = s0 + threadIdx.x; s < s1; s += blockDim.x) {
+        const int64_t first = (s - s0) * kSlotRows;
+        const int64_t left = total - first;
+        slots[s] = AdapterSlot{cls, (int)(start + first), (int)(left < 0 ? 0 : left < kSlotRows ? left : kSlotRows), 0};
+    }
+    if (threadIdx.x == 0) {
+        plan[cls] = start;
+        if (cls == adapters + 1) {
+            plan[adapters + 2] = (int32_t)rows;
+            if (total > 0) report_error(sink.dev, sink.host, FPEMU_ERR_INVALID, kWhereAdapterIndex, perm[start]);
+        }
+    }
+}
+
+struct AdapterParams {
+    int64_t rows, k, n;
+    int r, adapters;
+    const void* x;      // [rows, k]
+    int64_t x_row;
+    const void* w1;     // forward A [adapters, r, k]; transposed B [adapters, k, r]
+    int64_t w1_adapter, w1_row;
+    const void* w2;     // forward B [adapters, n, r]; transposed A [adapters, r, n]
+    int64_t w2_adapter, w2_row;
+    const void* base;   // [rows, n] or null
+    int64_t base_row;
+    void* y;            // [rows, n]
+    int64_t y_row;
+    const double* scales;  // one per adapter, or null: `scale` for all
+    double scale;
+    const void* index;
+    int index_wide;
+    const int32_t* plan;  // null: the kernel groups the (few) rows itself
+    void* u;              // [rows, r] of the sums' type, or null
+    ErrorSink sink;
+};
+
+// Rows without an adapter: base (or 0); rows with an id that is none: NaN, so
+// that a wrong index never looks like a result.
+template <typename T>
+__device__ void plain_row(const AdapterParams& P, int64_t row, bool bad, int64_t n0, int64_t n1) {
+    T* y = static_cast<T*>(P.y) + row * P.y_row;
+    const T* base = P.base ? static_cast<const T*>(P.base) + row * P.base_row : nullptr;
+    using Acc = typename AccOf<T>::type;
+    for (int64_t c = n0 + threadIdx.x; c < n1; c += blockDim.x)
+        y[c] = bad ? narrow<T>((Acc)__longlong_as_double(0x7ff8000000000000ll)) : base ? base[c] : narrow<T>((Acc)0);
+}
+
+// A cluster of kAdapterCluster blocks takes the rows of one slot (or, without a
+// plan, up to kGroupRows rows of one adapter, found by the row that leads them).
+// The blocks share the length k of the first product; their partial sums meet
+// through distributed shared memory in the blocks' order, and each block then
+// writes its own share of the n output columns.
+template <typename T, bool TR>
+__global__ void __launch_bounds__(kAdapterThreads) adapter_rows_kernel(AdapterParams P) {
+    using Acc = typename AccOf<T>::type;
+    constexpr int V = 16 / sizeof(T);
+    __shared__ Acc part[kGroupRows][kAdapterMaxRank];
+    __shared__ Acc us[kGroupRows][kAdapterMaxRank];
+    __shared__ Acc red[TR ? kGroupRows : 1][TR ? kAdapterThreads : 1];
+    __shared__ unsigned masks[kFewRows / 32];
+    __shared__ int list[kSlotRows];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int cr = (int)cluster.block_rank();
+    const int64_t unit = blockIdx.x / kAdapterCluster;
+    int cls, count;
+    if (P.plan) {
+        const AdapterSlot s = reinterpret_cast<const AdapterSlot*>(P.plan + plan_slot_word(P.adapters))[unit];
+        cls = s.cls, count = s.count;
+        if (count == 0) return;
+        if (tid < count) list[tid] = (P.plan + plan_perm_word(P.rows, P.adapters))[s.start + tid];
+    } else {
+        cls = row_class(P.index, P.index_wide, unit, P.adapters);
+        const bool same = tid < P.rows && row_class(P.index, P.index_wide, tid, P.adapters) == cls;
+        const unsigned m = __ballot_sync(0xffffffffu, same);
+        if (lane == 0) masks[warp] = m;
+        __syncthreads();
+        int rank = 0, before = 0, total = 0;  // of this unit's row; of this thread's row
+        for (int w = 0; w < kFewRows / 32; ++w) {
+            const int c = __popc(masks[w]);
+            if (w < (unit >> 5)) rank += c;
+            if (w < warp) before += c;
+            total += c;
+        }
+        rank += __popc(masks[unit >> 5] & ((1u << (unit & 31)) - 1));
+        if (rank % kGroupRows) return;  // another row leads this one
+        before += __popc(m & ((1u << lane) - 1));
+        if (same && before >= rank && before < rank + kGroupRows) list[before - rank] = tid;
+        count = total - rank < kGroupRows ? total - rank : kGroupRows;
+        if (cls == P.adapters + 1 && tid == 0 && cr == 0)
+            report_error(P.sink.dev, P.sink.host, FPEMU_ERR_INVALID, kWhereAdapterIndex, (int)unit);
+    }
+    __syncthreads();
+    const int64_t kshare = ((P.k + kAdapterCluster - 1) / kAdapterCluster + 7) / 8 * 8;
+    const int64_t nshare = ((P.n + kAdapterCluster - 1) / kAdapterCluster + 7) / 8 * 8;
+    const int64_t k0 = cr * kshare < P.k ? cr * kshare : P.k, k1 = k0 + kshare < P.k ? k0 + kshare : P.k;
+    const int64_t n0 = cr * nshare < P.n ? cr * nshare : P.n, n1 = n0 + nshare < P.n ? n0 + nshare : P.n;
+    if (cls >= P.adapters) {
+        for (int i = 0; i < count; ++i) plain_row<T>(P, list[i], cls != P.adapters, n0, n1);
+        return;
+    }
+    const T* w1 = static_cast<const T*>(P.w1) + cls * P.w1_adapter;
+    const T* w2 = static_cast<const T*>(P.w2) + cls * P.w2_adapter;
+    const T* x = static_cast<const T*>(P.x);
+    const Acc s = (Acc)(P.scales ? P.scales[cls] : P.scale);
+    const bool vec = (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w1)) % 16 == 0 &&
+                     (P.x_row * sizeof(T)) % 16 == 0 && (P.w1_row * sizeof(T)) % 16 == 0;
+    for (int first = 0; first < count; first += kGroupRows) {
+        const int g_n = count - first < kGroupRows ? count - first : kGroupRows;
+        const T* xr[kGroupRows];
+#pragma unroll
+        for (int g = 0; g < kGroupRows; ++g) xr[g] = x + (int64_t)list[first + (g < g_n ? g : 0)] * P.x_row;
+        if (!TR) {
+            for (int j = warp; j < P.r; j += kAdapterThreads / 32) {
+                const T* w = w1 + j * P.w1_row;
+                Acc acc[kGroupRows] = {};
+                if (vec) {
+                    int64_t c = k0 + lane * V;
+                    for (; c + V <= k1; c += 32 * V) {
+                        alignas(16) T wv[V], xv[V];
+                        *reinterpret_cast<uint4*>(wv) = *reinterpret_cast<const uint4*>(w + c);
+#pragma unroll
+                        for (int g = 0; g < kGroupRows; ++g)
+                            if (g < g_n) {
+                                *reinterpret_cast<uint4*>(xv) = *reinterpret_cast<const uint4*>(xr[g] + c);
+#pragma unroll
+                                for (int i = 0; i < V; ++i) acc[g] += widen(wv[i]) * widen(xv[i]);
+                            }
+                    }
+                    for (; c < k1; ++c)  // the lane that meets the end takes the last, short vector
+#pragma unroll
+                        for (int g = 0; g < kGroupRows; ++g)
+                            if (g < g_n) acc[g] += widen(w[c]) * widen(xr[g][c]);
+                } else {
+                    for (int64_t c = k0 + lane; c < k1; c += 32)
+#pragma unroll
+                        for (int g = 0; g < kGroupRows; ++g)
+                            if (g < g_n) acc[g] += widen(w[c]) * widen(xr[g][c]);
+                }
+#pragma unroll
+                for (int g = 0; g < kGroupRows; ++g) {
+                    if (g >= g_n) break;
+                    Acc v = acc[g];
+                    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                    if (lane == 0) part[g][j] = v;
+                }
+            }
+        } else {
+            int rp = 1;
+            while (rp < P.r) rp *= 2;
+            const int j = tid & (rp - 1), step = kAdapterThreads / rp;
+            Acc acc[kGroupRows] = {};
+            if (j < P.r)
+                for (int64_t c = k0 + tid / rp; c < k1; c += step) {
+                    const Acc wv = widen(w1[c * P.w1_row + j]);
+#pragma unroll
+                    for (int g = 0; g < kGroupRows; ++g)
+                        if (g < g_n) acc[g] += wv * widen(xr[g][c]);
+                }
+#pragma unroll
+            for (int g = 0; g < kGroupRows; ++g) red[g][tid] = acc[g];
+            __syncthreads();
+            for (int i = tid; i < g_n * P.r; i += kAdapterThreads) {
+                const int g = i / P.r, jj = i % P.r;
+                Acc v = 0;
+                for (int q = 0; q < step; ++q) v += red[g][q * rp + jj];
+                part[g][jj] = v;
+            }
+        }
+        cluster.sync();
+        for (int i = tid; i < g_n * P.r; i += kAdapterThreads) {
+            const int g = i / P.r, j = i % P.r;
+            Acc v = 0;
+            for (int b = 0; b < kAdapterCluster; ++b) v += *cluster.map_shared_rank(&part[g][j], b);
+            us[g][j] = v * s;
+            if (P.u && cr == 0) static_cast<Acc*>(P.u)[(int64_t)list[first + g] * P.r + j] = v * s;
+        }
+        cluster.sync();  // every block has read the partial sums
+        for (int64_t c = n0 + tid; c < n1; c += kAdapterThreads) {
+            Acc acc[kGroupRows] = {};
+            for (int j = 0; j < P.r; ++j) {
+                const Acc wv = widen(TR ? w2[j * P.w2_row + c] : w2[c * P.w2_row + j]);
+#pragma unroll
+                for (int g = 0; g < kGroupRows; ++g)
+                    if (g < g_n) acc[g] += wv * us[g][j];
+            }
+#pragma unroll
+            for (int g = 0; g < kGroupRows; ++g)
+                if (g < g_n) {
+                    const int64_t row = list[first + g];
+                    Acc v = acc[g];
+                    if (P.base) v += widen(static_cast<const T*>(P.base)[row * P.base_row + c]);
+                    static_cast<T*>(P.y)[row * P.y_row + c] = narrow<T>(v);
+                }
+        }
+        __syncthreads();  // `us` is rewritten by the next rows
+    }
+}
+
+// grad[i][j][c] = sum over the rows t of adapter i of p[t][j] * q[t][c]: dA from
+// (v, x) and dB from (u, dy).  A thread holds 16 values of j for one column.
+struct AdapterGradParams {
+    int64_t rows, cols;
+    int r, adapters;
+    const void* p;   // [rows, r] of the sums' type
+    const void* q;   // [rows, cols]
+    int64_t q_row;
+    void* grad;      // element (i, j, c) at i * r * cols + j * grad_j + c * grad_c
+    int64_t grad_j, grad_c;
+    const int32_t* plan;
+};
+
+constexpr int kGradJ = 16;
+constexpr int kGradChunk = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(128) adapter_grad_kernel(AdapterGradParams P) {
+    using Acc = typename AccOf<T>::type;
+    __shared__ int list[kGradChunk];
+    const int cls = blockIdx.y, j0 = blockIdx.z * kGradJ;
+    const int64_t c = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    const int start = P.plan[cls], end = P.plan[cls + 1];
+    const int32_t* perm = P.plan + plan_perm_word(P.rows, P.adapters);
+    const Acc* p = static_cast<const Acc*>(P.p);
+    const T* q = static_cast<const T*>(P.q);
+    Acc sum[kGradJ] = {};
+    for (int t = start; t < end; t += kGradChunk) {
+        const int m = end - t < kGradChunk ? end - t : kGradChunk;
+        __syncthreads();
+        if ((int)threadIdx.x < m) list[threadIdx.x] = perm[t + threadIdx.x];
+        __syncthreads();
+        if (c >= P.cols) continue;
+        Acc acc[kGradJ] = {};
+        for (int i = 0; i < m; ++i) {
+            const int64_t row = list[i];
+            const Acc v = widen(q[row * P.q_row + c]);
+#pragma unroll
+            for (int j = 0; j < kGradJ; ++j)
+                if (j0 + j < P.r) acc[j] += v * p[row * P.r + j0 + j];
+        }
+#pragma unroll
+        for (int j = 0; j < kGradJ; ++j) sum[j] += acc[j];
+    }
+    if (c < P.cols)
+#pragma unroll
+        for (int j = 0; j < kGradJ; ++j)
+            if (j0 + j < P.r)
+                static_cast<T*>(P.grad)[(int64_t)cls * P.r * P.cols + (j0 + j) * P.grad_j + c * P.grad_c] = narrow<T>(sum[j]);
+}
+
+}  // namespace fpemu

@@ -17,16 +17,17 @@
 #include <string>
 
 #include "crt_kernels.cuh"
+#include "fpemu_host.h"
 #include "gemm_kernel.cuh"
 #include "split_kernels.cuh"
 
 using namespace fpemu;
 
 namespace {
-
 thread_local std::string t_last_error;
+}
 
-int fail(int code, const char* fmt, ...) {
+int fpemu::fail(int code, const char* fmt, ...) {
     char buf[512];
     va_list ap;
     va_start(ap, fmt);
@@ -36,17 +37,7 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 
-#define FPEMU_CUDA(expr)                                                                        \
-    do {                                                                                        \
-        cudaError_t e_ = (expr);                                                                \
-        if (e_ != cudaSuccess) return fail(FPEMU_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(e_)); \
-    } while (0)
-
-#define FPEMU_TRY(expr)              \
-    do {                             \
-        int s_ = (expr);             \
-        if (s_ != FPEMU_OK) return s_; \
-    } while (0)
+namespace {
 
 // GEMM configurations.  Main: CTA pairs (2-SM MMA, M = 256) on 256 x 256
 // tiles, a 6-stage ring of 32 KB per CTA, 8 epilogue warps, 2 accumulators of
@@ -56,12 +47,9 @@ using MainCfg = GemmCfg<2, 256, 6, 8, 2>;
 using SingleCfg = GemmCfg<1, 256, 4, 8, 2>;
 static_assert(MainCfg::BN == SingleCfg::BN, "both configurations share the workspace layout");
 
-struct DevInfo {
-    int sms = 0;
-    int major = 0, minor = 0;
-};
+}  // namespace
 
-int device_info(DevInfo* out) {
+int fpemu::device_info(DevInfo* out) {
     static std::mutex mu;
     static DevInfo cache[64];
     static bool have[64] = {};
@@ -83,6 +71,8 @@ int device_info(DevInfo* out) {
                     out->major, out->minor);
     return FPEMU_OK;
 }
+
+namespace {
 
 // Split of a K-contiguous operand: 1 = both passes in one kernel (the row is
 // re-read from L2), 2 = an exponent kernel, then a residue kernel
@@ -559,6 +549,35 @@ int host_error_slot(volatile DeviceError** out, bool create) {
     *out = block + dev;
     return FPEMU_OK;
 }
+
+}  // namespace
+
+int fpemu::error_sink(ErrorSink* out) {
+    static std::mutex mu;
+    static ErrorSink cache[64] = {};
+    int dev = 0;
+    FPEMU_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return fail(FPEMU_ERR_NO_DEVICE, "device ordinal %d out of range", dev);
+    std::lock_guard<std::mutex> lk(mu);
+    if (cache[dev].dev == nullptr) {
+        void* p = nullptr;
+        FPEMU_CUDA(cudaGetSymbolAddress(&p, g_device_error));
+        cache[dev].dev = static_cast<DeviceError*>(p);
+    }
+    if (cache[dev].host == nullptr) {
+        volatile DeviceError* h = nullptr;
+        FPEMU_TRY(host_error_slot(&h, false));
+        if (h != nullptr) {
+            void* d = nullptr;
+            FPEMU_CUDA(cudaHostGetDevicePointer(&d, const_cast<DeviceError*>(h), 0));
+            cache[dev].host = static_cast<DeviceError*>(d);
+        }
+    }
+    *out = cache[dev];
+    return FPEMU_OK;
+}
+
+namespace {
 
 int check_gemm_args(int64_t m, int64_t n, int64_t k, int n_mod, const void* a_res, const void* b_res,
                     int64_t res_ld) {

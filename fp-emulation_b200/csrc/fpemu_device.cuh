@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "fpemu_error.cuh"
 #include "fpemu_internal.h"
 
 namespace fpemu {
@@ -16,13 +17,6 @@ namespace fpemu {
 // first failure here (code, role, block) and the kernel unwinds; the host
 // reads it back with fpemu_device_error().  Nothing traps.
 // ----------------------------------------------------------------------------
-struct DeviceError {
-    int code;    // FPEMU_ERR_TIMEOUT, ...
-    int where;   // which wait gave up (see kWait*)
-    int block;   // blockIdx.x of the first failing CTA
-    int detail;  // role-specific (unit index, stage, ...)
-};
-
 enum : int {
     kWaitFull = 1,       // MMA warp waiting for a TMA stage
     kWaitEmpty = 2,      // producer waiting for a free stage
@@ -42,21 +36,7 @@ __device__ DeviceError g_device_error;
 __device__ DeviceError* g_host_error;
 
 __device__ __forceinline__ void report_error(DeviceError* err, int code, int where, int detail) {
-    if (err != nullptr && atomicCAS(&err->code, 0, code) == 0) {
-        err->where = where;
-        err->block = (int)blockIdx.x;
-        err->detail = detail;
-        __threadfence();
-        volatile DeviceError* h = g_host_error;
-        if (h != nullptr) {
-            h->where = where;
-            h->block = (int)blockIdx.x;
-            h->detail = detail;
-            __threadfence_system();
-            h->code = code;  // last: a non-zero code means the other fields are set
-            __threadfence_system();
-        }
-    }
+    report_error(err, g_host_error, code, where, detail);
 }
 
 __device__ __forceinline__ uint64_t global_ns() {

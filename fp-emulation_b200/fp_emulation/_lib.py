@@ -24,6 +24,12 @@ FPEMU_ERR_TIMEOUT = 6
 FPEMU_ERR_NO_DEVICE = 7
 FPEMU_C_F64 = 0
 FPEMU_C_F32 = 1
+FPEMU_DT_F64, FPEMU_DT_F32, FPEMU_DT_F16, FPEMU_DT_BF16 = range(4)
+FPEMU_ADAPTER_MAX_RANK = 128
+FPEMU_ADAPTER_MAX_COUNT = 65000
+FPEMU_ADAPTER_MAX_ROWS = 0x40000000
+FPEMU_ADAPTER_FEW_ROWS = 256
+WHERE_ADAPTER_INDEX = 16  # `where` of device_error(): a row's adapter id is none
 
 # Every symbol include/fpemu.h declares, with its ctypes signature.
 _i64, _int, _sz, _vp, _dp = ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_double
@@ -52,6 +58,14 @@ SIGNATURES = {
     "fpemu_gemm_crt_segmented": (_int, [_i64, _i64, _i64, _int, _vp, _vp, _i64, _i64, _vp, _vp, _int, _vp, _i64,
                                         _i64, _i64, _int, _vp, _sz, _vp]),
     "fpemu_gemm_crt_noalloc": (_int, [_i64, _i64, _i64, _int, _vp, _vp, _i64, _vp, _vp, _int, _vp, _i64, _vp]),
+    "fpemu_adapter_plan_size": (_i64, [_i64, _i64]),
+    "fpemu_adapter_plan": (_int, [_vp, _int, _i64, _i64, _vp, _sz, _vp]),
+    "fpemu_adapter_matmul": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                                    _int, _vp, _i64, _vp, _i64, _vp, _dp, _vp, _int, _vp, _vp, _vp]),
+    "fpemu_adapter_grads": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
+                                   _vp]),
+    "fpemu_clip_workspace_size": (_sz, [_i64]),
+    "fpemu_clip_grads": (_int, [_i64, _vp, _vp, _vp, _vp, _int, _dp, _vp, _int, _vp, _sz, _vp]),
     "fpemu_device_error": (_int, [_IP, _IP, _IP, _IP, _int]),
     "fpemu_watch_errors": (_int, []),
     "fpemu_poll_error": (_int, [_IP, _IP, _IP, _IP]),

@@ -1,0 +1,338 @@
+"""Low-rank adapters of many requests beside a shared projection.
+
+A batch shares one projection ``base = x @ W.T`` (an emulated product, see
+``fp_emulation.ozaki``); every row adds the low-rank product of its own adapter:
+
+    y[t] = base[t] + scale_i * B[i] @ (A[i] @ x[t]),   i = index[t]
+
+``adapter_matmul`` is the operator, with its gradients; ``prepare_rows`` groups
+the rows of a batch by adapter once for all layers; ``Adapters`` holds the
+factors as parameters, and ``add_adapters`` / ``use_adapters`` put them beside
+the ``Linear`` layers of a model.  CUDA tensors only.  Nothing here has a
+counterpart in the reference.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from fp_emulation import _lib
+from fp_emulation.ozaki import _after_call, _dtype_bits, _require_cuda, _stream
+
+_DTYPE_CODE = {torch.float64: _lib.FPEMU_DT_F64, torch.float32: _lib.FPEMU_DT_F32,
+               torch.float16: _lib.FPEMU_DT_F16, torch.bfloat16: _lib.FPEMU_DT_BF16}
+
+
+class PreparedRows:
+    """The rows of a batch grouped by adapter (``prepare_rows``): a snapshot of
+    the index on the GPU, shared by every layer and by the backward pass."""
+
+    def __init__(self, index, adapters, shape=None):
+        if not isinstance(index, torch.Tensor) or index.dtype not in (torch.int32, torch.int64):
+            raise TypeError("adapter ids are an int32 or int64 tensor")
+        adapters = int(adapters)
+        if not 1 <= adapters <= _lib.FPEMU_ADAPTER_MAX_COUNT:
+            raise ValueError(f"{adapters} adapters; between 1 and {_lib.FPEMU_ADAPTER_MAX_COUNT} are supported")
+        dev = _require_cuda(index)
+        self.shape = index.shape if shape is None else torch.Size(shape)
+        self.adapters = adapters
+        self.index = _spread_index(index, self.shape).reshape(-1).clone()
+        rows = self.index.numel()
+        if rows > _lib.FPEMU_ADAPTER_MAX_ROWS:
+            raise ValueError(f"{rows} rows; at most {_lib.FPEMU_ADAPTER_MAX_ROWS} are supported")
+        lib = _lib.load()
+        self.plan = torch.empty((lib.fpemu_adapter_plan_size(rows, adapters) // 4,), dtype=torch.int32, device=dev)
+        with torch.cuda.device(dev):
+            st = lib.fpemu_adapter_plan(self.index.data_ptr(), self.index.element_size(), rows, adapters,
+                                        self.plan.data_ptr(), self.plan.numel() * 4, _stream(dev))
+        _lib.check(st, "prepare_rows")
+        _after_call("prepare_rows", dev)
+
+
+def prepare_rows(index, adapters, shape=None):
+    """Group the rows of a batch by adapter, once for every layer that the batch
+    passes.  ``index`` (int32 or int64, on the GPU) holds each row's adapter,
+    0 .. adapters - 1, or -1 for none; ``shape`` gives it the leading shape of the
+    layers' inputs where it has fewer dimensions (one id for each request of a
+    [requests, length, features] batch).  Later changes of ``index`` do not
+    change the result.  An id that is no adapter makes its rows NaN and raises
+    ``FpemuError`` in the first call that ends after the kernel has seen it."""
+    return PreparedRows(index, adapters, shape)
+
+
+def _spread_index(index, shape):
+    if index.shape == shape:
+        return index
+    if index.dim() > len(shape) or index.shape != shape[:index.dim()]:
+        raise RuntimeError(f"adapter ids of shape {tuple(index.shape)} do not match rows of shape {tuple(shape)}")
+    return index.reshape(index.shape + (1,) * (len(shape) - index.dim())).expand(shape)
+
+
+def _last_contiguous(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _launch(x, w1, w2, transposed, base, y, scale, index, plan, adapters, rank, k, n, u):
+    """One fpemu_adapter_matmul on the current stream of x's device."""
+    dev = x.device
+    scales = scale if isinstance(scale, torch.Tensor) else None
+    with torch.cuda.device(dev):
+        st = _lib.load().fpemu_adapter_matmul(
+            _DTYPE_CODE[x.dtype], x.shape[0], k, n, rank, adapters, x.data_ptr(), _row_stride(x),
+            w1.data_ptr(), w1.stride(0), w1.stride(1), w2.data_ptr(), w2.stride(0), w2.stride(1), transposed,
+            None if base is None else base.data_ptr(), 0 if base is None else base.stride(0),
+            None if y is None else y.data_ptr(), n if y is None else _row_stride(y),
+            None if scales is None else scales.data_ptr(), 0.0 if scales is not None else scale,
+            None if index is None else index.data_ptr(), 0 if index is None else index.element_size(),
+            None if plan is None else plan.data_ptr(), None if u is None else u.data_ptr(), _stream(dev))
+    _lib.check(st, "adapter_matmul")
+    _after_call("adapter_matmul", dev)
+
+
+def _sum_dtype(dtype):
+    return torch.float64 if dtype == torch.float64 else torch.float32
+
+
+class _AdapterMatmul(torch.autograd.Function):
+    """The operator and its gradients.  Products of the first factor (u) are kept
+    in the sums' type for dB; the backward pass makes v = scale * dy B the same
+    way while it makes dx, and sums dA and dB over the rows of each adapter."""
+
+    @staticmethod
+    def forward(ctx, x, A, B, base, rows, scale):
+        y = torch.empty((x.shape[0], B.shape[1]), dtype=x.dtype, device=x.device)
+        u = torch.empty((x.shape[0], A.shape[1]), dtype=_sum_dtype(x.dtype), device=x.device)
+        _launch(x, A, B, 0, base, y, scale, rows.index, _plan_of(rows), rows.adapters, A.shape[1], A.shape[2],
+                B.shape[1], u)
+        ctx.save_for_backward(x, A, B, u)
+        ctx.rows, ctx.scale = rows, scale
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, A, B, u = ctx.saved_tensors
+        rows, scale = ctx.rows, ctx.scale
+        need_x, need_A, need_B, need_base = ctx.needs_input_grad[:4]
+        n_ad, rank, k = A.shape
+        n = B.shape[1]
+        dyc = _last_contiguous(dy)
+        dx = dA = dB = v = None
+        if need_x or need_A:
+            v = torch.empty_like(u)
+            if need_x:
+                dx = torch.empty((x.shape[0], k), dtype=x.dtype, device=x.device)
+            _launch(dyc, B, A, 1, None, dx, scale, rows.index, _plan_of(rows), n_ad, rank, n, k if need_x else 0, v)
+        if need_A or need_B:
+            dA = torch.empty((n_ad, rank, k), dtype=A.dtype, device=A.device) if need_A else None
+            dB = torch.empty((n_ad, n, rank), dtype=B.dtype, device=B.device) if need_B else None
+            dev = x.device
+            with torch.cuda.device(dev):
+                st = _lib.load().fpemu_adapter_grads(
+                    _DTYPE_CODE[x.dtype], x.shape[0], k, n, rank, n_ad, x.data_ptr(), _row_stride(x),
+                    dyc.data_ptr(), _row_stride(dyc), u.data_ptr(), None if v is None else v.data_ptr(),
+                    rows.plan.data_ptr(), None if dA is None else dA.data_ptr(),
+                    None if dB is None else dB.data_ptr(), _stream(dev))
+            _lib.check(st, "adapter_matmul backward")
+            _after_call("adapter_matmul backward", dev)
+        return dx, dA, dB, dy if need_base else None, None, None
+
+
+def _plan_of(rows):
+    """Few rows are grouped inside the kernel; more go by the plan."""
+    return None if rows.index.numel() <= _lib.FPEMU_ADAPTER_FEW_ROWS else rows.plan
+
+
+def _span(t):
+    first = t.data_ptr()
+    return first, first + (sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _check_out(out, shape, x, base, others):
+    if out.shape != shape or out.dtype != x.dtype or out.device != x.device:
+        raise RuntimeError(f"out must be a {x.dtype} tensor of shape {tuple(shape)} on {x.device}")
+    o2 = out.view(-1, shape[-1]) if out.numel() else out.reshape(-1, shape[-1])
+    if out.numel() == 0:
+        return o2
+    if o2.stride(-1) != 1 and o2.shape[-1] > 1 or o2.shape[0] > 1 and o2.stride(0) < o2.shape[1]:
+        raise RuntimeError("out needs a contiguous last dimension and rows that do not overlap")
+    lo, hi = _span(o2)
+    for t in others:
+        if t.numel():
+            a, b = _span(t)
+            if a < hi and lo < b:
+                raise RuntimeError("out overlaps an input")
+    if base is not None:
+        a, b = _span(base)
+        if a < hi and lo < b and not (base.data_ptr() == out.data_ptr() and base.shape == out.shape
+                                      and base.stride() == out.stride()):
+            raise RuntimeError("out overlaps base without being base")
+    return o2
+
+
+def adapter_matmul(x, A, B, rows, base=None, scale=1.0, out=None):
+    """``base + scale_i * (x @ A[i].T) @ B[i].T`` with each row's own adapter i.
+
+    x: [..., k]; A: [adapters, rank, k]; B: [adapters, n, rank], all of one float
+    dtype (float64, float32, float16, bfloat16).  rows: ``prepare_rows(...)`` of
+    the batch, or an int32/int64 tensor of ids whose shape is x's leading shape or
+    the first dimensions of it (-1: no adapter; such a row returns ``base``).
+    base: broadcastable to [..., n], or None for zero.  scale: one number, or a
+    tensor with one value for each adapter (no gradient).  out: where to write the
+    result when autograd does not record; it may be ``base`` itself.
+
+    Sums are held in float64 for float64 and in float32 otherwise, and the result
+    is rounded once.  x, A, B and base have gradients (once; not twice
+    differentiable); repeated calls give the same bits."""
+    _dtype_bits(x.dtype)
+    tensors = [x, A, B] + ([base] if base is not None else [])
+    dev = _require_cuda(*tensors)
+    if any(t.dtype != x.dtype for t in tensors):
+        raise TypeError(f"adapter_matmul: operands of one dtype, got {', '.join(str(t.dtype) for t in tensors)}")
+    if x.dim() < 1 or A.dim() != 3 or B.dim() != 3 or A.shape[0] != B.shape[0] or A.shape[1] != B.shape[2] \
+            or A.shape[2] != x.shape[-1]:
+        raise RuntimeError(f"adapter_matmul: expected x [..., k], A [adapters, rank, k], B [adapters, n, rank], got "
+                           f"{tuple(x.shape)}, {tuple(A.shape)}, {tuple(B.shape)}")
+    adapters, rank, k = A.shape
+    n = B.shape[1]
+    if not 1 <= rank <= _lib.FPEMU_ADAPTER_MAX_RANK:
+        raise ValueError(f"adapter_matmul: rank {rank}; between 1 and {_lib.FPEMU_ADAPTER_MAX_RANK} is supported")
+    if not 1 <= adapters <= _lib.FPEMU_ADAPTER_MAX_COUNT:
+        raise ValueError(f"adapter_matmul: {adapters} adapters; between 1 and {_lib.FPEMU_ADAPTER_MAX_COUNT}")
+    if isinstance(scale, torch.Tensor):
+        if scale.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("adapter_matmul: scale has no gradient")
+        if scale.shape != (adapters,):
+            raise RuntimeError(f"adapter_matmul: scale of shape {tuple(scale.shape)} for {adapters} adapters")
+        scale = scale.detach().to(device=dev, dtype=torch.float64).contiguous()
+    else:
+        scale = float(scale)
+    lead = x.shape[:-1]
+    shape = lead + (n,)
+    count = math.prod(lead)
+    records = torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    if isinstance(rows, PreparedRows):
+        if rows.adapters != adapters:
+            raise RuntimeError(f"adapter_matmul: rows prepared for {rows.adapters} adapters, not {adapters}")
+        if rows.index.numel() != count:
+            raise RuntimeError(f"adapter_matmul: {rows.index.numel()} prepared rows for {count} rows of x")
+        if rows.index.device != dev:
+            raise RuntimeError(f"operands on different devices: {dev} and {rows.index.device}")
+    elif isinstance(rows, torch.Tensor):
+        if rows.dtype not in (torch.int32, torch.int64):
+            raise TypeError("adapter ids are an int32 or int64 tensor")
+        _require_cuda(x, rows)
+        index = _spread_index(rows, lead)
+        if records or count > _lib.FPEMU_ADAPTER_FEW_ROWS:
+            rows = PreparedRows(index, adapters)
+        else:
+            rows = None
+            index = index.reshape(-1).contiguous()
+    else:
+        raise TypeError("rows is a tensor of adapter ids or the result of prepare_rows")
+    if base is not None:
+        base = base.expand(shape)
+    if records:
+        if out is not None:
+            raise RuntimeError("adapter_matmul: out cannot be given while autograd records")
+        y = _AdapterMatmul.apply(_last_contiguous(x.reshape(count, k)), _last_contiguous(A), _last_contiguous(B),
+                                 None if base is None else _last_contiguous(base.reshape(count, n)), rows, scale)
+        return y.view(shape)
+    with torch.no_grad():
+        x2, A, B = _last_contiguous(x.reshape(count, k)), _last_contiguous(A), _last_contiguous(B)
+        if out is None:
+            y = torch.empty((count, n), dtype=x.dtype, device=dev)
+        else:
+            y = _check_out(out, shape, x, base, (x, A, B))
+        base2 = None if base is None else _last_contiguous(base.reshape(count, n))
+        plan = None if rows is None else _plan_of(rows)
+        _launch(x2, A, B, 0, base2, y, scale, index if rows is None else rows.index, plan, adapters, rank, k, n, None)
+    if out is None:
+        return y.view(shape)
+    torch.autograd.graph.increment_version(out)
+    return out
+
+
+class Adapters(nn.Module):
+    """The factors of ``adapters`` low-rank adapters of one projection: A
+    [adapters, rank, in_features] and B [adapters, out_features, rank], with B zero
+    at first so that a new adapter changes nothing.  ``scale`` is alpha / rank."""
+
+    def __init__(self, adapters, in_features, out_features, rank, alpha=None, device=None, dtype=torch.float64):
+        super().__init__()
+        _dtype_bits(dtype)
+        if not 1 <= rank <= _lib.FPEMU_ADAPTER_MAX_RANK:
+            raise ValueError(f"rank {rank}; between 1 and {_lib.FPEMU_ADAPTER_MAX_RANK} is supported")
+        self.scale = (rank if alpha is None else alpha) / rank
+        self.A = nn.Parameter(torch.empty((adapters, rank, in_features), device=device, dtype=dtype))
+        self.B = nn.Parameter(torch.zeros((adapters, out_features, rank), device=device, dtype=dtype))
+        bound = 1.0 / math.sqrt(max(in_features, 1))
+        nn.init.uniform_(self.A, -bound, bound)
+
+    @property
+    def adapters(self):
+        return self.A.shape[0]
+
+    def extra_repr(self):
+        n, rank, k = self.A.shape
+        return f"adapters={n}, in_features={k}, out_features={self.B.shape[1]}, rank={rank}, scale={self.scale}"
+
+    def forward(self, x, rows, base=None, out=None):
+        return adapter_matmul(x, self.A, self.B, rows, base=base, scale=self.scale, out=out)
+
+
+class _ActiveRows:
+    """The ids of the batch inside a ``use_adapters`` block; grouped once for each
+    leading shape that the layers meet."""
+
+    def __init__(self, index):
+        self.index = index
+        self.prepared = {}
+
+    def prepare(self, lead, adapters):
+        key = (tuple(lead), adapters)
+        if key not in self.prepared:
+            self.prepared[key] = PreparedRows(self.index, adapters, lead)
+        return self.prepared[key]
+
+
+@contextlib.contextmanager
+def use_adapters(model, index):
+    """Within the block, the model's layers that have adapters (``add_adapters``)
+    apply row t's adapter ``index[t]`` (-1: none).  ``index`` has the leading shape
+    of the layers' inputs, or the first dimensions of it."""
+    from fp_emulation.nn import Linear
+
+    layers = [m for m in model.modules() if isinstance(m, Linear) and m._modules.get("adapters") is not None]
+    if not layers:
+        raise RuntimeError("use_adapters: the model has no Linear with adapters (add_adapters)")
+    before = [m.active_rows for m in layers]
+    active = _ActiveRows(index)
+    for m in layers:
+        m.active_rows = active
+    try:
+        yield model
+    finally:
+        for m, rows in zip(layers, before):
+            m.active_rows = rows
+
+
+def add_adapters(model, adapters, rank, alpha=None):
+    """Put ``adapters`` low-rank adapters beside every ``fp_emulation.Linear`` of
+    ``model`` (as ``layer.adapters``, float64 like the layer) and return the model.
+    Outside a ``use_adapters`` block the layers compute as before."""
+    from fp_emulation.nn import Linear
+
+    for m in list(model.modules()):
+        if isinstance(m, Linear):
+            m.adapters = Adapters(adapters, m.in_features, m.out_features, rank, alpha, device=m.weight.device)
+    return model

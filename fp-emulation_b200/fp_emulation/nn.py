@@ -16,11 +16,17 @@ class Linear(nn.Linear):
     ``cache_weight_residues=True`` additionally keeps the split (int8 residues
     and column exponents) of the weight between such calls -- n_mod bytes per
     weight element -- and re-splits only when the weight's storage or version
-    changes (an optimizer step, ``load_state_dict``, any in-place update)."""
+    changes (an optimizer step, ``load_state_dict``, any in-place update).
+
+    ``adapters`` (None until ``add_adapters``) are low-rank adapters beside the
+    product; they act inside a ``use_adapters`` block, each row by its own."""
+
+    active_rows = None  # the batch's adapter ids, set by use_adapters
 
     def __init__(self, in_features, out_features, bias=True, device=None, cache_weight_residues=False):
         super().__init__(in_features, out_features, bias=bias, device=device, dtype=torch.float64)
         self.cache_weight_residues = cache_weight_residues
+        self.register_module("adapters", None)
         self._weight_op = None  # (the weight Parameter it was made for, PreparedOperand of W^T)
 
     def _records_grad(self, x):
@@ -48,6 +54,12 @@ class Linear(nn.Linear):
             y = _ozaki2_forward_prepared(x2d, self._weight_operand(), bias=self.bias)
         else:
             y = _ozaki2_forward(x2d, self.weight.T, bias=self.bias)
+        adapters = self._modules.get("adapters")  # absent from a layer pickled before there were any
+        if adapters is not None and self.active_rows is not None:
+            rows = self.active_rows.prepare(lead, adapters.adapters)
+            records = torch.is_grad_enabled() and (y.requires_grad or x2d.requires_grad or any(
+                p.requires_grad for p in adapters.parameters()))
+            y = adapters(x2d, rows, base=y, out=None if records else y)
         return y.reshape(*lead, self.out_features)
 
 

@@ -96,6 +96,9 @@ def _after_call(what: str, dev) -> None:
         if _CHECK_MODE == "poll" and _lib.poll_error()[0] == 0:
             return
         code, where, block, detail = _lib.device_error(clear=True)
+    if code == _lib.FPEMU_ERR_INVALID and where == _lib.WHERE_ADAPTER_INDEX:
+        raise _lib.FpemuError(code, f"{what}: row {detail} of a batch on {dev} has an adapter id that is neither -1 "
+                                    "nor an adapter; its outputs are NaN")
     if code:
         raise _lib.FpemuError(code, f"{what}: a kernel of fp_emulation on {dev} gave up waiting (where={where} "
                                     f"block={block} detail={detail}); the outputs it could not finish are NaN")

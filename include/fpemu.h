@@ -194,6 +194,68 @@ int fpemu_gemm_kernels(int64_t m, int64_t n);
  * per-CTA residue staging, or the split form's residues). */
 size_t fpemu_gemm_workspace_size(int64_t m, int64_t n, int n_mod);
 
+/* ---- adapters and gradients: no counterpart in the reference --------------- */
+
+/* Element types of the entry points below. */
+#define FPEMU_DT_F64 0
+#define FPEMU_DT_F32 1
+#define FPEMU_DT_F16 2
+#define FPEMU_DT_BF16 3
+
+#define FPEMU_ADAPTER_MAX_RANK 128
+#define FPEMU_ADAPTER_MAX_COUNT 65000
+#define FPEMU_ADAPTER_MAX_ROWS 0x40000000
+#define FPEMU_ADAPTER_FEW_ROWS 256
+
+/* The plan of a batch: its rows grouped by adapter.  `index` holds one id per
+ * row (index_bytes 4 or 8): 0 .. adapters - 1, or -1 for a row without an
+ * adapter.  Any other id is recorded as a device error (FPEMU_ERR_INVALID) and
+ * that row's output becomes NaN.  A plan serves every fpemu_adapter_matmul and
+ * fpemu_adapter_grads of the batch; it is a snapshot of the index. */
+int64_t fpemu_adapter_plan_size(int64_t rows, int64_t adapters); /* bytes; 0 when out of range */
+int fpemu_adapter_plan(const void *index, int index_bytes, int64_t rows, int64_t adapters,
+                       void *plan, size_t plan_bytes, void *stream);
+
+/* y[t] = base[t] + W2_i (s_i W1_i x[t]) for every row t with adapter i;
+ * base[t] (0 when base is NULL) for a row without one.  x is rows x k, y and
+ * base rows x n; strides are in elements and the last dimension is contiguous.
+ *   transposed 0: w1 is [adapters][rank][k], w2 is [adapters][n][rank]
+ *                 (the forward product, w1 = A, w2 = B);
+ *   transposed 1: w1 is [adapters][k][rank], w2 is [adapters][rank][n]
+ *                 (its gradient by x: x = dy, w1 = B, w2 = A).
+ * scales: one double per adapter, or NULL for `scale` everywhere.
+ * u (or NULL): rows x rank values s_i W1_i x[t] -- double for FPEMU_DT_F64, else
+ * float; rows without an adapter are not written.
+ * y may be base itself; otherwise it overlaps no input.
+ * plan NULL: rows <= FPEMU_ADAPTER_FEW_ROWS, grouped by the kernel from index. */
+int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank,
+                         int64_t adapters, const void *x, int64_t x_row, const void *w1,
+                         int64_t w1_adapter, int64_t w1_row, const void *w2, int64_t w2_adapter,
+                         int64_t w2_row, int transposed, const void *base, int64_t base_row,
+                         void *y, int64_t y_row, const double *scales, double scale,
+                         const void *index, int index_bytes, const void *plan, void *u,
+                         void *stream);
+
+/* Gradients of the factors, each [adapters][...] packed, zero for an adapter
+ * without rows: dA[i] = sum_t v[t]^T x[t] (rank x k) and dB[i] = sum_t dy[t]^T u[t]
+ * (n x rank) over the rows t of adapter i, in the rows' order.  u and v are what
+ * fpemu_adapter_matmul left (forward, and transposed on dy).  dA or dB may be NULL. */
+int fpemu_adapter_grads(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank,
+                        int64_t adapters, const void *x, int64_t x_row, const void *dy,
+                        int64_t dy_row, const void *u, const void *v, const void *plan, void *dA,
+                        void *dB, void *stream);
+
+/* The norm over every element of `count` tensors of any types (arrays of
+ * pointers, sizes and FPEMU_DT_ codes in host memory), norm_type 1, 2, or 0 for
+ * the largest magnitude; summed in double.  *norm (device) is a double or, with
+ * norm_f64 = 0, a float.  dst NULL: the norm alone.  Otherwise tensor i times
+ * min(1, max_norm / (norm + 1e-6)) goes to dst[i], which is src[i] or overlaps
+ * no tensor. */
+size_t fpemu_clip_workspace_size(int64_t count);
+int fpemu_clip_grads(int64_t count, const void *const *src, void *const *dst, const int64_t *numel,
+                     const int32_t *dtype, int norm_type, double max_norm, void *norm, int norm_f64,
+                     void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- device status ---------------------------------------------------------- */
 
 /* Synchronise the current device and read (optionally clear) the first error a
