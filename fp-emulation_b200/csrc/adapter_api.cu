@@ -2,7 +2,10 @@
 // (declared in include/fpemu.h).
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "adapter_kernels.cuh"
+#include "adapter_tiles.cuh"
 #include "fpemu_host.h"
 
 using namespace fpemu;
@@ -49,6 +52,38 @@ int launch_rows(const AdapterParams& P, bool transposed, cudaStream_t st) {
     cfg.numAttrs = 1;
     FPEMU_CUDA(cudaLaunchKernelEx(&cfg, transposed ? adapter_rows_kernel<T, true> : adapter_rows_kernel<T, false>, P));
     return FPEMU_OK;
+}
+
+template <typename T, bool TR, int RP>
+int launch_tiles_rank(const AdapterParams& P, const DevInfo& d, cudaStream_t st) {
+    auto kern = adapter_tile_kernel<T, TR, RP>;
+    using Tile = AdapterTile<T, TR, RP>;
+    FPEMU_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem));
+    const int64_t slots = plan_slots(P.rows, P.adapters);
+    int cluster = 1;
+    while (cluster < 8 && P.rows / kSlotRows * cluster < d.sms * 4) cluster *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(slots * cluster));
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = Tile::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    FPEMU_CUDA(cudaLaunchKernelEx(&cfg, kern, P));
+    return FPEMU_OK;
+}
+
+template <typename T, bool TR>
+int launch_tiles(const AdapterParams& P, const DevInfo& d, cudaStream_t st) {
+    if (P.r <= 16) return launch_tiles_rank<T, TR, 16>(P, d, st);
+    if (P.r <= 32) return launch_tiles_rank<T, TR, 32>(P, d, st);
+    if (P.r <= 64) return launch_tiles_rank<T, TR, 64>(P, d, st);
+    return launch_tiles_rank<T, TR, 128>(P, d, st);
 }
 
 template <typename T>
@@ -127,7 +162,9 @@ int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t 
     FPEMU_TRY(error_sink(&P.sink));
     return with_type(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows<T>(P, transposed != 0, static_cast<cudaStream_t>(stream));
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (P.plan) return transposed ? launch_tiles<T, true>(P, d, st) : launch_tiles<T, false>(P, d, st);
+        return launch_rows<T>(P, transposed != 0, st);
     });
 }
 
