@@ -86,13 +86,41 @@ int launch_tiles(const AdapterParams& P, const DevInfo& d, cudaStream_t st) {
     return launch_tiles_rank<T, TR, 128>(P, d, st);
 }
 
-template <typename T>
-int launch_grad(const AdapterGradParams& P, cudaStream_t st) {
-    if (P.cols == 0) return FPEMU_OK;
-    const dim3 grid((unsigned)((P.cols + 127) / 128), (unsigned)P.adapters, (unsigned)((P.r + kGradJ - 1) / kGradJ));
-    adapter_grad_kernel<T><<<grid, 128, 0, st>>>(P);
-    FPEMU_CUDA(cudaGetLastError());
+template <typename T, int RP>
+int launch_grad_rank(AdapterGradParams& P, const DevInfo& d, cudaStream_t st) {
+    using Tile = AdapterGradTile<T, RP>;
+    auto kern = adapter_grad_kernel<T, RP>;
+    FPEMU_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem));
+    int64_t blocks[2];
+    for (int i = 0; i < 2; ++i) blocks[i] = P.side[i].grad ? (P.side[i].cols + Tile::COLS - 1) / Tile::COLS : 0;
+    if (blocks[0] + blocks[1] == 0) return FPEMU_OK;
+    int cluster = 1;
+    while (cluster < 8 && (blocks[0] + blocks[1]) * P.adapters * cluster < d.sms * 4 &&
+           P.rows / P.adapters > cluster * 4 * Tile::KT)
+        cluster *= 2;
+    P.first_blocks = blocks[0] * cluster;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((blocks[0] + blocks[1]) * cluster), (unsigned)P.adapters);
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = Tile::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    FPEMU_CUDA(cudaLaunchKernelEx(&cfg, kern, P));
     return FPEMU_OK;
+}
+
+template <typename T>
+int launch_grad(AdapterGradParams& P, const DevInfo& d, cudaStream_t st) {
+    if (P.r <= 16) return launch_grad_rank<T, 16>(P, d, st);
+    if (P.r <= 32) return launch_grad_rank<T, 32>(P, d, st);
+    if (P.r <= 64) return launch_grad_rank<T, 64>(P, d, st);
+    return launch_grad_rank<T, 128>(P, d, st);
 }
 
 template <typename F>
@@ -158,7 +186,8 @@ int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t 
     P.w2 = w2, P.w2_adapter = w2_adapter, P.w2_row = w2_row;
     P.base = base, P.base_row = base_row, P.y = y, P.y_row = y_row;
     P.scales = scales, P.scale = scale;
-    P.index = index, P.index_wide = index_bytes == 8, P.plan = static_cast<const int32_t*>(plan), P.u = u;
+    P.index = index, P.index_wide = index_bytes == 8, P.plan = static_cast<const int32_t*>(plan);
+    P.u = u, P.u_row = middle_row((int)rank);
     FPEMU_TRY(error_sink(&P.sink));
     return with_type(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
@@ -175,21 +204,18 @@ int fpemu_adapter_grads(int dtype, int64_t rows, int64_t k, int64_t n, int64_t r
     FPEMU_TRY(check_sizes("adapter_grads", dtype, rows, k, n, rank, adapters));
     if (plan == nullptr || (dA && (!x || !v) && rows * k > 0) || (dB && (!dy || !u) && rows * n > 0))
         return fail(FPEMU_ERR_INVALID, "adapter_grads: null pointer");
+    if ((reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(v)) % 16 != 0)
+        return fail(FPEMU_ERR_INVALID, "adapter_grads: u and v start on a 16-byte boundary");
     if (x_row < 0 || dy_row < 0) return fail(FPEMU_ERR_INVALID, "adapter_grads: negative stride");
     FPEMU_TRY(device_info(&d));
     return with_type(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         AdapterGradParams P = {};
-        P.rows = rows, P.r = (int)rank, P.adapters = (int)adapters, P.plan = static_cast<const int32_t*>(plan);
-        if (dA) {
-            P.cols = k, P.p = v, P.q = x, P.q_row = x_row, P.grad = dA, P.grad_j = k, P.grad_c = 1;
-            FPEMU_TRY(launch_grad<T>(P, static_cast<cudaStream_t>(stream)));
-        }
-        if (dB) {
-            P.cols = n, P.p = u, P.q = dy, P.q_row = dy_row, P.grad = dB, P.grad_j = 1, P.grad_c = rank;
-            FPEMU_TRY(launch_grad<T>(P, static_cast<cudaStream_t>(stream)));
-        }
-        return (int)FPEMU_OK;
+        P.rows = rows, P.r = (int)rank, P.p_row = middle_row((int)rank), P.adapters = (int)adapters;
+        P.plan = static_cast<const int32_t*>(plan);
+        P.side[0] = AdapterGradSide{v, x, x_row, k, dA, 0};
+        P.side[1] = AdapterGradSide{u, dy, dy_row, n, dB, 1};
+        return launch_grad<T>(P, d, static_cast<cudaStream_t>(stream));
     });
 }
 

@@ -76,6 +76,9 @@ __host__ __device__ __forceinline__ int64_t plan_words(int64_t rows, int64_t ada
     return plan_perm_word(rows, adapters) + rows;
 }
 
+// Elements of a row of the middle (u and v): 16-byte units of 4 floats or 2 doubles.
+__host__ __device__ __forceinline__ int middle_row(int r) { return (r + 3) / 4 * 4; }
+
 __device__ __forceinline__ int row_class(const void* index, int wide, int64_t t, int adapters) {
     const int64_t id = wide ? static_cast<const int64_t*>(index)[t] : (int64_t) static_cast<const int32_t*>(index)[t];
     return id == -1 ? adapters : (id < 0 || id >= adapters) ? adapters + 1 : (int)id;
@@ -150,7 +153,8 @@ struct AdapterParams {
     const void* index;
     int index_wide;
     const int32_t* plan;  // null: the kernel groups the (few) rows itself
-    void* u;              // [rows, r] of the sums' type, or null
+    void* u;              // [rows, u_row] of the sums' type, or null
+    int u_row;
     ErrorSink sink;
 };
 
@@ -293,7 +297,7 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_rows_kernel(AdapterPa
             Acc v = 0;
             for (int b = 0; b < kAdapterCluster; ++b) v += *cluster.map_shared_rank(&part[g][j], b);
             us[g][j] = v * s;
-            if (P.u && cr == 0) static_cast<Acc*>(P.u)[(int64_t)list[first + g] * P.r + j] = v * s;
+            if (P.u && cr == 0) static_cast<Acc*>(P.u)[(int64_t)list[first + g] * P.u_row + j] = v * s;
         }
         cluster.sync();  // every block has read the partial sums
         for (int64_t c = n0 + tid; c < n1; c += kAdapterThreads) {
@@ -315,57 +319,6 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_rows_kernel(AdapterPa
         }
         __syncthreads();  // `us` is rewritten by the next rows
     }
-}
-
-// grad[i][j][c] = sum over the rows t of adapter i of p[t][j] * q[t][c]: dA from
-// (v, x) and dB from (u, dy).  A thread holds 16 values of j for one column.
-struct AdapterGradParams {
-    int64_t rows, cols;
-    int r, adapters;
-    const void* p;   // [rows, r] of the sums' type
-    const void* q;   // [rows, cols]
-    int64_t q_row;
-    void* grad;      // element (i, j, c) at i * r * cols + j * grad_j + c * grad_c
-    int64_t grad_j, grad_c;
-    const int32_t* plan;
-};
-
-constexpr int kGradJ = 16;
-constexpr int kGradChunk = 128;
-
-template <typename T>
-__global__ void __launch_bounds__(128) adapter_grad_kernel(AdapterGradParams P) {
-    using Acc = typename AccOf<T>::type;
-    __shared__ int list[kGradChunk];
-    const int cls = blockIdx.y, j0 = blockIdx.z * kGradJ;
-    const int64_t c = (int64_t)blockIdx.x * 128 + threadIdx.x;
-    const int start = P.plan[cls], end = P.plan[cls + 1];
-    const int32_t* perm = P.plan + plan_perm_word(P.rows, P.adapters);
-    const Acc* p = static_cast<const Acc*>(P.p);
-    const T* q = static_cast<const T*>(P.q);
-    Acc sum[kGradJ] = {};
-    for (int t = start; t < end; t += kGradChunk) {
-        const int m = end - t < kGradChunk ? end - t : kGradChunk;
-        __syncthreads();
-        if ((int)threadIdx.x < m) list[threadIdx.x] = perm[t + threadIdx.x];
-        __syncthreads();
-        if (c >= P.cols) continue;
-        Acc acc[kGradJ] = {};
-        for (int i = 0; i < m; ++i) {
-            const int64_t row = list[i];
-            const Acc v = widen(q[row * P.q_row + c]);
-#pragma unroll
-            for (int j = 0; j < kGradJ; ++j)
-                if (j0 + j < P.r) acc[j] += v * p[row * P.r + j0 + j];
-        }
-#pragma unroll
-        for (int j = 0; j < kGradJ; ++j) sum[j] += acc[j];
-    }
-    if (c < P.cols)
-#pragma unroll
-        for (int j = 0; j < kGradJ; ++j)
-            if (j0 + j < P.r)
-                static_cast<T*>(P.grad)[(int64_t)cls * P.r * P.cols + (j0 + j) * P.grad_j + c * P.grad_c] = narrow<T>(sum[j]);
 }
 
 }  // namespace fpemu

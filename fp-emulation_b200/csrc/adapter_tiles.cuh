@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kTileThreads) adapter_tile_kernel(AdapterParam
         };
         auto keep = [&](int row, int j, Acc v) {
             if (P.u && cr == 0 && j < P.r && warp * 16 + row < count)
-                static_cast<Acc*>(P.u)[(int64_t)list[warp * 16 + row] * P.r + j] = v;
+                static_cast<Acc*>(P.u)[(int64_t)list[warp * 16 + row] * P.u_row + j] = v;
         };
         if (busy) {
             if constexpr (E == 2) {
@@ -500,6 +500,248 @@ __global__ void __launch_bounds__(kTileThreads) adapter_tile_kernel(AdapterParam
     }
     if (total == nk) exchange();
     cluster.sync();  // no block leaves while another may read its partial sums
+}
+
+// Gradients of the factors: grad[i][j][c] = sum over the rows t of adapter i of
+// p[t][j] * q[t][c], dA from (v, x) and dB from (u, dy), in one launch.
+//
+// A block holds a stretch of columns and all of the rank in registers and walks
+// the adapter's rows, so q is read once and p (rank values a row) by every block
+// of columns.  Where that gives too few blocks, a cluster splits the rows into
+// consecutive parts, whose sums meet in the blocks' order.
+struct AdapterGradSide {
+    const void* p;  // [rows, p_row] of the sums' type
+    const void* q;  // [rows, cols]
+    int64_t q_row, cols;
+    void* grad;     // [adapters, r, cols] or, by_column, [adapters, cols, r]
+    int by_column;
+};
+struct AdapterGradParams {
+    AdapterGradSide side[2];
+    int64_t first_blocks;  // blocks of side 0; the others are side 1's
+    int64_t rows;
+    int r, p_row, adapters;
+    const int32_t* plan;
+};
+
+template <typename T, int RP>
+struct AdapterGradTile {
+    using Acc = typename AccOf<T>::type;
+    static constexpr int E = sizeof(T), V = 16 / E;
+    static constexpr int MT = E == 2 && RP < 128 ? 2 : 1;     // 16-column tiles a warp holds
+    static constexpr int COLS = 64 * MT;
+    static constexpr int KT = E == 8 ? 16 : 32;               // rows of a chunk
+    static constexpr int kPitchQ = COLS * E + (E == 2 ? 16 : 32);
+    static constexpr int kPitchP = (RP + (E == 4 ? 8 : 4)) * (int)sizeof(Acc);
+    static constexpr int kStage = KT * (kPitchQ + kPitchP);
+    static constexpr int kStages = RP <= 64 ? 4 : 3;
+    static constexpr int kPitchD = RP + 1;                    // the block's sums, after the rows
+    static constexpr int kJoin = COLS * kPitchD * (int)sizeof(Acc);
+    static constexpr int kSmem = kStages * kStage > kJoin ? kStages * kStage : kJoin;
+    static constexpr int kFlush = E == 2 ? 8 : 1;             // chunks that the tensor cores sum by themselves
+};
+
+template <typename T, int RP>
+__global__ void __launch_bounds__(kTileThreads) adapter_grad_kernel(const __grid_constant__ AdapterGradParams P) {
+    using Tile = AdapterGradTile<T, RP>;
+    using Acc = typename Tile::Acc;
+    constexpr int E = Tile::E, V = Tile::V, KT = Tile::KT, S = Tile::kStages, MT = Tile::MT, COLS = Tile::COLS;
+    extern __shared__ __align__(16) uint8_t smem[];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+    const int cr = (int)cluster.block_rank(), cs = (int)cluster.num_blocks();
+    const bool second = blockIdx.x >= P.first_blocks;
+    const AdapterGradSide& side = P.side[second];
+    const int64_t c0 = (blockIdx.x - (second ? P.first_blocks : 0)) / cs * COLS;
+    const int cls = blockIdx.y;
+    const int start = P.plan[cls], rows = P.plan[cls + 1] - start;
+    const int32_t* perm = P.plan + plan_perm_word(P.rows, P.adapters) + start;
+    const int share = (rows + KT * cs - 1) / (KT * cs) * KT;
+    const int t0 = cr * share < rows ? cr * share : rows, t1 = t0 + share < rows ? t0 + share : rows;
+    const int chunks = (t1 - t0 + KT - 1) / KT;
+    const T* qs = static_cast<const T*>(side.q);
+    const Acc* ps = static_cast<const Acc*>(side.p);
+    const bool vec = ((reinterpret_cast<uintptr_t>(qs) | (uintptr_t)(side.q_row * E)) & 15) == 0;
+
+    // Row ids of a thread's copies, one chunk ahead of the copies themselves.
+    constexpr int QU = COLS / V, QI = KT * QU / kTileThreads;          // 16-byte units of a q row; copies a thread
+    constexpr int PV = 16 / (int)sizeof(Acc), PU = RP / PV, PI = KT * PU / kTileThreads;
+    int q_id[QI], p_id[PI];
+    auto ids = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < QI; ++i) {
+            const int t = t0 + c * KT + (tid + i * kTileThreads) / QU;
+            q_id[i] = t < t1 ? perm[t] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < PI; ++i) {
+            const int t = t0 + c * KT + (tid + i * kTileThreads) / PU;
+            p_id[i] = t < t1 ? perm[t] : -1;
+        }
+    };
+    auto fetch = [&](int c) {
+        uint8_t* st = smem + c % S * Tile::kStage;
+#pragma unroll
+        for (int i = 0; i < QI; ++i) {
+            const int u = tid + i * kTileThreads;
+            const int64_t col = c0 + u % QU * V, left = side.cols - col;
+            const int avail = q_id[i] < 0 || left < 0 ? 0 : left > V ? V : (int)left;
+            fetch16(st + u / QU * Tile::kPitchQ + u % QU * 16, qs + q_id[i] * side.q_row + col, qs, avail, vec);
+        }
+#pragma unroll
+        for (int i = 0; i < PI; ++i) {
+            const int u = tid + i * kTileThreads, j = u % PU * PV;
+            const int avail = p_id[i] < 0 || j >= P.p_row ? 0 : PV;  // p_row is a multiple of PV
+            fetch16(st + KT * Tile::kPitchQ + u / PU * Tile::kPitchP + u % PU * 16,
+                    ps + (int64_t)p_id[i] * P.p_row + j, ps, avail, true);
+        }
+    };
+
+    Acc acc[MT][RP / 8][4] = {}, sum[E == 8 ? 1 : MT][E == 8 ? 1 : RP / 8][4] = {};
+    auto flush = [&]() {
+        if constexpr (E != 8) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int t = 0; t < RP / 8; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[m][t][e] += sum[m][t][e], sum[m][t][e] = 0;
+        }
+    };
+    auto compute = [&](const uint8_t* st) {
+        const uint8_t* pt = st + KT * Tile::kPitchQ;
+        auto p_at = [&](int row, int j) {
+            return *reinterpret_cast<const Acc*>(pt + row * Tile::kPitchP + j * (int)sizeof(Acc));
+        };
+        if constexpr (E == 2) {
+            const uint32_t qa = shared_address(st) + ((lane & 7) + (lane >> 4) * 8) * Tile::kPitchQ +
+                                (warp * 16 * MT + (lane >> 3 & 1) * 8) * 2;
+#pragma unroll
+            for (int ks = 0; ks < KT / 16; ++ks) {
+                uint32_t a[MT][4];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) ldsm4t(a[m], qa + ks * 16 * Tile::kPitchQ + m * 32);
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+                    for (int t = 0; t < RP / 8; ++t) {
+                        uint32_t hi[2], lo[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int row = ks * 16 + 2 * q + e * 8, j = t * 8 + g;
+                            split16<T>(p_at(row, j), p_at(row + 1, j), hi[e], lo[e]);
+                        }
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            mma16<T>(sum[m][t], a[m], lo[0], lo[1]);
+                            mma16<T>(sum[m][t], a[m], hi[0], hi[1]);
+                        }
+                    }
+                } else {
+                    // A half is a tf32 value as it is; the middle, whose range is a float's, is split
+                    // in two.  The order of rows within the sum is free: rows 2q and 2q + 1 stand
+                    // where the instruction has q and q + 4.
+                    uint32_t w[MT][2][4];
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[m][e]));
+                            w[m][e >> 1][e & 1] = __float_as_uint(f.x);
+                            w[m][e >> 1][(e & 1) + 2] = __float_as_uint(f.y);
+                        }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int t = 0; t < RP / 8; ++t) {
+                            const int row = ks * 16 + h * 8 + 2 * q, j = t * 8 + g;
+                            const Tf32Pair b0 = tf32_split(p_at(row, j)), b1 = tf32_split(p_at(row + 1, j));
+#pragma unroll
+                            for (int m = 0; m < MT; ++m) {
+                                mma_tf32(sum[m][t], w[m][h], b0.lo, b1.lo);
+                                mma_tf32(sum[m][t], w[m][h], b0.hi, b1.hi);
+                            }
+                        }
+                }
+            }
+        } else if constexpr (E == 4) {
+#pragma unroll
+            for (int ks = 0; ks < KT / 8; ++ks) {
+                uint32_t ah[4], al[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const Tf32Pair p = tf32_split(*reinterpret_cast<const float*>(
+                        st + (ks * 8 + q + (e >> 1) * 4) * Tile::kPitchQ + (warp * 16 + g + (e & 1) * 8) * 4));
+                    ah[e] = p.hi, al[e] = p.lo;
+                }
+#pragma unroll
+                for (int t = 0; t < RP / 8; ++t) {
+                    const Tf32Pair b0 = tf32_split(p_at(ks * 8 + q, t * 8 + g));
+                    const Tf32Pair b1 = tf32_split(p_at(ks * 8 + q + 4, t * 8 + g));
+                    mma_tf32(sum[0][t], ah, b0.lo, b1.lo);
+                    mma_tf32(sum[0][t], al, b0.hi, b1.hi);
+                    mma_tf32(sum[0][t], ah, b0.hi, b1.hi);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < KT / 4; ++ks) {
+                const uint8_t* qa = st + (ks * 4 + q) * Tile::kPitchQ + (warp * 16 + g) * 8;
+                const double a0 = *reinterpret_cast<const double*>(qa), a1 = *reinterpret_cast<const double*>(qa + 64);
+#pragma unroll
+                for (int t = 0; t < RP / 8; ++t) mma_f64(acc[0][t], a0, a1, p_at(ks * 4 + q, t * 8 + g));
+            }
+        }
+    };
+
+    ids(0);
+#pragma unroll
+    for (int c = 0; c < S - 1; ++c) {
+        if (c < chunks) {
+            fetch(c);
+            ids(c + 1);
+        }
+        copy_commit();
+    }
+    for (int c = 0; c < chunks; ++c) {
+        copy_wait<S - 2>();
+        __syncthreads();
+        if (c + S - 1 < chunks) {
+            fetch(c + S - 1);
+            ids(c + S);
+        }
+        copy_commit();
+        compute(smem + c % S * Tile::kStage);
+        if (c % Tile::kFlush == Tile::kFlush - 1) flush();
+    }
+    flush();
+    copy_wait<0>();
+    __syncthreads();
+    Acc* mine = reinterpret_cast<Acc*>(smem);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < RP / 8; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                mine[((warp * MT + m) * 16 + g + (e >> 1) * 8) * Tile::kPitchD + t * 8 + 2 * q + (e & 1)] = acc[m][t][e];
+    cluster.sync();
+    const Acc* parts[8];
+#pragma unroll
+    for (int b = 0; b < 8; ++b) parts[b] = b < cs ? cluster.map_shared_rank(mine, b) : nullptr;
+    const int cols = side.cols - c0 < COLS ? (int)(side.cols - c0) : COLS, own = COLS / cs;
+    const int first = cr * own, last = first + own < cols ? first + own : cols;
+    T* grad = static_cast<T*>(side.grad) + (int64_t)cls * P.r * side.cols;
+    const int many = last > first ? (last - first) * P.r : 0;
+    for (int i = tid; i < many; i += kTileThreads) {
+        const int c = first + (side.by_column ? i / P.r : i % (last - first));
+        const int j = side.by_column ? i % P.r : i / (last - first);
+        Acc v = 0;
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+            if (b < cs) v += parts[b][c * Tile::kPitchD + j];
+        grad[side.by_column ? (c0 + c) * P.r + j : j * side.cols + c0 + c] = narrow<T>(v);
+    }
+    cluster.sync();
 }
 
 }  // namespace fpemu

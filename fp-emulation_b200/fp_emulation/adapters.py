@@ -110,7 +110,7 @@ class _AdapterMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, A, B, base, rows, scale):
         y = torch.empty((x.shape[0], B.shape[1]), dtype=x.dtype, device=x.device)
-        u = torch.empty((x.shape[0], A.shape[1]), dtype=_sum_dtype(x.dtype), device=x.device)
+        u = torch.empty((x.shape[0], (A.shape[1] + 3) // 4 * 4), dtype=_sum_dtype(x.dtype), device=x.device)
         _launch(x, A, B, 0, base, y, scale, rows.index, _plan_of(rows), rows.adapters, A.shape[1], A.shape[2],
                 B.shape[1], u)
         ctx.save_for_backward(x, A, B, u)

@@ -224,8 +224,9 @@ int fpemu_adapter_plan(const void *index, int index_bytes, int64_t rows, int64_t
  *   transposed 1: w1 is [adapters][k][rank], w2 is [adapters][rank][n]
  *                 (its gradient by x: x = dy, w1 = B, w2 = A).
  * scales: one double per adapter, or NULL for `scale` everywhere.
- * u (or NULL): rows x rank values s_i W1_i x[t] -- double for FPEMU_DT_F64, else
- * float; rows without an adapter are not written.
+ * u (or NULL): rows of `rank` values s_i W1_i x[t], each row rank rounded up to a
+ * multiple of 4 apart -- double for FPEMU_DT_F64, else float; rows without an
+ * adapter are not written.
  * y may be base itself; otherwise it overlaps no input.
  * plan NULL: rows <= FPEMU_ADAPTER_FEW_ROWS, grouped by the kernel from index. */
 int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank,
