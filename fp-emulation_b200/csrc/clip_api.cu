@@ -16,7 +16,15 @@ constexpr int kSmallTable = 32, kLargeTable = 512;
 
 int clip_grid(const DevInfo& d, int64_t chunks) { return (int)std::min<int64_t>(chunks, (int64_t)d.sms * 4); }
 
-int64_t chunks_of(int64_t numel) { return (numel + kClipChunk - 1) / kClipChunk; }
+// Elements of a chunk: enough chunks for every block where there are elements enough.
+int chunk_size(const DevInfo& d, int64_t count, const int64_t* numel) {
+    int64_t all = 0;
+    for (int64_t i = 0; i < count; ++i) all += numel[i];
+    const int64_t even = all / ((int64_t)d.sms * 4);
+    int size = kClipChunkMin;
+    while (size < kClipChunkMax && size < even) size *= 2;
+    return size;
+}
 
 // The scaling kernel's blocks read and write in any order, so no output may meet
 // another output, or an input that is not its own.
@@ -69,8 +77,9 @@ int clip_check(int64_t count, const void* const* src, void* const* dst, const in
 // Fills the table with the next tensors that hold anything; returns where the list goes on.
 template <int N>
 int64_t fill(ClipTable<N>& t, int64_t from, int64_t count, const void* const* src, void* const* dst,
-             const int64_t* numel, const int32_t* dtype) {
+             const int64_t* numel, const int32_t* dtype, int size) {
     t.count = 0;
+    t.chunk_size = size;
     int64_t chunk = 0;
     for (; from < count && t.count < N; ++from) {
         if (numel[from] == 0) continue;
@@ -80,7 +89,7 @@ int64_t fill(ClipTable<N>& t, int64_t from, int64_t count, const void* const* sr
         t.numel[i] = numel[from];
         t.dtype[i] = (uint8_t)dtype[from];
         t.chunk[i] = chunk;
-        chunk += chunks_of(numel[from]);
+        chunk += (numel[from] + size - 1) / size;
     }
     t.chunk[t.count] = chunk;
     return from;
@@ -90,9 +99,10 @@ template <int N, int P>
 int clip_run(const DevInfo& d, int64_t count, const void* const* src, void* const* dst, const int64_t* numel,
              const int32_t* dtype, double max_norm, void* norm, int norm_f64, double* partial, cudaStream_t st) {
     ClipTable<N> t;
+    const int size = chunk_size(d, count, numel);
     int partials = 0;
     for (int64_t from = 0; from < count;) {
-        from = fill(t, from, count, src, dst, numel, dtype);
+        from = fill(t, from, count, src, dst, numel, dtype, size);
         const int grid = clip_grid(d, t.chunk[t.count]);
         if (grid == 0) continue;
         norm_partial_kernel<N, P><<<grid, kClipThreads, 0, st>>>(t, partial + (int64_t)partials * kClipSums);
@@ -105,7 +115,7 @@ int clip_run(const DevInfo& d, int64_t count, const void* const* src, void* cons
         return FPEMU_OK;
     }
     for (int64_t from = 0; from < count;) {
-        from = fill(t, from, count, src, dst, numel, dtype);
+        from = fill(t, from, count, src, dst, numel, dtype, size);
         const int grid = clip_grid(d, t.chunk[t.count]);
         if (grid == 0) continue;
         clip_scale_kernel<N, P><<<grid, kClipThreads, 0, st>>>(t, partial, partials, max_norm, norm, norm_f64);

@@ -15,12 +15,15 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "fpemu_internal.h"
 
 namespace fpemu {
 
 constexpr int kClipThreads = 256;
-constexpr int64_t kClipChunk = 16384;  // elements of one tensor that a block takes at a time
+constexpr int kClipChunkMin = 1024;    // elements of one tensor that a block takes at a time,
+constexpr int kClipChunkMax = 16384;   // by how many there are for every block
 constexpr int kClipSums = 3;           // doubles a block leaves (see NormSum)
 
 // Up to N tensors, passed in the launch's parameters: no copy of a pointer table.
@@ -32,6 +35,7 @@ struct ClipTable {
     int64_t chunk[N + 1];  // first chunk of each tensor, then their number
     uint8_t dtype[N];
     int count;
+    int chunk_size;
 };
 
 // p = 2: squares of doubles leave the range long before their norm does, so
@@ -120,65 +124,86 @@ __device__ NormSum block_join(NormSum v) {
 
 // Elements of type T before the first 16-byte boundary.
 template <typename T>
-__device__ __forceinline__ int64_t clip_head(const void* p, int64_t n) {
-    const int64_t h = ((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T);
+__device__ __forceinline__ int clip_head(const void* p, int n) {
+    const int h = ((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T);
     return h < n ? h : n;
 }
 
 template <typename T, int P>
-__device__ void chunk_norm(const T* p, int64_t n, NormSum& sum) {
-    constexpr int V = 16 / sizeof(T);
-    const int64_t head = clip_head<T>(p, n), vecs = (n - head) / V;
+__device__ __forceinline__ void add_vector(const uint4& raw, NormSum (&s)[2]) {
+    const T* v = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int e = 0; e < (int)(16 / sizeof(T)); ++e) s[e & 1].template add<P>(clip_widen(v[e]));
+}
+
+template <typename T, int P>
+__device__ void chunk_norm(const T* p, int n, NormSum& sum) {
+    constexpr int V = 16 / sizeof(T), U = 4;
+    const int head = clip_head<T>(p, n), vecs = (n - head) / V;
     NormSum s[2];
     const uint4* q = reinterpret_cast<const uint4*>(p + head);
-#pragma unroll 4
-    for (int64_t i = threadIdx.x; i < vecs; i += kClipThreads) {
-        alignas(16) T v[V];
-        *reinterpret_cast<uint4*>(v) = q[i];
+    int i = threadIdx.x;
+    for (; i + (U - 1) * kClipThreads < vecs; i += U * kClipThreads) {
+        uint4 raw[U];
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[e & 1].template add<P>(clip_widen(v[e]));
+        for (int u = 0; u < U; ++u) raw[u] = q[i + u * kClipThreads];
+#pragma unroll
+        for (int u = 0; u < U; ++u) add_vector<T, P>(raw[u], s);
     }
-    for (int64_t i = threadIdx.x; i < head; i += kClipThreads) s[0].template add<P>(clip_widen(p[i]));
-    for (int64_t i = head + vecs * V + threadIdx.x; i < n; i += kClipThreads) s[0].template add<P>(clip_widen(p[i]));
+    for (; i < vecs; i += kClipThreads) add_vector<T, P>(q[i], s);
+    if (threadIdx.x < head) s[0].template add<P>(clip_widen(p[threadIdx.x]));
+    const int t = head + vecs * V + threadIdx.x;
+    if (t < n) s[0].template add<P>(clip_widen(p[t]));
     sum.join<P>(s[0].mid, s[0].big, s[0].small);
     sum.join<P>(s[1].mid, s[1].big, s[1].small);
 }
 
 template <typename T>
-__device__ void chunk_scale(const T* p, T* o, int64_t n, const ClipFactor& f) {
-    constexpr int V = 16 / sizeof(T);
+__device__ void chunk_scale(const T* p, T* o, int n, const ClipFactor& f) {
+    constexpr int V = 16 / sizeof(T), U = 4;
     const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(o)) & 15) == 0;
-    const int64_t head = same ? clip_head<T>(p, n) : 0, vecs = same ? (n - head) / V : 0;
+    const int head = same ? clip_head<T>(p, n) : 0, vecs = same ? (n - head) / V : 0;
     const uint4* q = reinterpret_cast<const uint4*>(p + head);
     uint4* w = reinterpret_cast<uint4*>(o + head);
-#pragma unroll 4
-    for (int64_t i = threadIdx.x; i < vecs; i += kClipThreads) {
-        alignas(16) T v[V];
-        *reinterpret_cast<uint4*>(v) = q[i];
+    auto scaled = [&](uint4 raw) {
+        T* v = reinterpret_cast<T*>(&raw);
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = clip_scale(v[e], f);
-        w[i] = *reinterpret_cast<uint4*>(v);
+        return raw;
+    };
+    int i = threadIdx.x;
+    for (; i + (U - 1) * kClipThreads < vecs; i += U * kClipThreads) {
+        uint4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = __ldcs(q + i + u * kClipThreads);
+#pragma unroll
+        for (int u = 0; u < U; ++u) __stcs(w + i + u * kClipThreads, scaled(raw[u]));
     }
-    for (int64_t i = threadIdx.x; i < head; i += kClipThreads) o[i] = clip_scale(p[i], f);
-    for (int64_t i = head + vecs * V + threadIdx.x; i < n; i += kClipThreads) o[i] = clip_scale(p[i], f);
+    for (; i < vecs; i += kClipThreads) __stcs(w + i, scaled(__ldcs(q + i)));
+    if (threadIdx.x < head) o[threadIdx.x] = clip_scale(p[threadIdx.x], f);
+    for (int t = head + vecs * V + threadIdx.x; t < n; t += kClipThreads) o[t] = clip_scale(p[t], f);
 }
 
-// Calls f(tensor, first element, elements) for this block's share of the chunks.
-template <int N, typename F>
+// Calls f(tensor, first element, elements) for this block's share of the chunks,
+// first to last or, BACK, last to first: what the norm's pass read last is still in
+// the L2 when the scaling begins with it.
+template <bool BACK, int N, typename F>
 __device__ __forceinline__ void for_chunks(const ClipTable<N>& t, F&& f) {
     const int64_t chunks = t.chunk[t.count];
-    int64_t c = chunks * blockIdx.x / gridDim.x;
-    const int64_t end = chunks * (blockIdx.x + 1) / gridDim.x;
-    int lo = 0, hi = t.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (t.chunk[mid] <= c) lo = mid;
+    const int64_t begin = chunks * blockIdx.x / gridDim.x, end = chunks * (blockIdx.x + 1) / gridDim.x;
+    const int64_t from = BACK ? end - 1 : begin;
+    int i = 0, hi = t.count - 1;
+    while (i < hi) {
+        const int mid = (i + hi + 1) / 2;
+        if (t.chunk[mid] <= from) i = mid;
         else hi = mid - 1;
     }
-    for (; c < end; ++c) {
-        while (c >= t.chunk[lo + 1]) ++lo;
-        const int64_t at = (c - t.chunk[lo]) * kClipChunk, left = t.numel[lo] - at;
-        f(lo, at, left < kClipChunk ? left : kClipChunk);
+    for (int64_t n = 0; n < end - begin; ++n) {
+        const int64_t c = BACK ? end - 1 - n : begin + n;
+        if (BACK) while (c < t.chunk[i]) --i;
+        else while (c >= t.chunk[i + 1]) ++i;
+        const int64_t at = (c - t.chunk[i]) * t.chunk_size, left = t.numel[i] - at;
+        f(i, at, (int)(left < t.chunk_size ? left : t.chunk_size));
     }
 }
 
@@ -186,12 +211,15 @@ template <int N, int P>
 __global__ void __launch_bounds__(kClipThreads) norm_partial_kernel(const __grid_constant__ ClipTable<N> t,
                                                                     double* partial) {
     NormSum sum;
-    for_chunks(t, [&](int i, int64_t at, int64_t n) {
+    for_chunks<false>(t, [&](int i, int64_t at, int n) {
+        const void* p = t.src[i];
         switch (t.dtype[i]) {
-            case FPEMU_DT_F64: chunk_norm<double, P>(static_cast<const double*>(t.src[i]) + at, n, sum); break;
-            case FPEMU_DT_F32: chunk_norm<float, P>(static_cast<const float*>(t.src[i]) + at, n, sum); break;
-            case FPEMU_DT_F16: chunk_norm<__half, P>(static_cast<const __half*>(t.src[i]) + at, n, sum); break;
-            default: chunk_norm<__nv_bfloat16, P>(static_cast<const __nv_bfloat16*>(t.src[i]) + at, n, sum);
+            case FPEMU_DT_F64:
+                chunk_norm<double, P>(static_cast<const double*>(p) + at, n, sum);
+                break;
+            case FPEMU_DT_F32: chunk_norm<float, P>(static_cast<const float*>(p) + at, n, sum); break;
+            case FPEMU_DT_F16: chunk_norm<__half, P>(static_cast<const __half*>(p) + at, n, sum); break;
+            default: chunk_norm<__nv_bfloat16, P>(static_cast<const __nv_bfloat16*>(p) + at, n, sum);
         }
     });
     sum = block_join<P>(sum);
@@ -233,7 +261,7 @@ __global__ void __launch_bounds__(kClipThreads) clip_scale_kernel(const __grid_c
     f.c = c > 1.0 ? 1.0 : c;  // NaN stays
     f.hi = (float)f.c;
     f.lo = (float)(f.c - (double)f.hi);
-    for_chunks(t, [&](int i, int64_t at, int64_t n) {
+    for_chunks<true>(t, [&](int i, int64_t at, int n) {
         if (t.src[i] == t.dst[i] && f.c == 1.0) return;
         switch (t.dtype[i]) {
             case FPEMU_DT_F64:

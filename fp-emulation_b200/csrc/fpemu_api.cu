@@ -993,4 +993,13 @@ int fpemu_poll_error(int* code, int* where, int* block, int* detail) {
     return FPEMU_OK;
 }
 
+int fpemu_error_word(const volatile int** word) {
+    if (word == nullptr) return fail(FPEMU_ERR_INVALID, "word is null");
+    volatile DeviceError* h = nullptr;
+    FPEMU_TRY(host_error_slot(&h, false));
+    if (h == nullptr) return fail(FPEMU_ERR_INVALID, "fpemu_error_word: fpemu_watch_errors was not called on this device");
+    *word = &h->code;
+    return FPEMU_OK;
+}
+
 }  // extern "C"

@@ -69,6 +69,7 @@ SIGNATURES = {
     "fpemu_device_error": (_int, [_IP, _IP, _IP, _IP, _int]),
     "fpemu_watch_errors": (_int, []),
     "fpemu_poll_error": (_int, [_IP, _IP, _IP, _IP]),
+    "fpemu_error_word": (_int, [_vp]),
 }
 
 _lock = threading.RLock()
@@ -153,3 +154,14 @@ def poll_error():
     vals = [ctypes.c_int(0) for _ in range(4)]
     check(lib.fpemu_poll_error(*[ctypes.byref(v) for v in vals]), "poll_error")
     return tuple(v.value for v in vals)
+
+
+error_words = {}  # device index -> the c_int that poll_error() reads `code` from
+
+
+def remember_error_word(device_index: int) -> None:
+    """Keep the address behind poll_error() for this device (which must be current
+    and watched), so that a call's look at it costs no library call."""
+    address = ctypes.c_void_p()
+    check(load().fpemu_error_word(ctypes.byref(address)), "fpemu_error_word")
+    error_words[device_index] = ctypes.c_int.from_address(address.value)

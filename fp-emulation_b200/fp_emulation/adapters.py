@@ -14,7 +14,6 @@ counterpart in the reference.
 from __future__ import annotations
 
 import contextlib
-import ctypes
 import math
 
 import torch
@@ -22,7 +21,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from fp_emulation import _lib
-from fp_emulation.ozaki import _after_call, _dtype_bits, _require_cuda, _stream
+from fp_emulation.ozaki import _after_call, _dtype_bits, _on, _require_cuda, _stream
 
 _DTYPE_CODE = {torch.float64: _lib.FPEMU_DT_F64, torch.float32: _lib.FPEMU_DT_F32,
                torch.float16: _lib.FPEMU_DT_F16, torch.bfloat16: _lib.FPEMU_DT_BF16}
@@ -82,19 +81,21 @@ def _row_stride(t):
 
 
 def _launch(x, w1, w2, transposed, base, y, scale, index, plan, adapters, rank, k, n, u):
-    """One fpemu_adapter_matmul on the current stream of x's device."""
+    """One fpemu_adapter_matmul on the current stream of x's device (2-D x, base and y)."""
     dev = x.device
-    scales = scale if isinstance(scale, torch.Tensor) else None
-    with torch.cuda.device(dev):
+    d = dev.index
+    with _on(d):
         st = _lib.load().fpemu_adapter_matmul(
             _DTYPE_CODE[x.dtype], x.shape[0], k, n, rank, adapters, x.data_ptr(), _row_stride(x),
             w1.data_ptr(), w1.stride(0), w1.stride(1), w2.data_ptr(), w2.stride(0), w2.stride(1), transposed,
             None if base is None else base.data_ptr(), 0 if base is None else base.stride(0),
             None if y is None else y.data_ptr(), n if y is None else _row_stride(y),
-            None if scales is None else scales.data_ptr(), 0.0 if scales is not None else scale,
-            None if index is None else index.data_ptr(), 0 if index is None else index.element_size(),
-            None if plan is None else plan.data_ptr(), None if u is None else u.data_ptr(), _stream(dev))
-    _lib.check(st, "adapter_matmul")
+            None if scale.__class__ is float else scale.data_ptr(), scale if scale.__class__ is float else 0.0,
+            None if plan is not None else index.data_ptr(), 0 if plan is not None else index.element_size(),
+            None if plan is None else plan.data_ptr(), None if u is None else u.data_ptr(),
+            torch.cuda.current_stream(d).cuda_stream)
+    if st:
+        _lib.check(st, "adapter_matmul")
     _after_call("adapter_matmul", dev)
 
 
@@ -136,7 +137,7 @@ class _AdapterMatmul(torch.autograd.Function):
             dA = torch.empty((n_ad, rank, k), dtype=A.dtype, device=A.device) if need_A else None
             dB = torch.empty((n_ad, n, rank), dtype=B.dtype, device=B.device) if need_B else None
             dev = x.device
-            with torch.cuda.device(dev):
+            with _on(dev.index):
                 st = _lib.load().fpemu_adapter_grads(
                     _DTYPE_CODE[x.dtype], x.shape[0], k, n, rank, n_ad, x.data_ptr(), _row_stride(x),
                     dyc.data_ptr(), _row_stride(dyc), u.data_ptr(), None if v is None else v.data_ptr(),
@@ -149,7 +150,7 @@ class _AdapterMatmul(torch.autograd.Function):
 
 def _plan_of(rows):
     """Few rows are grouped inside the kernel; more go by the plan."""
-    return None if rows.index.numel() <= _lib.FPEMU_ADAPTER_FEW_ROWS else rows.plan
+    return None if rows.index.shape[0] <= _lib.FPEMU_ADAPTER_FEW_ROWS else rows.plan
 
 
 def _span(t):
@@ -193,17 +194,22 @@ def adapter_matmul(x, A, B, rows, base=None, scale=1.0, out=None):
     Sums are held in float64 for float64 and in float32 otherwise, and the result
     is rounded once.  x, A, B and base have gradients (once; not twice
     differentiable); repeated calls give the same bits."""
-    _dtype_bits(x.dtype)
-    tensors = [x, A, B] + ([base] if base is not None else [])
-    dev = _require_cuda(*tensors)
-    if any(t.dtype != x.dtype for t in tensors):
-        raise TypeError(f"adapter_matmul: operands of one dtype, got {', '.join(str(t.dtype) for t in tensors)}")
-    if x.dim() < 1 or A.dim() != 3 or B.dim() != 3 or A.shape[0] != B.shape[0] or A.shape[1] != B.shape[2] \
-            or A.shape[2] != x.shape[-1]:
+    dtype = x.dtype
+    _dtype_bits(dtype)
+    d = x.get_device()
+    if d < 0 or A.get_device() != d or B.get_device() != d or (base is not None and base.get_device() != d) \
+            or d not in _lib._watched:
+        _require_cuda(x, A, B, *(() if base is None else (base,)))
+    if A.dtype is not dtype or B.dtype is not dtype or (base is not None and base.dtype is not dtype):
+        raise TypeError("adapter_matmul: operands of one dtype, got " +
+                        ", ".join(str(t.dtype) for t in (x, A, B, base) if t is not None))
+    shape_x, shape_A, shape_B = x.shape, A.shape, B.shape
+    if len(shape_x) < 1 or len(shape_A) != 3 or len(shape_B) != 3 or shape_A[0] != shape_B[0] \
+            or shape_A[1] != shape_B[2] or shape_A[2] != shape_x[-1]:
         raise RuntimeError(f"adapter_matmul: expected x [..., k], A [adapters, rank, k], B [adapters, n, rank], got "
-                           f"{tuple(x.shape)}, {tuple(A.shape)}, {tuple(B.shape)}")
-    adapters, rank, k = A.shape
-    n = B.shape[1]
+                           f"{tuple(shape_x)}, {tuple(shape_A)}, {tuple(shape_B)}")
+    adapters, rank, k = shape_A
+    n = shape_B[1]
     if not 1 <= rank <= _lib.FPEMU_ADAPTER_MAX_RANK:
         raise ValueError(f"adapter_matmul: rank {rank}; between 1 and {_lib.FPEMU_ADAPTER_MAX_RANK} is supported")
     if not 1 <= adapters <= _lib.FPEMU_ADAPTER_MAX_COUNT:
@@ -213,24 +219,29 @@ def adapter_matmul(x, A, B, rows, base=None, scale=1.0, out=None):
             raise RuntimeError("adapter_matmul: scale has no gradient")
         if scale.shape != (adapters,):
             raise RuntimeError(f"adapter_matmul: scale of shape {tuple(scale.shape)} for {adapters} adapters")
-        scale = scale.detach().to(device=dev, dtype=torch.float64).contiguous()
+        if scale.dtype is not torch.float64 or scale.get_device() != d or not scale.is_contiguous():
+            scale = scale.detach().to(device=x.device, dtype=torch.float64).contiguous()
     else:
         scale = float(scale)
-    lead = x.shape[:-1]
+    flat = len(shape_x) == 2
+    lead = shape_x[:-1]
+    count = shape_x[0] if flat else math.prod(lead)
     shape = lead + (n,)
-    count = math.prod(lead)
-    records = torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    records = torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad
+                                           or (base is not None and base.requires_grad))
     if isinstance(rows, PreparedRows):
         if rows.adapters != adapters:
             raise RuntimeError(f"adapter_matmul: rows prepared for {rows.adapters} adapters, not {adapters}")
-        if rows.index.numel() != count:
-            raise RuntimeError(f"adapter_matmul: {rows.index.numel()} prepared rows for {count} rows of x")
-        if rows.index.device != dev:
-            raise RuntimeError(f"operands on different devices: {dev} and {rows.index.device}")
+        index = rows.index
+        if index.shape[0] != count:
+            raise RuntimeError(f"adapter_matmul: {index.shape[0]} prepared rows for {count} rows of x")
+        if index.get_device() != d:
+            raise RuntimeError(f"operands on different devices: {x.device} and {index.device}")
     elif isinstance(rows, torch.Tensor):
         if rows.dtype not in (torch.int32, torch.int64):
             raise TypeError("adapter ids are an int32 or int64 tensor")
-        _require_cuda(x, rows)
+        if rows.get_device() != d:
+            _require_cuda(x, rows)
         index = _spread_index(rows, lead)
         if records or count > _lib.FPEMU_ADAPTER_FEW_ROWS:
             rows = PreparedRows(index, adapters)
@@ -239,25 +250,24 @@ def adapter_matmul(x, A, B, rows, base=None, scale=1.0, out=None):
             index = index.reshape(-1).contiguous()
     else:
         raise TypeError("rows is a tensor of adapter ids or the result of prepare_rows")
+    x2, A, B = _last_contiguous(x if flat else x.reshape(count, k)), _last_contiguous(A), _last_contiguous(B)
+    base2 = None
     if base is not None:
-        base = base.expand(shape)
+        if base.shape != shape:
+            base = base.expand(shape)
+        base2 = _last_contiguous(base if flat else base.reshape(count, n))
     if records:
         if out is not None:
             raise RuntimeError("adapter_matmul: out cannot be given while autograd records")
-        y = _AdapterMatmul.apply(_last_contiguous(x.reshape(count, k)), _last_contiguous(A), _last_contiguous(B),
-                                 None if base is None else _last_contiguous(base.reshape(count, n)), rows, scale)
-        return y.view(shape)
-    with torch.no_grad():
-        x2, A, B = _last_contiguous(x.reshape(count, k)), _last_contiguous(A), _last_contiguous(B)
-        if out is None:
-            y = torch.empty((count, n), dtype=x.dtype, device=dev)
-        else:
-            y = _check_out(out, shape, x, base, (x, A, B))
-        base2 = None if base is None else _last_contiguous(base.reshape(count, n))
-        plan = None if rows is None else _plan_of(rows)
-        _launch(x2, A, B, 0, base2, y, scale, index if rows is None else rows.index, plan, adapters, rank, k, n, None)
+        y = _AdapterMatmul.apply(x2, A, B, base2, rows, scale)
+        return y if flat else y.view(shape)
     if out is None:
-        return y.view(shape)
+        y = torch.empty((count, n), dtype=dtype, device=x.device)
+    else:
+        y = _check_out(out, shape, x, base, (x2, A, B))
+    _launch(x2, A, B, 0, base2, y, scale, index, None if rows is None else _plan_of(rows), adapters, rank, k, n, None)
+    if out is None:
+        return y if flat else y.view(shape)
     torch.autograd.graph.increment_version(out)
     return out
 

@@ -8,14 +8,15 @@ the reference.
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import operator
+from array import array
 
 import torch
 
 from fp_emulation import _lib
 from fp_emulation.adapters import _DTYPE_CODE
-from fp_emulation.ozaki import _after_call, _dtype_bits, _require_cuda, _stream
+from fp_emulation.ozaki import _after_call, _dtype_bits, _on, _require_cuda
 
 _NORMS = {1.0: 1, 2.0: 2, math.inf: 0}
 
@@ -39,33 +40,54 @@ def _dense(t):
     return True
 
 
+_layout, _dtype, _grad = map(operator.attrgetter, ("layout", "dtype", "grad"))
+
+
 def _check_list(tensors, what):
+    """The tensors' dtype codes; refuses what the kernels do not take."""
+    try:
+        devices = set(map(torch.Tensor.get_device, tensors))
+        codes = list(map(_DTYPE_CODE.__getitem__, map(_dtype, tensors)))
+        if len(devices) == 1 and devices <= _lib._watched and set(map(_layout, tensors)) == {torch.strided}:
+            return codes
+    except (TypeError, KeyError):
+        pass
     for t in tensors:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}: a list of tensors, got {type(t).__name__}")
-        if t.layout != torch.strided:
+        if t.layout is not torch.strided:
             raise TypeError(f"{what}: strided tensors only, got {t.layout}")
-        if t.dtype not in _DTYPE_CODE:
-            _dtype_bits(t.dtype)  # raises
-    return _require_cuda(*tensors)
+        _dtype_bits(t.dtype)
+    _require_cuda(*tensors)
+    return [_DTYPE_CODE[t.dtype] for t in tensors]
 
 
-def _run(src, dst, code, max_norm, dev, what):
+def _in_one_stretch(tensors):
+    """The tensors, with copies in place of those that are not dense."""
+    if all(map(torch.Tensor.is_contiguous, tensors)):
+        return tensors
+    return [t if _dense(t) else t.contiguous() for t in tensors]
+
+
+def _run(src, dst, codes, norm_code, max_norm, what):
     """One fpemu_clip_grads: the norm of `src` and, with `dst`, the scaled tensors.
-    float64 if any tensor is, else float32."""
+    The norm is float64 if any tensor is, else float32."""
     n = len(src)
-    wide = any(t.dtype == torch.float64 for t in src)
+    dev = src[0].device
+    wide = _lib.FPEMU_DT_F64 in codes
     lib = _lib.load()
-    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in src])
-    outs = None if dst is None else (ctypes.c_void_p * n)(*[t.data_ptr() for t in dst])
-    sizes = (ctypes.c_int64 * n)(*[t.numel() for t in src])
-    dtypes = (ctypes.c_int32 * n)(*[_DTYPE_CODE[t.dtype] for t in src])
-    with torch.cuda.device(dev):
+    ptrs, sizes = array("Q", map(torch.Tensor.data_ptr, src)), array("q", map(torch.Tensor.numel, src))
+    outs = None if dst is None else ptrs if dst is src else array("Q", map(torch.Tensor.data_ptr, dst))
+    kinds = array("i", codes)
+    with _on(dev.index):
         norm = torch.empty((), dtype=torch.float64 if wide else torch.float32, device=dev)
         ws = torch.empty((lib.fpemu_clip_workspace_size(n),), dtype=torch.uint8, device=dev)
-        st = lib.fpemu_clip_grads(n, ptrs, outs, sizes, dtypes, code, max_norm, norm.data_ptr(), int(wide),
-                                  ws.data_ptr(), ws.numel(), _stream(dev))
-    _lib.check(st, what)
+        st = lib.fpemu_clip_grads(n, ptrs.buffer_info()[0], None if outs is None else outs.buffer_info()[0],
+                                  sizes.buffer_info()[0], kinds.buffer_info()[0], norm_code, max_norm,
+                                  norm.data_ptr(), int(wide), ws.data_ptr(), ws.numel(),
+                                  torch.cuda.current_stream(dev.index).cuda_stream)
+    if st:
+        _lib.check(st, what)
     _after_call(what, dev)
     return norm
 
@@ -87,8 +109,8 @@ def grad_norm(tensors, norm_type=2.0):
     code = _norm_code(norm_type)
     if not tensors:
         return torch.tensor(0.0)
-    dev = _check_list(tensors, "grad_norm")
-    return _run([t if _dense(t) else t.contiguous() for t in tensors], None, code, 0.0, dev, "grad_norm")
+    codes = _check_list(tensors, "grad_norm")
+    return _run(_in_one_stretch(tensors), None, codes, code, 0.0, "grad_norm")
 
 
 @torch.no_grad()
@@ -102,26 +124,28 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     code, max_norm = _norm_code(norm_type), _max_norm(max_norm)
     if not grads:
         return [], torch.tensor(0.0)
-    dev = _check_list(grads, "clip_grads")
-    src = [g if _dense(g) else g.contiguous() for g in grads]
+    codes = _check_list(grads, "clip_grads")
+    src = _in_one_stretch(grads)
     if out is None:
         out = dst = [torch.empty_like(s) for s in src]
-    else:
-        out = list(out)
-        if len(out) != len(grads):
-            raise RuntimeError(f"clip_grads: {len(out)} outputs for {len(grads)} gradients")
-        _check_list(grads + out, "clip_grads")
-        for g, o in zip(grads, out):
-            if g.shape != o.shape or g.dtype != o.dtype:
-                raise RuntimeError("clip_grads: an output has another shape or dtype than its gradient")
-        dst = [o if _dense(o) and o.stride() == s.stride() else torch.empty_like(s) for s, o in zip(src, out)]
-    norm = _run(src, dst, code, max_norm, dev, "clip_grads")
-    if dst is not out:
-        for o, d in zip(out, dst):
-            if o is d:
-                torch.autograd.graph.increment_version(o)
-            else:
-                o.copy_(d)
+        return out, _run(src, dst, codes, code, max_norm, "clip_grads")
+    out = list(out)
+    if len(out) != len(grads):
+        raise RuntimeError(f"clip_grads: {len(out)} outputs for {len(grads)} gradients")
+    if all(map(operator.is_, out, src)):
+        norm = _run(src, src, codes, code, max_norm, "clip_grads")
+        torch.autograd.graph.increment_version(out)
+        return out, norm
+    _check_list(grads + out, "clip_grads")
+    for g, o in zip(grads, out):
+        if g.shape != o.shape or g.dtype != o.dtype:
+            raise RuntimeError("clip_grads: an output has another shape or dtype than its gradient")
+    dst = [o if _dense(o) and o.stride() == s.stride() else torch.empty_like(s) for s, o in zip(src, out)]
+    norm = _run(src, dst, codes, code, max_norm, "clip_grads")
+    torch.autograd.graph.increment_version([o for o, d in zip(out, dst) if o is d])
+    for o, d in zip(out, dst):
+        if o is not d:
+            o.copy_(d)
     return out, norm
 
 
@@ -134,7 +158,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     appear once."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     code, max_norm = _norm_code(norm_type), _max_norm(max_norm)
-    grads = [p.grad for p in parameters if p.grad is not None]
+    grads = [g for g in map(_grad, parameters) if g is not None]
     if not grads:
         return torch.tensor(0.0)
     if error_if_nonfinite:

@@ -13,6 +13,7 @@ reference on its own; the production call goes through one C entry point.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -68,6 +69,14 @@ def _stream(device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_NO_CONTEXT = contextlib.nullcontext()
+
+
+def _on(index):
+    """A context in which CUDA device `index` is current (free when it is already)."""
+    return _NO_CONTEXT if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
 def _require_cuda(*tensors):
     for t in tensors:
         if not t.is_cuda:
@@ -92,8 +101,12 @@ def _after_call(what: str, dev) -> None:
     """Surface a device-side failure recorded on `dev` (see _CHECK_MODE)."""
     if _CHECK_MODE == "off":
         return
+    word = _lib.error_words.get(dev.index)
+    if _CHECK_MODE == "poll" and word is not None and word.value == 0:
+        return
     with torch.cuda.device(dev):
         if _CHECK_MODE == "poll" and _lib.poll_error()[0] == 0:
+            _lib.remember_error_word(dev.index)
             return
         code, where, block, detail = _lib.device_error(clear=True)
     if code == _lib.FPEMU_ERR_INVALID and where == _lib.WHERE_ADAPTER_INDEX:

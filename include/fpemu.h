@@ -280,6 +280,11 @@ int fpemu_watch_errors(void);
  * reference. */
 int fpemu_poll_error(int *code, int *where, int *block, int *detail);
 
+/* Where fpemu_poll_error reads `code` for the current device: a host address
+ * that stays valid, for callers that look after every call.  Needs
+ * fpemu_watch_errors on this device.  No counterpart in the reference. */
+int fpemu_error_word(const volatile int **word);
+
 #ifdef __cplusplus
 }
 #endif
