@@ -2,6 +2,7 @@
 // (declared in include/fpemu.h).
 #include <cuda_runtime.h>
 
+#include <cstdlib>
 #include <type_traits>
 
 #include "adapter_kernels.cuh"
@@ -27,6 +28,8 @@ int check_sizes(const char* what, int dtype, int64_t rows, int64_t k, int64_t n,
     if (rows < 0 || rows > FPEMU_ADAPTER_MAX_ROWS || k < 0 || n < 0)
         return fail(FPEMU_ERR_INVALID, "%s: bad sizes rows=%lld k=%lld n=%lld", what, (long long)rows, (long long)k,
                     (long long)n);
+    if (k >= 1 << 30 || n >= 1 << 30)
+        return fail(FPEMU_ERR_UNSUPPORTED, "%s: k=%lld n=%lld: below 2^30", what, (long long)k, (long long)n);
     if (rank < 1 || rank > FPEMU_ADAPTER_MAX_RANK)
         return fail(FPEMU_ERR_UNSUPPORTED, "%s: rank %lld outside [1, %d]", what, (long long)rank,
                     FPEMU_ADAPTER_MAX_RANK);
@@ -61,7 +64,9 @@ int launch_tiles_rank(const AdapterParams& P, const DevInfo& d, cudaStream_t st)
     FPEMU_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem));
     const int64_t slots = plan_slots(P.rows, P.adapters);
     int cluster = 1;
+    static const char* force = getenv("FPEMU_PROBE_C");
     while (cluster < 8 && P.rows / kSlotRows * cluster < d.sms * 4) cluster *= 2;
+    if (force) cluster = atoi(force);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(slots * cluster));
     cfg.blockDim = dim3(kTileThreads);
@@ -101,7 +106,7 @@ int launch_grad_rank(AdapterGradParams& P, const DevInfo& d, cudaStream_t st) {
     P.first_blocks = blocks[0] * cluster;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((blocks[0] + blocks[1]) * cluster), (unsigned)P.adapters);
-    cfg.blockDim = dim3(kTileThreads);
+    cfg.blockDim = dim3(kGradThreads);
     cfg.dynamicSmemBytes = Tile::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr;

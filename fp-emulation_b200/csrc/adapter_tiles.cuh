@@ -17,8 +17,6 @@
 
 namespace fpemu {
 
-constexpr int kTileThreads = 128;  // four warps of 16 rows
-
 __device__ __forceinline__ uint32_t shared_address(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
@@ -33,15 +31,13 @@ __device__ __forceinline__ void copy_wait() {
 
 // 16 bytes of a tile: `avail` elements from src, zeros after them.
 template <typename T>
-__device__ __forceinline__ void fetch16(uint8_t* dst, const T* src, const T* safe, int avail, bool vec) {
+__device__ __forceinline__ void fetch16(uint8_t* dst, const T* src, int avail, bool vec) {
     constexpr int V = 16 / sizeof(T);
     if (vec) {
-        copy16(shared_address(dst), avail > 0 ? src : safe, avail * (int)sizeof(T));
+        copy16(shared_address(dst), src, avail * (int)sizeof(T));  // src is not read where avail is 0
     } else {
-        alignas(16) T v[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = i < avail ? src[i] : T(0.0f);
-        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(v);
+#pragma unroll 1
+        for (int i = 0; i < V; ++i) reinterpret_cast<T*>(dst)[i] = i < avail ? src[i] : T(0.0f);
     }
 }
 
@@ -131,6 +127,15 @@ struct AdapterTile {
     static constexpr int kStages = RP <= 32 ? 4 : 3;
     static constexpr int kPitchU = E == 2 ? RP + 8 : RP + 4;  // elements of Acc
     static constexpr int kSmem = kStages * kStage + kSlotRows * kPitchU * (int)sizeof(Acc);
+    static constexpr int kBlocks = kSmem <= 57000 ? 4 : RP <= 32 && kSmem <= 76000 ? 3 : kSmem <= 114000 ? 2 : 1;  // per SM
+    // The results of a warp's two rows are 16 bytes of neighbouring columns for each thread: column
+    // q * V + 2 t + b of a group of 4 V stands where the instruction has column 2 q + b of its tile t.
+    // Long-major weights are laid out in that order; 16-bit rank-major ones (read transposed, eight
+    // neighbours at a time) are not, and their results go through the tile instead.
+    static constexpr bool kDirect = !(TR && E == 2);
+    __host__ __device__ static constexpr int place(int c) {
+        return kDirect ? c / (4 * V) * (4 * V) + c % V / 2 * 8 + c % (4 * V) / V * 2 + c % 2 : c;
+    }
 };
 
 // Rows without an adapter or with a bad id, this block's share of the columns.
@@ -156,15 +161,22 @@ __device__ void plain_rows(const AdapterParams& P, const int* list, int count, b
     }
 }
 
+// Eight warps: four groups of 16 rows, twice.  In the first product the two
+// warps of a group hold half of the rank each, in the second one half of the
+// chunk's columns.
+constexpr int kTileThreads = 256;
+
 template <typename T, bool TR, int RP>
-__global__ void __launch_bounds__(kTileThreads) adapter_tile_kernel(AdapterParams P) {
+__global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
+    adapter_tile_kernel(const __grid_constant__ AdapterParams P) {
     using Tile = AdapterTile<T, TR, RP>;
     using Acc = typename Tile::Acc;
-    constexpr int E = Tile::E, V = Tile::V, KC = Tile::KC, S = Tile::kStages;
+    constexpr int E = Tile::E, V = Tile::V, KC = Tile::KC, S = Tile::kStages, HT = RP / 16;  // HT: 8-rank tiles a warp
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int list[kSlotRows];
     cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, q = lane & 3;
+    const int rows0 = (tid >> 5 & 3) * 16, half = tid >> 7;
     const int cr = (int)cluster.block_rank(), cs = (int)cluster.num_blocks();
     const AdapterSlot slot =
         reinterpret_cast<const AdapterSlot*>(P.plan + plan_slot_word(P.adapters))[blockIdx.x / cs];
@@ -173,118 +185,135 @@ __global__ void __launch_bounds__(kTileThreads) adapter_tile_kernel(AdapterParam
     if (tid < kSlotRows)
         list[tid] = (P.plan + plan_perm_word(P.rows, P.adapters))[slot.start + (tid < count ? tid : 0)];
     __syncthreads();
-    const int64_t kshare = (P.k + (int64_t)KC * cs - 1) / ((int64_t)KC * cs) * KC;
-    const int64_t nshare = (P.n + (int64_t)KC * cs - 1) / ((int64_t)KC * cs) * KC;
-    const int64_t k0 = cr * kshare < P.k ? cr * kshare : P.k, k1 = k0 + kshare < P.k ? k0 + kshare : P.k;
-    const int64_t n0 = cr * nshare < P.n ? cr * nshare : P.n, n1 = n0 + nshare < P.n ? n0 + nshare : P.n;
+    // This block's share of k and of n, in whole chunks but for the last block's (k and n stay below 2^30).
+    const int k = (int)P.k, n = (int)P.n;
+    const int kshare = (k + KC * cs - 1) / (KC * cs) * KC, nshare = (n + KC * cs - 1) / (KC * cs) * KC;
+    const int k0 = min(cr * kshare, k), n0 = min(cr * nshare, n);
+    const int klen = min(kshare, k - k0), nlen = min(nshare, n - n0);
     if (slot.cls >= P.adapters) {
-        plain_rows<T>(P, list, count, slot.cls != P.adapters, n0, n1);
+        plain_rows<T>(P, list, count, slot.cls != P.adapters, n0, n0 + nlen);
         return;
     }
-    const int nk = (int)((k1 - k0 + KC - 1) / KC), total = nk + (int)((n1 - n0 + KC - 1) / KC);
+    const int nk = (klen + KC - 1) / KC, total = nk + (nlen + KC - 1) / KC;
     const T* w1 = static_cast<const T*>(P.w1) + slot.cls * P.w1_adapter;
     const T* w2 = static_cast<const T*>(P.w2) + slot.cls * P.w2_adapter;
     const T* x = static_cast<const T*>(P.x);
     const T* base = static_cast<const T*>(P.base);
-    T* y = static_cast<T*>(P.y);
     auto aligned = [](const void* p, int64_t stride) {
         return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * E)) & 15) == 0;
     };
     const bool vec_x = aligned(x, P.x_row), vec_w1 = aligned(w1, P.w1_row), vec_w2 = aligned(w2, P.w2_row);
-    const bool vec_base = aligned(base, P.base_row), vec_y = aligned(y, P.y_row);
+    const bool vec_base = aligned(base, P.base_row), vec_y = aligned(P.y, P.y_row);
 
-    auto clamp = [](int64_t v) { return v < 0 ? 0 : v > V ? V : (int)v; };
-    auto fetch_rows = [&](uint8_t* st, const T* src, int64_t stride, int64_t c0, int64_t c1, bool vec) {
+    auto clamp = [](int v) { return v < 0 ? 0 : v > V ? V : v; };
+    // This thread's 16-byte units of a tile: one of rows tid / 8 and tid / 8 + 32, and NW of the weights,
+    // UPR units along and SKIP rows apart.  The pointers advance from chunk to chunk; whole chunks of
+    // aligned operands are copied as they are, others element by element where they must.
+    constexpr int NW = (RP + 31) / 32;
+    const int unit = tid % 8 * V;
+    const T *rp[2], *wp;
+    auto aim_rows = [&](const T* src, int64_t stride, int c0) {
 #pragma unroll
-        for (int i = 0; i < kSlotRows / 16; ++i) {
-            const int row = tid / 8 + 16 * i;
-            const int64_t c = c0 + (tid % 8) * V;
-            fetch16(st + row * Tile::kPitchX + (tid % 8) * 16, src + list[row] * stride + c, src,
-                    row < count ? clamp(c1 - c) : 0, vec);
+        for (int i = 0; i < 2; ++i) rp[i] = src + list[tid / 8 + 32 * i] * stride + c0 + unit;
+    };
+    auto fetch_weights = [&](auto by_long, uint8_t* wt, int64_t stride, int left, bool vec) {
+        constexpr bool LONG = decltype(by_long)::value, PLACED = LONG && !TR;  // the second product's
+        constexpr int UPR = LONG ? RP * E / 16 : 8, SKIP = kTileThreads / UPR;
+        const int l = tid / UPR, j = tid % UPR * V;
+        if (RP >= 32 || tid < 8 * RP) {
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                const int row = l + i * SKIP;
+                uint8_t* dst = wt + (PLACED ? Tile::place(row) : row) * (LONG ? Tile::kPitchLong : Tile::kPitchRank) + j * E;
+                const int avail = LONG ? (row < left ? clamp(P.r - j) : 0) : row < P.r ? clamp(left - j) : 0;
+                fetch16(dst, wp + i * SKIP * stride, avail, vec);
+            }
+        }
+        wp += LONG ? KC * stride : KC;
+    };
+    auto aim_weights = [&](auto by_long, const T* w, int64_t stride, int c0) {
+        constexpr bool LONG = decltype(by_long)::value;
+        constexpr int UPR = LONG ? RP * E / 16 : 8;
+        wp = w + (tid / UPR + (LONG ? c0 : 0)) * stride + tid % UPR * V + (LONG ? 0 : c0);
+    };
+    constexpr std::integral_constant<bool, TR> first_long{};
+    constexpr std::integral_constant<bool, !TR> second_long{};
+    auto fetch_rows = [&](uint8_t* st, int left, bool vec) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            fetch16(st + (tid / 8 + i * 32) * Tile::kPitchX + tid % 8 * 16, rp[i],
+                    tid / 8 + i * 32 < count ? clamp(left - unit) : 0, vec);
+            rp[i] += KC;
         }
     };
-    auto fetch_rank = [&](uint8_t* st, const T* w, int64_t stride, int64_t c0, int64_t c1, bool vec) {
-#pragma unroll
-        for (int i = 0; i < RP * 8 / kTileThreads; ++i) {
-            const int j = tid / 8 + 16 * i;
-            const int64_t c = c0 + (tid % 8) * V;
-            fetch16(st + j * Tile::kPitchRank + (tid % 8) * 16, w + j * stride + c, w, j < P.r ? clamp(c1 - c) : 0, vec);
-        }
+    auto fetch_first = [&](int c, uint8_t* st) {
+        fetch_rows(st, klen - c * KC, vec_x);
+        fetch_weights(first_long, st + Tile::kStageX, P.w1_row, klen - c * KC, vec_w1);
     };
-    auto fetch_long = [&](uint8_t* st, const T* w, int64_t stride, int64_t c0, int64_t c1, bool vec) {
-        constexpr int per = RP * E / 16;
-#pragma unroll
-        for (int i = 0; i < (KC * per + kTileThreads - 1) / kTileThreads; ++i) {
-            const int idx = tid + i * kTileThreads, l = idx / per, j = idx % per * V;
-            if (KC * per % kTileThreads == 0 || idx < KC * per)
-                fetch16(st + l * Tile::kPitchLong + j * E, w + (c0 + l) * stride + j, w,
-                        c0 + l < c1 ? clamp(P.r - j) : 0, vec);
+    auto fetch_second = [&](int c, uint8_t* st) {
+        if (c == 0) {
+            if (base) aim_rows(base, P.base_row, n0);
+            aim_weights(second_long, w2, P.w2_row, n0);
         }
-    };
-    auto fetch = [&](int c) {
-        uint8_t* st = smem + c % S * Tile::kStage;
-        if (c < nk) {
-            const int64_t c0 = k0 + (int64_t)c * KC;
-            fetch_rows(st, x, P.x_row, c0, k1, vec_x);
-            if (TR) fetch_long(st + Tile::kStageX, w1, P.w1_row, c0, k1, vec_w1);
-            else fetch_rank(st + Tile::kStageX, w1, P.w1_row, c0, k1, vec_w1);
-        } else {
-            const int64_t c0 = n0 + (int64_t)(c - nk) * KC;
-            if (base) fetch_rows(st, base, P.base_row, c0, n1, vec_base);
-            if (TR) fetch_rank(st + Tile::kStageX, w2, P.w2_row, c0, n1, vec_w2);
-            else fetch_long(st + Tile::kStageX, w2, P.w2_row, c0, n1, vec_w2);
-        }
+        if (base) fetch_rows(st, nlen - c * KC, vec_base);
+        fetch_weights(second_long, st + Tile::kStageX, P.w2_row, nlen - c * KC, vec_w2);
     };
 
     Acc* us = reinterpret_cast<Acc*>(smem + S * Tile::kStage);
-    Acc acc[RP / 8][4] = {};
+    Acc acc[HT][4] = {};
     // The middle as this thread's part of the left operand: 16-bit data split in
     // two and, for halves, scaled by a power of two per row; f32 and f64 plain.
     uint32_t uh[E == 2 ? RP / 16 : 1][4], ul[E == 2 ? RP / 16 : 1][4];
     Acc uf[E == 2 ? 1 : RP / (E == 4 ? 8 : 4)][E == 4 ? 4 : 2];
     float back[2] = {1.f, 1.f};
-    const bool busy = warp * 16 < count;
+    const bool busy = rows0 < count;
 
     auto exchange = [&]() {
-        Acc* own = us + warp * 16 * Tile::kPitchU;
+        Acc* own = us + rows0 * Tile::kPitchU;
 #pragma unroll
-        for (int t = 0; t < RP / 8; ++t) {
-            own[g * Tile::kPitchU + t * 8 + 2 * q] = acc[t][0];
-            own[g * Tile::kPitchU + t * 8 + 2 * q + 1] = acc[t][1];
-            own[(g + 8) * Tile::kPitchU + t * 8 + 2 * q] = acc[t][2];
-            own[(g + 8) * Tile::kPitchU + t * 8 + 2 * q + 1] = acc[t][3];
+        for (int t = 0; t < HT; ++t) {
+            Acc* o = own + g * Tile::kPitchU + (half * HT + t) * 8 + 2 * q;
+            o[0] = acc[t][0], o[1] = acc[t][1];
+            o[8 * Tile::kPitchU] = acc[t][2], o[8 * Tile::kPitchU + 1] = acc[t][3];
         }
         cluster.sync();
         const Acc s = (Acc)(P.scales ? P.scales[slot.cls] : P.scale);
-        const Acc* parts[8];
+        // Sums of the blocks' parts in their order, in place of v; past the rank, where an infinite x
+        // met a zero, 0.
+        auto join = [&](auto& v, auto row_of, auto rank_of) {
+            constexpr int M = sizeof(v) / sizeof(v[0]), N = sizeof(v[0]) / sizeof(v[0][0]);
+            for (int b = 0; b < cs; ++b) {
+                const Acc* part = cluster.map_shared_rank(own, b);
 #pragma unroll
-        for (int b = 0; b < 8; ++b) parts[b] = b < cs ? cluster.map_shared_rank(own, b) : nullptr;
-        auto at = [&](int row, int j) {
-            Acc v = 0;
+                for (int t = 0; t < M; ++t)
 #pragma unroll
-            for (int b = 0; b < 8; ++b)
-                if (b < cs) v += parts[b][row * Tile::kPitchU + j];
-            return j < P.r ? v * s : Acc(0);  // past the rank, an infinite x met a zero: NaN
-        };
-        auto keep = [&](int row, int j, Acc v) {
-            if (P.u && cr == 0 && j < P.r && warp * 16 + row < count)
-                static_cast<Acc*>(P.u)[(int64_t)list[warp * 16 + row] * P.u_row + j] = v;
+                    for (int e = 0; e < N; ++e) {
+                        const Acc p = part[row_of(e) * Tile::kPitchU + rank_of(t, e)];
+                        v[t][e] = b ? v[t][e] + p : p;
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < M; ++t)
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const int row = row_of(e), r = rank_of(t, e);
+                    v[t][e] = r < P.r ? v[t][e] * s : Acc(0);
+                    if (P.u && cr == 0 && half == 0 && r < P.r && rows0 + row < count)
+                        static_cast<Acc*>(P.u)[(int64_t)list[rows0 + row] * P.u_row + r] = v[t][e];
+                }
         };
         if (busy) {
             if constexpr (E == 2) {
-                float v[RP / 16][8];
-                float top[2] = {0.f, 0.f};
-#pragma unroll
-                for (int t = 0; t < RP / 16; ++t)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {  // a0..a3 of two: rows g, g + 8, then columns + 8
-                        const int row = g + (e >> 1 & 1) * 8, j = t * 16 + 2 * q + (e & 1) + (e >> 2) * 8;
-                        v[t][e] = at(row, j);
-                        keep(row, j, v[t][e]);
-                        top[e >> 1 & 1] = fmaxf(top[e >> 1 & 1], fabsf(v[t][e]));
-                    }
+                float v[RP / 16][8];  // a0..a3 of two: rows g, g + 8, then columns + 8
+                join(v, [&](int e) { return g + (e >> 1 & 1) * 8; },
+                     [&](int t, int e) { return t * 16 + 2 * q + (e & 1) + (e >> 2) * 8; });
                 float down[2] = {1.f, 1.f};
                 if constexpr (std::is_same<T, __half>::value) {
+                    float top[2] = {0.f, 0.f};
+#pragma unroll
+                    for (int t = 0; t < RP / 16; ++t)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) top[e >> 1 & 1] = fmaxf(top[e >> 1 & 1], fabsf(v[t][e]));
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
@@ -302,22 +331,9 @@ __global__ void __launch_bounds__(kTileThreads) adapter_tile_kernel(AdapterParam
                     for (int e = 0; e < 4; ++e)
                         split16<T>(v[t][2 * e] * down[e & 1], v[t][2 * e + 1] * down[e & 1], uh[t][e], ul[t][e]);
             } else if constexpr (E == 4) {
-#pragma unroll
-                for (int t = 0; t < RP / 8; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = g + (e & 1) * 8, j = t * 8 + q + (e >> 1) * 4;
-                        uf[t][e] = at(row, j);
-                        keep(row, j, uf[t][e]);
-                    }
+                join(uf, [&](int e) { return g + (e & 1) * 8; }, [&](int t, int e) { return t * 8 + q + (e >> 1) * 4; });
             } else {
-#pragma unroll
-                for (int t = 0; t < RP / 4; ++t)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        uf[t][e] = at(g + e * 8, t * 4 + q);
-                        keep(g + e * 8, t * 4 + q, uf[t][e]);
-                    }
+                join(uf, [&](int e) { return g + e * 8; }, [&](int t, int) { return t * 4 + q; });
             }
         }
     };
@@ -325,40 +341,57 @@ __global__ void __launch_bounds__(kTileThreads) adapter_tile_kernel(AdapterParam
     auto shrink = [&](const uint8_t* st) {
         const uint8_t* wt = st + Tile::kStageX;
         if constexpr (E == 2) {
-            const uint32_t xa = shared_address(st) + (warp * 16 + (lane & 15)) * Tile::kPitchX + (lane >> 4) * 16;
-            const uint32_t wa = shared_address(wt) +
-                                (TR ? (lane & 15) * Tile::kPitchLong + (lane >> 4) * 16
-                                    : ((lane & 7) + (lane >> 4) * 8) * Tile::kPitchRank + (lane >> 3 & 1) * 16);
+            const uint32_t xa = shared_address(st) + (rows0 + (lane & 15)) * Tile::kPitchX + (lane >> 4) * 16;
+            uint32_t b[4];
+            if constexpr (RP == 16) {  // one 8-rank tile: four 8-element pieces of k at a time
+                const uint32_t wa = shared_address(wt) + (TR ? lane * Tile::kPitchLong + half * 16
+                                                             : (half * 8 + (lane & 7)) * Tile::kPitchRank + (lane >> 3) * 16);
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-                uint32_t a[4], b[4];
-                ldsm4(a, xa + ks * 32);
+                for (int kp = 0; kp < 2; ++kp) {
+                    uint32_t a[4];
+                    if (TR) ldsm4t(b, wa + kp * 32 * Tile::kPitchLong);
+                    else ldsm4(b, wa + kp * 64);
+                    ldsm4(a, xa + kp * 64);
+                    mma16<T>(acc[0], a, b[0], b[1]);
+                    ldsm4(a, xa + kp * 64 + 32);
+                    mma16<T>(acc[0], a, b[2], b[3]);
+                }
+            } else {
+                const int j0 = half * HT * 8;
+                const uint32_t wa = shared_address(wt) +
+                                    (TR ? (lane & 15) * Tile::kPitchLong + (j0 + (lane >> 4) * 8) * 2
+                                        : (j0 + (lane & 7) + (lane >> 4) * 8) * Tile::kPitchRank + (lane >> 3 & 1) * 16);
 #pragma unroll
-                for (int p = 0; p < RP / 16; ++p) {
-                    if (TR) ldsm4t(b, wa + ks * 16 * Tile::kPitchLong + p * 32);
-                    else ldsm4(b, wa + p * 16 * Tile::kPitchRank + ks * 32);
-                    mma16<T>(acc[2 * p], a, b[0], b[1]);
-                    mma16<T>(acc[2 * p + 1], a, b[2], b[3]);
+                for (int ks = 0; ks < 4; ++ks) {
+                    uint32_t a[4];
+                    ldsm4(a, xa + ks * 32);
+#pragma unroll
+                    for (int p = 0; p < HT / 2; ++p) {
+                        if (TR) ldsm4t(b, wa + ks * 16 * Tile::kPitchLong + p * 32);
+                        else ldsm4(b, wa + p * 16 * Tile::kPitchRank + ks * 32);
+                        mma16<T>(acc[2 * p], a, b[0], b[1]);
+                        mma16<T>(acc[2 * p + 1], a, b[2], b[3]);
+                    }
                 }
             }
         } else if constexpr (E == 4) {
             // The tensor cores' sums run over one chunk; chunks are added in registers, rounded to nearest.
-            float sum[RP / 8][4] = {};
+            float sum[HT][4] = {};
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
                 uint32_t ah[4], al[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const Tf32Pair p = tf32_split(*reinterpret_cast<const float*>(
-                        st + (warp * 16 + g + (e & 1) * 8) * Tile::kPitchX + (ks * 8 + q + (e >> 1) * 4) * 4));
+                        st + (rows0 + g + (e & 1) * 8) * Tile::kPitchX + (ks * 8 + q + (e >> 1) * 4) * 4));
                     ah[e] = p.hi, al[e] = p.lo;
                 }
 #pragma unroll
-                for (int t = 0; t < RP / 8; ++t) {
+                for (int t = 0; t < HT; ++t) {
                     Tf32Pair b[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const int kk = ks * 8 + q + e * 4, j = t * 8 + g;
+                        const int kk = ks * 8 + q + e * 4, j = (half * HT + t) * 8 + g;
                         b[e] = tf32_split(*reinterpret_cast<const float*>(
                             wt + (TR ? kk * Tile::kPitchLong + j * 4 : j * Tile::kPitchRank + kk * 4)));
                     }
@@ -368,18 +401,18 @@ __global__ void __launch_bounds__(kTileThreads) adapter_tile_kernel(AdapterParam
                 }
             }
 #pragma unroll
-            for (int t = 0; t < RP / 8; ++t)
+            for (int t = 0; t < HT; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[t][e] += sum[t][e];
         } else {
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-                const uint8_t* xa = st + (warp * 16 + g) * Tile::kPitchX + (ks * 4 + q) * 8;
+                const uint8_t* xa = st + (rows0 + g) * Tile::kPitchX + (ks * 4 + q) * 8;
                 const double a0 = *reinterpret_cast<const double*>(xa);
                 const double a1 = *reinterpret_cast<const double*>(xa + 8 * Tile::kPitchX);
 #pragma unroll
-                for (int t = 0; t < RP / 8; ++t) {
-                    const int kk = ks * 4 + q, j = t * 8 + g;
+                for (int t = 0; t < HT; ++t) {
+                    const int kk = ks * 4 + q, j = (half * HT + t) * 8 + g;
                     mma_f64(acc[t], a0, a1, *reinterpret_cast<const double*>(
                         wt + (TR ? kk * Tile::kPitchLong + j * 8 : j * Tile::kPitchRank + kk * 8)));
                 }
@@ -387,46 +420,34 @@ __global__ void __launch_bounds__(kTileThreads) adapter_tile_kernel(AdapterParam
         }
     };
 
-    // Two neighbouring results of rows g and g + 8 at column `col` of the chunk: base plus the
-    // product, rounded once, left where base was.
-    auto finish = [&](uint8_t* st, int col, Acc c0, Acc c1, Acc c2, Acc c3) {
+    // This thread's rows of y at its 16 bytes of the warp's group of columns.
+    const int col0 = half * (KC / 2) + q * V;
+    T* yp[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            T* o = reinterpret_cast<T*>(st + (warp * 16 + g + h * 8) * Tile::kPitchX) + col;
-            Acc a = h ? c2 : c0, b = h ? c3 : c1;
-            if constexpr (std::is_same<T, __half>::value) a *= back[h], b *= back[h];
-            if (base) a += widen(o[0]), b += widen(o[1]);
-            alignas(16) T v[2] = {narrow<T>(a), narrow<T>(b)};
-            if constexpr (E == 2) *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<uint32_t*>(v);
-            else if constexpr (E == 4) *reinterpret_cast<uint2*>(o) = *reinterpret_cast<uint2*>(v);
-            else *reinterpret_cast<uint4*>(o) = *reinterpret_cast<uint4*>(v);
-        }
-    };
+    for (int h = 0; h < 2; ++h) yp[h] = static_cast<T*>(P.y) + list[rows0 + g + h * 8] * P.y_row + n0 + col0;
 
-    auto expand = [&](uint8_t* st, int64_t c0) {
+    auto expand = [&](uint8_t* st, int left) {
+        constexpr int NT = V / 2;  // 8-column tiles of a group
         const uint8_t* wt = st + Tile::kStageX;
+        Acc c[NT][4] = {};
         if constexpr (E == 2) {
             const uint32_t wa = shared_address(wt) +
-                                (TR ? (lane & 15) * Tile::kPitchRank + (lane >> 4) * 16
-                                    : ((lane & 7) + (lane >> 4) * 8) * Tile::kPitchLong + (lane >> 3 & 1) * 16);
+                                (TR ? (lane & 15) * Tile::kPitchRank + (half * 32 + (lane >> 4) * 8) * 2
+                                    : (half * 32 + (lane & 7) + (lane >> 4) * 8) * Tile::kPitchLong + (lane >> 3 & 1) * 16);
 #pragma unroll
-            for (int p = 0; p < KC / 16; ++p) {
-                float c[2][4] = {};
+            for (int t = 0; t < RP / 16; ++t) {
 #pragma unroll
-                for (int t = 0; t < RP / 16; ++t) {
+                for (int p = 0; p < 2; ++p) {
                     uint32_t b[4];
                     if (TR) ldsm4t(b, wa + t * 16 * Tile::kPitchRank + p * 32);
                     else ldsm4(b, wa + p * 16 * Tile::kPitchLong + t * 32);
-                    mma16<T>(c[0], ul[t], b[0], b[1]);
-                    mma16<T>(c[1], ul[t], b[2], b[3]);
-                    mma16<T>(c[0], uh[t], b[0], b[1]);
-                    mma16<T>(c[1], uh[t], b[2], b[3]);
+                    mma16<T>(c[2 * p], ul[t], b[0], b[1]);
+                    mma16<T>(c[2 * p + 1], ul[t], b[2], b[3]);
+                    mma16<T>(c[2 * p], uh[t], b[0], b[1]);
+                    mma16<T>(c[2 * p + 1], uh[t], b[2], b[3]);
                 }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) finish(st, p * 16 + h * 8 + 2 * q, c[h][0], c[h][1], c[h][2], c[h][3]);
             }
         } else if constexpr (E == 4) {
-            float c[KC / 8][4] = {};
 #pragma unroll
             for (int t = 0; t < RP / 8; ++t) {
                 uint32_t ah[4], al[4];
@@ -436,69 +457,101 @@ __global__ void __launch_bounds__(kTileThreads) adapter_tile_kernel(AdapterParam
                     ah[e] = p.hi, al[e] = p.lo;
                 }
 #pragma unroll
-                for (int p = 0; p < KC / 8; ++p) {
+                for (int p = 0; p < NT; ++p) {
                     Tf32Pair b[2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int j = t * 8 + q + e * 4, l = p * 8 + g;
+                    for (int e = 0; e < 2; ++e) {  // slot p * 8 + g of the group is its column g / 2 * V + 2 p + g % 2
+                        const int j = t * 8 + q + e * 4;
                         b[e] = tf32_split(*reinterpret_cast<const float*>(
-                            wt + (TR ? j * Tile::kPitchRank + l * 4 : l * Tile::kPitchLong + j * 4)));
+                            wt + (TR ? j * Tile::kPitchRank + (half * 16 + g / 2 * V + 2 * p + g % 2) * 4
+                                     : (half * 16 + p * 8 + g) * Tile::kPitchLong + j * 4)));
                     }
                     mma_tf32(c[p], ah, b[0].lo, b[1].lo);
                     mma_tf32(c[p], al, b[0].hi, b[1].hi);
                     mma_tf32(c[p], ah, b[0].hi, b[1].hi);
                 }
             }
-#pragma unroll
-            for (int p = 0; p < KC / 8; ++p) finish(st, p * 8 + 2 * q, c[p][0], c[p][1], c[p][2], c[p][3]);
         } else {
-            double c[KC / 8][4] = {};
 #pragma unroll
-            for (int t = 0; t < RP / 4; ++t)
-#pragma unroll
-                for (int p = 0; p < KC / 8; ++p) {
-                    const int j = t * 4 + q, l = p * 8 + g;
-                    mma_f64(c[p], uf[t][0], uf[t][1], *reinterpret_cast<const double*>(
-                        wt + (TR ? j * Tile::kPitchRank + l * 8 : l * Tile::kPitchLong + j * 8)));
-                }
-#pragma unroll
-            for (int p = 0; p < KC / 8; ++p) finish(st, p * 8 + 2 * q, c[p][0], c[p][1], c[p][2], c[p][3]);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {  // 8 lanes a row, 16 bytes each
-            const int row = warp * 16 + i * 4 + lane / 8;
-            const int64_t c = c0 + (lane % 8) * V;
-            const int avail = row < count ? clamp(n1 - c) : 0;
-            const uint8_t* src = st + row * Tile::kPitchX + (lane % 8) * 16;
-            T* dst = y + list[row] * P.y_row + c;
-            if (vec_y && avail == V) {
-                *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-            } else {
-                for (int e = 0; e < avail; ++e) dst[e] = reinterpret_cast<const T*>(src)[e];
+            for (int t = 0; t < RP / 4; ++t) {
+                const int j = t * 4 + q, l = half * 8 + g;
+                mma_f64(c[0], uf[t][0], uf[t][1], *reinterpret_cast<const double*>(
+                    wt + (TR ? j * Tile::kPitchRank + l * 8 : l * Tile::kPitchLong + j * 8)));
             }
+        }
+        if constexpr (!Tile::kDirect) {
+            // Through the tile: pairs of columns in, 16 bytes of a row out; base waits in the tile meanwhile.
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int p = 0; p < NT; ++p) {
+                    T* o = reinterpret_cast<T*>(st + (rows0 + g + h * 8) * Tile::kPitchX) + half * 32 + p * 8 + 2 * q;
+                    alignas(4) T v[2];
+                    float a = c[p][2 * h], b = c[p][2 * h + 1];
+                    if constexpr (std::is_same<T, __half>::value) a *= back[h], b *= back[h];
+                    if (base) a += widen(o[0]), b += widen(o[1]);
+                    v[0] = narrow<T>(a), v[1] = narrow<T>(b);
+                    *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<uint32_t*>(v);
+                }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            alignas(16) T v[V];
+            const uint8_t* tile = st + (rows0 + g + h * 8) * Tile::kPitchX + half * 64 + q * 16;
+            if (!Tile::kDirect || base) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(tile);
+            if constexpr (Tile::kDirect) {
+#pragma unroll
+                for (int p = 0; p < NT; ++p)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        Acc a = c[p][2 * h + b];
+                        if constexpr (std::is_same<T, __half>::value) a *= back[h];
+                        v[2 * p + b] = narrow<T>(base ? a + (Acc)widen(v[2 * p + b]) : a);
+                    }
+            }
+            if (rows0 + g + h * 8 < count) {
+                if (vec_y && left >= KC) {
+                    *reinterpret_cast<uint4*>(yp[h]) = *reinterpret_cast<uint4*>(v);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (e + col0 < left) yp[h][e] = v[e];
+                }
+            }
+            yp[h] += KC;
         }
     };
 
-#pragma unroll
-    for (int c = 0; c < S - 1; ++c) {
-        if (c < total) fetch(c);
+    // Stages by their offset: `load` is where the next chunk goes, `use` what is computed.
+    uint32_t load = 0, use = 0;
+    auto next = [](uint32_t& stage) { stage = stage == (S - 1) * Tile::kStage ? 0 : stage + Tile::kStage; };
+    aim_rows(x, P.x_row, k0);
+    aim_weights(first_long, w1, P.w1_row, k0);
+    for (int c = 1 - S; c < nk; ++c) {
+        if (c >= 0) {
+            copy_wait<S - 2>();
+            __syncthreads();  // chunk c has arrived for all; chunk c - 1's buffer is free
+        }
+        if (c + S - 1 < nk) fetch_first(c + S - 1, smem + load);
+        else if (c + S - 1 < total) fetch_second(c + S - 1 - nk, smem + load);
+        next(load);
         copy_commit();
-    }
-    for (int c = 0; c < total; ++c) {
-        copy_wait<S - 2>();
-        __syncthreads();  // chunk c has arrived for all; chunk c - 1's buffer is free
-        if (c + S - 1 < total) fetch(c + S - 1);
-        copy_commit();
-        uint8_t* st = smem + c % S * Tile::kStage;
-        if (c < nk) {
-            if (busy) shrink(st);
-        } else {
-            if (c == nk) exchange();
-            if (busy) expand(st, n0 + (int64_t)(c - nk) * KC);
+        if (c >= 0) {
+            if (busy) shrink(smem + use);
+            next(use);
         }
     }
-    if (total == nk) exchange();
+    exchange();
+    for (int c = nk; c < total; ++c) {
+        copy_wait<S - 2>();
+        __syncthreads();
+        if (c + S - 1 < total) fetch_second(c + S - 1 - nk, smem + load);
+        next(load);
+        copy_commit();
+        if (busy) expand(smem + use, nlen - (c - nk) * KC);
+        next(use);
+    }
     cluster.sync();  // no block leaves while another may read its partial sums
 }
 
@@ -509,6 +562,8 @@ __global__ void __launch_bounds__(kTileThreads) adapter_tile_kernel(AdapterParam
 // the adapter's rows, so q is read once and p (rank values a row) by every block
 // of columns.  Where that gives too few blocks, a cluster splits the rows into
 // consecutive parts, whose sums meet in the blocks' order.
+constexpr int kGradThreads = 128;
+
 struct AdapterGradSide {
     const void* p;  // [rows, p_row] of the sums' type
     const void* q;  // [rows, cols]
@@ -542,7 +597,7 @@ struct AdapterGradTile {
 };
 
 template <typename T, int RP>
-__global__ void __launch_bounds__(kTileThreads) adapter_grad_kernel(const __grid_constant__ AdapterGradParams P) {
+__global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid_constant__ AdapterGradParams P) {
     using Tile = AdapterGradTile<T, RP>;
     using Acc = typename Tile::Acc;
     constexpr int E = Tile::E, V = Tile::V, KT = Tile::KT, S = Tile::kStages, MT = Tile::MT, COLS = Tile::COLS;
@@ -564,18 +619,18 @@ __global__ void __launch_bounds__(kTileThreads) adapter_grad_kernel(const __grid
     const bool vec = ((reinterpret_cast<uintptr_t>(qs) | (uintptr_t)(side.q_row * E)) & 15) == 0;
 
     // Row ids of a thread's copies, one chunk ahead of the copies themselves.
-    constexpr int QU = COLS / V, QI = KT * QU / kTileThreads;          // 16-byte units of a q row; copies a thread
-    constexpr int PV = 16 / (int)sizeof(Acc), PU = RP / PV, PI = KT * PU / kTileThreads;
+    constexpr int QU = COLS / V, QI = KT * QU / kGradThreads;          // 16-byte units of a q row; copies a thread
+    constexpr int PV = 16 / (int)sizeof(Acc), PU = RP / PV, PI = KT * PU / kGradThreads;
     int q_id[QI], p_id[PI];
     auto ids = [&](int c) {
 #pragma unroll
         for (int i = 0; i < QI; ++i) {
-            const int t = t0 + c * KT + (tid + i * kTileThreads) / QU;
+            const int t = t0 + c * KT + (tid + i * kGradThreads) / QU;
             q_id[i] = t < t1 ? perm[t] : -1;
         }
 #pragma unroll
         for (int i = 0; i < PI; ++i) {
-            const int t = t0 + c * KT + (tid + i * kTileThreads) / PU;
+            const int t = t0 + c * KT + (tid + i * kGradThreads) / PU;
             p_id[i] = t < t1 ? perm[t] : -1;
         }
     };
@@ -583,17 +638,17 @@ __global__ void __launch_bounds__(kTileThreads) adapter_grad_kernel(const __grid
         uint8_t* st = smem + c % S * Tile::kStage;
 #pragma unroll
         for (int i = 0; i < QI; ++i) {
-            const int u = tid + i * kTileThreads;
+            const int u = tid + i * kGradThreads;
             const int64_t col = c0 + u % QU * V, left = side.cols - col;
             const int avail = q_id[i] < 0 || left < 0 ? 0 : left > V ? V : (int)left;
-            fetch16(st + u / QU * Tile::kPitchQ + u % QU * 16, qs + q_id[i] * side.q_row + col, qs, avail, vec);
+            fetch16(st + u / QU * Tile::kPitchQ + u % QU * 16, qs + q_id[i] * side.q_row + col, avail, vec);
         }
 #pragma unroll
         for (int i = 0; i < PI; ++i) {
-            const int u = tid + i * kTileThreads, j = u % PU * PV;
+            const int u = tid + i * kGradThreads, j = u % PU * PV;
             const int avail = p_id[i] < 0 || j >= P.p_row ? 0 : PV;  // p_row is a multiple of PV
             fetch16(st + KT * Tile::kPitchQ + u / PU * Tile::kPitchP + u % PU * 16,
-                    ps + (int64_t)p_id[i] * P.p_row + j, ps, avail, true);
+                    ps + (int64_t)p_id[i] * P.p_row + j, avail, true);
         }
     };
 
@@ -732,7 +787,7 @@ __global__ void __launch_bounds__(kTileThreads) adapter_grad_kernel(const __grid
     const int first = cr * own, last = first + own < cols ? first + own : cols;
     T* grad = static_cast<T*>(side.grad) + (int64_t)cls * P.r * side.cols;
     const int many = last > first ? (last - first) * P.r : 0;
-    for (int i = tid; i < many; i += kTileThreads) {
+    for (int i = tid; i < many; i += kGradThreads) {
         const int c = first + (side.by_column ? i / P.r : i % (last - first));
         const int j = side.by_column ? i % P.r : i / (last - first);
         Acc v = 0;
