@@ -2,10 +2,11 @@
 // (declared in include/fpemu.h).
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdlib>
 #include <type_traits>
 
-#include "adapter_kernels.cuh"
+#include "adapter_few.cuh"
 #include "adapter_tiles.cuh"
 #include "fpemu_host.h"
 
@@ -39,22 +40,38 @@ int check_sizes(const char* what, int dtype, int64_t rows, int64_t k, int64_t n,
     return FPEMU_OK;
 }
 
-template <typename T>
-int launch_rows(const AdapterParams& P, bool transposed, cudaStream_t st) {
-    const int64_t units = P.plan ? plan_slots(P.rows, P.adapters) : P.rows;
+template <typename T, int RP>
+int launch_few_rank(const AdapterParams& P, const DevInfo& d, cudaStream_t st) {
+    auto kern = adapter_few_kernel<T, RP>;
+    using Tile = FewTile<T, RP>;
+    if (Tile::kSmem > 48 * 1024)
+        FPEMU_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem));
+    // Groups of eight rows of one adapter, of none, or with a bad id: never more than this.
+    const int64_t units = std::min<int64_t>(P.rows, P.rows / kGroupRows + P.adapters + 2);
+    int cluster = 8;
+    while (cluster > 2 && units * cluster > d.sms * 4) cluster /= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(units * kAdapterCluster));
-    cfg.blockDim = dim3(kAdapterThreads);
+    cfg.gridDim = dim3((unsigned)(units * cluster));
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = Tile::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = kAdapterCluster;
+    attr.val.clusterDim.x = cluster;
     attr.val.clusterDim.y = 1;
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    FPEMU_CUDA(cudaLaunchKernelEx(&cfg, transposed ? adapter_rows_kernel<T, true> : adapter_rows_kernel<T, false>, P));
+    FPEMU_CUDA(cudaLaunchKernelEx(&cfg, kern, P));
     return FPEMU_OK;
+}
+
+template <typename T>
+int launch_few(const AdapterParams& P, const DevInfo& d, cudaStream_t st) {
+    if (P.r <= 16) return launch_few_rank<T, 16>(P, d, st);
+    if (P.r <= 32) return launch_few_rank<T, 32>(P, d, st);
+    if (P.r <= 64) return launch_few_rank<T, 64>(P, d, st);
+    return launch_few_rank<T, 128>(P, d, st);
 }
 
 template <typename T, bool TR, int RP>
@@ -180,9 +197,9 @@ int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t 
     if (x_row < 0 || base_row < 0 || w1_adapter < 0 || w2_adapter < 0 || w1_row < 0 || w2_row < 0 ||
         (y_row < n && rows > 1))
         return fail(FPEMU_ERR_INVALID, "adapter_matmul: negative stride or output rows that overlap");
-    if (plan == nullptr && (rows > FPEMU_ADAPTER_FEW_ROWS || index == nullptr || (index_bytes != 4 && index_bytes != 8)))
-        return fail(FPEMU_ERR_INVALID, "adapter_matmul: %lld rows need a plan, fewer an index of 4 or 8 bytes",
-                    (long long)rows);
+    if (plan == nullptr && (rows > FPEMU_ADAPTER_FEW_ROWS || transposed || index == nullptr || (index_bytes != 4 && index_bytes != 8)))
+        return fail(FPEMU_ERR_INVALID, "adapter_matmul: %lld rows%s need a plan, few rows an index of 4 or 8 bytes",
+                    (long long)rows, transposed ? ", transposed," : "");
     FPEMU_TRY(device_info(&d));
     AdapterParams P = {};
     P.rows = rows, P.k = k, P.n = n, P.r = (int)rank, P.adapters = (int)adapters;
@@ -198,7 +215,7 @@ int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t 
         using T = std::remove_pointer_t<decltype(t)>;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         if (P.plan) return transposed ? launch_tiles<T, true>(P, d, st) : launch_tiles<T, false>(P, d, st);
-        return launch_rows<T>(P, transposed != 0, st);
+        return launch_few<T>(P, d, st);
     });
 }
 

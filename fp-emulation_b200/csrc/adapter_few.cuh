@@ -1,0 +1,298 @@
+// adapter_few.cuh -- the adapter products of a few rows (single tokens, small
+// batches), where the weights are what there is to read.
+//
+// A cluster of blocks takes up to eight rows of one adapter and shares the
+// lengths k and n.  Weights and rows go from memory straight into the operands
+// of mma.sync: the order of k inside a sum is free, so a thread's 16 contiguous
+// bytes of a weight row and of an input row stand for the same slots, and no
+// value passes through shared memory.  Eight rows fill the narrow side of the
+// instruction; in the second product the sixteen rows of its wide side hold the
+// eight rows twice, as the high and the low part of the middle.
+#pragma once
+
+#include "adapter_tiles.cuh"
+
+namespace fpemu {
+
+constexpr int kFewThreads = 256;
+constexpr int kGroupRows = 8;
+
+__device__ __forceinline__ void mma_f64_8(double (&c)[2], double a, double b) {
+    asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};"
+                 : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
+}
+
+// 16 bytes of a row: `avail` elements, zeros after them.
+template <typename T>
+__device__ __forceinline__ uint4 load16(const T* p, int avail, bool vec) {
+    constexpr int V = 16 / sizeof(T);
+    if (vec && avail >= V) return __ldg(reinterpret_cast<const uint4*>(p));
+    alignas(16) T v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = i < avail ? p[i] : T(0.0f);
+    return *reinterpret_cast<uint4*>(v);
+}
+
+template <typename T, int RP>
+struct FewTile {
+    using Acc = typename AccOf<T>::type;
+    static constexpr int E = sizeof(T), V = 16 / E, KS = 4 * V;     // elements of k a warp takes at a step
+    static constexpr int MR = E == 8 ? 8 : 16;                      // ranks of an instruction
+    static constexpr int RT = RP / MR, PA = E == 8 ? 2 : 4;         // rank tiles; sums a thread holds of one
+    static constexpr int UN = RP <= 16 ? 4 : RP <= 32 ? 2 : 1;      // steps with their loads in flight together
+    static constexpr int JS = (RP + KS - 1) / KS;                   // 16-byte steps along the rank
+    static constexpr int UG = JS * V >= 16 ? 1 : JS * V >= 8 ? 2 : 4;  // column groups, likewise
+    static constexpr int kWarps = kFewThreads / 32;
+    static constexpr int kSmem = (kWarps + 2) * RP * kGroupRows * (int)sizeof(Acc);
+};
+
+template <typename T, int RP>
+__global__ void __launch_bounds__(kFewThreads) adapter_few_kernel(const __grid_constant__ AdapterParams P) {
+    using Tile = FewTile<T, RP>;
+    using Acc = typename Tile::Acc;
+    constexpr int E = Tile::E, V = Tile::V, KS = Tile::KS, RT = Tile::RT, MR = Tile::MR, UN = Tile::UN, JS = Tile::JS;
+    constexpr int W = Tile::kWarps;
+    extern __shared__ __align__(16) uint8_t smem[];
+    Acc* red = reinterpret_cast<Acc*>(smem);           // [warp][rank][row]
+    Acc* part = red + W * RP * kGroupRows;             // [rank][row], read by the cluster
+    Acc* us = part + RP * kGroupRows;                  // [rank][row], the cluster's sums
+    __shared__ __align__(16) int ids[kFewRows];
+    __shared__ unsigned leaders[W];
+    __shared__ int list[kGroupRows], lead[2];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+    const int cr = (int)cluster.block_rank(), cs = (int)cluster.num_blocks();
+    const int rows = (int)P.rows, unit = blockIdx.x / cs;
+
+    // Rows of a class in groups of eight, by the rows' order; this cluster's group is the one whose
+    // first row is the unit-th of all groups' first rows.
+    const int mine = tid < rows ? row_class(P.index, P.index_wide, tid, P.adapters) : -1;
+    ids[tid] = mine;
+    __syncthreads();
+    int rank = 0;
+    for (int t = 0; t < tid; t += 4) {
+        const int4 v = *reinterpret_cast<const int4*>(ids + t);
+        rank += (v.x == mine) + (v.y == mine && t + 1 < tid) + (v.z == mine && t + 2 < tid) + (v.w == mine && t + 3 < tid);
+    }
+    const bool leader = tid < rows && rank % kGroupRows == 0;
+    const unsigned ballot = __ballot_sync(0xffffffffu, leader);
+    if (lane == 0) leaders[warp] = ballot;
+    __syncthreads();
+    int before = __popc(ballot & ((1u << lane) - 1)), groups = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        if (w < warp) before += __popc(leaders[w]);
+        groups += __popc(leaders[w]);
+    }
+    if (unit >= groups) return;
+    if (leader && before == unit) lead[0] = mine, lead[1] = rank;
+    __syncthreads();
+    const int cls = lead[0], place = rank - lead[1];
+    const bool in = tid < rows && mine == cls && place >= 0 && place < kGroupRows;
+    if (in) list[place] = tid;
+    const int count = __syncthreads_count(in);
+
+    const int k = (int)P.k, n = (int)P.n;
+    const int kshare = (k + KS * cs - 1) / (KS * cs) * KS, nshare = (n + KS * cs - 1) / (KS * cs) * KS;
+    const int k0 = min(cr * kshare, k), n0 = min(cr * nshare, n);
+    const int k1 = min(k0 + kshare, k), n1 = min(n0 + nshare, n);
+    if (cls >= P.adapters) {
+        if (cls > P.adapters && cr == 0 && tid == 0)
+            report_error(P.sink.dev, P.sink.host, FPEMU_ERR_INVALID, kWhereAdapterIndex, list[0]);
+        plain_rows<T>(P, list, count, cls != P.adapters, n0, n1);
+        return;
+    }
+    const T* w1 = static_cast<const T*>(P.w1) + cls * P.w1_adapter;
+    const T* w2 = static_cast<const T*>(P.w2) + cls * P.w2_adapter;
+    const int64_t row = list[g < count ? g : 0];
+    const T* xp = static_cast<const T*>(P.x) + row * P.x_row;
+    const T* base = P.base ? static_cast<const T*>(P.base) + row * P.base_row : nullptr;
+    T* y = static_cast<T*>(P.y) + row * P.y_row;
+    auto aligned = [](const void* p, int64_t stride) {
+        return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * E)) & 15) == 0;
+    };
+    const bool vec_x = aligned(P.x, P.x_row), vec_w1 = aligned(w1, P.w1_row), vec_w2 = aligned(w2, P.w2_row);
+    const bool vec_y = aligned(P.y, P.y_row), vec_base = aligned(P.base, P.base_row);
+
+    // The second product's weights start towards the L2 now.
+    if (P.w2_row == P.r) {
+        const char* from = reinterpret_cast<const char*>(w2 + (int64_t)n0 * P.r);
+        const int64_t bytes = (int64_t)(n1 - n0) * P.r * E;
+        for (int64_t at = (int64_t)tid * 128; at < bytes; at += kFewThreads * 128)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(from + at));
+    }
+
+    Acc acc[RT][Tile::PA] = {};
+    for (int c = k0 + warp * KS; c < k1; c += W * KS * UN) {
+        uint4 xv[UN], wv[UN][RT][MR / 8];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int at = c + u * W * KS + q * V, avail = k1 - at;
+            xv[u] = load16(xp + at, avail, vec_x);
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int h = 0; h < MR / 8; ++h) {
+                    const int j = t * MR + h * 8 + g;
+                    wv[u][t][h] = load16(w1 + (j < P.r ? j : 0) * P.w1_row + at, avail, vec_w1);
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const uint32_t* xr = reinterpret_cast<const uint32_t*>(&xv[u]);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                if constexpr (E == 8) {
+                    const double* xd = reinterpret_cast<const double*>(&xv[u]);
+                    const double* wd = reinterpret_cast<const double*>(&wv[u][t][0]);
+                    mma_f64_8(acc[t], wd[0], xd[0]);
+                    mma_f64_8(acc[t], wd[1], xd[1]);
+                } else {
+                    const uint32_t* wa = reinterpret_cast<const uint32_t*>(&wv[u][t][0]);
+                    const uint32_t* wb = reinterpret_cast<const uint32_t*>(&wv[u][t][MR / 8 - 1]);
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        if constexpr (E == 2) {
+                            const uint32_t a[4] = {wa[2 * m], wb[2 * m], wa[2 * m + 1], wb[2 * m + 1]};
+                            mma16<T>(acc[t], a, xr[2 * m], xr[2 * m + 1]);
+                        } else {
+                            const Tf32Pair p0 = tf32_split(__uint_as_float(wa[2 * m]));
+                            const Tf32Pair p1 = tf32_split(__uint_as_float(wb[2 * m]));
+                            const Tf32Pair p2 = tf32_split(__uint_as_float(wa[2 * m + 1]));
+                            const Tf32Pair p3 = tf32_split(__uint_as_float(wb[2 * m + 1]));
+                            const Tf32Pair b0 = tf32_split(__uint_as_float(xr[2 * m]));
+                            const Tf32Pair b1 = tf32_split(__uint_as_float(xr[2 * m + 1]));
+                            const uint32_t hi[4] = {p0.hi, p1.hi, p2.hi, p3.hi}, lo[4] = {p0.lo, p1.lo, p2.lo, p3.lo};
+                            mma_tf32(acc[t], hi, b0.lo, b1.lo);
+                            mma_tf32(acc[t], lo, b0.hi, b1.hi);
+                            mma_tf32(acc[t], hi, b0.hi, b1.hi);
+                        }
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int e = 0; e < Tile::PA; ++e)
+            red[(warp * RP + t * MR + (e >> 1) * 8 + g) * kGroupRows + 2 * q + (e & 1)] = acc[t][e];
+    __syncthreads();
+    for (int i = tid; i < RP * kGroupRows; i += kFewThreads) {
+        Acc v = red[i];
+#pragma unroll
+        for (int w = 1; w < W; ++w) v += red[w * RP * kGroupRows + i];
+        part[i] = v;
+    }
+    cluster.sync();
+    const Acc s = (Acc)(P.scales ? P.scales[cls] : P.scale);
+    join_parts<RP * kGroupRows>(cluster, cr, cs, part, us, [](int e) { return e; }, [&](int e, Acc v) {
+        const int j = e / kGroupRows, r = e % kGroupRows;
+        v = j < P.r ? v * s : Acc(0);
+        if (P.u && j < P.r && r < count) static_cast<Acc*>(P.u)[(int64_t)list[r] * P.u_row + j] = v;
+        return v;
+    });
+    cluster.sync();
+
+    // The middle as the left operand: rows g; where there are sixteen, rows g + 8 hold the low parts.
+    constexpr int UA = E == 8 ? 2 : E == 4 ? 8 : 8;
+    using Part = typename std::conditional<E == 8, double, uint32_t>::type;
+    Part ua[JS][UA];
+    float back = 1.f;
+    if constexpr (E == 2 && std::is_same<T, __half>::value) {
+        float top = 0.f;
+        for (int j = q; j < RP; j += 4) top = fmaxf(top, fabsf((float)us[j * kGroupRows + g]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = (int)(__float_as_uint(top) >> 23);
+        if (e > 0 && e < 254) back = __uint_as_float(e << 23);
+    }
+    const float down = back == 1.f ? 1.f : __uint_as_float((254u << 23) - __float_as_uint(back));
+#pragma unroll
+    for (int t = 0; t < JS; ++t) {
+        const int j0 = t * KS + q * V;
+        auto at = [&](int i) { return RP % KS == 0 || j0 + i < RP ? us[(j0 + i) * kGroupRows + g] : Acc(0); };
+        if constexpr (E == 8) {
+            ua[t][0] = at(0), ua[t][1] = at(1);
+        } else if constexpr (E == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const Tf32Pair p = tf32_split(at(i));
+                ua[t][2 * i] = p.hi, ua[t][2 * i + 1] = p.lo;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                split16<T>(at(2 * i) * down, at(2 * i + 1) * down, ua[t][2 * i], ua[t][2 * i + 1]);
+        }
+    }
+    constexpr int NT = V / 2;  // 8-column tiles of a group of KS columns, laid out as in AdapterTile::place
+    constexpr int UG = Tile::UG;
+    for (int first = n0 + warp * KS; first < n1; first += W * KS * UG) {
+        uint4 wv[UG][NT][JS], held[UG];
+#pragma unroll
+        for (int u = 0; u < UG; ++u) {
+            const int c0 = first + u * W * KS;
+#pragma unroll
+            for (int p = 0; p < NT; ++p)
+#pragma unroll
+                for (int t = 0; t < JS; ++t) {
+                    const int c = c0 + g / 2 * V + 2 * p + g % 2, j = t * KS + q * V;
+                    wv[u][p][t] = c < n1 && j < P.r ? load16(w2 + c * P.w2_row + j, P.r - j, vec_w2) : uint4{0, 0, 0, 0};
+                }
+            const int avail = g < count ? n1 - c0 - q * V : 0;
+            held[u] = base && avail > 0 ? load16(base + c0 + q * V, avail, vec_base) : uint4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < UG; ++u) {
+            const int col = first + u * W * KS + q * V, avail = g < count ? n1 - col : 0;
+            T* v = reinterpret_cast<T*>(&held[u]);
+#pragma unroll
+            for (int p = 0; p < NT; ++p) {
+                Acc r0, r1;
+                if constexpr (E == 8) {
+                    double c[2] = {};
+#pragma unroll
+                    for (int t = 0; t < JS; ++t) {
+                        const double* wd = reinterpret_cast<const double*>(&wv[u][p][t]);
+                        mma_f64_8(c, ua[t][0], wd[0]);
+                        mma_f64_8(c, ua[t][1], wd[1]);
+                    }
+                    r0 = c[0], r1 = c[1];
+                } else {
+                    float c[4] = {};
+#pragma unroll
+                    for (int t = 0; t < JS; ++t) {
+                        const uint32_t* wr = reinterpret_cast<const uint32_t*>(&wv[u][p][t]);
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            const uint32_t a[4] = {ua[t][4 * m], ua[t][4 * m + 1], ua[t][4 * m + 2], ua[t][4 * m + 3]};
+                            if constexpr (E == 2) {
+                                mma16<T>(c, a, wr[2 * m], wr[2 * m + 1]);
+                            } else {
+                                const Tf32Pair b0 = tf32_split(__uint_as_float(wr[2 * m]));
+                                const Tf32Pair b1 = tf32_split(__uint_as_float(wr[2 * m + 1]));
+                                // Low parts meet high ones alone: an infinite middle is all in its low part.
+                                const uint32_t high[4] = {a[0], 0, a[2], 0};
+                                mma_tf32(c, high, b0.lo, b1.lo);
+                                mma_tf32(c, a, b0.hi, b1.hi);
+                            }
+                        }
+                    }
+                    r0 = (c[2] + c[0]) * back, r1 = (c[3] + c[1]) * back;
+                }
+                if (base) r0 += widen(v[2 * p]), r1 += widen(v[2 * p + 1]);
+                v[2 * p] = narrow<T>(r0), v[2 * p + 1] = narrow<T>(r1);
+            }
+            if (vec_y && avail >= V) {
+                *reinterpret_cast<uint4*>(y + col) = held[u];
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (e < avail) y[col + e] = v[e];
+            }
+        }
+    }
+}
+
+}  // namespace fpemu

@@ -23,10 +23,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kAdapterMaxRank = 128;
 constexpr int kSlotRows = 64;      // rows of one adapter that a slot of the plan holds
-constexpr int kFewRows = 256;      // up to here the kernels group the rows themselves
-constexpr int kAdapterThreads = 256;
-constexpr int kAdapterCluster = 8;
-constexpr int kGroupRows = 8;      // rows that share one read of a weight
+constexpr int kFewRows = 256;      // up to here the forward kernel groups the rows itself
 
 // Sums are held in float for 16- and 32-bit data and in double for float64.
 template <typename T>
@@ -167,158 +164,6 @@ __device__ void plain_row(const AdapterParams& P, int64_t row, bool bad, int64_t
     using Acc = typename AccOf<T>::type;
     for (int64_t c = n0 + threadIdx.x; c < n1; c += blockDim.x)
         y[c] = bad ? narrow<T>((Acc)__longlong_as_double(0x7ff8000000000000ll)) : base ? base[c] : narrow<T>((Acc)0);
-}
-
-// A cluster of kAdapterCluster blocks takes the rows of one slot (or, without a
-// plan, up to kGroupRows rows of one adapter, found by the row that leads them).
-// The blocks share the length k of the first product; their partial sums meet
-// through distributed shared memory in the blocks' order, and each block then
-// writes its own share of the n output columns.
-template <typename T, bool TR>
-__global__ void __launch_bounds__(kAdapterThreads) adapter_rows_kernel(AdapterParams P) {
-    using Acc = typename AccOf<T>::type;
-    constexpr int V = 16 / sizeof(T);
-    __shared__ Acc part[kGroupRows][kAdapterMaxRank];
-    __shared__ Acc us[kGroupRows][kAdapterMaxRank];
-    __shared__ Acc red[TR ? kGroupRows : 1][TR ? kAdapterThreads : 1];
-    __shared__ unsigned masks[kFewRows / 32];
-    __shared__ int list[kSlotRows];
-    cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int cr = (int)cluster.block_rank();
-    const int64_t unit = blockIdx.x / kAdapterCluster;
-    int cls, count;
-    if (P.plan) {
-        const AdapterSlot s = reinterpret_cast<const AdapterSlot*>(P.plan + plan_slot_word(P.adapters))[unit];
-        cls = s.cls, count = s.count;
-        if (count == 0) return;
-        if (tid < count) list[tid] = (P.plan + plan_perm_word(P.rows, P.adapters))[s.start + tid];
-    } else {
-        cls = row_class(P.index, P.index_wide, unit, P.adapters);
-        const bool same = tid < P.rows && row_class(P.index, P.index_wide, tid, P.adapters) == cls;
-        const unsigned m = __ballot_sync(0xffffffffu, same);
-        if (lane == 0) masks[warp] = m;
-        __syncthreads();
-        int rank = 0, before = 0, total = 0;  // of this unit's row; of this thread's row
-        for (int w = 0; w < kFewRows / 32; ++w) {
-            const int c = __popc(masks[w]);
-            if (w < (unit >> 5)) rank += c;
-            if (w < warp) before += c;
-            total += c;
-        }
-        rank += __popc(masks[unit >> 5] & ((1u << (unit & 31)) - 1));
-        if (rank % kGroupRows) return;  // another row leads this one
-        before += __popc(m & ((1u << lane) - 1));
-        if (same && before >= rank && before < rank + kGroupRows) list[before - rank] = tid;
-        count = total - rank < kGroupRows ? total - rank : kGroupRows;
-        if (cls == P.adapters + 1 && tid == 0 && cr == 0)
-            report_error(P.sink.dev, P.sink.host, FPEMU_ERR_INVALID, kWhereAdapterIndex, (int)unit);
-    }
-    __syncthreads();
-    const int64_t kshare = ((P.k + kAdapterCluster - 1) / kAdapterCluster + 7) / 8 * 8;
-    const int64_t nshare = ((P.n + kAdapterCluster - 1) / kAdapterCluster + 7) / 8 * 8;
-    const int64_t k0 = cr * kshare < P.k ? cr * kshare : P.k, k1 = k0 + kshare < P.k ? k0 + kshare : P.k;
-    const int64_t n0 = cr * nshare < P.n ? cr * nshare : P.n, n1 = n0 + nshare < P.n ? n0 + nshare : P.n;
-    if (cls >= P.adapters) {
-        for (int i = 0; i < count; ++i) plain_row<T>(P, list[i], cls != P.adapters, n0, n1);
-        return;
-    }
-    const T* w1 = static_cast<const T*>(P.w1) + cls * P.w1_adapter;
-    const T* w2 = static_cast<const T*>(P.w2) + cls * P.w2_adapter;
-    const T* x = static_cast<const T*>(P.x);
-    const Acc s = (Acc)(P.scales ? P.scales[cls] : P.scale);
-    const bool vec = (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w1)) % 16 == 0 &&
-                     (P.x_row * sizeof(T)) % 16 == 0 && (P.w1_row * sizeof(T)) % 16 == 0;
-    for (int first = 0; first < count; first += kGroupRows) {
-        const int g_n = count - first < kGroupRows ? count - first : kGroupRows;
-        const T* xr[kGroupRows];
-#pragma unroll
-        for (int g = 0; g < kGroupRows; ++g) xr[g] = x + (int64_t)list[first + (g < g_n ? g : 0)] * P.x_row;
-        if (!TR) {
-            for (int j = warp; j < P.r; j += kAdapterThreads / 32) {
-                const T* w = w1 + j * P.w1_row;
-                Acc acc[kGroupRows] = {};
-                if (vec) {
-                    int64_t c = k0 + lane * V;
-                    for (; c + V <= k1; c += 32 * V) {
-                        alignas(16) T wv[V], xv[V];
-                        *reinterpret_cast<uint4*>(wv) = *reinterpret_cast<const uint4*>(w + c);
-#pragma unroll
-                        for (int g = 0; g < kGroupRows; ++g)
-                            if (g < g_n) {
-                                *reinterpret_cast<uint4*>(xv) = *reinterpret_cast<const uint4*>(xr[g] + c);
-#pragma unroll
-                                for (int i = 0; i < V; ++i) acc[g] += widen(wv[i]) * widen(xv[i]);
-                            }
-                    }
-                    for (; c < k1; ++c)  // the lane that meets the end takes the last, short vector
-#pragma unroll
-                        for (int g = 0; g < kGroupRows; ++g)
-                            if (g < g_n) acc[g] += widen(w[c]) * widen(xr[g][c]);
-                } else {
-                    for (int64_t c = k0 + lane; c < k1; c += 32)
-#pragma unroll
-                        for (int g = 0; g < kGroupRows; ++g)
-                            if (g < g_n) acc[g] += widen(w[c]) * widen(xr[g][c]);
-                }
-#pragma unroll
-                for (int g = 0; g < kGroupRows; ++g) {
-                    if (g >= g_n) break;
-                    Acc v = acc[g];
-                    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                    if (lane == 0) part[g][j] = v;
-                }
-            }
-        } else {
-            int rp = 1;
-            while (rp < P.r) rp *= 2;
-            const int j = tid & (rp - 1), step = kAdapterThreads / rp;
-            Acc acc[kGroupRows] = {};
-            if (j < P.r)
-                for (int64_t c = k0 + tid / rp; c < k1; c += step) {
-                    const Acc wv = widen(w1[c * P.w1_row + j]);
-#pragma unroll
-                    for (int g = 0; g < kGroupRows; ++g)
-                        if (g < g_n) acc[g] += wv * widen(xr[g][c]);
-                }
-#pragma unroll
-            for (int g = 0; g < kGroupRows; ++g) red[g][tid] = acc[g];
-            __syncthreads();
-            for (int i = tid; i < g_n * P.r; i += kAdapterThreads) {
-                const int g = i / P.r, jj = i % P.r;
-                Acc v = 0;
-                for (int q = 0; q < step; ++q) v += red[g][q * rp + jj];
-                part[g][jj] = v;
-            }
-        }
-        cluster.sync();
-        for (int i = tid; i < g_n * P.r; i += kAdapterThreads) {
-            const int g = i / P.r, j = i % P.r;
-            Acc v = 0;
-            for (int b = 0; b < kAdapterCluster; ++b) v += *cluster.map_shared_rank(&part[g][j], b);
-            us[g][j] = v * s;
-            if (P.u && cr == 0) static_cast<Acc*>(P.u)[(int64_t)list[first + g] * P.u_row + j] = v * s;
-        }
-        cluster.sync();  // every block has read the partial sums
-        for (int64_t c = n0 + tid; c < n1; c += kAdapterThreads) {
-            Acc acc[kGroupRows] = {};
-            for (int j = 0; j < P.r; ++j) {
-                const Acc wv = widen(TR ? w2[j * P.w2_row + c] : w2[c * P.w2_row + j]);
-#pragma unroll
-                for (int g = 0; g < kGroupRows; ++g)
-                    if (g < g_n) acc[g] += wv * us[g][j];
-            }
-#pragma unroll
-            for (int g = 0; g < kGroupRows; ++g)
-                if (g < g_n) {
-                    const int64_t row = list[first + g];
-                    Acc v = acc[g];
-                    if (P.base) v += widen(static_cast<const T*>(P.base)[row * P.base_row + c]);
-                    static_cast<T*>(P.y)[row * P.y_row + c] = narrow<T>(v);
-                }
-        }
-        __syncthreads();  // `us` is rewritten by the next rows
-    }
 }
 
 }  // namespace fpemu

@@ -126,7 +126,7 @@ struct AdapterTile {
     static constexpr int kStage = kStageX + (kRankBytes > kLongBytes ? kRankBytes : kLongBytes);
     static constexpr int kStages = RP <= 32 ? 4 : 3;
     static constexpr int kPitchU = E == 2 ? RP + 8 : RP + 4;  // elements of Acc
-    static constexpr int kSmem = kStages * kStage + kSlotRows * kPitchU * (int)sizeof(Acc);
+    static constexpr int kSmem = kStages * kStage + 2 * kSlotRows * kPitchU * (int)sizeof(Acc);
     static constexpr int kBlocks = kSmem <= 57000 ? 4 : RP <= 32 && kSmem <= 76000 ? 3 : kSmem <= 114000 ? 2 : 1;  // per SM
     // The results of a warp's two rows are 16 bytes of neighbouring columns for each thread: column
     // q * V + 2 t + b of a group of 4 V stands where the instruction has column 2 q + b of its tile t.
@@ -158,6 +158,30 @@ __device__ void plain_rows(const AdapterParams& P, const int* list, int count, b
             c += vecs * V;
         }
         if (c < n1) plain_row<T>(P, row, bad, c, n1);
+    }
+}
+
+// Joins the blocks' parts of N sums: each block takes its share of them, adds
+// the parts in the blocks' order, and stores done(e, sum) to every block.  A
+// cluster barrier before makes the parts visible, one after the results; after
+// that no block reads or writes another's memory.
+template <int N, typename Acc, typename At, typename Done>
+__device__ __forceinline__ void join_parts(cg::cluster_group& cluster, int cr, int cs, Acc* part, Acc* out, At at,
+                                           Done done) {
+    for (int i = threadIdx.x; i < N / cs; i += blockDim.x) {
+        const int e = cr * (N / cs) + i, o = at(e);
+        Acc p[8];
+#pragma unroll
+        for (int b = 0; b < 8; ++b)  // all loads in flight before the first addition
+            if (b < cs) p[b] = *cluster.map_shared_rank(part + o, b);
+        Acc v = p[0];
+#pragma unroll
+        for (int b = 1; b < 8; ++b)
+            if (b < cs) v += p[b];
+        v = done(e, v);
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+            if (b < cs) *cluster.map_shared_rank(out + o, b) = v;
     }
 }
 
@@ -259,7 +283,8 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
         fetch_weights(second_long, st + Tile::kStageX, P.w2_row, nlen - c * KC, vec_w2);
     };
 
-    Acc* us = reinterpret_cast<Acc*>(smem + S * Tile::kStage);
+    Acc* part = reinterpret_cast<Acc*>(smem + S * Tile::kStage);  // this block's sums, read by the cluster
+    Acc* us = part + kSlotRows * Tile::kPitchU;                   // the cluster's sums
     Acc acc[HT][4] = {};
     // The middle as this thread's part of the left operand: 16-bit data split in
     // two and, for halves, scaled by a power of two per row; f32 and f64 plain.
@@ -269,44 +294,34 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
     const bool busy = rows0 < count;
 
     auto exchange = [&]() {
-        Acc* own = us + rows0 * Tile::kPitchU;
+        Acc* own = part + (rows0 + g) * Tile::kPitchU + half * HT * 8 + 2 * q;
 #pragma unroll
         for (int t = 0; t < HT; ++t) {
-            Acc* o = own + g * Tile::kPitchU + (half * HT + t) * 8 + 2 * q;
-            o[0] = acc[t][0], o[1] = acc[t][1];
-            o[8 * Tile::kPitchU] = acc[t][2], o[8 * Tile::kPitchU + 1] = acc[t][3];
+            own[t * 8] = acc[t][0], own[t * 8 + 1] = acc[t][1];
+            own[t * 8 + 8 * Tile::kPitchU] = acc[t][2], own[t * 8 + 8 * Tile::kPitchU + 1] = acc[t][3];
         }
         cluster.sync();
         const Acc s = (Acc)(P.scales ? P.scales[slot.cls] : P.scale);
-        // Sums of the blocks' parts in their order, in place of v; past the rank, where an infinite x
-        // met a zero, 0.
-        auto join = [&](auto& v, auto row_of, auto rank_of) {
-            constexpr int M = sizeof(v) / sizeof(v[0]), N = sizeof(v[0]) / sizeof(v[0][0]);
-            for (int b = 0; b < cs; ++b) {
-                const Acc* part = cluster.map_shared_rank(own, b);
-#pragma unroll
-                for (int t = 0; t < M; ++t)
-#pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const Acc p = part[row_of(e) * Tile::kPitchU + rank_of(t, e)];
-                        v[t][e] = b ? v[t][e] + p : p;
-                    }
-            }
-#pragma unroll
-            for (int t = 0; t < M; ++t)
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const int row = row_of(e), r = rank_of(t, e);
-                    v[t][e] = r < P.r ? v[t][e] * s : Acc(0);
-                    if (P.u && cr == 0 && half == 0 && r < P.r && rows0 + row < count)
-                        static_cast<Acc*>(P.u)[(int64_t)list[rows0 + row] * P.u_row + r] = v[t][e];
-                }
-        };
+        join_parts<kSlotRows * RP>(cluster, cr, cs, part, us, [](int e) { return e / RP * Tile::kPitchU + e % RP; },
+                                   [&](int e, Acc v) {
+            const int row = e / RP, r = e % RP;
+            v = r < P.r ? v * s : Acc(0);  // past the rank, an infinite x met a zero: NaN
+            if (P.u && r < P.r && row < count) static_cast<Acc*>(P.u)[(int64_t)list[row] * P.u_row + r] = v;
+            return v;
+        });
+        cluster.sync();
         if (busy) {
+            const Acc* from = us + (rows0 + g) * Tile::kPitchU;
             if constexpr (E == 2) {
                 float v[RP / 16][8];  // a0..a3 of two: rows g, g + 8, then columns + 8
-                join(v, [&](int e) { return g + (e >> 1 & 1) * 8; },
-                     [&](int t, int e) { return t * 16 + 2 * q + (e & 1) + (e >> 2) * 8; });
+#pragma unroll
+                for (int t = 0; t < RP / 16; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 f = *reinterpret_cast<const float2*>(
+                            from + (e & 1) * 8 * Tile::kPitchU + t * 16 + 2 * q + (e >> 1) * 8);
+                        v[t][2 * e] = f.x, v[t][2 * e + 1] = f.y;
+                    }
                 float down[2] = {1.f, 1.f};
                 if constexpr (std::is_same<T, __half>::value) {
                     float top[2] = {0.f, 0.f};
@@ -330,10 +345,13 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         split16<T>(v[t][2 * e] * down[e & 1], v[t][2 * e + 1] * down[e & 1], uh[t][e], ul[t][e]);
-            } else if constexpr (E == 4) {
-                join(uf, [&](int e) { return g + (e & 1) * 8; }, [&](int t, int e) { return t * 8 + q + (e >> 1) * 4; });
             } else {
-                join(uf, [&](int e) { return g + e * 8; }, [&](int t, int) { return t * 4 + q; });
+                constexpr int step = E == 4 ? 8 : 4;  // a0, a1 of rows g, g + 8; f32 two more, four columns on
+#pragma unroll
+                for (int t = 0; t < RP / step; ++t)
+#pragma unroll
+                    for (int e = 0; e < step / 2; ++e)
+                        uf[t][e] = from[(e & 1) * 8 * Tile::kPitchU + t * step + q + (e >> 1) * 4];
             }
         }
     };
@@ -552,7 +570,6 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
         if (busy) expand(smem + use, nlen - (c - nk) * KC);
         next(use);
     }
-    cluster.sync();  // no block leaves while another may read its partial sums
 }
 
 // Gradients of the factors: grad[i][j][c] = sum over the rows t of adapter i of

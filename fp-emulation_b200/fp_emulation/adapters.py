@@ -21,7 +21,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from fp_emulation import _lib
-from fp_emulation.ozaki import _after_call, _dtype_bits, _on, _require_cuda, _stream
+from fp_emulation.ozaki import _after_call, _dtype_bits, _on, _raw_stream, _require_cuda, _stream
 
 _DTYPE_CODE = {torch.float64: _lib.FPEMU_DT_F64, torch.float32: _lib.FPEMU_DT_F32,
                torch.float16: _lib.FPEMU_DT_F16, torch.bfloat16: _lib.FPEMU_DT_BF16}
@@ -93,7 +93,7 @@ def _launch(x, w1, w2, transposed, base, y, scale, index, plan, adapters, rank, 
             None if scale.__class__ is float else scale.data_ptr(), scale if scale.__class__ is float else 0.0,
             None if plan is not None else index.data_ptr(), 0 if plan is not None else index.element_size(),
             None if plan is None else plan.data_ptr(), None if u is None else u.data_ptr(),
-            torch.cuda.current_stream(d).cuda_stream)
+            _raw_stream(d))
     if st:
         _lib.check(st, "adapter_matmul")
     _after_call("adapter_matmul", dev)
@@ -132,7 +132,7 @@ class _AdapterMatmul(torch.autograd.Function):
             v = torch.empty_like(u)
             if need_x:
                 dx = torch.empty((x.shape[0], k), dtype=x.dtype, device=x.device)
-            _launch(dyc, B, A, 1, None, dx, scale, rows.index, _plan_of(rows), n_ad, rank, n, k if need_x else 0, v)
+            _launch(dyc, B, A, 1, None, dx, scale, rows.index, rows.plan, n_ad, rank, n, k if need_x else 0, v)
         if need_A or need_B:
             dA = torch.empty((n_ad, rank, k), dtype=A.dtype, device=A.device) if need_A else None
             dB = torch.empty((n_ad, n, rank), dtype=B.dtype, device=B.device) if need_B else None

@@ -16,7 +16,7 @@ import torch
 
 from fp_emulation import _lib
 from fp_emulation.adapters import _DTYPE_CODE
-from fp_emulation.ozaki import _after_call, _dtype_bits, _on, _require_cuda
+from fp_emulation.ozaki import _after_call, _dtype_bits, _on, _raw_stream, _require_cuda
 
 _NORMS = {1.0: 1, 2.0: 2, math.inf: 0}
 
@@ -85,7 +85,7 @@ def _run(src, dst, codes, norm_code, max_norm, what):
         st = lib.fpemu_clip_grads(n, ptrs.buffer_info()[0], None if outs is None else outs.buffer_info()[0],
                                   sizes.buffer_info()[0], kinds.buffer_info()[0], norm_code, max_norm,
                                   norm.data_ptr(), int(wide), ws.data_ptr(), ws.numel(),
-                                  torch.cuda.current_stream(dev.index).cuda_stream)
+                                  _raw_stream(dev.index))
     if st:
         _lib.check(st, what)
     _after_call(what, dev)

@@ -69,12 +69,15 @@ def _stream(device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+# torch's own query of the current stream's handle (torch.cuda.current_stream builds a Stream object
+# around it, 2 us a call).
+_raw_stream = torch._C._cuda_getCurrentRawStream
 _NO_CONTEXT = contextlib.nullcontext()
 
 
 def _on(index):
     """A context in which CUDA device `index` is current (free when it is already)."""
-    return _NO_CONTEXT if torch.cuda.current_device() == index else torch.cuda.device(index)
+    return _NO_CONTEXT if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
 def _require_cuda(*tensors):

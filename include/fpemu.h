@@ -228,7 +228,8 @@ int fpemu_adapter_plan(const void *index, int index_bytes, int64_t rows, int64_t
  * multiple of 4 apart -- double for FPEMU_DT_F64, else float; rows without an
  * adapter are not written.
  * y may be base itself; otherwise it overlaps no input.
- * plan NULL: rows <= FPEMU_ADAPTER_FEW_ROWS, grouped by the kernel from index. */
+ * plan NULL: rows <= FPEMU_ADAPTER_FEW_ROWS and not transposed, grouped by the
+ * kernel from index. */
 int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank,
                          int64_t adapters, const void *x, int64_t x_row, const void *w1,
                          int64_t w1_adapter, int64_t w1_row, const void *w2, int64_t w2_adapter,
