@@ -155,15 +155,4 @@ struct AdapterParams {
     ErrorSink sink;
 };
 
-// Rows without an adapter: base (or 0); rows with an id that is none: NaN, so
-// that a wrong index never looks like a result.
-template <typename T>
-__device__ void plain_row(const AdapterParams& P, int64_t row, bool bad, int64_t n0, int64_t n1) {
-    T* y = static_cast<T*>(P.y) + row * P.y_row;
-    const T* base = P.base ? static_cast<const T*>(P.base) + row * P.base_row : nullptr;
-    using Acc = typename AccOf<T>::type;
-    for (int64_t c = n0 + threadIdx.x; c < n1; c += blockDim.x)
-        y[c] = bad ? narrow<T>((Acc)__longlong_as_double(0x7ff8000000000000ll)) : base ? base[c] : narrow<T>((Acc)0);
-}
-
 }  // namespace fpemu

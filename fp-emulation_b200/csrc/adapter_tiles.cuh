@@ -29,15 +29,38 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// 16 bytes of a tile: `avail` elements from src, zeros after them.
+template <int B>
+__device__ __forceinline__ void copy_small(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(B), "r"(bytes) : "memory");
+}
+
+// How an operand's rows may be copied: 16 bytes at a time; 4 (floats and even
+// pairs of 16-bit values) or 8 (doubles); or, 0, 16-bit values at odd places, one
+// by one through registers.
 template <typename T>
-__device__ __forceinline__ void fetch16(uint8_t* dst, const T* src, int avail, bool vec) {
-    constexpr int V = 16 / sizeof(T);
-    if (vec) {
-        copy16(shared_address(dst), src, avail * (int)sizeof(T));  // src is not read where avail is 0
-    } else {
-#pragma unroll 1
-        for (int i = 0; i < V; ++i) reinterpret_cast<T*>(dst)[i] = i < avail ? src[i] : T(0.0f);
+__device__ __forceinline__ int copy_unit(const void* p, int64_t stride) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * (int64_t)sizeof(T));
+    return (a & 15) == 0 ? 16 : sizeof(T) >= 4 ? (int)sizeof(T) : (a & 3) == 0 ? 4 : 0;
+}
+
+// 16 bytes of a tile: `avail` elements from src, zeros after them.  What is not
+// available is not read.
+template <typename T>
+__device__ __forceinline__ void fetch16(uint8_t* dst, const T* src, int avail, int unit) {
+    constexpr int E = sizeof(T), V = 16 / E, B = E == 8 ? 8 : 4;
+    if (unit == 16) {
+        copy16(shared_address(dst), src, avail * E);
+    } else if (unit != 0) {
+#pragma unroll
+        for (int i = 0; i < 16 / B; ++i) {
+            const int left = avail * E - i * B;
+            copy_small<B>(shared_address(dst) + i * B, src + i * (B / E), left < 0 ? 0 : left < B ? left : B);
+        }
+    } else if (E == 2) {
+        alignas(16) T v[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = i < avail ? src[i] : T(0.0f);
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(v);
     }
 }
 
@@ -138,26 +161,40 @@ struct AdapterTile {
     }
 };
 
-// Rows without an adapter or with a bad id, this block's share of the columns.
+// Rows without an adapter (base, or 0) or with an id that is none (NaN, so that a
+// wrong index never looks like a result), this block's share of the columns.
 template <typename T>
-__device__ void plain_rows(const AdapterParams& P, const int* list, int count, bool bad, int64_t n0, int64_t n1) {
-    constexpr int V = 16 / sizeof(T);
-    if (!bad && P.base == P.y && P.base_row == P.y_row) return;
+__device__ void plain_rows(const AdapterParams& P, const int* list, int count, bool bad, int n0, int n1) {
+    using Acc = typename AccOf<T>::type;
+    constexpr int V = 16 / (int)sizeof(T);
+    if ((!bad && P.base == P.y && P.base_row == P.y_row) || n1 <= n0) return;
     const T* base = static_cast<const T*>(P.base);
     T* y = static_cast<T*>(P.y);
-    const bool vec = !bad && ((reinterpret_cast<uintptr_t>(base) | reinterpret_cast<uintptr_t>(y)) & 15) == 0 &&
-                     (P.base_row * sizeof(T)) % 16 == 0 && (P.y_row * sizeof(T)) % 16 == 0;
-    for (int i = 0; i < count; ++i) {
-        const int64_t row = list[i];
-        int64_t c = n0;
-        if (vec) {
-            const int64_t vecs = (n1 - n0) / V;
-            for (int64_t v = threadIdx.x; v < vecs; v += blockDim.x)
-                *reinterpret_cast<uint4*>(y + row * P.y_row + n0 + v * V) =
-                    base ? *reinterpret_cast<const uint4*>(base + row * P.base_row + n0 + v * V) : uint4{0, 0, 0, 0};
-            c += vecs * V;
-        }
-        if (c < n1) plain_row<T>(P, row, bad, c, n1);
+    const T fill = narrow<T>(bad ? (Acc)__longlong_as_double(0x7ff8000000000000ll) : (Acc)0);
+    const bool vec = !bad && base && copy_unit<T>(base, P.base_row) == 16 && copy_unit<T>(y, P.y_row) == 16;
+    const int warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32, len = n1 - n0;
+    const int whole = vec ? len / V * V : 0;  // of a row, copied 16 bytes at a time
+    for (int first = warp; first < count; first += 8 * warps) {
+        // Eight rows of a warp with their loads in flight together.
+        auto columns = [&](auto unit, int from, int to, int step) {
+            using U = decltype(unit);
+            for (int c = from; c < to; c += step) {
+                U v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int t = first + i * warps;
+                    if (t < count && !bad && base) v[i] = *reinterpret_cast<const U*>(base + list[t] * P.base_row + n0 + c);
+                    else if constexpr (std::is_same<U, T>::value) v[i] = fill;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int t = first + i * warps;
+                    if (t < count) *reinterpret_cast<U*>(y + list[t] * P.y_row + n0 + c) = v[i];
+                }
+            }
+        };
+        columns(uint4{}, lane * V, whole, 32 * V);
+        columns(T(0.0f), whole + lane, len, 32);
     }
 }
 
@@ -223,16 +260,13 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
     const T* w2 = static_cast<const T*>(P.w2) + slot.cls * P.w2_adapter;
     const T* x = static_cast<const T*>(P.x);
     const T* base = static_cast<const T*>(P.base);
-    auto aligned = [](const void* p, int64_t stride) {
-        return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * E)) & 15) == 0;
-    };
-    const bool vec_x = aligned(x, P.x_row), vec_w1 = aligned(w1, P.w1_row), vec_w2 = aligned(w2, P.w2_row);
-    const bool vec_base = aligned(base, P.base_row), vec_y = aligned(P.y, P.y_row);
+    const int vec_x = copy_unit<T>(x, P.x_row), vec_w1 = copy_unit<T>(w1, P.w1_row), vec_w2 = copy_unit<T>(w2, P.w2_row);
+    const int vec_base = copy_unit<T>(base, P.base_row);
+    const bool vec_y = copy_unit<T>(P.y, P.y_row) == 16;
 
     auto clamp = [](int v) { return v < 0 ? 0 : v > V ? V : v; };
     // This thread's 16-byte units of a tile: one of rows tid / 8 and tid / 8 + 32, and NW of the weights,
-    // UPR units along and SKIP rows apart.  The pointers advance from chunk to chunk; whole chunks of
-    // aligned operands are copied as they are, others element by element where they must.
+    // UPR units along and SKIP rows apart.  The pointers advance from chunk to chunk.
     constexpr int NW = (RP + 31) / 32;
     const int unit = tid % 8 * V;
     const T *rp[2], *wp;
@@ -240,7 +274,7 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
 #pragma unroll
         for (int i = 0; i < 2; ++i) rp[i] = src + list[tid / 8 + 32 * i] * stride + c0 + unit;
     };
-    auto fetch_weights = [&](auto by_long, uint8_t* wt, int64_t stride, int left, bool vec) {
+    auto fetch_weights = [&](auto by_long, uint8_t* wt, int64_t stride, int left, int vec) {
         constexpr bool LONG = decltype(by_long)::value, PLACED = LONG && !TR;  // the second product's
         constexpr int UPR = LONG ? RP * E / 16 : 8, SKIP = kTileThreads / UPR;
         const int l = tid / UPR, j = tid % UPR * V;
@@ -262,7 +296,7 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
     };
     constexpr std::integral_constant<bool, TR> first_long{};
     constexpr std::integral_constant<bool, !TR> second_long{};
-    auto fetch_rows = [&](uint8_t* st, int left, bool vec) {
+    auto fetch_rows = [&](uint8_t* st, int left, int vec) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             fetch16(st + (tid / 8 + i * 32) * Tile::kPitchX + tid % 8 * 16, rp[i],
@@ -528,16 +562,24 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
                         v[2 * p + b] = narrow<T>(base ? a + (Acc)widen(v[2 * p + b]) : a);
                     }
             }
-            if (rows0 + g + h * 8 < count) {
-                if (vec_y && left >= KC) {
-                    *reinterpret_cast<uint4*>(yp[h]) = *reinterpret_cast<uint4*>(v);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (e + col0 < left) yp[h][e] = v[e];
-                }
+            if (vec_y && left >= KC) {
+                if (rows0 + g + h * 8 < count) *reinterpret_cast<uint4*>(yp[h]) = *reinterpret_cast<uint4*>(v);
+            } else {
+                *reinterpret_cast<uint4*>(st + (rows0 + g + h * 8) * Tile::kPitchX + half * 64 + q * 16) =
+                    *reinterpret_cast<uint4*>(v);
             }
             yp[h] += KC;
+        }
+        if (!vec_y || left < KC) {  // element by element, neighbouring lanes on neighbouring columns
+            constexpr int H = KC / 2;
+            __syncwarp();
+#pragma unroll 4
+            for (int i = lane; i < 16 * H; i += 32) {
+                const int row = rows0 + i / H, c = half * H + i % H;
+                if (row < count && c < left)
+                    static_cast<T*>(P.y)[list[row] * P.y_row + n0 + nlen - left + c] =
+                        *reinterpret_cast<const T*>(st + row * Tile::kPitchX + c * E);
+            }
         }
     };
 
@@ -633,7 +675,7 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
     const int chunks = (t1 - t0 + KT - 1) / KT;
     const T* qs = static_cast<const T*>(side.q);
     const Acc* ps = static_cast<const Acc*>(side.p);
-    const bool vec = ((reinterpret_cast<uintptr_t>(qs) | (uintptr_t)(side.q_row * E)) & 15) == 0;
+    const int vec = copy_unit<T>(qs, side.q_row);
 
     // Row ids of a thread's copies, one chunk ahead of the copies themselves.
     constexpr int QU = COLS / V, QI = KT * QU / kGradThreads;          // 16-byte units of a q row; copies a thread
@@ -665,7 +707,7 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
             const int u = tid + i * kGradThreads, j = u % PU * PV;
             const int avail = p_id[i] < 0 || j >= P.p_row ? 0 : PV;  // p_row is a multiple of PV
             fetch16(st + KT * Tile::kPitchQ + u / PU * Tile::kPitchP + u % PU * 16,
-                    ps + (int64_t)p_id[i] * P.p_row + j, avail, true);
+                    ps + (int64_t)p_id[i] * P.p_row + j, avail, 16);
         }
     };
 
