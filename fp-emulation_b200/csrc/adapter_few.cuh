@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kFewThreads) adapter_few_kernel(const __grid_c
     join_parts<RP * kGroupRows>(cluster, cr, cs, part, us, [](int e) { return e; }, [&](int e, Acc v) {
         const int j = e / kGroupRows, r = e % kGroupRows;
         v = j < P.r ? v * s : Acc(0);
-        if (P.u && j < P.r && r < count) static_cast<Acc*>(P.u)[(int64_t)list[r] * P.u_row + j] = v;
+        if (P.u && j < P.r && r < count) static_cast<typename MiddleOf<T>::type*>(P.u)[(int64_t)list[r] * P.u_row + j] = MiddleOf<T>::pack(v);
         return v;
     });
     cluster.sync();

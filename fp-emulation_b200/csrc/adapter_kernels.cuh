@@ -150,7 +150,7 @@ struct AdapterParams {
     const void* index;
     int index_wide;
     const int32_t* plan;  // null: the kernel groups the (few) rows itself
-    void* u;              // [rows, u_row] of the sums' type, or null
+    void* u;              // [rows, u_row], kept for the gradients, or null
     int u_row;
     ErrorSink sink;
 };

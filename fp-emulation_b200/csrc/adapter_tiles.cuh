@@ -130,6 +130,24 @@ __device__ __forceinline__ void split16(float x, float y, uint32_t& hi, uint32_t
     }
 }
 
+// How u and v are kept for the gradients: as they are, or, for bfloat16 data, as
+// the two parts that the products use (high in the upper half of the word), which
+// saves every block of the gradient kernel the splitting.
+template <typename T>
+struct MiddleOf {
+    using type = typename AccOf<T>::type;
+    static __device__ __forceinline__ type pack(type v) { return v; }
+};
+template <>
+struct MiddleOf<__nv_bfloat16> {
+    using type = uint32_t;
+    static __device__ __forceinline__ uint32_t pack(float v) {
+        uint32_t hi, lo;
+        split16<__nv_bfloat16>(v, 0.f, hi, lo);
+        return hi << 16 | (lo & 0xffffu);
+    }
+};
+
 // Tiles in shared memory.  "Rank-major" weights have a row for each rank and
 // 128 bytes along the long dimension, "long-major" ones a row for each of its
 // elements and the rank along it.  The pitches keep the warps' fragment loads
@@ -340,7 +358,7 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
                                    [&](int e, Acc v) {
             const int row = e / RP, r = e % RP;
             v = r < P.r ? v * s : Acc(0);  // past the rank, an infinite x met a zero: NaN
-            if (P.u && r < P.r && row < count) static_cast<Acc*>(P.u)[(int64_t)list[row] * P.u_row + r] = v;
+            if (P.u && r < P.r && row < count) static_cast<typename MiddleOf<T>::type*>(P.u)[(int64_t)list[row] * P.u_row + r] = MiddleOf<T>::pack(v);
             return v;
         });
         cluster.sync();
@@ -677,37 +695,32 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
     const Acc* ps = static_cast<const Acc*>(side.p);
     const int vec = copy_unit<T>(qs, side.q_row);
 
-    // Row ids of a thread's copies, one chunk ahead of the copies themselves.
-    constexpr int QU = COLS / V, QI = KT * QU / kGradThreads;          // 16-byte units of a q row; copies a thread
-    constexpr int PV = 16 / (int)sizeof(Acc), PU = RP / PV, PI = KT * PU / kGradThreads;
-    int q_id[QI], p_id[PI];
+    // A thread's copies of a chunk: 16 bytes of QI rows of q, 16 of PI rows of p, each at one place along
+    // the row.  Every warp reads the chunk's row ids, one chunk ahead of the copies that need them.
+    constexpr int QU = COLS / V, QI = KT * QU / kGradThreads, QS = kGradThreads / QU;
+    constexpr int PV = 16 / (int)sizeof(Acc), PU = RP / PV, PI = KT * PU / kGradThreads, PS = kGradThreads / PU;
+    const int64_t col = c0 + tid % QU * V, cols_left = side.cols - col;
+    const int q_avail = cols_left < 0 ? 0 : cols_left > V ? V : (int)cols_left;
+    const int p_bytes = tid % PU * PV < P.p_row ? 16 : 0;  // p_row is a multiple of PV
+    const Acc* pc = ps + tid % PU * PV;
+    int id = 0;
     auto ids = [&](int c) {
-#pragma unroll
-        for (int i = 0; i < QI; ++i) {
-            const int t = t0 + c * KT + (tid + i * kGradThreads) / QU;
-            q_id[i] = t < t1 ? perm[t] : -1;
-        }
-#pragma unroll
-        for (int i = 0; i < PI; ++i) {
-            const int t = t0 + c * KT + (tid + i * kGradThreads) / PU;
-            p_id[i] = t < t1 ? perm[t] : -1;
-        }
+        const int t = t0 + c * KT + lane;
+        id = lane < KT && t < t1 ? perm[t] : -1;
     };
     auto fetch = [&](int c) {
         uint8_t* st = smem + c % S * Tile::kStage;
 #pragma unroll
         for (int i = 0; i < QI; ++i) {
-            const int u = tid + i * kGradThreads;
-            const int64_t col = c0 + u % QU * V, left = side.cols - col;
-            const int avail = q_id[i] < 0 || left < 0 ? 0 : left > V ? V : (int)left;
-            fetch16(st + u / QU * Tile::kPitchQ + u % QU * 16, qs + q_id[i] * side.q_row + col, avail, vec);
+            const int r = __shfl_sync(0xffffffffu, id, tid / QU + i * QS);
+            fetch16(st + (tid / QU + i * QS) * Tile::kPitchQ + tid % QU * 16, qs + r * side.q_row + col,
+                    r < 0 ? 0 : q_avail, vec);
         }
 #pragma unroll
         for (int i = 0; i < PI; ++i) {
-            const int u = tid + i * kGradThreads, j = u % PU * PV;
-            const int avail = p_id[i] < 0 || j >= P.p_row ? 0 : PV;  // p_row is a multiple of PV
-            fetch16(st + KT * Tile::kPitchQ + u / PU * Tile::kPitchP + u % PU * 16,
-                    ps + (int64_t)p_id[i] * P.p_row + j, avail, 16);
+            const int r = __shfl_sync(0xffffffffu, id, tid / PU + i * PS);
+            copy16(shared_address(st + KT * Tile::kPitchQ + (tid / PU + i * PS) * Tile::kPitchP + tid % PU * 16),
+                   pc + (int64_t)r * P.p_row, r < 0 ? 0 : p_bytes);
         }
     };
 
@@ -735,46 +748,51 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
                 uint32_t a[MT][4];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) ldsm4t(a[m], qa + ks * 16 * Tile::kPitchQ + m * 32);
-                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                // Two 8-rank tiles at a time: rank 2 n + t of 16 stands where the instruction has column n of
+                // tile t, so that one 8-byte load serves both.
 #pragma unroll
-                    for (int t = 0; t < RP / 8; ++t) {
-                        uint32_t hi[2], lo[2];
+                for (int t = 0; t < RP / 16; ++t) {
+                    uint2 w[2][2];  // rows 2 q, 2 q + 1, then 8 on; .x for tile 2 t, .y for 2 t + 1
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int row = ks * 16 + 2 * q + e * 8, j = t * 8 + g;
-                            split16<T>(p_at(row, j), p_at(row + 1, j), hi[e], lo[e]);
-                        }
+                    for (int e = 0; e < 4; ++e)
+                        w[e >> 1][e & 1] = *reinterpret_cast<const uint2*>(
+                            pt + (ks * 16 + 2 * q + (e >> 1) * 8 + (e & 1)) * Tile::kPitchP + (t * 16 + 2 * g) * 4);
+                    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            mma16<T>(sum[m][t], a[m], lo[0], lo[1]);
-                            mma16<T>(sum[m][t], a[m], hi[0], hi[1]);
-                        }
-                    }
-                } else {
-                    // A half is a tf32 value as it is; the middle, whose range is a float's, is split
-                    // in two.  The order of rows within the sum is free: rows 2q and 2q + 1 stand
-                    // where the instruction has q and q + 4.
-                    uint32_t w[MT][2][4];
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t hi[2], lo[2];
 #pragma unroll
-                    for (int m = 0; m < MT; ++m)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[m][e]));
-                            w[m][e >> 1][e & 1] = __float_as_uint(f.x);
-                            w[m][e >> 1][(e & 1) + 2] = __float_as_uint(f.y);
-                        }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int t = 0; t < RP / 8; ++t) {
-                            const int row = ks * 16 + h * 8 + 2 * q, j = t * 8 + g;
-                            const Tf32Pair b0 = tf32_split(p_at(row, j)), b1 = tf32_split(p_at(row + 1, j));
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t a = h ? w[e][0].y : w[e][0].x, b = h ? w[e][1].y : w[e][1].x;
+                                hi[e] = __byte_perm(a, b, 0x7632), lo[e] = __byte_perm(a, b, 0x5410);
+                            }
 #pragma unroll
                             for (int m = 0; m < MT; ++m) {
-                                mma_tf32(sum[m][t], w[m][h], b0.lo, b1.lo);
-                                mma_tf32(sum[m][t], w[m][h], b0.hi, b1.hi);
+                                mma16<T>(sum[m][2 * t + h], a[m], lo[0], lo[1]);
+                                mma16<T>(sum[m][2 * t + h], a[m], hi[0], hi[1]);
                             }
                         }
+                    } else {
+                        // A half is a tf32 value as it is; the middle, whose range is a float's, is split in two.
+                        // The order of rows within the sum is free: rows 2q and 2q + 1 stand where the
+                        // instruction has q and q + 4.
+#pragma unroll
+                        for (int k8 = 0; k8 < 2; ++k8)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const Tf32Pair b0 = tf32_split(__uint_as_float(h ? w[k8][0].y : w[k8][0].x));
+                                const Tf32Pair b1 = tf32_split(__uint_as_float(h ? w[k8][1].y : w[k8][1].x));
+#pragma unroll
+                                for (int m = 0; m < MT; ++m) {
+                                    const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&a[m][2 * k8]));
+                                    const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&a[m][2 * k8 + 1]));
+                                    const uint32_t x[4] = {__float_as_uint(f0.x), __float_as_uint(f1.x),
+                                                           __float_as_uint(f0.y), __float_as_uint(f1.y)};
+                                    mma_tf32(sum[m][2 * t + h], x, b0.lo, b1.lo);
+                                    mma_tf32(sum[m][2 * t + h], x, b0.hi, b1.hi);
+                                }
+                            }
+                    }
                 }
             }
         } else if constexpr (E == 4) {
@@ -837,7 +855,8 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
         for (int t = 0; t < RP / 8; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                mine[((warp * MT + m) * 16 + g + (e >> 1) * 8) * Tile::kPitchD + t * 8 + 2 * q + (e & 1)] = acc[m][t][e];
+                mine[((warp * MT + m) * 16 + g + (e >> 1) * 8) * Tile::kPitchD +
+                     (E == 2 ? t / 2 * 16 + 2 * (2 * q + (e & 1)) + t % 2 : t * 8 + 2 * q + (e & 1))] = acc[m][t][e];
     cluster.sync();
     const Acc* parts[8];
 #pragma unroll

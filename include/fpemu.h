@@ -225,8 +225,9 @@ int fpemu_adapter_plan(const void *index, int index_bytes, int64_t rows, int64_t
  *                 (its gradient by x: x = dy, w1 = B, w2 = A).
  * scales: one double per adapter, or NULL for `scale` everywhere.
  * u (or NULL): rows of `rank` values s_i W1_i x[t], each row rank rounded up to a
- * multiple of 4 apart -- double for FPEMU_DT_F64, else float; rows without an
- * adapter are not written.
+ * multiple of 4 apart, for fpemu_adapter_grads -- doubles for FPEMU_DT_F64, floats,
+ * or for FPEMU_DT_BF16 the float cut into two bfloat16 parts; rows without an adapter
+ * are not written.
  * y may be base itself; otherwise it overlaps no input.
  * plan NULL: rows <= FPEMU_ADAPTER_FEW_ROWS and not transposed, grouped by the
  * kernel from index. */
