@@ -73,37 +73,43 @@ int launch_few(const AdapterParams& P, const DevInfo& d, cudaStream_t st) {
     return launch_few_rank<T, 128>(P, d, st);
 }
 
+int padded_rank(int64_t r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128; }
+
+constexpr int kMostBlocks = 3;  // of a tile kernel on an SM
+
 template <typename T, bool TR, int RP>
-int launch_tiles_rank(const AdapterParams& P, const DevInfo& d, cudaStream_t st) {
-    auto kern = adapter_tile_kernel<T, TR, RP>;
+int launch_tiles_rank(AdapterParams& P, const DevInfo& d, cudaStream_t st) {
     using Tile = AdapterTile<T, TR, RP>;
-    FPEMU_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem));
+    static_assert(Tile::kBlocks <= kMostBlocks, "the workspace holds a part of every block");
+    auto shrink = adapter_shrink_kernel<T, TR, RP>;
+    auto expand = adapter_expand_kernel<T, TR, RP>;
+    FPEMU_CUDA(cudaFuncSetAttribute(shrink, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem));
+    FPEMU_CUDA(cudaFuncSetAttribute(expand, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem));
     const int64_t slots = plan_slots(P.rows, P.adapters);
-    // Blocks for a slot: enough slots fill the device by themselves and pay for no exchange between
-    // blocks; few are split.  Measured (1 / 2 / 4 / 8 blocks, us): 256 slots of 4096 x 8192 half rank 64
-    // 199 / 212 / 223 / 265; 78 slots of 1000 x 777 float 74 / 41 / 33 / 46; 24 of 4096 x 4096 double
-    // - / 114 / 59 / 35.
-    const int64_t filled = P.rows / kSlotRows + std::min<int64_t>(P.adapters, P.rows) / 2;
-    int cluster = 1;
-    while (cluster < 8 && filled * cluster < d.sms * 4 / 3) cluster *= 2;
+    auto grid = [&](int64_t length) {
+        const int64_t chunks = std::max<int64_t>((length + Tile::KC - 1) / Tile::KC, 1);
+        return (int)std::min<int64_t>((int64_t)d.sms * Tile::kBlocks, slots * chunks);
+    };
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(slots * cluster));
     cfg.blockDim = dim3(kTileThreads);
     cfg.dynamicSmemBytes = Tile::kSmem;
     cfg.stream = st;
+    P.shrink_grid = grid(P.k);
+    cfg.gridDim = dim3((unsigned)P.shrink_grid);
+    if (P.k > 0) FPEMU_CUDA(cudaLaunchKernelEx(&cfg, shrink, P));
+    // The second kernel's blocks start as the first one's end, and wait for it before they read u.
     cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = cluster;
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    FPEMU_CUDA(cudaLaunchKernelEx(&cfg, kern, P));
+    cfg.numAttrs = P.k > 0 ? 1 : 0;
+    cfg.gridDim = dim3((unsigned)grid(P.n));
+    FPEMU_CUDA(cudaLaunchKernelEx(&cfg, expand, P));
     return FPEMU_OK;
 }
 
 template <typename T, bool TR>
-int launch_tiles(const AdapterParams& P, const DevInfo& d, cudaStream_t st) {
+int launch_tiles(AdapterParams& P, const DevInfo& d, cudaStream_t st) {
     if (P.r <= 16) return launch_tiles_rank<T, TR, 16>(P, d, st);
     if (P.r <= 32) return launch_tiles_rank<T, TR, 32>(P, d, st);
     if (P.r <= 64) return launch_tiles_rank<T, TR, 64>(P, d, st);
@@ -183,14 +189,27 @@ int fpemu_adapter_plan(const void* index, int index_bytes, int64_t rows, int64_t
     adapter_plan_kernel<<<(unsigned)(adapters + 2), 1024, 0, static_cast<cudaStream_t>(stream)>>>(
         index, index_bytes == 8, rows, (int)adapters, static_cast<int32_t*>(plan), sink);
     FPEMU_CUDA(cudaGetLastError());
+    adapter_pack_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(rows, (int)adapters,
+                                                                            static_cast<int32_t*>(plan));
+    FPEMU_CUDA(cudaGetLastError());
     return FPEMU_OK;
+}
+
+size_t fpemu_adapter_workspace_size(int dtype, int64_t rows, int64_t rank, int64_t adapters) {
+    DevInfo d;
+    if (check_sizes("adapter_workspace_size", dtype, rows, 0, 0, rank, adapters) != FPEMU_OK || device_info(&d) != FPEMU_OK)
+        return 0;
+    // A part for every block of the first kernel and every slot, one of which begins or ends with each.
+    return (size_t)(plan_slots(rows, adapters) + (int64_t)d.sms * kMostBlocks) * kSlotRows * padded_rank(rank) *
+           (dtype == FPEMU_DT_F64 ? 8 : 4);
 }
 
 int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters,
                          const void* x, int64_t x_row, const void* w1, int64_t w1_adapter, int64_t w1_row,
                          const void* w2, int64_t w2_adapter, int64_t w2_row, int transposed, const void* base,
                          int64_t base_row, void* y, int64_t y_row, const double* scales, double scale,
-                         const void* index, int index_bytes, const void* plan, void* u, void* stream) {
+                         const void* index, int index_bytes, const void* plan, void* u, void* workspace,
+                         size_t workspace_bytes, void* stream) {
     DevInfo d;
     FPEMU_TRY(check_sizes("adapter_matmul", dtype, rows, k, n, rank, adapters));
     if (rows == 0) return FPEMU_OK;
@@ -203,6 +222,10 @@ int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t 
         return fail(FPEMU_ERR_INVALID, "adapter_matmul: %lld rows%s need a plan, few rows an index of 4 or 8 bytes",
                     (long long)rows, transposed ? ", transposed," : "");
     FPEMU_TRY(device_info(&d));
+    if (plan != nullptr && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
+                            workspace_bytes < fpemu_adapter_workspace_size(dtype, rows, rank, adapters)))
+        return fail(FPEMU_ERR_WORKSPACE, "adapter_matmul: need %zu bytes of 16-byte aligned workspace, got %zu",
+                    fpemu_adapter_workspace_size(dtype, rows, rank, adapters), workspace_bytes);
     AdapterParams P = {};
     P.rows = rows, P.k = k, P.n = n, P.r = (int)rank, P.adapters = (int)adapters;
     P.x = x, P.x_row = x_row;
@@ -211,7 +234,7 @@ int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t 
     P.base = base, P.base_row = base_row, P.y = y, P.y_row = y_row;
     P.scales = scales, P.scale = scale;
     P.index = index, P.index_wide = index_bytes == 8, P.plan = static_cast<const int32_t*>(plan);
-    P.u = u, P.u_row = middle_row((int)rank);
+    P.u = u, P.u_row = middle_row((int)rank), P.parts = workspace;
     FPEMU_TRY(error_sink(&P.sink));
     return with_type(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;

@@ -33,6 +33,30 @@ __device__ __forceinline__ uint4 load16(const T* p, int avail, bool vec) {
     return *reinterpret_cast<uint4*>(v);
 }
 
+// Joins the blocks' parts of N sums: each block takes its share of them, adds
+// the parts in the blocks' order, and stores done(e, sum) to every block.  A
+// cluster barrier before makes the parts visible, one after the results; after
+// that no block reads or writes another's memory.
+template <int N, typename Acc, typename At, typename Done>
+__device__ __forceinline__ void join_parts(cg::cluster_group& cluster, int cr, int cs, Acc* part, Acc* out, At at,
+                                           Done done) {
+    for (int i = threadIdx.x; i < N / cs; i += blockDim.x) {
+        const int e = cr * (N / cs) + i, o = at(e);
+        Acc p[8];
+#pragma unroll
+        for (int b = 0; b < 8; ++b)  // all loads in flight before the first addition
+            if (b < cs) p[b] = *cluster.map_shared_rank(part + o, b);
+        Acc v = p[0];
+#pragma unroll
+        for (int b = 1; b < 8; ++b)
+            if (b < cs) v += p[b];
+        v = done(e, v);
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+            if (b < cs) *cluster.map_shared_rank(out + o, b) = v;
+    }
+}
+
 template <typename T, int RP>
 struct FewTile {
     using Acc = typename AccOf<T>::type;
@@ -226,7 +250,7 @@ __global__ void __launch_bounds__(kFewThreads) adapter_few_kernel(const __grid_c
                 split16<T>(at(2 * i) * down, at(2 * i + 1) * down, ua[t][2 * i], ua[t][2 * i + 1]);
         }
     }
-    constexpr int NT = V / 2;  // 8-column tiles of a group of KS columns, laid out as in AdapterTile::place
+    constexpr int NT = V / 2;  // 8-column tiles of a group of KS columns, laid out as in AdapterTile::at
     constexpr int UG = Tile::UG;
     for (int first = n0 + warp * KS; first < n1; first += W * KS * UG) {
         uint4 wv[UG][NT][JS], held[UG];

@@ -58,16 +58,25 @@ struct AdapterSlot {
 };
 
 // The plan: int32 words [0, adapters + 3) are the first position of each class
-// in `perm` (classes in order; the last word is the number of rows), then the
-// slots (16-byte aligned), then perm, the rows sorted by class and in their own
-// order within one.  A class's slots begin at start/kSlotRows + class: ranges of
-// two classes never meet because ceil(c/S) <= (start + c)/S - start/S + 1.
+// in `perm` (classes in order; the last word is the number of rows); then
+// (16-byte aligned) the classes' slots, in which a class begins at
+// start/kSlotRows + class -- ranges of two classes never meet because
+// ceil(c/S) <= (start + c)/S - start/S + 1 -- and some stay empty; then the slots
+// that hold rows, those of adapters from the front and the others from the back,
+// and how many there are of each; then perm, the rows sorted by class and in their
+// own order within one.
 __host__ __device__ __forceinline__ int64_t plan_slots(int64_t rows, int64_t adapters) {
     return rows / kSlotRows + adapters + 2;
 }
 __host__ __device__ __forceinline__ int64_t plan_slot_word(int64_t adapters) { return (adapters + 3 + 3) / 4 * 4; }
-__host__ __device__ __forceinline__ int64_t plan_perm_word(int64_t rows, int64_t adapters) {
+__host__ __device__ __forceinline__ int64_t plan_busy_word(int64_t rows, int64_t adapters) {
     return plan_slot_word(adapters) + 4 * plan_slots(rows, adapters);
+}
+__host__ __device__ __forceinline__ int64_t plan_header_word(int64_t rows, int64_t adapters) {
+    return plan_busy_word(rows, adapters) + 4 * plan_slots(rows, adapters);
+}
+__host__ __device__ __forceinline__ int64_t plan_perm_word(int64_t rows, int64_t adapters) {
+    return plan_header_word(rows, adapters) + 4;
 }
 __host__ __device__ __forceinline__ int64_t plan_words(int64_t rows, int64_t adapters) {
     return plan_perm_word(rows, adapters) + rows;
@@ -132,6 +141,39 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const void* index, i
     }
 }
 
+// The slots that hold rows, one block.
+__global__ void __launch_bounds__(1024) adapter_pack_kernel(int64_t rows, int adapters, int32_t* plan) {
+    __shared__ int counts[2][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t slots = plan_slots(rows, adapters);
+    const AdapterSlot* from = reinterpret_cast<const AdapterSlot*>(plan + plan_slot_word(adapters));
+    AdapterSlot* to = reinterpret_cast<AdapterSlot*>(plan + plan_busy_word(rows, adapters));
+    int done[2] = {0, 0};  // adapters' slots, others
+    for (int64_t first = 0; first < slots; first += 1024) {
+        const int64_t i = first + threadIdx.x;
+        const AdapterSlot s = i < slots ? from[i] : AdapterSlot{0, 0, 0, 0};
+        const bool kind[2] = {s.count > 0 && s.cls < adapters, s.count > 0 && s.cls >= adapters};
+        unsigned m[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            m[h] = __ballot_sync(0xffffffffu, kind[h]);
+            if (lane == 0) counts[h][warp] = __popc(m[h]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            int at = done[h] + __popc(m[h] & ((1u << lane) - 1));
+            for (int w = 0; w < 32; ++w) {
+                if (w < warp) at += counts[h][w];
+                done[h] += counts[h][w];
+            }
+            if (kind[h]) to[h ? slots - 1 - at : at] = s;
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x < 2) plan[plan_header_word(rows, adapters) + threadIdx.x] = done[threadIdx.x];
+}
+
 struct AdapterParams {
     int64_t rows, k, n;
     int r, adapters;
@@ -152,7 +194,16 @@ struct AdapterParams {
     const int32_t* plan;  // null: the kernel groups the (few) rows itself
     void* u;              // [rows, u_row], kept for the gradients, or null
     int u_row;
+    void* parts;          // with a plan: the first product's partial sums
+    int shrink_grid;      // blocks that leave them
     ErrorSink sink;
 };
+
+__device__ __forceinline__ const AdapterSlot* plan_busy(const AdapterParams& P) {
+    return reinterpret_cast<const AdapterSlot*>(P.plan + plan_busy_word(P.rows, P.adapters));
+}
+__device__ __forceinline__ const int32_t* plan_perm(const AdapterParams& P) {
+    return P.plan + plan_perm_word(P.rows, P.adapters);
+}
 
 }  // namespace fpemu

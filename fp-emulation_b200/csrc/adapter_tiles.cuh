@@ -1,11 +1,13 @@
 // adapter_tiles.cuh -- the adapter products of long batches on the tensor cores.
 //
-// A cluster of blocks takes one slot of the plan, up to 64 rows of one adapter.
-// The blocks share the length k of the first product and the columns n of the
-// second one; every element of x, base and y passes through one block, once.
-// The chunks of both products (64 rows by 128 bytes of x and W1, then of base
-// and W2) go through one ring of asynchronous copies, so the second product's
-// first chunks arrive while the blocks exchange the rank-long middle.
+// Two kernels: u = s W1 x (k long, rank wide), then y = base + W2 u.  Their work
+// is a list of chunks, 64 rows of one adapter (a slot of the plan) by 128 bytes
+// along k or n, dealt out in equal consecutive stretches to as many blocks as the
+// device holds, whatever the adapters' shares of the batch.  A block streams its
+// stretch through one ring of asynchronous copies without a pause from slot to
+// slot.  A slot whose k is divided between blocks leaves partial sums in the
+// workspace, which the second kernel adds in the blocks' order.  x, base and y
+// pass through one block once; u and its parts are a rank wide and stay in the L2.
 //
 // What a chunk costs: the rank is small, so both products are bound by the
 // bytes of x, base and y for float64 up to rank 16 and for 16-bit data up to
@@ -41,6 +43,12 @@ template <typename T>
 __device__ __forceinline__ int copy_unit(const void* p, int64_t stride) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * (int64_t)sizeof(T));
     return (a & 15) == 0 ? 16 : sizeof(T) >= 4 ? (int)sizeof(T) : (a & 3) == 0 ? 4 : 0;
+}
+
+template <typename T>
+__device__ __forceinline__ int copy_unit2(const void* p, int64_t row, int64_t adapter) {
+    const int a = copy_unit<T>(p, row), b = copy_unit<T>(p, adapter);
+    return a < b ? a : b;
 }
 
 // 16 bytes of a tile: `avail` elements from src, zeros after them.  What is not
@@ -148,6 +156,8 @@ struct MiddleOf<__nv_bfloat16> {
     }
 };
 
+constexpr int kTileThreads = 256;
+
 // Tiles in shared memory.  "Rank-major" weights have a row for each rank and
 // 128 bytes along the long dimension, "long-major" ones a row for each of its
 // elements and the rank along it.  The pitches keep the warps' fragment loads
@@ -167,14 +177,16 @@ struct AdapterTile {
     static constexpr int kStage = kStageX + (kRankBytes > kLongBytes ? kRankBytes : kLongBytes);
     static constexpr int kStages = RP <= 32 ? 4 : 3;
     static constexpr int kPitchU = E == 2 ? RP + 8 : RP + 4;  // elements of Acc
-    static constexpr int kSmem = kStages * kStage + 2 * kSlotRows * kPitchU * (int)sizeof(Acc);
-    static constexpr int kBlocks = kSmem <= 57000 ? 4 : RP <= 32 && kSmem <= 76000 ? 3 : kSmem <= 114000 ? 2 : 1;  // per SM
+    static constexpr int kSmem = kStages * kStage + kSlotRows * kPitchU * (int)sizeof(Acc);
+    // Blocks an SM: by the registers that the sums need, and by shared memory.
+    static constexpr int kWant = RP * E <= 64 ? 3 : RP * E <= 256 ? 2 : 1, kFit = 232448 / (kSmem + 4096);
+    static constexpr int kBlocks = kWant < kFit ? kWant : kFit;
     // The results of a warp's two rows are 16 bytes of neighbouring columns for each thread: column
     // q * V + 2 t + b of a group of 4 V stands where the instruction has column 2 q + b of its tile t.
     // Long-major weights are laid out in that order; 16-bit rank-major ones (read transposed, eight
     // neighbours at a time) are not, and their results go through the tile instead.
     static constexpr bool kDirect = !(TR && E == 2);
-    __host__ __device__ static constexpr int place(int c) {
+    __host__ __device__ static constexpr int at(int c) {
         return kDirect ? c / (4 * V) * (4 * V) + c % V / 2 * 8 + c % (4 * V) / V * 2 + c % 2 : c;
     }
 };
@@ -216,287 +228,405 @@ __device__ void plain_rows(const AdapterParams& P, const int* list, int count, b
     }
 }
 
-// Joins the blocks' parts of N sums: each block takes its share of them, adds
-// the parts in the blocks' order, and stores done(e, sum) to every block.  A
-// cluster barrier before makes the parts visible, one after the results; after
-// that no block reads or writes another's memory.
-template <int N, typename Acc, typename At, typename Done>
-__device__ __forceinline__ void join_parts(cg::cluster_group& cluster, int cr, int cs, Acc* part, Acc* out, At at,
-                                           Done done) {
-    for (int i = threadIdx.x; i < N / cs; i += blockDim.x) {
-        const int e = cr * (N / cs) + i, o = at(e);
-        Acc p[8];
+// 64 gathered rows by 128 bytes: this thread's 16 bytes of rows tid / 8 and tid / 8 + 32.
+template <typename T, int PITCH>
+struct RowTile {
+    static constexpr int V = 16 / (int)sizeof(T), KC = 8 * V;
+    const T* p[2];
+    bool ok[2];
+    __device__ __forceinline__ void aim(const T* src, int64_t stride, const int* list, int count, int64_t c0) {
 #pragma unroll
-        for (int b = 0; b < 8; ++b)  // all loads in flight before the first addition
-            if (b < cs) p[b] = *cluster.map_shared_rank(part + o, b);
-        Acc v = p[0];
+        for (int i = 0; i < 2; ++i) {
+            const int t = threadIdx.x / 8 + 32 * i;
+            p[i] = src + list[t] * stride + c0 + threadIdx.x % 8 * V;
+            ok[i] = t < count;
+        }
+    }
+    // `left` elements of the rows are there; moves on to the next chunk.
+    __device__ __forceinline__ void fetch(uint8_t* st, int left, int unit) {
+        const int here = left - (int)(threadIdx.x % 8) * V, avail = here < 0 ? 0 : here > V ? V : here;
 #pragma unroll
-        for (int b = 1; b < 8; ++b)
-            if (b < cs) v += p[b];
-        v = done(e, v);
+        for (int i = 0; i < 2; ++i) {
+            fetch16(st + (threadIdx.x / 8 + 32 * i) * PITCH + threadIdx.x % 8 * 16, p[i], ok[i] ? avail : 0, unit);
+            p[i] += KC;
+        }
+    }
+};
+
+// The weights of a chunk: LONG, a row of the rank for each of KC elements (laid
+// out by PLACE), or RP rows of KC elements.
+template <typename T, int RP, bool LONG, int PITCH, typename Place>
+struct WeightTile {
+    static constexpr int E = sizeof(T), V = 16 / E, KC = 8 * V;
+    static constexpr int UPR = LONG ? RP * E / 16 : 8, SKIP = kTileThreads / UPR, N = (RP + 31) / 32;
+    const T* p;
+    __device__ __forceinline__ void aim(const T* w, int64_t stride, int64_t c0) {
+        p = w + (threadIdx.x / UPR + (LONG ? c0 : 0)) * stride + threadIdx.x % UPR * V + (LONG ? 0 : c0);
+    }
+    __device__ __forceinline__ void fetch(uint8_t* wt, int64_t stride, int r, int left, int unit) {
+        const int l = threadIdx.x / UPR, j = threadIdx.x % UPR * V;
+        if (RP >= 32 || threadIdx.x < 8 * RP) {
 #pragma unroll
-        for (int b = 0; b < 8; ++b)
-            if (b < cs) *cluster.map_shared_rank(out + o, b) = v;
+            for (int i = 0; i < N; ++i) {
+                const int row = l + i * SKIP, here = LONG ? r - j : left - j;
+                const int avail = (LONG ? row >= left : row >= r) || here < 0 ? 0 : here > V ? V : here;
+                fetch16(wt + (LONG ? Place::at(row) : row) * PITCH + j * E, p + i * SKIP * stride, avail, unit);
+            }
+        }
+        p += LONG ? KC * stride : KC;
+    }
+};
+struct InPlace {
+    static __device__ __forceinline__ int at(int c) { return c; }
+};
+
+// The slots of a block's stretch: rows and record of the slot that is being
+// fetched and of those behind it that are still being computed, with the loads of
+// the next ones under way.
+struct SlotFeed {
+    static constexpr int kRing = 8;
+    int (*list)[kSlotRows];   // [kRing], shared
+    AdapterSlot* rec;         // [kRing], shared
+    const AdapterSlot* slots;
+    const int32_t* perm;
+    int busy, slot;           // how many; the one that enter() makes current next
+    AdapterSlot next, after;
+    int id;
+    __device__ __forceinline__ int load_id(const AdapterSlot& s) {
+        const int t = threadIdx.x;
+        return t < kSlotRows ? perm[s.start + (t < s.count ? t : 0)] : 0;
+    }
+    __device__ __forceinline__ AdapterSlot load(int i) const { return slots[i < busy ? i : busy - 1]; }
+    __device__ __forceinline__ void begin(int first) {
+        slot = first;
+        next = load(first), after = load(first + 1);
+        id = load_id(next);
+    }
+    // All threads; returns the slot whose rows are now in list[slot % kRing].
+    __device__ __forceinline__ AdapterSlot enter() {
+        const int at = slot % kRing;
+        if (threadIdx.x < kSlotRows) list[at][threadIdx.x] = id;
+        if (threadIdx.x == 0) rec[at] = next;
+        __syncthreads();
+        const AdapterSlot now = next;
+        next = after;
+        id = load_id(next);
+        ++slot;
+        after = load(slot + 1);
+        return now;
+    }
+};
+
+// Block b of `blocks` takes chunks [total b / blocks, total (b + 1) / blocks).  A
+// stretch is an eighth of a slot at least, so that a slot has few parts.
+struct ChunkShare {
+    int64_t total;
+    int blocks;
+    __device__ __forceinline__ ChunkShare(int busy, int per, int grid) {
+        total = (int64_t)busy * per;
+        const int64_t most = total / ((per + 7) / 8);
+        blocks = (int)(most < grid ? (most > 0 ? most : 1) : grid);
+    }
+    __device__ __forceinline__ int64_t first(int b) const { return total * b / blocks; }
+    __device__ __forceinline__ int owner(int64_t chunk) const { return (int)(((chunk + 1) * blocks - 1) / total); }
+};
+
+// u: eight warps, RG groups of rows by KW parts of every chunk's k; a warp holds
+// its rows' sums over its parts for the whole rank, and the KW sums are added when
+// the block leaves the slot.  (The warps of a group read each x once; with all of k
+// and half of the rank for each they would read it twice, and the loads from shared
+// memory would bind the kernel.)
+template <typename T, bool TR, int RP>
+__global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
+    adapter_shrink_kernel(const __grid_constant__ AdapterParams P) {
+    using Tile = AdapterTile<T, TR, RP>;
+    using Acc = typename Tile::Acc;
+    constexpr int E = Tile::E, KC = Tile::KC, S = Tile::kStages;
+    constexpr int MT = RP * (E == 4 ? 2 : 1) < 128 ? 2 : 1, RG = 4 / MT, KW = 8 / RG, NT = RP / 8;
+    constexpr int FLUSH = 4;  // chunks that the tensor cores sum by themselves, for floats
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int list[SlotFeed::kRing][kSlotRows];
+    __shared__ AdapterSlot rec[SlotFeed::kRing];
+    cudaTriggerProgrammaticLaunchCompletion();
+    const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, q = lane & 3;
+    const int rows0 = (tid >> 5) % RG * 16 * MT, kw = (tid >> 5) / RG;
+    const int busy = P.plan[plan_header_word(P.rows, P.adapters)];
+    const int k = (int)P.k, per = (k + KC - 1) / KC;
+    if (busy == 0) return;
+    const ChunkShare share(busy, per, gridDim.x);
+    if ((int)blockIdx.x >= share.blocks) return;
+    const int64_t begin = share.first(blockIdx.x);
+    const int chunks = (int)(share.first(blockIdx.x + 1) - begin);
+    SlotFeed feed{list, rec, plan_busy(P), plan_perm(P), busy};
+    feed.begin((int)(begin / per));
+    const T* x = static_cast<const T*>(P.x);
+    const T* w1 = static_cast<const T*>(P.w1);
+    const int unit_x = copy_unit<T>(x, P.x_row), unit_w = copy_unit2<T>(w1, P.w1_row, P.w1_adapter);
+
+    RowTile<T, Tile::kPitchX> xt;
+    WeightTile<T, RP, TR, TR ? Tile::kPitchLong : Tile::kPitchRank, InPlace> wt;
+    uint32_t load = 0, use = 0;
+    auto next = [](uint32_t& stage) { stage = stage == (S - 1) * Tile::kStage ? 0 : stage + Tile::kStage; };
+    int fetch_at = (int)(begin % per);  // the next chunk to fetch, within its slot
+    bool enter = true;
+    auto fetch = [&]() {
+        if (enter) {
+            const AdapterSlot s = feed.enter();
+            xt.aim(x, P.x_row, list[(feed.slot - 1) % SlotFeed::kRing], s.count, (int64_t)fetch_at * KC);
+            wt.aim(w1 + s.cls * P.w1_adapter, P.w1_row, (int64_t)fetch_at * KC);
+        }
+        const int left = k - fetch_at * KC;
+        xt.fetch(smem + load, left, unit_x);
+        wt.fetch(smem + load + Tile::kStageX, P.w1_row, P.r, left, unit_w);
+        enter = ++fetch_at == per;
+        if (enter) fetch_at = 0;
+    };
+
+    Acc acc[MT][NT][4] = {}, sum[E == 4 ? MT : 1][E == 4 ? NT : 1][4] = {};
+    auto flush = [&]() {
+        if constexpr (E == 4) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[m][t][e] += sum[m][t][e], sum[m][t][e] = 0;
+        }
+    };
+    auto shrink = [&](const uint8_t* st) {
+        const uint8_t* ws = st + Tile::kStageX;
+#pragma unroll
+        for (int i = 0; i < 4 / KW; ++i) {
+            const int ks = kw * (4 / KW) + i;
+            if constexpr (E == 2) {
+                const uint32_t xa = shared_address(st) + (rows0 + (lane & 15)) * Tile::kPitchX + (lane >> 4) * 16 + ks * 32;
+                const uint32_t wa = shared_address(ws) +
+                                    (TR ? (ks * 16 + (lane & 15)) * Tile::kPitchLong + (lane >> 4) * 16
+                                        : ((lane & 7) + (lane >> 4) * 8) * Tile::kPitchRank + (lane >> 3 & 1) * 16 + ks * 32);
+                uint32_t a[MT][4];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) ldsm4(a[m], xa + m * 16 * Tile::kPitchX);
+#pragma unroll
+                for (int p = 0; p < RP / 16; ++p) {
+                    uint32_t b[4];
+                    if (TR) ldsm4t(b, wa + p * 32);
+                    else ldsm4(b, wa + p * 16 * Tile::kPitchRank);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        mma16<T>(acc[m][2 * p], a[m], b[0], b[1]);
+                        mma16<T>(acc[m][2 * p + 1], a[m], b[2], b[3]);
+                    }
+                }
+            } else if constexpr (E == 4) {
+                uint32_t ah[MT][4], al[MT][4];
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const Tf32Pair p = tf32_split(*reinterpret_cast<const float*>(
+                            st + (rows0 + m * 16 + g + (e & 1) * 8) * Tile::kPitchX + (ks * 8 + q + (e >> 1) * 4) * 4));
+                        ah[m][e] = p.hi, al[m][e] = p.lo;
+                    }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    Tf32Pair b[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int kk = ks * 8 + q + e * 4, j = t * 8 + g;
+                        b[e] = tf32_split(*reinterpret_cast<const float*>(
+                            ws + (TR ? kk * Tile::kPitchLong + j * 4 : j * Tile::kPitchRank + kk * 4)));
+                    }
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) mma_tf32(sum[m][t], ah[m], b[0].lo, b[1].lo);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) mma_tf32(sum[m][t], al[m], b[0].hi, b[1].hi);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) mma_tf32(sum[m][t], ah[m], b[0].hi, b[1].hi);
+                }
+            } else {
+                double a[MT][2];
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        a[m][h] = *reinterpret_cast<const double*>(
+                            st + (rows0 + m * 16 + h * 8 + g) * Tile::kPitchX + (ks * 4 + q) * 8);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const int kk = ks * 4 + q, j = t * 8 + g;
+                    const double b = *reinterpret_cast<const double*>(
+                        ws + (TR ? kk * Tile::kPitchLong + j * 8 : j * Tile::kPitchRank + kk * 8));
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) mma_f64(acc[m][t], a[m][0], a[m][1], b);
+                }
+            }
+        }
+    };
+    // The block's sums of a slot to the workspace: the parts of k one after the other.
+    Acc* red = reinterpret_cast<Acc*>(smem + S * Tile::kStage);
+    auto leave = [&](int64_t part) {
+        flush();
+        for (int p = 0; p < KW; ++p) {
+            if (kw == p) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            Acc* o = red + (rows0 + m * 16 + g + (e >> 1) * 8) * Tile::kPitchU + t * 8 + 2 * q + (e & 1);
+                            *o = p ? *o + acc[m][t][e] : acc[m][t][e];
+                            acc[m][t][e] = 0;
+                        }
+            }
+            __syncthreads();
+        }
+        Acc* out = static_cast<Acc*>(P.parts) + part * (kSlotRows * RP);
+        for (int i = tid; i < kSlotRows * RP; i += kTileThreads) out[i] = red[i / RP * Tile::kPitchU + i % RP];
+    };
+
+    int at = (int)(begin % per), slot = (int)(begin / per);
+    for (int c = 1 - S; c < chunks; ++c) {
+        if (c >= 0) {
+            copy_wait<S - 2>();
+            __syncthreads();  // chunk c has arrived for all; chunk c - 1's buffer is free
+        }
+        if (c + S - 1 < chunks) fetch();
+        next(load);
+        copy_commit();
+        if (c < 0) continue;
+        if (rows0 < rec[slot % SlotFeed::kRing].count) shrink(smem + use);
+        next(use);
+        if (c % FLUSH == FLUSH - 1) flush();
+        if (++at == per || c + 1 == chunks) {
+            leave((int64_t)blockIdx.x + slot);
+            at = 0, ++slot;
+        }
     }
 }
 
-// Eight warps: four groups of 16 rows, twice.  In the first product the two
-// warps of a group hold half of the rank each, in the second one half of the
-// chunk's columns.
-constexpr int kTileThreads = 256;
-
+// y: eight warps, four groups of 16 rows by the halves of every chunk's columns.
 template <typename T, bool TR, int RP>
 __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
-    adapter_tile_kernel(const __grid_constant__ AdapterParams P) {
+    adapter_expand_kernel(const __grid_constant__ AdapterParams P) {
     using Tile = AdapterTile<T, TR, RP>;
     using Acc = typename Tile::Acc;
-    constexpr int E = Tile::E, V = Tile::V, KC = Tile::KC, S = Tile::kStages, HT = RP / 16;  // HT: 8-rank tiles a warp
+    constexpr int E = Tile::E, V = Tile::V, KC = Tile::KC, S = Tile::kStages;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int list[kSlotRows];
-    cg::cluster_group cluster = cg::this_cluster();
+    __shared__ int list[SlotFeed::kRing][kSlotRows];
+    __shared__ AdapterSlot rec[SlotFeed::kRing];
     const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, q = lane & 3;
     const int rows0 = (tid >> 5 & 3) * 16, half = tid >> 7;
-    const int cr = (int)cluster.block_rank(), cs = (int)cluster.num_blocks();
-    const AdapterSlot slot =
-        reinterpret_cast<const AdapterSlot*>(P.plan + plan_slot_word(P.adapters))[blockIdx.x / cs];
-    const int count = slot.count;
-    if (count == 0) return;
-    if (tid < kSlotRows)
-        list[tid] = (P.plan + plan_perm_word(P.rows, P.adapters))[slot.start + (tid < count ? tid : 0)];
-    __syncthreads();
-    // This block's share of k and of n, in whole chunks but for the last block's (k and n stay below 2^30).
-    const int k = (int)P.k, n = (int)P.n;
-    const int kshare = (k + KC * cs - 1) / (KC * cs) * KC, nshare = (n + KC * cs - 1) / (KC * cs) * KC;
-    const int k0 = min(cr * kshare, k), n0 = min(cr * nshare, n);
-    const int klen = min(kshare, k - k0), nlen = min(nshare, n - n0);
-    if (slot.cls >= P.adapters) {
-        plain_rows<T>(P, list, count, slot.cls != P.adapters, n0, n0 + nlen);
-        return;
-    }
-    const int nk = (klen + KC - 1) / KC, total = nk + (nlen + KC - 1) / KC;
-    const T* w1 = static_cast<const T*>(P.w1) + slot.cls * P.w1_adapter;
-    const T* w2 = static_cast<const T*>(P.w2) + slot.cls * P.w2_adapter;
-    const T* x = static_cast<const T*>(P.x);
+    const int32_t* header = P.plan + plan_header_word(P.rows, P.adapters);
+    const int busy = header[0], idle = header[1];
+    const int n = (int)P.n, per = n > 0 ? (n + KC - 1) / KC : 1;  // without columns, for u alone
     const T* base = static_cast<const T*>(P.base);
-    const int vec_x = copy_unit<T>(x, P.x_row), vec_w1 = copy_unit<T>(w1, P.w1_row), vec_w2 = copy_unit<T>(w2, P.w2_row);
-    const int vec_base = copy_unit<T>(base, P.base_row);
+    const T* w2 = static_cast<const T*>(P.w2);
+    const int unit_base = copy_unit<T>(base, P.base_row), unit_w = copy_unit2<T>(w2, P.w2_row, P.w2_adapter);
     const bool vec_y = copy_unit<T>(P.y, P.y_row) == 16;
+    const ChunkShare share(busy > 0 ? busy : 1, per, gridDim.x);
+    const bool here = busy > 0 && (int)blockIdx.x < share.blocks;
+    const int64_t begin = here ? share.first(blockIdx.x) : 0;
+    const int chunks = here ? (int)(share.first(blockIdx.x + 1) - begin) : 0;
+    const int kper = ((int)P.k + KC - 1) / KC;
+    const ChunkShare kshare(busy > 0 ? busy : 1, kper > 0 ? kper : 1, P.shrink_grid);
+    SlotFeed feed{list, rec, plan_busy(P), plan_perm(P), busy};
+    if (here) feed.begin((int)(begin / per));
 
-    auto clamp = [](int v) { return v < 0 ? 0 : v > V ? V : v; };
-    // This thread's 16-byte units of a tile: one of rows tid / 8 and tid / 8 + 32, and NW of the weights,
-    // UPR units along and SKIP rows apart.  The pointers advance from chunk to chunk.
-    constexpr int NW = (RP + 31) / 32;
-    const int unit = tid % 8 * V;
-    const T *rp[2], *wp;
-    auto aim_rows = [&](const T* src, int64_t stride, int c0) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) rp[i] = src + list[tid / 8 + 32 * i] * stride + c0 + unit;
-    };
-    auto fetch_weights = [&](auto by_long, uint8_t* wt, int64_t stride, int left, int vec) {
-        constexpr bool LONG = decltype(by_long)::value, PLACED = LONG && !TR;  // the second product's
-        constexpr int UPR = LONG ? RP * E / 16 : 8, SKIP = kTileThreads / UPR;
-        const int l = tid / UPR, j = tid % UPR * V;
-        if (RP >= 32 || tid < 8 * RP) {
-#pragma unroll
-            for (int i = 0; i < NW; ++i) {
-                const int row = l + i * SKIP;
-                uint8_t* dst = wt + (PLACED ? Tile::place(row) : row) * (LONG ? Tile::kPitchLong : Tile::kPitchRank) + j * E;
-                const int avail = LONG ? (row < left ? clamp(P.r - j) : 0) : row < P.r ? clamp(left - j) : 0;
-                fetch16(dst, wp + i * SKIP * stride, avail, vec);
-            }
+    RowTile<T, Tile::kPitchX> bt;
+    WeightTile<T, RP, !TR, TR ? Tile::kPitchRank : Tile::kPitchLong, Tile> wt;
+    uint32_t load = 0, use = 0;
+    auto next = [](uint32_t& stage) { stage = stage == (S - 1) * Tile::kStage ? 0 : stage + Tile::kStage; };
+    int fetch_at = (int)(begin % per);
+    bool enter = true;
+    auto fetch = [&]() {
+        if (enter) {
+            const AdapterSlot s = feed.enter();
+            if (base) bt.aim(base, P.base_row, list[(feed.slot - 1) % SlotFeed::kRing], s.count, (int64_t)fetch_at * KC);
+            wt.aim(w2 + s.cls * P.w2_adapter, P.w2_row, (int64_t)fetch_at * KC);
         }
-        wp += LONG ? KC * stride : KC;
-    };
-    auto aim_weights = [&](auto by_long, const T* w, int64_t stride, int c0) {
-        constexpr bool LONG = decltype(by_long)::value;
-        constexpr int UPR = LONG ? RP * E / 16 : 8;
-        wp = w + (tid / UPR + (LONG ? c0 : 0)) * stride + tid % UPR * V + (LONG ? 0 : c0);
-    };
-    constexpr std::integral_constant<bool, TR> first_long{};
-    constexpr std::integral_constant<bool, !TR> second_long{};
-    auto fetch_rows = [&](uint8_t* st, int left, int vec) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            fetch16(st + (tid / 8 + i * 32) * Tile::kPitchX + tid % 8 * 16, rp[i],
-                    tid / 8 + i * 32 < count ? clamp(left - unit) : 0, vec);
-            rp[i] += KC;
-        }
-    };
-    auto fetch_first = [&](int c, uint8_t* st) {
-        fetch_rows(st, klen - c * KC, vec_x);
-        fetch_weights(first_long, st + Tile::kStageX, P.w1_row, klen - c * KC, vec_w1);
-    };
-    auto fetch_second = [&](int c, uint8_t* st) {
-        if (c == 0) {
-            if (base) aim_rows(base, P.base_row, n0);
-            aim_weights(second_long, w2, P.w2_row, n0);
-        }
-        if (base) fetch_rows(st, nlen - c * KC, vec_base);
-        fetch_weights(second_long, st + Tile::kStageX, P.w2_row, nlen - c * KC, vec_w2);
+        const int left = n - fetch_at * KC;
+        if (base) bt.fetch(smem + load, left, unit_base);
+        wt.fetch(smem + load + Tile::kStageX, P.w2_row, P.r, left, unit_w);
+        enter = ++fetch_at == per;
+        if (enter) fetch_at = 0;
     };
 
-    Acc* part = reinterpret_cast<Acc*>(smem + S * Tile::kStage);  // this block's sums, read by the cluster
-    Acc* us = part + kSlotRows * Tile::kPitchU;                   // the cluster's sums
-    Acc acc[HT][4] = {};
+    Acc* us = reinterpret_cast<Acc*>(smem + S * Tile::kStage);
     // The middle as this thread's part of the left operand: 16-bit data split in
     // two and, for halves, scaled by a power of two per row; f32 and f64 plain.
     uint32_t uh[E == 2 ? RP / 16 : 1][4], ul[E == 2 ? RP / 16 : 1][4];
     Acc uf[E == 2 ? 1 : RP / (E == 4 ? 8 : 4)][E == 4 ? 4 : 2];
-    float back[2] = {1.f, 1.f};
-    const bool busy = rows0 < count;
-
-    auto exchange = [&]() {
-        Acc* own = part + (rows0 + g) * Tile::kPitchU + half * HT * 8 + 2 * q;
-#pragma unroll
-        for (int t = 0; t < HT; ++t) {
-            own[t * 8] = acc[t][0], own[t * 8 + 1] = acc[t][1];
-            own[t * 8 + 8 * Tile::kPitchU] = acc[t][2], own[t * 8 + 8 * Tile::kPitchU + 1] = acc[t][3];
-        }
-        cluster.sync();
-        const Acc s = (Acc)(P.scales ? P.scales[slot.cls] : P.scale);
-        join_parts<kSlotRows * RP>(cluster, cr, cs, part, us, [](int e) { return e / RP * Tile::kPitchU + e % RP; },
-                                   [&](int e, Acc v) {
-            const int row = e / RP, r = e % RP;
+    float back[2];
+    T* yp[2];
+    auto take_slot = [&](int slot, int at) {
+        const AdapterSlot& now = rec[slot % SlotFeed::kRing];
+        const int* rows = list[slot % SlotFeed::kRing];
+        const Acc s = (Acc)(P.scales ? P.scales[now.cls] : P.scale);
+        const int b0 = kper ? kshare.owner((int64_t)slot * kper) : 0;
+        const int b1 = kper ? kshare.owner((int64_t)(slot + 1) * kper - 1) : -1;
+        const Acc* parts = static_cast<const Acc*>(P.parts) + (int64_t)(b0 + slot) * (kSlotRows * RP);
+#pragma unroll 4
+        for (int i = tid; i < kSlotRows * RP; i += kTileThreads) {
+            Acc v = 0;
+            for (int b = 0; b <= b1 - b0; ++b) v += __ldcg(parts + (int64_t)b * (kSlotRows * RP) + i);
+            const int row = i / RP, r = i % RP;
             v = r < P.r ? v * s : Acc(0);  // past the rank, an infinite x met a zero: NaN
-            if (P.u && r < P.r && row < count) static_cast<typename MiddleOf<T>::type*>(P.u)[(int64_t)list[row] * P.u_row + r] = MiddleOf<T>::pack(v);
-            return v;
-        });
-        cluster.sync();
-        if (busy) {
-            const Acc* from = us + (rows0 + g) * Tile::kPitchU;
-            if constexpr (E == 2) {
-                float v[RP / 16][8];  // a0..a3 of two: rows g, g + 8, then columns + 8
-#pragma unroll
-                for (int t = 0; t < RP / 16; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 f = *reinterpret_cast<const float2*>(
-                            from + (e & 1) * 8 * Tile::kPitchU + t * 16 + 2 * q + (e >> 1) * 8);
-                        v[t][2 * e] = f.x, v[t][2 * e + 1] = f.y;
-                    }
-                float down[2] = {1.f, 1.f};
-                if constexpr (std::is_same<T, __half>::value) {
-                    float top[2] = {0.f, 0.f};
-#pragma unroll
-                    for (int t = 0; t < RP / 16; ++t)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) top[e >> 1 & 1] = fmaxf(top[e >> 1 & 1], fabsf(v[t][e]));
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-                        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-                        const int e = (int)(__float_as_uint(top[h]) >> 23);  // 0 and 255 stay unscaled
-                        if (e > 0 && e < 254) {
-                            down[h] = __uint_as_float((254 - e) << 23);
-                            back[h] = __uint_as_float(e << 23);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < RP / 16; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        split16<T>(v[t][2 * e] * down[e & 1], v[t][2 * e + 1] * down[e & 1], uh[t][e], ul[t][e]);
-            } else {
-                constexpr int step = E == 4 ? 8 : 4;  // a0, a1 of rows g, g + 8; f32 two more, four columns on
-#pragma unroll
-                for (int t = 0; t < RP / step; ++t)
-#pragma unroll
-                    for (int e = 0; e < step / 2; ++e)
-                        uf[t][e] = from[(e & 1) * 8 * Tile::kPitchU + t * step + q + (e >> 1) * 4];
-            }
+            us[row * Tile::kPitchU + r] = v;
+            if (P.u && at == 0 && r < P.r && row < now.count)
+                static_cast<typename MiddleOf<T>::type*>(P.u)[(int64_t)rows[row] * P.u_row + r] = MiddleOf<T>::pack(v);
         }
-    };
-
-    auto shrink = [&](const uint8_t* st) {
-        const uint8_t* wt = st + Tile::kStageX;
+        __syncthreads();
+        const Acc* from = us + (rows0 + g) * Tile::kPitchU;
         if constexpr (E == 2) {
-            const uint32_t xa = shared_address(st) + (rows0 + (lane & 15)) * Tile::kPitchX + (lane >> 4) * 16;
-            uint32_t b[4];
-            if constexpr (RP == 16) {  // one 8-rank tile: four 8-element pieces of k at a time
-                const uint32_t wa = shared_address(wt) + (TR ? lane * Tile::kPitchLong + half * 16
-                                                             : (half * 8 + (lane & 7)) * Tile::kPitchRank + (lane >> 3) * 16);
+            float v[RP / 16][8];  // a0..a3 of two: rows g, g + 8, then columns + 8
 #pragma unroll
-                for (int kp = 0; kp < 2; ++kp) {
-                    uint32_t a[4];
-                    if (TR) ldsm4t(b, wa + kp * 32 * Tile::kPitchLong);
-                    else ldsm4(b, wa + kp * 64);
-                    ldsm4(a, xa + kp * 64);
-                    mma16<T>(acc[0], a, b[0], b[1]);
-                    ldsm4(a, xa + kp * 64 + 32);
-                    mma16<T>(acc[0], a, b[2], b[3]);
-                }
-            } else {
-                const int j0 = half * HT * 8;
-                const uint32_t wa = shared_address(wt) +
-                                    (TR ? (lane & 15) * Tile::kPitchLong + (j0 + (lane >> 4) * 8) * 2
-                                        : (j0 + (lane & 7) + (lane >> 4) * 8) * Tile::kPitchRank + (lane >> 3 & 1) * 16);
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) {
-                    uint32_t a[4];
-                    ldsm4(a, xa + ks * 32);
-#pragma unroll
-                    for (int p = 0; p < HT / 2; ++p) {
-                        if (TR) ldsm4t(b, wa + ks * 16 * Tile::kPitchLong + p * 32);
-                        else ldsm4(b, wa + p * 16 * Tile::kPitchRank + ks * 32);
-                        mma16<T>(acc[2 * p], a, b[0], b[1]);
-                        mma16<T>(acc[2 * p + 1], a, b[2], b[3]);
-                    }
-                }
-            }
-        } else if constexpr (E == 4) {
-            // The tensor cores' sums run over one chunk; chunks are added in registers, rounded to nearest.
-            float sum[HT][4] = {};
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-                uint32_t ah[4], al[4];
+            for (int t = 0; t < RP / 16; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const Tf32Pair p = tf32_split(*reinterpret_cast<const float*>(
-                        st + (rows0 + g + (e & 1) * 8) * Tile::kPitchX + (ks * 8 + q + (e >> 1) * 4) * 4));
-                    ah[e] = p.hi, al[e] = p.lo;
+                    const float2 f = *reinterpret_cast<const float2*>(
+                        from + (e & 1) * 8 * Tile::kPitchU + t * 16 + 2 * q + (e >> 1) * 8);
+                    v[t][2 * e] = f.x, v[t][2 * e + 1] = f.y;
                 }
+            float down[2] = {1.f, 1.f};
+            if constexpr (std::is_same<T, __half>::value) {
+                float top[2] = {0.f, 0.f};
+                back[0] = back[1] = 1.f;
 #pragma unroll
-                for (int t = 0; t < HT; ++t) {
-                    Tf32Pair b[2];
+                for (int t = 0; t < RP / 16; ++t)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int kk = ks * 8 + q + e * 4, j = (half * HT + t) * 8 + g;
-                        b[e] = tf32_split(*reinterpret_cast<const float*>(
-                            wt + (TR ? kk * Tile::kPitchLong + j * 4 : j * Tile::kPitchRank + kk * 4)));
+                    for (int e = 0; e < 8; ++e) top[e >> 1 & 1] = fmaxf(top[e >> 1 & 1], fabsf(v[t][e]));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+                    const int e = (int)(__float_as_uint(top[h]) >> 23);  // 0 and 255 stay unscaled
+                    if (e > 0 && e < 254) {
+                        down[h] = __uint_as_float((254 - e) << 23);
+                        back[h] = __uint_as_float(e << 23);
                     }
-                    mma_tf32(sum[t], ah, b[0].lo, b[1].lo);
-                    mma_tf32(sum[t], al, b[0].hi, b[1].hi);
-                    mma_tf32(sum[t], ah, b[0].hi, b[1].hi);
                 }
             }
 #pragma unroll
-            for (int t = 0; t < HT; ++t)
+            for (int t = 0; t < RP / 16; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[t][e] += sum[t][e];
+                for (int e = 0; e < 4; ++e)
+                    split16<T>(v[t][2 * e] * down[e & 1], v[t][2 * e + 1] * down[e & 1], uh[t][e], ul[t][e]);
         } else {
+            constexpr int step = E == 4 ? 8 : 4;  // a0, a1 of rows g, g + 8; f32 two more, four columns on
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-                const uint8_t* xa = st + (rows0 + g) * Tile::kPitchX + (ks * 4 + q) * 8;
-                const double a0 = *reinterpret_cast<const double*>(xa);
-                const double a1 = *reinterpret_cast<const double*>(xa + 8 * Tile::kPitchX);
+            for (int t = 0; t < RP / step; ++t)
 #pragma unroll
-                for (int t = 0; t < HT; ++t) {
-                    const int kk = ks * 4 + q, j = (half * HT + t) * 8 + g;
-                    mma_f64(acc[t], a0, a1, *reinterpret_cast<const double*>(
-                        wt + (TR ? kk * Tile::kPitchLong + j * 8 : j * Tile::kPitchRank + kk * 8)));
-                }
-            }
+                for (int e = 0; e < step / 2; ++e)
+                    uf[t][e] = from[(e & 1) * 8 * Tile::kPitchU + t * step + q + (e >> 1) * 4];
         }
+        // This thread's rows of y at its 16 bytes of the warp's group of columns.
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            yp[h] = static_cast<T*>(P.y) + rows[rows0 + g + h * 8] * P.y_row + (int64_t)at * KC + half * (KC / 2) + q * V;
     };
 
-    // This thread's rows of y at its 16 bytes of the warp's group of columns.
-    const int col0 = half * (KC / 2) + q * V;
-    T* yp[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) yp[h] = static_cast<T*>(P.y) + list[rows0 + g + h * 8] * P.y_row + n0 + col0;
-
-    auto expand = [&](uint8_t* st, int left) {
+    auto expand = [&](uint8_t* st, int left, const int* rows, int count) {
         constexpr int NT = V / 2;  // 8-column tiles of a group
         const uint8_t* wt = st + Tile::kStageX;
         Acc c[NT][4] = {};
@@ -506,16 +636,16 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
                                     : (half * 32 + (lane & 7) + (lane >> 4) * 8) * Tile::kPitchLong + (lane >> 3 & 1) * 16);
 #pragma unroll
             for (int t = 0; t < RP / 16; ++t) {
+                uint32_t b[2][4];
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    uint32_t b[4];
-                    if (TR) ldsm4t(b, wa + t * 16 * Tile::kPitchRank + p * 32);
-                    else ldsm4(b, wa + p * 16 * Tile::kPitchLong + t * 32);
-                    mma16<T>(c[2 * p], ul[t], b[0], b[1]);
-                    mma16<T>(c[2 * p + 1], ul[t], b[2], b[3]);
-                    mma16<T>(c[2 * p], uh[t], b[0], b[1]);
-                    mma16<T>(c[2 * p + 1], uh[t], b[2], b[3]);
+                    if (TR) ldsm4t(b[p], wa + t * 16 * Tile::kPitchRank + p * 32);
+                    else ldsm4(b[p], wa + p * 16 * Tile::kPitchLong + t * 32);
                 }
+#pragma unroll
+                for (int p = 0; p < 4; ++p) mma16<T>(c[p], ul[t], b[p / 2][p % 2 * 2], b[p / 2][p % 2 * 2 + 1]);
+#pragma unroll
+                for (int p = 0; p < 4; ++p) mma16<T>(c[p], uh[t], b[p / 2][p % 2 * 2], b[p / 2][p % 2 * 2 + 1]);
             }
         } else if constexpr (E == 4) {
 #pragma unroll
@@ -595,40 +725,41 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
             for (int i = lane; i < 16 * H; i += 32) {
                 const int row = rows0 + i / H, c = half * H + i % H;
                 if (row < count && c < left)
-                    static_cast<T*>(P.y)[list[row] * P.y_row + n0 + nlen - left + c] =
+                    static_cast<T*>(P.y)[rows[row] * P.y_row + n - left + c] =
                         *reinterpret_cast<const T*>(st + row * Tile::kPitchX + c * E);
             }
         }
     };
 
-    // Stages by their offset: `load` is where the next chunk goes, `use` what is computed.
-    uint32_t load = 0, use = 0;
-    auto next = [](uint32_t& stage) { stage = stage == (S - 1) * Tile::kStage ? 0 : stage + Tile::kStage; };
-    aim_rows(x, P.x_row, k0);
-    aim_weights(first_long, w1, P.w1_row, k0);
-    for (int c = 1 - S; c < nk; ++c) {
+    cudaGridDependencySynchronize();  // the parts of u are there
+    int at = (int)(begin % per), slot = (int)(begin / per);
+    bool taken = false;
+    for (int c = 1 - S; c < chunks; ++c) {
         if (c >= 0) {
             copy_wait<S - 2>();
             __syncthreads();  // chunk c has arrived for all; chunk c - 1's buffer is free
         }
-        if (c + S - 1 < nk) fetch_first(c + S - 1, smem + load);
-        else if (c + S - 1 < total) fetch_second(c + S - 1 - nk, smem + load);
+        if (c + S - 1 < chunks) fetch();
         next(load);
         copy_commit();
-        if (c >= 0) {
-            if (busy) shrink(smem + use);
-            next(use);
-        }
-    }
-    exchange();
-    for (int c = nk; c < total; ++c) {
-        copy_wait<S - 2>();
-        __syncthreads();
-        if (c + S - 1 < total) fetch_second(c + S - 1 - nk, smem + load);
-        next(load);
-        copy_commit();
-        if (busy) expand(smem + use, nlen - (c - nk) * KC);
+        if (c < 0) continue;
+        if (!taken) take_slot(slot, at);
+        taken = true;
+        const int count = rec[slot % SlotFeed::kRing].count;
+        if (rows0 < count) expand(smem + use, n - at * KC, list[slot % SlotFeed::kRing], count);
         next(use);
+        if (++at == per) at = 0, ++slot, taken = false;
+    }
+    // Rows without an adapter, an eighth of the columns at a time.
+    constexpr int kParts = 8;
+    const AdapterSlot* last = plan_busy(P) + plan_slots(P.rows, P.adapters) - 1;
+    const int width = (n + kParts * V - 1) / (kParts * V) * V;
+    for (int i = blockIdx.x; i < idle * kParts; i += gridDim.x) {
+        const AdapterSlot s = last[-(i / kParts)];
+        __syncthreads();
+        if (tid < s.count) list[0][tid] = plan_perm(P)[s.start + tid];
+        __syncthreads();
+        plain_rows<T>(P, list[0], s.count, s.cls != P.adapters, min(i % kParts * width, n), min((i % kParts + 1) * width, n));
     }
 }
 

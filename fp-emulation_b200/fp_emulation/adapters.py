@@ -84,16 +84,22 @@ def _launch(x, w1, w2, transposed, base, y, scale, index, plan, adapters, rank, 
     """One fpemu_adapter_matmul on the current stream of x's device (2-D x, base and y)."""
     dev = x.device
     d = dev.index
+    lib = _lib.load()
+    code, rows = _DTYPE_CODE[x.dtype], x.shape[0]
     with _on(d):
-        st = _lib.load().fpemu_adapter_matmul(
-            _DTYPE_CODE[x.dtype], x.shape[0], k, n, rank, adapters, x.data_ptr(), _row_stride(x),
+        size = 0
+        if plan is not None:
+            size = lib.fpemu_adapter_workspace_size(code, rows, rank, adapters)
+            workspace = torch.empty((size,), dtype=torch.uint8, device=dev)
+        st = lib.fpemu_adapter_matmul(
+            code, rows, k, n, rank, adapters, x.data_ptr(), _row_stride(x),
             w1.data_ptr(), w1.stride(0), w1.stride(1), w2.data_ptr(), w2.stride(0), w2.stride(1), transposed,
             None if base is None else base.data_ptr(), 0 if base is None else base.stride(0),
             None if y is None else y.data_ptr(), n if y is None else _row_stride(y),
             None if scale.__class__ is float else scale.data_ptr(), scale if scale.__class__ is float else 0.0,
             None if plan is not None else index.data_ptr(), 0 if plan is not None else index.element_size(),
             None if plan is None else plan.data_ptr(), None if u is None else u.data_ptr(),
-            _raw_stream(d))
+            workspace.data_ptr() if size else None, size, _raw_stream(d))
     if st:
         _lib.check(st, "adapter_matmul")
     _after_call("adapter_matmul", dev)

@@ -230,14 +230,16 @@ int fpemu_adapter_plan(const void *index, int index_bytes, int64_t rows, int64_t
  * are not written.
  * y may be base itself; otherwise it overlaps no input.
  * plan NULL: rows <= FPEMU_ADAPTER_FEW_ROWS and not transposed, grouped by the
- * kernel from index. */
+ * kernel from index; no workspace.  With a plan: fpemu_adapter_workspace_size
+ * bytes, 16-byte aligned, for this call alone. */
 int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank,
                          int64_t adapters, const void *x, int64_t x_row, const void *w1,
                          int64_t w1_adapter, int64_t w1_row, const void *w2, int64_t w2_adapter,
                          int64_t w2_row, int transposed, const void *base, int64_t base_row,
                          void *y, int64_t y_row, const double *scales, double scale,
                          const void *index, int index_bytes, const void *plan, void *u,
-                         void *stream);
+                         void *workspace, size_t workspace_bytes, void *stream);
+size_t fpemu_adapter_workspace_size(int dtype, int64_t rows, int64_t rank, int64_t adapters);
 
 /* Gradients of the factors, each [adapters][...] packed, zero for an adapter
  * without rows: dA[i] = sum_t v[t]^T x[t] (rank x k) and dB[i] = sum_t dy[t]^T u[t]

@@ -92,16 +92,16 @@ def test_dense_means_each_element_once():
 
 def test_plan_size_and_c_refusals():
     lib = _lib.load()
-    # start words, slots and rows: (n + 3 rounded to 4) + 4 (rows // 64 + n + 2) + rows, in words
+    # start words (n + 3 rounded to 4), slots twice (4 words each, rows // 64 + n + 2), 4 words, rows
     for rows, n in ((0, 1), (1, 1), (63, 5), (64, 5), (1000, 64), (1 << 20, 65000)):
-        assert lib.fpemu_adapter_plan_size(rows, n) == 4 * ((n + 3 + 3) // 4 * 4 + 4 * (rows // 64 + n + 2) + rows)
+        assert lib.fpemu_adapter_plan_size(rows, n) == 4 * ((n + 3 + 3) // 4 * 4 + 8 * (rows // 64 + n + 2) + 4 + rows)
     assert lib.fpemu_adapter_plan_size(-1, 1) == 0 and lib.fpemu_adapter_plan_size(1, 0) == 0
     assert lib.fpemu_adapter_plan(None, 4, 1, 1, None, 0, None) == _lib.FPEMU_ERR_WORKSPACE
     assert lib.fpemu_adapter_plan(None, 2, 1, 1, None, 0, None) == _lib.FPEMU_ERR_INVALID
 
     def matmul(dtype=0, rows=4, k=8, n=8, rank=2, adapters=2, x=16, y=16, x_row=8, y_row=8, index=16, nbytes=4, plan=None):
         return lib.fpemu_adapter_matmul(dtype, rows, k, n, rank, adapters, x, x_row, 16, 16, 8, 16, 16, 2, 0, None, 0,
-                                        y, y_row, None, 1.0, index, nbytes, plan, None, None)
+                                        y, y_row, None, 1.0, index, nbytes, plan, None, None, 0, None)
 
     bad, unsupported = _lib.FPEMU_ERR_INVALID, _lib.FPEMU_ERR_UNSUPPORTED
     assert matmul(dtype=4) == bad and matmul(rows=-1) == bad and matmul(x=None) == bad and matmul(y=None) == bad
