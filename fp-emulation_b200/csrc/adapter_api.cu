@@ -75,7 +75,7 @@ int launch_few(const AdapterParams& P, const DevInfo& d, cudaStream_t st) {
 
 int padded_rank(int64_t r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128; }
 
-constexpr int kMostBlocks = 3;  // of a tile kernel on an SM
+constexpr int kMostBlocks = 2;  // of a tile kernel on an SM
 
 template <typename T, bool TR, int RP>
 int launch_tiles_rank(AdapterParams& P, const DevInfo& d, cudaStream_t st) {
@@ -91,7 +91,7 @@ int launch_tiles_rank(AdapterParams& P, const DevInfo& d, cudaStream_t st) {
         return (int)std::min<int64_t>((int64_t)d.sms * Tile::kBlocks, slots * chunks);
     };
     cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(kTileThreads);
+    cfg.blockDim = dim3(kTileThreads + kCopyThreads);
     cfg.dynamicSmemBytes = Tile::kSmem;
     cfg.stream = st;
     P.shrink_grid = grid(P.k);

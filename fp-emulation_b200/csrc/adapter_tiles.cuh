@@ -16,6 +16,7 @@
 #pragma once
 
 #include "adapter_kernels.cuh"
+#include "fpemu_barrier.cuh"
 
 namespace fpemu {
 
@@ -156,7 +157,9 @@ struct MiddleOf<__nv_bfloat16> {
     }
 };
 
-constexpr int kTileThreads = 256;
+constexpr int kTileThreads = 256;      // eight warps that compute
+constexpr int kCopyThreads = 64;       // and two that copy
+constexpr uint64_t kTileWaitNs = 2000000000ull;
 
 // Tiles in shared memory.  "Rank-major" weights have a row for each rank and
 // 128 bytes along the long dimension, "long-major" ones a row for each of its
@@ -175,12 +178,14 @@ struct AdapterTile {
     static constexpr int kRankBytes = RP * kPitchRank, kLongBytes = KC * kPitchLong;
     static constexpr int kStageX = kSlotRows * kPitchX;
     static constexpr int kStage = kStageX + (kRankBytes > kLongBytes ? kRankBytes : kLongBytes);
-    static constexpr int kStages = RP <= 32 ? 4 : 3;
     static constexpr int kPitchU = E == 2 ? RP + 8 : RP + 4;  // elements of Acc
-    static constexpr int kSmem = kStages * kStage + kSlotRows * kPitchU * (int)sizeof(Acc);
-    // Blocks an SM: by the registers that the sums need, and by shared memory.
-    static constexpr int kWant = RP * E <= 64 ? 3 : RP * E <= 256 ? 2 : 1, kFit = 232448 / (kSmem + 4096);
-    static constexpr int kBlocks = kWant < kFit ? kWant : kFit;
+    static constexpr int kMiddle = kSlotRows * kPitchU * (int)sizeof(Acc);
+    // Two blocks an SM where the registers for a rank's sums allow it, and as many chunks in flight as fit.
+    static constexpr int kBlocks = RP * E <= 128 ? 2 : 1;
+    static constexpr int kFit = ((kBlocks == 2 ? 110000 : 222000) - kMiddle) / kStage;
+    static constexpr int kStages = kFit < 8 ? kFit : 8;
+    static constexpr int kSmem = kStages * kStage + kMiddle;
+    static_assert(kStages >= 3, "the copies of a chunk overlap the work on others");
     // The results of a warp's two rows are 16 bytes of neighbouring columns for each thread: column
     // q * V + 2 t + b of a group of 4 V stands where the instruction has column 2 q + b of its tile t.
     // Long-major weights are laid out in that order; 16-bit rank-major ones (read transposed, eight
@@ -202,7 +207,8 @@ __device__ void plain_rows(const AdapterParams& P, const int* list, int count, b
     T* y = static_cast<T*>(P.y);
     const T fill = narrow<T>(bad ? (Acc)__longlong_as_double(0x7ff8000000000000ll) : (Acc)0);
     const bool vec = !bad && base && copy_unit<T>(base, P.base_row) == 16 && copy_unit<T>(y, P.y_row) == 16;
-    const int warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32, len = n1 - n0;
+    constexpr int warps = kTileThreads / 32;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, len = n1 - n0;
     const int whole = vec ? len / V * V : 0;  // of a row, copied 16 bytes at a time
     for (int first = warp; first < count; first += 8 * warps) {
         // Eight rows of a warp with their loads in flight together.
@@ -228,26 +234,23 @@ __device__ void plain_rows(const AdapterParams& P, const int* list, int count, b
     }
 }
 
-// 64 gathered rows by 128 bytes: this thread's 16 bytes of rows tid / 8 and tid / 8 + 32.
+// 64 gathered rows by 128 bytes: a copying thread's 16 bytes of every eighth row.
 template <typename T, int PITCH>
 struct RowTile {
-    static constexpr int V = 16 / (int)sizeof(T), KC = 8 * V;
-    const T* p[2];
-    bool ok[2];
-    __device__ __forceinline__ void aim(const T* src, int64_t stride, const int* list, int count, int64_t c0) {
+    static constexpr int V = 16 / (int)sizeof(T), KC = 8 * V, N = kSlotRows * 8 / kCopyThreads;
+    const T* p[N];
+    int count;
+    __device__ __forceinline__ void aim(int t, const T* src, int64_t stride, const int* list, int rows, int64_t c0) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int t = threadIdx.x / 8 + 32 * i;
-            p[i] = src + list[t] * stride + c0 + threadIdx.x % 8 * V;
-            ok[i] = t < count;
-        }
+        for (int i = 0; i < N; ++i) p[i] = src + list[t / 8 + 8 * i] * stride + c0 + t % 8 * V;
+        count = rows;
     }
     // `left` elements of the rows are there; moves on to the next chunk.
-    __device__ __forceinline__ void fetch(uint8_t* st, int left, int unit) {
-        const int here = left - (int)(threadIdx.x % 8) * V, avail = here < 0 ? 0 : here > V ? V : here;
+    __device__ __forceinline__ void fetch(int t, uint8_t* st, int left, int unit) {
+        const int here = left - t % 8 * V, avail = here < 0 ? 0 : here > V ? V : here;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            fetch16(st + (threadIdx.x / 8 + 32 * i) * PITCH + threadIdx.x % 8 * 16, p[i], ok[i] ? avail : 0, unit);
+        for (int i = 0; i < N; ++i) {
+            fetch16(st + (t / 8 + 8 * i) * PITCH + t % 8 * 16, p[i], t / 8 + 8 * i < count ? avail : 0, unit);
             p[i] += KC;
         }
     }
@@ -258,20 +261,19 @@ struct RowTile {
 template <typename T, int RP, bool LONG, int PITCH, typename Place>
 struct WeightTile {
     static constexpr int E = sizeof(T), V = 16 / E, KC = 8 * V;
-    static constexpr int UPR = LONG ? RP * E / 16 : 8, SKIP = kTileThreads / UPR, N = (RP + 31) / 32;
+    static constexpr int UPR = LONG ? RP * E / 16 : 8, SKIP = kCopyThreads / UPR, N = RP / 8;
     const T* p;
-    __device__ __forceinline__ void aim(const T* w, int64_t stride, int64_t c0) {
-        p = w + (threadIdx.x / UPR + (LONG ? c0 : 0)) * stride + threadIdx.x % UPR * V + (LONG ? 0 : c0);
+    __device__ __forceinline__ void aim(int t, const T* w, int64_t stride, int64_t c0) {
+        p = w + (t / UPR + (LONG ? c0 : 0)) * stride + t % UPR * V + (LONG ? 0 : c0);
     }
-    __device__ __forceinline__ void fetch(uint8_t* wt, int64_t stride, int r, int left, int unit) {
-        const int l = threadIdx.x / UPR, j = threadIdx.x % UPR * V;
-        if (RP >= 32 || threadIdx.x < 8 * RP) {
+    __device__ __forceinline__ void fetch(int t, uint8_t* wt, int64_t stride, int r, int left, int unit) {
+        const int l = t / UPR, j = t % UPR * V, here = LONG ? r - j : left - j;
+        const int avail = here < 0 ? 0 : here > V ? V : here;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int row = l + i * SKIP, here = LONG ? r - j : left - j;
-                const int avail = (LONG ? row >= left : row >= r) || here < 0 ? 0 : here > V ? V : here;
-                fetch16(wt + (LONG ? Place::at(row) : row) * PITCH + j * E, p + i * SKIP * stride, avail, unit);
-            }
+        for (int i = 0; i < N; ++i) {
+            const int row = l + i * SKIP;
+            fetch16(wt + (LONG ? Place::at(row) : row) * PITCH + j * E, p + i * SKIP * stride,
+                    (LONG ? row < left : row < r) ? avail : 0, unit);
         }
         p += LONG ? KC * stride : KC;
     }
@@ -280,34 +282,63 @@ struct InPlace {
     static __device__ __forceinline__ int at(int c) { return c; }
 };
 
-// The slots of a block's stretch: rows and record of the slot that is being
-// fetched and of those behind it that are still being computed, with the loads of
-// the next ones under way.
+template <int ID, int N>
+__device__ __forceinline__ void named_barrier() {
+    asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
+}
+constexpr int kCopyBarrier = 1, kWorkBarrier = 2;
+
+// The ring of chunks: a buffer is full when every copying thread's copies have
+// arrived (and what it wrote itself is visible), and free again when each of the
+// eight computing warps has left it.  So a warp runs ahead of another by as many
+// chunks as there are buffers, and loads, products and stores overlap.
+template <int S>
+struct ChunkRing {
+    uint64_t full[S], empty[S];
+    __device__ __forceinline__ void init() {
+        if (threadIdx.x == 0) {
+#pragma unroll
+            for (int i = 0; i < S; ++i) mbar_init(&full[i], 2 * kCopyThreads), mbar_init(&empty[i], kTileThreads / 32);
+            fence_barrier_init();
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ void copied(int s) {
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(shared_address(&full[s])) : "memory");
+        mbar_arrive(&full[s]);
+    }
+    __device__ __forceinline__ void left(int s) {
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&empty[s]);
+    }
+};
+
+// The slots of a block's stretch, for the copying threads: rows and record of the
+// slot that is being fetched and of those behind it that are still being computed,
+// with the loads of the next ones under way.
 struct SlotFeed {
-    static constexpr int kRing = 8;
+    static constexpr int kRing = 16;  // a chunk in flight each, at most
     int (*list)[kSlotRows];   // [kRing], shared
     AdapterSlot* rec;         // [kRing], shared
     const AdapterSlot* slots;
     const int32_t* perm;
-    int busy, slot;           // how many; the one that enter() makes current next
+    int busy, t;              // slots; this thread, of kCopyThreads
+    int slot;                 // the one that enter() makes current next
     AdapterSlot next, after;
     int id;
-    __device__ __forceinline__ int load_id(const AdapterSlot& s) {
-        const int t = threadIdx.x;
-        return t < kSlotRows ? perm[s.start + (t < s.count ? t : 0)] : 0;
-    }
+    __device__ __forceinline__ int load_id(const AdapterSlot& s) { return perm[s.start + (t < s.count ? t : 0)]; }
     __device__ __forceinline__ AdapterSlot load(int i) const { return slots[i < busy ? i : busy - 1]; }
     __device__ __forceinline__ void begin(int first) {
         slot = first;
         next = load(first), after = load(first + 1);
         id = load_id(next);
     }
-    // All threads; returns the slot whose rows are now in list[slot % kRing].
+    // All copying threads; returns the slot whose rows are now in list[(slot - 1) % kRing].
     __device__ __forceinline__ AdapterSlot enter() {
         const int at = slot % kRing;
-        if (threadIdx.x < kSlotRows) list[at][threadIdx.x] = id;
-        if (threadIdx.x == 0) rec[at] = next;
-        __syncthreads();
+        list[at][t] = id;
+        if (t == 0) rec[at] = next;
+        named_barrier<kCopyBarrier, kCopyThreads>();
         const AdapterSlot now = next;
         next = after;
         id = load_id(next);
@@ -337,16 +368,17 @@ struct ChunkShare {
 // and half of the rank for each they would read it twice, and the loads from shared
 // memory would bind the kernel.)
 template <typename T, bool TR, int RP>
-__global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
+__global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR, RP>::kBlocks)
     adapter_shrink_kernel(const __grid_constant__ AdapterParams P) {
     using Tile = AdapterTile<T, TR, RP>;
     using Acc = typename Tile::Acc;
     constexpr int E = Tile::E, KC = Tile::KC, S = Tile::kStages;
-    constexpr int MT = RP * (E == 4 ? 2 : 1) < 128 ? 2 : 1, RG = 4 / MT, KW = 8 / RG, NT = RP / 8;
+    constexpr int MT = RP < (E == 4 ? 32 : 128) ? 2 : 1, RG = 4 / MT, KW = 8 / RG, NT = RP / 8;
     constexpr int FLUSH = 4;  // chunks that the tensor cores sum by themselves, for floats
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int list[SlotFeed::kRing][kSlotRows];
     __shared__ AdapterSlot rec[SlotFeed::kRing];
+    __shared__ ChunkRing<S> ring;
     cudaTriggerProgrammaticLaunchCompletion();
     const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, q = lane & 3;
     const int rows0 = (tid >> 5) % RG * 16 * MT, kw = (tid >> 5) / RG;
@@ -357,30 +389,39 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
     if ((int)blockIdx.x >= share.blocks) return;
     const int64_t begin = share.first(blockIdx.x);
     const int chunks = (int)(share.first(blockIdx.x + 1) - begin);
-    SlotFeed feed{list, rec, plan_busy(P), plan_perm(P), busy};
-    feed.begin((int)(begin / per));
-    const T* x = static_cast<const T*>(P.x);
-    const T* w1 = static_cast<const T*>(P.w1);
-    const int unit_x = copy_unit<T>(x, P.x_row), unit_w = copy_unit2<T>(w1, P.w1_row, P.w1_adapter);
-
-    RowTile<T, Tile::kPitchX> xt;
-    WeightTile<T, RP, TR, TR ? Tile::kPitchLong : Tile::kPitchRank, InPlace> wt;
-    uint32_t load = 0, use = 0;
-    auto next = [](uint32_t& stage) { stage = stage == (S - 1) * Tile::kStage ? 0 : stage + Tile::kStage; };
-    int fetch_at = (int)(begin % per);  // the next chunk to fetch, within its slot
-    bool enter = true;
-    auto fetch = [&]() {
-        if (enter) {
-            const AdapterSlot s = feed.enter();
-            xt.aim(x, P.x_row, list[(feed.slot - 1) % SlotFeed::kRing], s.count, (int64_t)fetch_at * KC);
-            wt.aim(w1 + s.cls * P.w1_adapter, P.w1_row, (int64_t)fetch_at * KC);
+    ring.init();
+    if (tid >= kTileThreads) {
+        const int t = tid - kTileThreads;
+        const T* x = static_cast<const T*>(P.x);
+        const T* w1 = static_cast<const T*>(P.w1);
+        const int unit_x = copy_unit<T>(x, P.x_row), unit_w = copy_unit2<T>(w1, P.w1_row, P.w1_adapter);
+        RowTile<T, Tile::kPitchX> xt;
+        WeightTile<T, RP, TR, TR ? Tile::kPitchLong : Tile::kPitchRank, InPlace> wt;
+        SlotFeed feed{list, rec, plan_busy(P), plan_perm(P), busy, t};
+        feed.begin((int)(begin / per));
+        int at = (int)(begin % per), stage = 0;
+        uint32_t round = 1;
+        for (int c = 0; c < chunks; ++c) {
+            if (c >= S && !mbar_wait(&ring.empty[stage], round, kTileWaitNs)) {
+                report_error(P.sink.dev, P.sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterEmpty, c);
+                break;
+            }
+            if (c == 0 || at == 0) {
+                const AdapterSlot s = feed.enter();
+                xt.aim(t, x, P.x_row, list[(feed.slot - 1) % SlotFeed::kRing], s.count, (int64_t)at * KC);
+                wt.aim(t, w1 + s.cls * P.w1_adapter, P.w1_row, (int64_t)at * KC);
+            }
+            uint8_t* st = smem + stage * Tile::kStage;
+            xt.fetch(t, st, k - at * KC, unit_x);
+            wt.fetch(t, st + Tile::kStageX, P.w1_row, P.r, k - at * KC, unit_w);
+            ring.copied(stage);
+            if (++at == per) at = 0;
+            if (++stage == S) stage = 0, round ^= 1;
         }
-        const int left = k - fetch_at * KC;
-        xt.fetch(smem + load, left, unit_x);
-        wt.fetch(smem + load + Tile::kStageX, P.w1_row, P.r, left, unit_w);
-        enter = ++fetch_at == per;
-        if (enter) fetch_at = 0;
-    };
+        copy_commit();
+        copy_wait<0>();
+        return;
+    }
 
     Acc acc[MT][NT][4] = {}, sum[E == 4 ? MT : 1][E == 4 ? NT : 1][4] = {};
     auto flush = [&]() {
@@ -479,24 +520,25 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
                             acc[m][t][e] = 0;
                         }
             }
-            __syncthreads();
+            named_barrier<kWorkBarrier, kTileThreads>();
         }
         Acc* out = static_cast<Acc*>(P.parts) + part * (kSlotRows * RP);
         for (int i = tid; i < kSlotRows * RP; i += kTileThreads) out[i] = red[i / RP * Tile::kPitchU + i % RP];
     };
 
-    int at = (int)(begin % per), slot = (int)(begin / per);
-    for (int c = 1 - S; c < chunks; ++c) {
-        if (c >= 0) {
-            copy_wait<S - 2>();
-            __syncthreads();  // chunk c has arrived for all; chunk c - 1's buffer is free
+    int at = (int)(begin % per), slot = (int)(begin / per), stage = 0;
+    uint32_t round = 0;
+    bool ok = true;
+    for (int c = 0; c < chunks; ++c) {
+        if (ok && !mbar_wait(&ring.full[stage], round, kTileWaitNs)) {
+            report_error(P.sink.dev, P.sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterFull, c);
+            ok = false;  // what is left becomes NaN
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[m][0][0] = (Acc)__longlong_as_double(0x7ff8000000000000ll);
         }
-        if (c + S - 1 < chunks) fetch();
-        next(load);
-        copy_commit();
-        if (c < 0) continue;
-        if (rows0 < rec[slot % SlotFeed::kRing].count) shrink(smem + use);
-        next(use);
+        if (ok && rows0 < rec[slot % SlotFeed::kRing].count) shrink(smem + stage * Tile::kStage);
+        ring.left(stage);
+        if (++stage == S) stage = 0, round ^= 1;
         if (c % FLUSH == FLUSH - 1) flush();
         if (++at == per || c + 1 == chunks) {
             leave((int64_t)blockIdx.x + slot);
@@ -507,7 +549,7 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
 
 // y: eight warps, four groups of 16 rows by the halves of every chunk's columns.
 template <typename T, bool TR, int RP>
-__global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
+__global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR, RP>::kBlocks)
     adapter_expand_kernel(const __grid_constant__ AdapterParams P) {
     using Tile = AdapterTile<T, TR, RP>;
     using Acc = typename Tile::Acc;
@@ -515,6 +557,7 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int list[SlotFeed::kRing][kSlotRows];
     __shared__ AdapterSlot rec[SlotFeed::kRing];
+    __shared__ ChunkRing<S> ring;
     const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, q = lane & 3;
     const int rows0 = (tid >> 5 & 3) * 16, half = tid >> 7;
     const int32_t* header = P.plan + plan_header_word(P.rows, P.adapters);
@@ -530,27 +573,40 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
     const int chunks = here ? (int)(share.first(blockIdx.x + 1) - begin) : 0;
     const int kper = ((int)P.k + KC - 1) / KC;
     const ChunkShare kshare(busy > 0 ? busy : 1, kper > 0 ? kper : 1, P.shrink_grid);
-    SlotFeed feed{list, rec, plan_busy(P), plan_perm(P), busy};
-    if (here) feed.begin((int)(begin / per));
-
-    RowTile<T, Tile::kPitchX> bt;
-    WeightTile<T, RP, !TR, TR ? Tile::kPitchRank : Tile::kPitchLong, Tile> wt;
-    uint32_t load = 0, use = 0;
-    auto next = [](uint32_t& stage) { stage = stage == (S - 1) * Tile::kStage ? 0 : stage + Tile::kStage; };
-    int fetch_at = (int)(begin % per);
-    bool enter = true;
-    auto fetch = [&]() {
-        if (enter) {
-            const AdapterSlot s = feed.enter();
-            if (base) bt.aim(base, P.base_row, list[(feed.slot - 1) % SlotFeed::kRing], s.count, (int64_t)fetch_at * KC);
-            wt.aim(w2 + s.cls * P.w2_adapter, P.w2_row, (int64_t)fetch_at * KC);
+    ring.init();
+    // Rows without an adapter, an eighth of the columns at a time, by the threads that compute.
+    constexpr int kParts = 8;
+    const int width = (n + kParts * V - 1) / (kParts * V) * V;
+    if (tid >= kTileThreads) {
+        const int t = tid - kTileThreads;
+        RowTile<T, Tile::kPitchX> bt;
+        WeightTile<T, RP, !TR, TR ? Tile::kPitchRank : Tile::kPitchLong, Tile> wt;
+        SlotFeed feed{list, rec, plan_busy(P), plan_perm(P), busy, t};
+        if (here) feed.begin((int)(begin / per));
+        int at = (int)(begin % per), stage = 0;
+        uint32_t round = 1;
+        for (int c = 0; c < chunks; ++c) {
+            if (c >= S && !mbar_wait(&ring.empty[stage], round, kTileWaitNs)) {
+                report_error(P.sink.dev, P.sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterEmpty, c);
+                break;
+            }
+            if (c == 0 || at == 0) {
+                const AdapterSlot s = feed.enter();
+                if (base) bt.aim(t, base, P.base_row, list[(feed.slot - 1) % SlotFeed::kRing], s.count, (int64_t)at * KC);
+                wt.aim(t, w2 + s.cls * P.w2_adapter, P.w2_row, (int64_t)at * KC);
+            }
+            uint8_t* st = smem + stage * Tile::kStage;
+            if (base) bt.fetch(t, st, n - at * KC, unit_base);
+            wt.fetch(t, st + Tile::kStageX, P.w2_row, P.r, n - at * KC, unit_w);
+            ring.copied(stage);
+            if (++at == per) at = 0;
+            if (++stage == S) stage = 0, round ^= 1;
         }
-        const int left = n - fetch_at * KC;
-        if (base) bt.fetch(smem + load, left, unit_base);
-        wt.fetch(smem + load + Tile::kStageX, P.w2_row, P.r, left, unit_w);
-        enter = ++fetch_at == per;
-        if (enter) fetch_at = 0;
-    };
+        copy_commit();
+        copy_wait<0>();
+        cudaGridDependencySynchronize();
+        return;
+    }
 
     Acc* us = reinterpret_cast<Acc*>(smem + S * Tile::kStage);
     // The middle as this thread's part of the left operand: 16-bit data split in
@@ -559,6 +615,7 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
     Acc uf[E == 2 ? 1 : RP / (E == 4 ? 8 : 4)][E == 4 ? 4 : 2];
     float back[2];
     T* yp[2];
+    bool ok = true;
     auto take_slot = [&](int slot, int at) {
         const AdapterSlot& now = rec[slot % SlotFeed::kRing];
         const int* rows = list[slot % SlotFeed::kRing];
@@ -576,7 +633,7 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
             if (P.u && at == 0 && r < P.r && row < now.count)
                 static_cast<typename MiddleOf<T>::type*>(P.u)[(int64_t)rows[row] * P.u_row + r] = MiddleOf<T>::pack(v);
         }
-        __syncthreads();
+        named_barrier<kWorkBarrier, kTileThreads>();
         const Acc* from = us + (rows0 + g) * Tile::kPitchU;
         if constexpr (E == 2) {
             float v[RP / 16][8];  // a0..a3 of two: rows g, g + 8, then columns + 8
@@ -732,33 +789,36 @@ __global__ void __launch_bounds__(kTileThreads, AdapterTile<T, TR, RP>::kBlocks)
     };
 
     cudaGridDependencySynchronize();  // the parts of u are there
-    int at = (int)(begin % per), slot = (int)(begin / per);
-    bool taken = false;
-    for (int c = 1 - S; c < chunks; ++c) {
-        if (c >= 0) {
-            copy_wait<S - 2>();
-            __syncthreads();  // chunk c has arrived for all; chunk c - 1's buffer is free
+    int at = (int)(begin % per), slot = (int)(begin / per), stage = 0;
+    uint32_t round = 0;
+    for (int c = 0; c < chunks; ++c) {
+        if (ok && !mbar_wait(&ring.full[stage], round, kTileWaitNs)) {
+            report_error(P.sink.dev, P.sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterFull, c);
+            ok = false;
         }
-        if (c + S - 1 < chunks) fetch();
-        next(load);
-        copy_commit();
-        if (c < 0) continue;
-        if (!taken) take_slot(slot, at);
-        taken = true;
+        if (!ok) {  // what is left becomes NaN
+            const AdapterSlot s = plan_busy(P)[slot];
+            const T nan = narrow<T>((Acc)__longlong_as_double(0x7ff8000000000000ll));
+            for (int i = lane; i < 16 * (KC / 2); i += 32) {
+                const int row = rows0 + i / (KC / 2), col = at * KC + half * (KC / 2) + i % (KC / 2);
+                if (row < s.count && col < n) static_cast<T*>(P.y)[plan_perm(P)[s.start + row] * P.y_row + col] = nan;
+            }
+            if (++at == per) at = 0, ++slot;
+            continue;
+        }
+        if (c == 0 || at == 0) take_slot(slot, at);
         const int count = rec[slot % SlotFeed::kRing].count;
-        if (rows0 < count) expand(smem + use, n - at * KC, list[slot % SlotFeed::kRing], count);
-        next(use);
-        if (++at == per) at = 0, ++slot, taken = false;
+        if (rows0 < count) expand(smem + stage * Tile::kStage, n - at * KC, list[slot % SlotFeed::kRing], count);
+        ring.left(stage);
+        if (++stage == S) stage = 0, round ^= 1;
+        if (++at == per) at = 0, ++slot;
     }
-    // Rows without an adapter, an eighth of the columns at a time.
-    constexpr int kParts = 8;
     const AdapterSlot* last = plan_busy(P) + plan_slots(P.rows, P.adapters) - 1;
-    const int width = (n + kParts * V - 1) / (kParts * V) * V;
     for (int i = blockIdx.x; i < idle * kParts; i += gridDim.x) {
         const AdapterSlot s = last[-(i / kParts)];
-        __syncthreads();
+        named_barrier<kWorkBarrier, kTileThreads>();
         if (tid < s.count) list[0][tid] = plan_perm(P)[s.start + tid];
-        __syncthreads();
+        named_barrier<kWorkBarrier, kTileThreads>();
         plain_rows<T>(P, list[0], s.count, s.cls != P.adapters, min(i % kParts * width, n), min((i % kParts + 1) * width, n));
     }
 }

@@ -17,6 +17,8 @@ struct DeviceError {
 
 enum : int {
     kWhereAdapterIndex = 16,  // a row's adapter id is neither -1 nor an adapter
+    kWaitAdapterFull = 17,    // an adapter kernel's warp waiting for a chunk
+    kWaitAdapterEmpty = 18,   // its copying warps waiting for a free buffer
 };
 
 // First failure wins; `host` is the pinned mirror (null until it is watched).
