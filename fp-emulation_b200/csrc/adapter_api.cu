@@ -77,6 +77,49 @@ int padded_rank(int64_t r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 :
 
 constexpr int kMostBlocks = 2;  // of a tile kernel on an SM
 
+template <typename T>
+constexpr CUtensorMapDataType map_type() {
+    return sizeof(T) == 8 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT64
+           : sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+           : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+template <typename T>
+bool map_ok(const void* p, int64_t stride) {
+    return p != nullptr && reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride > 0 && stride * (int64_t)sizeof(T) % 16 == 0 &&
+           stride < (int64_t(1) << 36);
+}
+
+// Rows of `length` elements that are gathered four at a time, 128 bytes of each.
+template <typename T>
+bool make_row_map(CUtensorMap* map, const void* p, int64_t stride, int64_t length, int64_t rows) {
+    auto enc = tensor_map_encoder();
+    if (enc == nullptr || !map_ok<T>(p, stride) || stride < length) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)length, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * sizeof(T)};
+    const cuuint32_t box[2] = {128 / (cuuint32_t)sizeof(T), 1}, step[2] = {1, 1};
+    return enc(map, map_type<T>(), 2, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// All adapters' weights as (inner, outer / turns, turns, adapter): element `turns` i + p of the outer
+// dimension is (i, p), so that a box can hold them in the order of p.
+template <typename T>
+bool make_weight_map(CUtensorMap* map, const void* p, int64_t row, int64_t adapter, int64_t inner, int64_t outer,
+                     int64_t adapters, int turns, int inner_box, int outer_box) {
+    auto enc = tensor_map_encoder();
+    if (adapters == 1) adapter = row;  // unused, but it has to be a stride
+    if (enc == nullptr || !map_ok<T>(p, row) || !map_ok<T>(p, adapter) || outer % turns != 0) return false;
+    const cuuint64_t e = sizeof(T);
+    const cuuint64_t dims[4] = {(cuuint64_t)inner, (cuuint64_t)(outer / turns), (cuuint64_t)turns, (cuuint64_t)adapters};
+    const cuuint64_t strides[3] = {(cuuint64_t)(turns * row) * e, (cuuint64_t)row * e, (cuuint64_t)adapter * e};
+    const cuuint32_t box[4] = {(cuuint32_t)inner_box, (cuuint32_t)outer_box, (cuuint32_t)turns, 1}, step[4] = {1, 1, 1, 1};
+    const int bytes = inner_box * (int)e;
+    return enc(map, map_type<T>(), 4, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, bool TR, int RP>
 int launch_tiles_rank(AdapterParams& P, const DevInfo& d, cudaStream_t st) {
     using Tile = AdapterTile<T, TR, RP>;
@@ -90,13 +133,24 @@ int launch_tiles_rank(AdapterParams& P, const DevInfo& d, cudaStream_t st) {
         const int64_t chunks = std::max<int64_t>((length + Tile::KC - 1) / Tile::KC, 1);
         return (int)std::min<int64_t>((int64_t)d.sms * Tile::kBlocks, slots * chunks);
     };
+    // Each product's rows and weights by TMA where they are aligned for it (few strides are not).
+    CUtensorMap maps[4] = {};
+    constexpr int inner = Tile::kInner / (int)sizeof(T);
+    auto weights = [&](CUtensorMap* map, const void* w, int64_t row, int64_t adapter, int64_t length, bool by_long, int turns) {
+        return by_long ? make_weight_map<T>(map, w, row, adapter, P.r, length, P.adapters, turns, inner, Tile::KC / turns)
+                       : make_weight_map<T>(map, w, row, adapter, length, P.r, P.adapters, 1, Tile::KC, RP);
+    };
+    P.tma1 = P.k > 0 && make_row_map<T>(&maps[0], P.x, P.x_row, P.k, P.rows) &&
+             weights(&maps[1], P.w1, P.w1_row, P.w1_adapter, P.k, TR, 1);
+    P.tma2 = P.n > 0 && (P.base == nullptr || make_row_map<T>(&maps[2], P.base, P.base_row, P.n, P.rows)) &&
+             weights(&maps[3], P.w2, P.w2_row, P.w2_adapter, P.n, !TR, TR ? 1 : Tile::NT);
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(kTileThreads + kCopyThreads);
     cfg.dynamicSmemBytes = Tile::kSmem;
     cfg.stream = st;
     P.shrink_grid = grid(P.k);
     cfg.gridDim = dim3((unsigned)P.shrink_grid);
-    if (P.k > 0) FPEMU_CUDA(cudaLaunchKernelEx(&cfg, shrink, P));
+    if (P.k > 0) FPEMU_CUDA(cudaLaunchKernelEx(&cfg, shrink, P, maps[0], maps[1]));
     // The second kernel's blocks start as the first one's end, and wait for it before they read u.
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -104,7 +158,7 @@ int launch_tiles_rank(AdapterParams& P, const DevInfo& d, cudaStream_t st) {
     cfg.attrs = &attr;
     cfg.numAttrs = P.k > 0 ? 1 : 0;
     cfg.gridDim = dim3((unsigned)grid(P.n));
-    FPEMU_CUDA(cudaLaunchKernelEx(&cfg, expand, P));
+    FPEMU_CUDA(cudaLaunchKernelEx(&cfg, expand, P, maps[2], maps[3]));
     return FPEMU_OK;
 }
 

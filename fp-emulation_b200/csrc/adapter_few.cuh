@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kFewThreads) adapter_few_kernel(const __grid_c
                 split16<T>(at(2 * i) * down, at(2 * i + 1) * down, ua[t][2 * i], ua[t][2 * i + 1]);
         }
     }
-    constexpr int NT = V / 2;  // 8-column tiles of a group of KS columns, laid out as in AdapterTile::at
+    constexpr int NT = V / 2;  // 8-column tiles of a group of KS columns; a thread's results are 16 bytes of neighbours
     constexpr int UG = Tile::UG;
     for (int first = n0 + warp * KS; first < n1; first += W * KS * UG) {
         uint4 wv[UG][NT][JS], held[UG];

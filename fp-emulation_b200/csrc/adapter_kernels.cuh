@@ -196,6 +196,7 @@ struct AdapterParams {
     int u_row;
     void* parts;          // with a plan: the first product's partial sums
     int shrink_grid;      // blocks that leave them
+    int tma1, tma2;       // whether TMA copies what the first and the second product read
     ErrorSink sink;
 };
 

@@ -15,6 +15,8 @@
 // for 16-bit and 273 for tf32 data, which is enough there.
 #pragma once
 
+#include <cuda.h>
+
 #include "adapter_kernels.cuh"
 #include "fpemu_barrier.cuh"
 
@@ -161,39 +163,42 @@ constexpr int kTileThreads = 256;      // eight warps that compute
 constexpr int kCopyThreads = 64;       // and two that copy
 constexpr uint64_t kTileWaitNs = 2000000000ull;
 
-// Tiles in shared memory.  "Rank-major" weights have a row for each rank and
-// 128 bytes along the long dimension, "long-major" ones a row for each of its
-// elements and the rank along it.  The pitches keep the warps' fragment loads
-// free of bank conflicts: odd numbers of 16-byte units for ldmatrix; 4 (mod 16)
-// 8-byte units for f64; for f32, 4 or 8 (mod 32) words as the fragment runs
-// along the row or across rows.
+// Tiles in shared memory, as TMA writes them with 128-byte swizzle: rows of 128
+// bytes whose 16-byte units change places by the row.  "Rank-major" weights have a
+// row for each rank and 128 bytes along the long dimension.  "Long-major" ones have
+// a row for each of its elements and the rank along it, in sub-tiles of at most 128
+// bytes of rank (narrower rows have the narrower swizzles).  A warp's fragment loads
+// are free of bank conflicts, but for weights read across their rows by f32 and f64.
+__device__ __forceinline__ uint32_t tile_at(int row, int byte) { return row * 128 + (byte ^ (row & 7) << 4); }
+
 template <typename T, bool TR, int RP>
 struct AdapterTile {
     using Acc = typename AccOf<T>::type;
     static constexpr int E = sizeof(T), V = 16 / E;
-    static constexpr int KC = 128 / E;
-    static constexpr int kPitchX = E == 8 ? 160 : 144;
-    static constexpr int kPitchRank = E == 8 || (E == 4 && TR) ? 160 : 144;
-    static constexpr int kPitchLong = E == 8 ? (RP + 4) * 8 : E == 4 ? (RP + (TR ? 8 : 4)) * 4 : RP * 2 + 16;
-    static constexpr int kRankBytes = RP * kPitchRank, kLongBytes = KC * kPitchLong;
-    static constexpr int kStageX = kSlotRows * kPitchX;
-    static constexpr int kStage = kStageX + (kRankBytes > kLongBytes ? kRankBytes : kLongBytes);
-    static constexpr int kPitchU = E == 2 ? RP + 8 : RP + 4;  // elements of Acc
+    static constexpr int KC = 128 / E;                             // elements of a chunk along k or n
+    static constexpr int kStageX = kSlotRows * 128, kStage = kStageX + RP * 128;
+    static constexpr int kInner = RP * E < 128 ? RP * E : 128;     // bytes of a long-major row
+    static constexpr int kSubs = RP * E / kInner;
+    static constexpr int kPitchU = E == 2 ? RP + 8 : RP + 4;       // elements of Acc
     static constexpr int kMiddle = kSlotRows * kPitchU * (int)sizeof(Acc);
     // Two blocks an SM where the registers for a rank's sums allow it, and as many chunks in flight as fit.
     static constexpr int kBlocks = RP * E <= 128 ? 2 : 1;
-    static constexpr int kFit = ((kBlocks == 2 ? 110000 : 222000) - kMiddle) / kStage;
+    static constexpr int kFit = ((kBlocks == 2 ? 108000 : 220000) - kMiddle) / kStage;
     static constexpr int kStages = kFit < 8 ? kFit : 8;
-    static constexpr int kSmem = kStages * kStage + kMiddle;
+    static constexpr int kSmem = kStages * kStage + kMiddle + 1024;  // and room to align
     static_assert(kStages >= 3, "the copies of a chunk overlap the work on others");
-    // The results of a warp's two rows are 16 bytes of neighbouring columns for each thread: column
-    // q * V + 2 t + b of a group of 4 V stands where the instruction has column 2 q + b of its tile t.
-    // Long-major weights are laid out in that order; 16-bit rank-major ones (read transposed, eight
-    // neighbours at a time) are not, and their results go through the tile instead.
-    static constexpr bool kDirect = !(TR && E == 2);
-    __host__ __device__ static constexpr int at(int c) {
-        return kDirect ? c / (4 * V) * (4 * V) + c % V / 2 * 8 + c % (4 * V) / V * 2 + c % 2 : c;
+    static __device__ __forceinline__ uint32_t long_at(int row, int byte) {
+        const int sub = byte / kInner, in = byte % kInner;
+        const int turn = kInner == 128 ? row & 7 : kInner == 64 ? row >> 1 & 3 : row >> 2 & 1;
+        return sub * (KC * kInner) + row * kInner + (in ^ turn << 4);
     }
+    // The results of a warp's two rows are 16 bytes of neighbouring columns for each thread: column
+    // NT i + p of a chunk stands where the instruction has column i of its tile p.  Long-major weights of
+    // the second product are laid out in that order; 16-bit rank-major ones (read transposed, eight
+    // neighbours at a time) are not, and their results go through the tile instead.
+    static constexpr int NT = V / 2;
+    static constexpr bool kDirect = !(TR && E == 2);
+    static __device__ __forceinline__ int at(int c) { return c % NT * 16 + c / NT; }
 };
 
 // Rows without an adapter (base, or 0) or with an id that is none (NaN, so that a
@@ -235,7 +240,7 @@ __device__ void plain_rows(const AdapterParams& P, const int* list, int count, b
 }
 
 // 64 gathered rows by 128 bytes: a copying thread's 16 bytes of every eighth row.
-template <typename T, int PITCH>
+template <typename T>
 struct RowTile {
     static constexpr int V = 16 / (int)sizeof(T), KC = 8 * V, N = kSlotRows * 8 / kCopyThreads;
     const T* p[N];
@@ -250,15 +255,15 @@ struct RowTile {
         const int here = left - t % 8 * V, avail = here < 0 ? 0 : here > V ? V : here;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            fetch16(st + (t / 8 + 8 * i) * PITCH + t % 8 * 16, p[i], t / 8 + 8 * i < count ? avail : 0, unit);
+            fetch16(st + tile_at(t / 8 + 8 * i, t % 8 * 16), p[i], t / 8 + 8 * i < count ? avail : 0, unit);
             p[i] += KC;
         }
     }
 };
 
-// The weights of a chunk: LONG, a row of the rank for each of KC elements (laid
-// out by PLACE), or RP rows of KC elements.
-template <typename T, int RP, bool LONG, int PITCH, typename Place>
+// The weights of a chunk: LONG, a row of the rank for each of KC elements (in the
+// order of the results where PLACED), or RP rows of KC elements.
+template <typename T, typename Tile, int RP, bool LONG, bool PLACED>
 struct WeightTile {
     static constexpr int E = sizeof(T), V = 16 / E, KC = 8 * V;
     static constexpr int UPR = LONG ? RP * E / 16 : 8, SKIP = kCopyThreads / UPR, N = RP / 8;
@@ -272,15 +277,25 @@ struct WeightTile {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int row = l + i * SKIP;
-            fetch16(wt + (LONG ? Place::at(row) : row) * PITCH + j * E, p + i * SKIP * stride,
-                    (LONG ? row < left : row < r) ? avail : 0, unit);
+            fetch16(wt + (LONG ? Tile::long_at(PLACED ? Tile::at(row) : row, j * E) : tile_at(row, j * E)),
+                    p + i * SKIP * stride, (LONG ? row < left : row < r) ? avail : 0, unit);
         }
         p += LONG ? KC * stride : KC;
     }
 };
-struct InPlace {
-    static __device__ __forceinline__ int at(int c) { return c; }
-};
+
+// TMA: four gathered rows of a two-dimensional map, or a box of the weights' map
+// (see make_weight_map).  Alignment and bounds are the maps'; what lies outside is zero.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int col, const int (&r)[4]) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+                 " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(smem_u32(bar)), "r"(col), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ void tma_box4(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c3) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+                 " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(0), "r"(c3) : "memory");
+}
 
 template <int ID, int N>
 __device__ __forceinline__ void named_barrier() {
@@ -288,17 +303,18 @@ __device__ __forceinline__ void named_barrier() {
 }
 constexpr int kCopyBarrier = 1, kWorkBarrier = 2;
 
-// The ring of chunks: a buffer is full when every copying thread's copies have
-// arrived (and what it wrote itself is visible), and free again when each of the
-// eight computing warps has left it.  So a warp runs ahead of another by as many
+// The ring of chunks: a buffer is full when TMA's bytes or every copying thread's
+// copies have arrived (and what they wrote themselves is visible), and free again
+// when each of the eight computing warps has left it.  So a warp runs ahead of another by as many
 // chunks as there are buffers, and loads, products and stores overlap.
 template <int S>
 struct ChunkRing {
     uint64_t full[S], empty[S];
-    __device__ __forceinline__ void init() {
+    __device__ __forceinline__ void init(bool tma) {
         if (threadIdx.x == 0) {
 #pragma unroll
-            for (int i = 0; i < S; ++i) mbar_init(&full[i], 2 * kCopyThreads), mbar_init(&empty[i], kTileThreads / 32);
+            for (int i = 0; i < S; ++i)
+                mbar_init(&full[i], tma ? 1 : 2 * kCopyThreads), mbar_init(&empty[i], kTileThreads / 32);
             fence_barrier_init();
         }
         __syncthreads();
@@ -348,6 +364,109 @@ struct SlotFeed {
     }
 };
 
+// What a kernel streams: gathered rows (or none) and weights, `length` elements long.
+struct StreamParams {
+    const void *rows, *w;
+    int64_t row_stride, w_adapter, w_row;
+    int length, rank, no_row;      // no_row: a row index past the map's rows
+    const CUtensorMap *row_map, *w_map;
+    int tma;
+};
+
+// The copying warps of a block: its chunks from `at` of slot `slot` on.  By TMA
+// (the rows' strides and the pointers are multiples of 16 bytes): one warp, sixteen
+// lanes of which fetch four rows each, others a sub-tile of the weights.  Else both
+// warps copy 16 bytes, 4 or 8, or single values a thread, whatever the alignment.
+template <typename T, typename Tile, int RP, bool LONG, bool PLACED>
+__device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<Tile::kStages>& ring, uint8_t* smem,
+                                              int (*list)[kSlotRows], AdapterSlot* rec, const AdapterSlot* slots,
+                                              const int32_t* perm, int busy, int slot, int at, int per, int chunks,
+                                              ErrorSink sink) {
+    constexpr int S = Tile::kStages, KC = Tile::KC;
+    const int t = threadIdx.x - kTileThreads;
+    const T* rows = static_cast<const T*>(q.rows);
+    const T* w = static_cast<const T*>(q.w);
+    int stage = 0;
+    uint32_t round = 1;
+    auto free_stage = [&](int c) {
+        if (c < S || mbar_wait(&ring.empty[stage], round, kTileWaitNs)) return true;
+        report_error(sink.dev, sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterEmpty, c);
+        return false;
+    };
+    auto next_stage = [&]() {
+        if (++at == per) at = 0;
+        if (++stage == S) stage = 0, round ^= 1;
+    };
+    if (q.tma) {
+        if (t >= 32) return;
+        constexpr int kBoxes = LONG ? Tile::kSubs : 1, kNT = PLACED ? Tile::NT : 1;
+        auto load = [&](int i) { return slots[i < busy ? i : busy - 1]; };
+        int next_id[4], id[4] = {};
+        auto load_ids = [&](const AdapterSlot& s) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) next_id[i] = t < 16 && 4 * t + i < s.count ? perm[s.start + 4 * t + i] : -1;
+        };
+        AdapterSlot now{}, next = load(slot), after = load(slot + 1);
+        load_ids(next);
+        int c = 0;
+        for (; c < chunks; ++c) {
+            if (!free_stage(c)) break;
+            if (c == 0 || at == 0) {  // the next slot's rows; the loads of those behind it stay under way
+                now = next;
+                const int ring_at = slot % SlotFeed::kRing;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (t < 16) list[ring_at][4 * t + i] = next_id[i] < 0 ? 0 : next_id[i];
+                    id[i] = next_id[i] < 0 ? q.no_row : next_id[i];
+                }
+                if (t == 0) rec[ring_at] = now;
+                next = after;
+                load_ids(next);
+                ++slot;
+                after = load(slot + 1);
+            }
+            __syncwarp();
+            if (t == 0) mbar_arrive_expect_tx(&ring.full[stage], (rows ? Tile::kStageX : 0) + RP * 128);
+            __syncwarp();
+            const uint32_t st = shared_address(smem + stage * Tile::kStage);
+            if (t < 16) {
+                if (rows) tma_gather4(st + t * 512, q.row_map, &ring.full[stage], at * KC, id);
+            } else if (t - 16 < kBoxes) {
+                const int b = t - 16;
+                if (LONG)
+                    tma_box4(st + Tile::kStageX + b * (KC * Tile::kInner), q.w_map, &ring.full[stage],
+                             b * (Tile::kInner / Tile::E), at * (KC / kNT), now.cls);
+                else tma_box4(st + Tile::kStageX, q.w_map, &ring.full[stage], at * KC, 0, now.cls);
+            }
+            next_stage();
+        }
+        // Given up: what is under way has to land before the block may end.
+        if (c < chunks)
+            for (int i = c < S ? 0 : c - S; i < c; ++i) mbar_wait(&ring.full[i % S], i / S & 1, kTileWaitNs);
+        return;
+    }
+    RowTile<T> xt;
+    WeightTile<T, Tile, RP, LONG, PLACED> wt;
+    const int unit_rows = copy_unit<T>(rows, q.row_stride), unit_w = copy_unit2<T>(w, q.w_row, q.w_adapter);
+    SlotFeed feed{list, rec, slots, perm, busy, t};
+    if (chunks > 0) feed.begin(slot);
+    for (int c = 0; c < chunks; ++c) {
+        if (!free_stage(c)) break;
+        if (c == 0 || at == 0) {
+            const AdapterSlot s = feed.enter();
+            if (rows) xt.aim(t, rows, q.row_stride, list[(feed.slot - 1) % SlotFeed::kRing], s.count, (int64_t)at * KC);
+            wt.aim(t, w + s.cls * q.w_adapter, q.w_row, (int64_t)at * KC);
+        }
+        uint8_t* st = smem + stage * Tile::kStage;
+        if (rows) xt.fetch(t, st, q.length - at * KC, unit_rows);
+        wt.fetch(t, st + Tile::kStageX, q.w_row, q.rank, q.length - at * KC, unit_w);
+        ring.copied(stage);
+        next_stage();
+    }
+    copy_commit();
+    copy_wait<0>();
+}
+
 // Block b of `blocks` takes chunks [total b / blocks, total (b + 1) / blocks).  A
 // stretch is an eighth of a slot at least, so that a slot has few parts.
 struct ChunkShare {
@@ -369,13 +488,15 @@ struct ChunkShare {
 // memory would bind the kernel.)
 template <typename T, bool TR, int RP>
 __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR, RP>::kBlocks)
-    adapter_shrink_kernel(const __grid_constant__ AdapterParams P) {
+    adapter_shrink_kernel(const __grid_constant__ AdapterParams P, const __grid_constant__ CUtensorMap row_map,
+                          const __grid_constant__ CUtensorMap w_map) {
     using Tile = AdapterTile<T, TR, RP>;
     using Acc = typename Tile::Acc;
     constexpr int E = Tile::E, KC = Tile::KC, S = Tile::kStages;
     constexpr int MT = RP < (E == 4 ? 32 : 128) ? 2 : 1, RG = 4 / MT, KW = 8 / RG, NT = RP / 8;
     constexpr int FLUSH = 4;  // chunks that the tensor cores sum by themselves, for floats
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = raw + ((1024 - (shared_address(raw) & 1023)) & 1023);  // the swizzles repeat every 1024 bytes
     __shared__ int list[SlotFeed::kRing][kSlotRows];
     __shared__ AdapterSlot rec[SlotFeed::kRing];
     __shared__ ChunkRing<S> ring;
@@ -389,37 +510,11 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     if ((int)blockIdx.x >= share.blocks) return;
     const int64_t begin = share.first(blockIdx.x);
     const int chunks = (int)(share.first(blockIdx.x + 1) - begin);
-    ring.init();
+    ring.init(P.tma1);
     if (tid >= kTileThreads) {
-        const int t = tid - kTileThreads;
-        const T* x = static_cast<const T*>(P.x);
-        const T* w1 = static_cast<const T*>(P.w1);
-        const int unit_x = copy_unit<T>(x, P.x_row), unit_w = copy_unit2<T>(w1, P.w1_row, P.w1_adapter);
-        RowTile<T, Tile::kPitchX> xt;
-        WeightTile<T, RP, TR, TR ? Tile::kPitchLong : Tile::kPitchRank, InPlace> wt;
-        SlotFeed feed{list, rec, plan_busy(P), plan_perm(P), busy, t};
-        feed.begin((int)(begin / per));
-        int at = (int)(begin % per), stage = 0;
-        uint32_t round = 1;
-        for (int c = 0; c < chunks; ++c) {
-            if (c >= S && !mbar_wait(&ring.empty[stage], round, kTileWaitNs)) {
-                report_error(P.sink.dev, P.sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterEmpty, c);
-                break;
-            }
-            if (c == 0 || at == 0) {
-                const AdapterSlot s = feed.enter();
-                xt.aim(t, x, P.x_row, list[(feed.slot - 1) % SlotFeed::kRing], s.count, (int64_t)at * KC);
-                wt.aim(t, w1 + s.cls * P.w1_adapter, P.w1_row, (int64_t)at * KC);
-            }
-            uint8_t* st = smem + stage * Tile::kStage;
-            xt.fetch(t, st, k - at * KC, unit_x);
-            wt.fetch(t, st + Tile::kStageX, P.w1_row, P.r, k - at * KC, unit_w);
-            ring.copied(stage);
-            if (++at == per) at = 0;
-            if (++stage == S) stage = 0, round ^= 1;
-        }
-        copy_commit();
-        copy_wait<0>();
+        const StreamParams q{P.x, P.w1, P.x_row, P.w1_adapter, P.w1_row, k, P.r, (int)P.rows, &row_map, &w_map, P.tma1};
+        stream_chunks<T, Tile, RP, TR, false>(q, ring, smem, list, rec, plan_busy(P), plan_perm(P), busy,
+                                              (int)(begin / per), (int)(begin % per), per, chunks, P.sink);
         return;
     }
 
@@ -440,18 +535,15 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
         for (int i = 0; i < 4 / KW; ++i) {
             const int ks = kw * (4 / KW) + i;
             if constexpr (E == 2) {
-                const uint32_t xa = shared_address(st) + (rows0 + (lane & 15)) * Tile::kPitchX + (lane >> 4) * 16 + ks * 32;
-                const uint32_t wa = shared_address(ws) +
-                                    (TR ? (ks * 16 + (lane & 15)) * Tile::kPitchLong + (lane >> 4) * 16
-                                        : ((lane & 7) + (lane >> 4) * 8) * Tile::kPitchRank + (lane >> 3 & 1) * 16 + ks * 32);
+                const uint32_t xa = shared_address(st) + tile_at(rows0 + (lane & 15), ks * 32 + (lane >> 4) * 16);
                 uint32_t a[MT][4];
 #pragma unroll
-                for (int m = 0; m < MT; ++m) ldsm4(a[m], xa + m * 16 * Tile::kPitchX);
+                for (int m = 0; m < MT; ++m) ldsm4(a[m], xa + m * 16 * 128);
 #pragma unroll
                 for (int p = 0; p < RP / 16; ++p) {
                     uint32_t b[4];
-                    if (TR) ldsm4t(b, wa + p * 32);
-                    else ldsm4(b, wa + p * 16 * Tile::kPitchRank);
+                    if (TR) ldsm4t(b, shared_address(ws) + Tile::long_at(ks * 16 + (lane & 15), p * 32 + (lane >> 4) * 16));
+                    else ldsm4(b, shared_address(ws) + tile_at(p * 16 + (lane & 7) + (lane >> 4) * 8, ks * 32 + (lane >> 3 & 1) * 16));
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
                         mma16<T>(acc[m][2 * p], a[m], b[0], b[1]);
@@ -465,7 +557,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const Tf32Pair p = tf32_split(*reinterpret_cast<const float*>(
-                            st + (rows0 + m * 16 + g + (e & 1) * 8) * Tile::kPitchX + (ks * 8 + q + (e >> 1) * 4) * 4));
+                            st + tile_at(rows0 + m * 16 + g + (e & 1) * 8, (ks * 8 + q + (e >> 1) * 4) * 4)));
                         ah[m][e] = p.hi, al[m][e] = p.lo;
                     }
 #pragma unroll
@@ -475,7 +567,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
                     for (int e = 0; e < 2; ++e) {
                         const int kk = ks * 8 + q + e * 4, j = t * 8 + g;
                         b[e] = tf32_split(*reinterpret_cast<const float*>(
-                            ws + (TR ? kk * Tile::kPitchLong + j * 4 : j * Tile::kPitchRank + kk * 4)));
+                            ws + (TR ? Tile::long_at(kk, j * 4) : tile_at(j, kk * 4))));
                     }
 #pragma unroll
                     for (int m = 0; m < MT; ++m) mma_tf32(sum[m][t], ah[m], b[0].lo, b[1].lo);
@@ -485,18 +577,19 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
                     for (int m = 0; m < MT; ++m) mma_tf32(sum[m][t], ah[m], b[0].hi, b[1].hi);
                 }
             } else {
+                // The order of k is free: this one puts the four threads of a row into different banks.
+                const int kk = (q >> 1) * 8 + ks * 2 + (q & 1);
                 double a[MT][2];
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
                         a[m][h] = *reinterpret_cast<const double*>(
-                            st + (rows0 + m * 16 + h * 8 + g) * Tile::kPitchX + (ks * 4 + q) * 8);
+                            st + tile_at(rows0 + m * 16 + h * 8 + g, kk * 8));
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const int kk = ks * 4 + q, j = t * 8 + g;
-                    const double b = *reinterpret_cast<const double*>(
-                        ws + (TR ? kk * Tile::kPitchLong + j * 8 : j * Tile::kPitchRank + kk * 8));
+                    const int j = t * 8 + g;
+                    const double b = *reinterpret_cast<const double*>(ws + (TR ? Tile::long_at(kk, j * 8) : tile_at(j, kk * 8)));
 #pragma unroll
                     for (int m = 0; m < MT; ++m) mma_f64(acc[m][t], a[m][0], a[m][1], b);
                 }
@@ -550,11 +643,13 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
 // y: eight warps, four groups of 16 rows by the halves of every chunk's columns.
 template <typename T, bool TR, int RP>
 __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR, RP>::kBlocks)
-    adapter_expand_kernel(const __grid_constant__ AdapterParams P) {
+    adapter_expand_kernel(const __grid_constant__ AdapterParams P, const __grid_constant__ CUtensorMap row_map,
+                          const __grid_constant__ CUtensorMap w_map) {
     using Tile = AdapterTile<T, TR, RP>;
     using Acc = typename Tile::Acc;
     constexpr int E = Tile::E, V = Tile::V, KC = Tile::KC, S = Tile::kStages;
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = raw + ((1024 - (shared_address(raw) & 1023)) & 1023);  // the swizzles repeat every 1024 bytes
     __shared__ int list[SlotFeed::kRing][kSlotRows];
     __shared__ AdapterSlot rec[SlotFeed::kRing];
     __shared__ ChunkRing<S> ring;
@@ -564,8 +659,6 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     const int busy = header[0], idle = header[1];
     const int n = (int)P.n, per = n > 0 ? (n + KC - 1) / KC : 1;  // without columns, for u alone
     const T* base = static_cast<const T*>(P.base);
-    const T* w2 = static_cast<const T*>(P.w2);
-    const int unit_base = copy_unit<T>(base, P.base_row), unit_w = copy_unit2<T>(w2, P.w2_row, P.w2_adapter);
     const bool vec_y = copy_unit<T>(P.y, P.y_row) == 16;
     const ChunkShare share(busy > 0 ? busy : 1, per, gridDim.x);
     const bool here = busy > 0 && (int)blockIdx.x < share.blocks;
@@ -573,41 +666,20 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     const int chunks = here ? (int)(share.first(blockIdx.x + 1) - begin) : 0;
     const int kper = ((int)P.k + KC - 1) / KC;
     const ChunkShare kshare(busy > 0 ? busy : 1, kper > 0 ? kper : 1, P.shrink_grid);
-    ring.init();
+    ring.init(P.tma2);
     // Rows without an adapter, an eighth of the columns at a time, by the threads that compute.
     constexpr int kParts = 8;
     const int width = (n + kParts * V - 1) / (kParts * V) * V;
     if (tid >= kTileThreads) {
-        const int t = tid - kTileThreads;
-        RowTile<T, Tile::kPitchX> bt;
-        WeightTile<T, RP, !TR, TR ? Tile::kPitchRank : Tile::kPitchLong, Tile> wt;
-        SlotFeed feed{list, rec, plan_busy(P), plan_perm(P), busy, t};
-        if (here) feed.begin((int)(begin / per));
-        int at = (int)(begin % per), stage = 0;
-        uint32_t round = 1;
-        for (int c = 0; c < chunks; ++c) {
-            if (c >= S && !mbar_wait(&ring.empty[stage], round, kTileWaitNs)) {
-                report_error(P.sink.dev, P.sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterEmpty, c);
-                break;
-            }
-            if (c == 0 || at == 0) {
-                const AdapterSlot s = feed.enter();
-                if (base) bt.aim(t, base, P.base_row, list[(feed.slot - 1) % SlotFeed::kRing], s.count, (int64_t)at * KC);
-                wt.aim(t, w2 + s.cls * P.w2_adapter, P.w2_row, (int64_t)at * KC);
-            }
-            uint8_t* st = smem + stage * Tile::kStage;
-            if (base) bt.fetch(t, st, n - at * KC, unit_base);
-            wt.fetch(t, st + Tile::kStageX, P.w2_row, P.r, n - at * KC, unit_w);
-            ring.copied(stage);
-            if (++at == per) at = 0;
-            if (++stage == S) stage = 0, round ^= 1;
-        }
-        copy_commit();
-        copy_wait<0>();
+        const StreamParams q{P.base, P.w2, P.base_row, P.w2_adapter, P.w2_row, n, P.r, (int)P.rows, &row_map, &w_map, P.tma2};
+        stream_chunks<T, Tile, RP, !TR, !TR>(q, ring, smem, list, rec, plan_busy(P), plan_perm(P), busy,
+                                             (int)(begin / per), (int)(begin % per), per, chunks, P.sink);
         cudaGridDependencySynchronize();
         return;
     }
 
+    // f64: the rank that step t of this thread stands for (any order will do; this one spreads the banks).
+    auto rank_of = [&](int t) { return t / 4 * 16 + (q >> 1) * 8 + t % 4 * 2 + (q & 1); };
     Acc* us = reinterpret_cast<Acc*>(smem + S * Tile::kStage);
     // The middle as this thread's part of the left operand: 16-bit data split in
     // two and, for halves, scaled by a power of two per row; f32 and f64 plain.
@@ -675,7 +747,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
             for (int t = 0; t < RP / step; ++t)
 #pragma unroll
                 for (int e = 0; e < step / 2; ++e)
-                    uf[t][e] = from[(e & 1) * 8 * Tile::kPitchU + t * step + q + (e >> 1) * 4];
+                    uf[t][e] = from[(e & 1) * 8 * Tile::kPitchU + (E == 8 ? rank_of(t) : t * step + q + (e >> 1) * 4)];
         }
         // This thread's rows of y at its 16 bytes of the warp's group of columns.
 #pragma unroll
@@ -684,20 +756,18 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     };
 
     auto expand = [&](uint8_t* st, int left, const int* rows, int count) {
-        constexpr int NT = V / 2;  // 8-column tiles of a group
+        constexpr int NT = Tile::NT;  // 8-column tiles of the warp's half chunk
         const uint8_t* wt = st + Tile::kStageX;
         Acc c[NT][4] = {};
         if constexpr (E == 2) {
-            const uint32_t wa = shared_address(wt) +
-                                (TR ? (lane & 15) * Tile::kPitchRank + (half * 32 + (lane >> 4) * 8) * 2
-                                    : (half * 32 + (lane & 7) + (lane >> 4) * 8) * Tile::kPitchLong + (lane >> 3 & 1) * 16);
 #pragma unroll
             for (int t = 0; t < RP / 16; ++t) {
                 uint32_t b[2][4];
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    if (TR) ldsm4t(b[p], wa + t * 16 * Tile::kPitchRank + p * 32);
-                    else ldsm4(b[p], wa + p * 16 * Tile::kPitchLong + t * 32);
+                    if (TR) ldsm4t(b[p], shared_address(wt) + tile_at(t * 16 + (lane & 15), (half * 32 + p * 16 + (lane >> 4) * 8) * 2));
+                    else ldsm4(b[p], shared_address(wt) + Tile::long_at((2 * p + (lane >> 4)) * 16 + half * 8 + (lane & 7),
+                                                                        t * 32 + (lane >> 3 & 1) * 16));
                 }
 #pragma unroll
                 for (int p = 0; p < 4; ++p) mma16<T>(c[p], ul[t], b[p / 2][p % 2 * 2], b[p / 2][p % 2 * 2 + 1]);
@@ -705,6 +775,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
                 for (int p = 0; p < 4; ++p) mma16<T>(c[p], uh[t], b[p / 2][p % 2 * 2], b[p / 2][p % 2 * 2 + 1]);
             }
         } else if constexpr (E == 4) {
+            float rest[NT][4] = {};
 #pragma unroll
             for (int t = 0; t < RP / 8; ++t) {
                 uint32_t ah[4], al[4];
@@ -717,24 +788,30 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
                 for (int p = 0; p < NT; ++p) {
                     Tf32Pair b[2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {  // slot p * 8 + g of the group is its column g / 2 * V + 2 p + g % 2
+                    for (int e = 0; e < 2; ++e) {
                         const int j = t * 8 + q + e * 4;
                         b[e] = tf32_split(*reinterpret_cast<const float*>(
-                            wt + (TR ? j * Tile::kPitchRank + (half * 16 + g / 2 * V + 2 * p + g % 2) * 4
-                                     : (half * 16 + p * 8 + g) * Tile::kPitchLong + j * 4)));
+                            wt + (TR ? tile_at(j, (half * 16 + NT * g + p) * 4) : Tile::long_at(p * 16 + half * 8 + g, j * 4))));
                     }
-                    mma_tf32(c[p], ah, b[0].lo, b[1].lo);
-                    mma_tf32(c[p], al, b[0].hi, b[1].hi);
+                    mma_tf32(rest[p], ah, b[0].lo, b[1].lo);
                     mma_tf32(c[p], ah, b[0].hi, b[1].hi);
+                    mma_tf32(rest[p], al, b[0].hi, b[1].hi);
                 }
             }
+#pragma unroll
+            for (int p = 0; p < NT; ++p)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[p][e] += rest[p][e];
         } else {
+            double odd[4] = {};
 #pragma unroll
             for (int t = 0; t < RP / 4; ++t) {
-                const int j = t * 4 + q, l = half * 8 + g;
-                mma_f64(c[0], uf[t][0], uf[t][1], *reinterpret_cast<const double*>(
-                    wt + (TR ? j * Tile::kPitchRank + l * 8 : l * Tile::kPitchLong + j * 8)));
+                const int j = rank_of(t), l = half * 8 + g;
+                mma_f64(t % 2 ? odd : c[0], uf[t][0], uf[t][1], *reinterpret_cast<const double*>(
+                    wt + (TR ? tile_at(j, l * 8) : Tile::long_at(l, j * 8))));
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[0][e] += odd[e];
         }
         if constexpr (!Tile::kDirect) {
             // Through the tile: pairs of columns in, 16 bytes of a row out; base waits in the tile meanwhile.
@@ -742,7 +819,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int p = 0; p < NT; ++p) {
-                    T* o = reinterpret_cast<T*>(st + (rows0 + g + h * 8) * Tile::kPitchX) + half * 32 + p * 8 + 2 * q;
+                    T* o = reinterpret_cast<T*>(st + tile_at(rows0 + g + h * 8, half * 64 + p * 16 + 4 * q));
                     alignas(4) T v[2];
                     float a = c[p][2 * h], b = c[p][2 * h + 1];
                     if constexpr (std::is_same<T, __half>::value) a *= back[h], b *= back[h];
@@ -752,10 +829,11 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
                 }
             __syncwarp();
         }
+        const bool whole = vec_y && left >= KC;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             alignas(16) T v[V];
-            const uint8_t* tile = st + (rows0 + g + h * 8) * Tile::kPitchX + half * 64 + q * 16;
+            uint8_t* tile = st + tile_at(rows0 + g + h * 8, half * 64 + q * 16);
             if (!Tile::kDirect || base) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(tile);
             if constexpr (Tile::kDirect) {
 #pragma unroll
@@ -764,28 +842,29 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
                     for (int b = 0; b < 2; ++b) {
                         Acc a = c[p][2 * h + b];
                         if constexpr (std::is_same<T, __half>::value) a *= back[h];
-                        v[2 * p + b] = narrow<T>(base ? a + (Acc)widen(v[2 * p + b]) : a);
+                        v[NT * b + p] = narrow<T>(base ? a + (Acc)widen(v[NT * b + p]) : a);
                     }
             }
-            if (vec_y && left >= KC) {
+            if (whole) {
                 if (rows0 + g + h * 8 < count) *reinterpret_cast<uint4*>(yp[h]) = *reinterpret_cast<uint4*>(v);
             } else {
-                *reinterpret_cast<uint4*>(st + (rows0 + g + h * 8) * Tile::kPitchX + half * 64 + q * 16) =
-                    *reinterpret_cast<uint4*>(v);
+                *reinterpret_cast<uint4*>(tile) = *reinterpret_cast<uint4*>(v);
             }
             yp[h] += KC;
         }
-        if (!vec_y || left < KC) {  // element by element, neighbouring lanes on neighbouring columns
+        if (!whole) {  // element by element, neighbouring lanes on neighbouring columns
             constexpr int H = KC / 2;
             __syncwarp();
 #pragma unroll 4
             for (int i = lane; i < 16 * H; i += 32) {
-                const int row = rows0 + i / H, c = half * H + i % H;
-                if (row < count && c < left)
-                    static_cast<T*>(P.y)[rows[row] * P.y_row + n - left + c] =
-                        *reinterpret_cast<const T*>(st + row * Tile::kPitchX + c * E);
+                const int row = rows0 + i / H, col = half * H + i % H;
+                if (row < count && col < left)
+                    static_cast<T*>(P.y)[rows[row] * P.y_row + n - left + col] =
+                        *reinterpret_cast<const T*>(st + tile_at(row, col * E));
             }
         }
+        // The tile was written here and is next written by TMA.
+        if (!Tile::kDirect || !whole) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     };
 
     cudaGridDependencySynchronize();  // the parts of u are there

@@ -108,7 +108,9 @@ uint64_t wait_budget_ns() {
     return v;
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+}  // namespace
+
+PFN_cuTensorMapEncodeTiled_v12000 fpemu::tensor_map_encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -119,6 +121,8 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     }();
     return fn;
 }
+
+namespace {
 
 // 3-D map over int8 residues [n_mod][rows][res_ld] (K innermost), box
 // [1][box_rows][128 B], SWIZZLE_128B.  Out-of-range K and rows read as zero.

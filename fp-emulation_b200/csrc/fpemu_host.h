@@ -2,6 +2,8 @@
 // libfpemu.so: error text, device check, and where kernels record a failure.
 #pragma once
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -22,6 +24,9 @@ struct DevInfo {
 
 // The current device; fails unless it is sm_100.
 int device_info(DevInfo* out);
+
+// The driver's encoder of TMA tensor maps (null if the driver has none).
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
 // Device address of the record that fpemu_device_error() reads, and of its
 // host-visible copy (null until fpemu_watch_errors), for the current device.
