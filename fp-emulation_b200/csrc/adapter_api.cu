@@ -90,13 +90,13 @@ bool map_ok(const void* p, int64_t stride) {
            stride < (int64_t(1) << 36);
 }
 
-// Rows of `length` elements that are gathered four at a time, 128 bytes of each.
+// Rows of `length` elements in boxes of a slot's rows by 128 bytes.
 template <typename T>
 bool make_row_map(CUtensorMap* map, const void* p, int64_t stride, int64_t length, int64_t rows) {
     auto enc = tensor_map_encoder();
     if (enc == nullptr || !map_ok<T>(p, stride) || stride < length) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)length, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * sizeof(T)};
-    const cuuint32_t box[2] = {128 / (cuuint32_t)sizeof(T), 1}, step[2] = {1, 1};
+    const cuuint32_t box[2] = {128 / (cuuint32_t)sizeof(T), kSlotRows}, step[2] = {1, 1};
     return enc(map, map_type<T>(), 2, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -140,10 +140,11 @@ int launch_tiles_rank(AdapterParams& P, const DevInfo& d, cudaStream_t st) {
         return by_long ? make_weight_map<T>(map, w, row, adapter, P.r, length, P.adapters, turns, inner, Tile::KC / turns)
                        : make_weight_map<T>(map, w, row, adapter, length, P.r, P.adapters, 1, Tile::KC, RP);
     };
-    P.tma1 = P.k > 0 && make_row_map<T>(&maps[0], P.x, P.x_row, P.k, P.rows) &&
-             weights(&maps[1], P.w1, P.w1_row, P.w1_adapter, P.k, TR, 1);
-    P.tma2 = P.n > 0 && (P.base == nullptr || make_row_map<T>(&maps[2], P.base, P.base_row, P.n, P.rows)) &&
-             weights(&maps[3], P.w2, P.w2_row, P.w2_adapter, P.n, !TR, TR ? 1 : Tile::NT);
+    P.tma1 = P.tma2 = 0;
+    if (P.k > 0 && make_row_map<T>(&maps[0], P.x, P.x_row, P.k, P.rows)) P.tma1 |= kTmaRows;
+    if (P.k > 0 && weights(&maps[1], P.w1, P.w1_row, P.w1_adapter, P.k, TR, 1)) P.tma1 |= kTmaWeights;
+    if (P.n > 0 && make_row_map<T>(&maps[2], P.base, P.base_row, P.n, P.rows)) P.tma2 |= kTmaRows;
+    if (P.n > 0 && weights(&maps[3], P.w2, P.w2_row, P.w2_adapter, P.n, !TR, TR ? 1 : Tile::NT)) P.tma2 |= kTmaWeights;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(kTileThreads + kCopyThreads);
     cfg.dynamicSmemBytes = Tile::kSmem;

@@ -174,6 +174,8 @@ __global__ void __launch_bounds__(1024) adapter_pack_kernel(int64_t rows, int ad
     if (threadIdx.x < 2) plan[plan_header_word(rows, adapters) + threadIdx.x] = done[threadIdx.x];
 }
 
+constexpr int kTmaRows = 1, kTmaWeights = 2;
+
 struct AdapterParams {
     int64_t rows, k, n;
     int r, adapters;
@@ -196,7 +198,7 @@ struct AdapterParams {
     int u_row;
     void* parts;          // with a plan: the first product's partial sums
     int shrink_grid;      // blocks that leave them
-    int tma1, tma2;       // whether TMA copies what the first and the second product read
+    int tma1, tma2;       // which maps there are for the first and the second product
     ErrorSink sink;
 };
 

@@ -284,12 +284,14 @@ struct WeightTile {
     }
 };
 
-// TMA: four gathered rows of a two-dimensional map, or a box of the weights' map
-// (see make_weight_map).  Alignment and bounds are the maps'; what lies outside is zero.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int col, const int (&r)[4]) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
-                 " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)),
-                 "r"(smem_u32(bar)), "r"(col), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+// TMA: a box of consecutive rows, or of the weights' map (see make_weight_map).
+// What lies outside the maps is zero.  (Rows that do not follow one another are
+// copied by the threads: TMA's gather of four rows by 128 bytes took some 50 cycles
+// an instruction on an SM, 2.9 TB/s in all, where two warps' copies reach 4.2.)
+__device__ __forceinline__ void tma_box2(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+                 " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(smem_u32(bar)), "r"(c0), "r"(c1) : "memory");
 }
 __device__ __forceinline__ void tma_box4(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c3) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
@@ -303,25 +305,33 @@ __device__ __forceinline__ void named_barrier() {
 }
 constexpr int kCopyBarrier = 1, kWorkBarrier = 2;
 
-// The ring of chunks: a buffer is full when TMA's bytes or every copying thread's
+// The ring of chunks: a buffer is full when TMA's bytes and every copying thread's
 // copies have arrived (and what they wrote themselves is visible), and free again
 // when each of the eight computing warps has left it.  So a warp runs ahead of another by as many
 // chunks as there are buffers, and loads, products and stores overlap.
 template <int S>
 struct ChunkRing {
     uint64_t full[S], empty[S];
-    __device__ __forceinline__ void init(bool tma) {
+    __device__ __forceinline__ void init() {
         if (threadIdx.x == 0) {
 #pragma unroll
             for (int i = 0; i < S; ++i)
-                mbar_init(&full[i], tma ? 1 : 2 * kCopyThreads), mbar_init(&empty[i], kTileThreads / 32);
+                mbar_init(&full[i], 2 * kCopyThreads), mbar_init(&empty[i], kTileThreads / 32);
             fence_barrier_init();
         }
         __syncthreads();
     }
-    __device__ __forceinline__ void copied(int s) {
+    // One chunk: the threads' copies, and what thread 0 asks of TMA (`bytes` in all).  Every copying thread
+    // arrives twice, when its copies have landed and for what it wrote itself.
+    template <typename Copies, typename Tma>
+    __device__ __forceinline__ void copied_after(int s, int t, uint32_t bytes, Copies copies, Tma tma) {
+        if (t == 0 && bytes > 0) {
+            mbar_arrive_expect_tx(&full[s], bytes);
+            tma();
+        }
+        copies();
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(shared_address(&full[s])) : "memory");
-        mbar_arrive(&full[s]);
+        if (t > 0 || bytes == 0) mbar_arrive(&full[s]);
     }
     __device__ __forceinline__ void left(int s) {
         __syncwarp();
@@ -368,103 +378,71 @@ struct SlotFeed {
 struct StreamParams {
     const void *rows, *w;
     int64_t row_stride, w_adapter, w_row;
-    int length, rank, no_row;      // no_row: a row index past the map's rows
+    int length, rank;
     const CUtensorMap *row_map, *w_map;
-    int tma;
+    int tma;  // kTmaRows, kTmaWeights: which maps there are
 };
 
-// The copying warps of a block: its chunks from `at` of slot `slot` on.  By TMA
-// (the rows' strides and the pointers are multiples of 16 bytes): one warp, sixteen
-// lanes of which fetch four rows each, others a sub-tile of the weights.  Else both
-// warps copy 16 bytes, 4 or 8, or single values a thread, whatever the alignment.
+// The copying warps of a block: its chunks from `at` of slot `slot` on.  Weights,
+// and the rows of a slot that follow one another in memory, come by TMA where
+// pointers and strides are multiples of 16 bytes (rows past the slot's are then some
+// other slot's: no result meets them).  The rest is copied by the threads, 16 bytes
+// at a time, 4 or 8, or single values, whatever the alignment.
 template <typename T, typename Tile, int RP, bool LONG, bool PLACED>
 __device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<Tile::kStages>& ring, uint8_t* smem,
                                               int (*list)[kSlotRows], AdapterSlot* rec, const AdapterSlot* slots,
                                               const int32_t* perm, int busy, int slot, int at, int per, int chunks,
                                               ErrorSink sink) {
-    constexpr int S = Tile::kStages, KC = Tile::KC;
+    constexpr int S = Tile::kStages, KC = Tile::KC, kNT = PLACED ? Tile::NT : 1;
     const int t = threadIdx.x - kTileThreads;
     const T* rows = static_cast<const T*>(q.rows);
     const T* w = static_cast<const T*>(q.w);
-    int stage = 0;
-    uint32_t round = 1;
-    auto free_stage = [&](int c) {
-        if (c < S || mbar_wait(&ring.empty[stage], round, kTileWaitNs)) return true;
-        report_error(sink.dev, sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterEmpty, c);
-        return false;
-    };
-    auto next_stage = [&]() {
-        if (++at == per) at = 0;
-        if (++stage == S) stage = 0, round ^= 1;
-    };
-    if (q.tma) {
-        if (t >= 32) return;
-        constexpr int kBoxes = LONG ? Tile::kSubs : 1, kNT = PLACED ? Tile::NT : 1;
-        auto load = [&](int i) { return slots[i < busy ? i : busy - 1]; };
-        int next_id[4], id[4] = {};
-        auto load_ids = [&](const AdapterSlot& s) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) next_id[i] = t < 16 && 4 * t + i < s.count ? perm[s.start + 4 * t + i] : -1;
-        };
-        AdapterSlot now{}, next = load(slot), after = load(slot + 1);
-        load_ids(next);
-        int c = 0;
-        for (; c < chunks; ++c) {
-            if (!free_stage(c)) break;
-            if (c == 0 || at == 0) {  // the next slot's rows; the loads of those behind it stay under way
-                now = next;
-                const int ring_at = slot % SlotFeed::kRing;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (t < 16) list[ring_at][4 * t + i] = next_id[i] < 0 ? 0 : next_id[i];
-                    id[i] = next_id[i] < 0 ? q.no_row : next_id[i];
-                }
-                if (t == 0) rec[ring_at] = now;
-                next = after;
-                load_ids(next);
-                ++slot;
-                after = load(slot + 1);
-            }
-            __syncwarp();
-            if (t == 0) mbar_arrive_expect_tx(&ring.full[stage], (rows ? Tile::kStageX : 0) + RP * 128);
-            __syncwarp();
-            const uint32_t st = shared_address(smem + stage * Tile::kStage);
-            if (t < 16) {
-                if (rows) tma_gather4(st + t * 512, q.row_map, &ring.full[stage], at * KC, id);
-            } else if (t - 16 < kBoxes) {
-                const int b = t - 16;
-                if (LONG)
-                    tma_box4(st + Tile::kStageX + b * (KC * Tile::kInner), q.w_map, &ring.full[stage],
-                             b * (Tile::kInner / Tile::E), at * (KC / kNT), now.cls);
-                else tma_box4(st + Tile::kStageX, q.w_map, &ring.full[stage], at * KC, 0, now.cls);
-            }
-            next_stage();
-        }
-        // Given up: what is under way has to land before the block may end.
-        if (c < chunks)
-            for (int i = c < S ? 0 : c - S; i < c; ++i) mbar_wait(&ring.full[i % S], i / S & 1, kTileWaitNs);
-        return;
-    }
+    const bool tma_w = q.tma & kTmaWeights;
     RowTile<T> xt;
     WeightTile<T, Tile, RP, LONG, PLACED> wt;
     const int unit_rows = copy_unit<T>(rows, q.row_stride), unit_w = copy_unit2<T>(w, q.w_row, q.w_adapter);
     SlotFeed feed{list, rec, slots, perm, busy, t};
     if (chunks > 0) feed.begin(slot);
-    for (int c = 0; c < chunks; ++c) {
-        if (!free_stage(c)) break;
+    int stage = 0, cls = 0, first = 0, c = 0;
+    uint32_t round = 1;
+    bool box = false;
+    for (; c < chunks; ++c) {
+        if (c >= S && !mbar_wait(&ring.empty[stage], round, kTileWaitNs)) {
+            report_error(sink.dev, sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterEmpty, c);
+            break;
+        }
         if (c == 0 || at == 0) {
             const AdapterSlot s = feed.enter();
-            if (rows) xt.aim(t, rows, q.row_stride, list[(feed.slot - 1) % SlotFeed::kRing], s.count, (int64_t)at * KC);
-            wt.aim(t, w + s.cls * q.w_adapter, q.w_row, (int64_t)at * KC);
+            const int* ids = list[(feed.slot - 1) % SlotFeed::kRing];
+            cls = s.cls, first = ids[0];
+            box = (q.tma & kTmaRows) && ids[s.count - 1] - first == s.count - 1;
+            if (rows && !box) xt.aim(t, rows, q.row_stride, ids, s.count, (int64_t)at * KC);
+            if (!tma_w) wt.aim(t, w + s.cls * q.w_adapter, q.w_row, (int64_t)at * KC);
         }
         uint8_t* st = smem + stage * Tile::kStage;
-        if (rows) xt.fetch(t, st, q.length - at * KC, unit_rows);
-        wt.fetch(t, st + Tile::kStageX, q.w_row, q.rank, q.length - at * KC, unit_w);
-        ring.copied(stage);
-        next_stage();
+        ring.copied_after(stage, t, (rows && box ? Tile::kStageX : 0) + (tma_w ? RP * 128 : 0), [&]() {
+            if (rows && !box) xt.fetch(t, st, q.length - at * KC, unit_rows);
+            if (!tma_w) wt.fetch(t, st + Tile::kStageX, q.w_row, q.rank, q.length - at * KC, unit_w);
+        }, [&]() {
+            const uint32_t to = shared_address(st);
+            if (rows && box) tma_box2(to, q.row_map, &ring.full[stage], at * KC, first);
+            if (tma_w) {
+                if (LONG)
+#pragma unroll
+                    for (int b = 0; b < Tile::kSubs; ++b)
+                        tma_box4(to + Tile::kStageX + b * (KC * Tile::kInner), q.w_map, &ring.full[stage],
+                                 b * (Tile::kInner / Tile::E), at * (KC / kNT), cls);
+                else tma_box4(to + Tile::kStageX, q.w_map, &ring.full[stage], at * KC, 0, cls);
+            }
+        });
+        if (++at == per) at = 0;
+        if (++stage == S) stage = 0, round ^= 1;
     }
     copy_commit();
     copy_wait<0>();
+    // Given up: what TMA has under way has to land before the block may end.
+    if (c < chunks)
+        for (int i = c < S ? 0 : c - S; i < c; ++i) mbar_wait(&ring.full[i % S], i / S & 1, kTileWaitNs);
 }
 
 // Block b of `blocks` takes chunks [total b / blocks, total (b + 1) / blocks).  A
@@ -510,9 +488,9 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     if ((int)blockIdx.x >= share.blocks) return;
     const int64_t begin = share.first(blockIdx.x);
     const int chunks = (int)(share.first(blockIdx.x + 1) - begin);
-    ring.init(P.tma1);
+    ring.init();
     if (tid >= kTileThreads) {
-        const StreamParams q{P.x, P.w1, P.x_row, P.w1_adapter, P.w1_row, k, P.r, (int)P.rows, &row_map, &w_map, P.tma1};
+        const StreamParams q{P.x, P.w1, P.x_row, P.w1_adapter, P.w1_row, k, P.r, &row_map, &w_map, P.tma1};
         stream_chunks<T, Tile, RP, TR, false>(q, ring, smem, list, rec, plan_busy(P), plan_perm(P), busy,
                                               (int)(begin / per), (int)(begin % per), per, chunks, P.sink);
         return;
@@ -666,12 +644,12 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     const int chunks = here ? (int)(share.first(blockIdx.x + 1) - begin) : 0;
     const int kper = ((int)P.k + KC - 1) / KC;
     const ChunkShare kshare(busy > 0 ? busy : 1, kper > 0 ? kper : 1, P.shrink_grid);
-    ring.init(P.tma2);
+    ring.init();
     // Rows without an adapter, an eighth of the columns at a time, by the threads that compute.
     constexpr int kParts = 8;
     const int width = (n + kParts * V - 1) / (kParts * V) * V;
     if (tid >= kTileThreads) {
-        const StreamParams q{P.base, P.w2, P.base_row, P.w2_adapter, P.w2_row, n, P.r, (int)P.rows, &row_map, &w_map, P.tma2};
+        const StreamParams q{P.base, P.w2, P.base_row, P.w2_adapter, P.w2_row, n, P.r, &row_map, &w_map, P.tma2};
         stream_chunks<T, Tile, RP, !TR, !TR>(q, ring, smem, list, rec, plan_busy(P), plan_perm(P), busy,
                                              (int)(begin / per), (int)(begin % per), per, chunks, P.sink);
         cudaGridDependencySynchronize();
