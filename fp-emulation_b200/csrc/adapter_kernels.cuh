@@ -51,6 +51,22 @@ __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Two neighbours at a time (one conversion for 16-bit types).
+__device__ __forceinline__ float2 widen2(const float* v) { return make_float2(v[0], v[1]); }
+__device__ __forceinline__ double2 widen2(const double* v) { return make_double2(v[0], v[1]); }
+__device__ __forceinline__ float2 widen2(const __half* v) { return __half22float2(*reinterpret_cast<const __half2*>(v)); }
+__device__ __forceinline__ float2 widen2(const __nv_bfloat16* v) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(v));
+}
+__device__ __forceinline__ void narrow2(float* v, float a, float b) { v[0] = a, v[1] = b; }
+__device__ __forceinline__ void narrow2(double* v, double a, double b) { v[0] = a, v[1] = b; }
+__device__ __forceinline__ void narrow2(__half* v, float a, float b) {
+    *reinterpret_cast<__half2*>(v) = __floats2half2_rn(a, b);
+}
+__device__ __forceinline__ void narrow2(__nv_bfloat16* v, float a, float b) {
+    *reinterpret_cast<__nv_bfloat162*>(v) = __floats2bfloat162_rn(a, b);
+}
+
 // One slot of the plan: up to kSlotRows rows of one adapter (class `cls`:
 // an adapter, `adapters` for rows without one, `adapters + 1` for bad ids).
 struct AdapterSlot {

@@ -733,19 +733,31 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
             yp[h] = static_cast<T*>(P.y) + rows[rows0 + g + h * 8] * P.y_row + (int64_t)at * KC + half * (KC / 2) + q * V;
     };
 
+    // 16-bit weights: where this thread's loads of a chunk start, from the chunk's buffer.
+    uint32_t w_at[E == 2 ? (TR ? 2 : RP / 16) : 1];
+    if constexpr (E == 2) {
+        if constexpr (TR) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) w_at[p] = tile_at(lane & 15, (half * 32 + p * 16 + (lane >> 4) * 8) * 2);
+        } else {
+#pragma unroll
+            for (int t = 0; t < RP / 16; ++t)
+                w_at[t] = Tile::long_at((lane >> 4) * 16 + half * 8 + (lane & 7), t * 32 + (lane >> 3 & 1) * 16);
+        }
+    }
     auto expand = [&](uint8_t* st, int left, const int* rows, int count) {
         constexpr int NT = Tile::NT;  // 8-column tiles of the warp's half chunk
         const uint8_t* wt = st + Tile::kStageX;
         Acc c[NT][4] = {};
         if constexpr (E == 2) {
+            const uint32_t w0 = shared_address(wt);
 #pragma unroll
             for (int t = 0; t < RP / 16; ++t) {
                 uint32_t b[2][4];
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    if (TR) ldsm4t(b[p], shared_address(wt) + tile_at(t * 16 + (lane & 15), (half * 32 + p * 16 + (lane >> 4) * 8) * 2));
-                    else ldsm4(b[p], shared_address(wt) + Tile::long_at((2 * p + (lane >> 4)) * 16 + half * 8 + (lane & 7),
-                                                                        t * 32 + (lane >> 3 & 1) * 16));
+                    if (TR) ldsm4t(b[p], w0 + w_at[p] + t * 16 * 128);
+                    else ldsm4(b[p], w0 + w_at[t] + p * 32 * Tile::kInner);
                 }
 #pragma unroll
                 for (int p = 0; p < 4; ++p) mma16<T>(c[p], ul[t], b[p / 2][p % 2 * 2], b[p / 2][p % 2 * 2 + 1]);
@@ -801,8 +813,11 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
                     alignas(4) T v[2];
                     float a = c[p][2 * h], b = c[p][2 * h + 1];
                     if constexpr (std::is_same<T, __half>::value) a *= back[h], b *= back[h];
-                    if (base) a += widen(o[0]), b += widen(o[1]);
-                    v[0] = narrow<T>(a), v[1] = narrow<T>(b);
+                    if (base) {
+                        const float2 old = widen2(o);
+                        a += old.x, b += old.y;
+                    }
+                    narrow2(v, a, b);
                     *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<uint32_t*>(v);
                 }
             __syncwarp();
@@ -814,14 +829,20 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
             uint8_t* tile = st + tile_at(rows0 + g + h * 8, half * 64 + q * 16);
             if (!Tile::kDirect || base) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(tile);
             if constexpr (Tile::kDirect) {
+                Acc r[V];  // element NT b + p is column b of tile p
 #pragma unroll
-                for (int p = 0; p < NT; ++p)
+                for (int e = 0; e < V; ++e) {
+                    r[e] = c[e % NT][2 * h + e / NT];
+                    if constexpr (std::is_same<T, __half>::value) r[e] *= back[h];
+                }
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        Acc a = c[p][2 * h + b];
-                        if constexpr (std::is_same<T, __half>::value) a *= back[h];
-                        v[NT * b + p] = narrow<T>(base ? a + (Acc)widen(v[NT * b + p]) : a);
+                for (int e = 0; e < V; e += 2) {
+                    if (base) {
+                        const auto old = widen2(v + e);
+                        r[e] += old.x, r[e + 1] += old.y;
                     }
+                    narrow2(v + e, r[e], r[e + 1]);
+                }
             }
             if (whole) {
                 if (rows0 + g + h * 8 < count) *reinterpret_cast<uint4*>(yp[h]) = *reinterpret_cast<uint4*>(v);
