@@ -208,6 +208,22 @@ int launch_grad(AdapterGradParams& P, const DevInfo& d, cudaStream_t st) {
     return launch_grad_rank<T, 128>(P, d, st);
 }
 
+size_t workspace_size(const DevInfo& d, int dtype, int64_t rows, int64_t rank, int64_t adapters) {
+    // A part for every block of the first kernel and every slot, one of which begins or ends with each.
+    return (size_t)(plan_slots(rows, adapters) + (int64_t)d.sms * kMostBlocks) * kSlotRows * padded_rank(rank) *
+           (dtype == FPEMU_DT_F64 ? 8 : 4);
+}
+
+int check_workspace(const char* what, int dtype, int64_t rows, int64_t rank, int64_t adapters, const void* workspace,
+                    size_t bytes) {
+    DevInfo d;
+    FPEMU_TRY(device_info(&d));
+    const size_t need = workspace_size(d, dtype, rows, rank, adapters);
+    if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || bytes < need)
+        return fail(FPEMU_ERR_WORKSPACE, "%s: need %zu bytes of 16-byte aligned workspace, got %zu", what, need, bytes);
+    return FPEMU_OK;
+}
+
 template <typename F>
 int with_type(int dtype, F&& f) {
     switch (dtype) {
@@ -254,38 +270,31 @@ size_t fpemu_adapter_workspace_size(int dtype, int64_t rows, int64_t rank, int64
     DevInfo d;
     if (check_sizes("adapter_workspace_size", dtype, rows, 0, 0, rank, adapters) != FPEMU_OK || device_info(&d) != FPEMU_OK)
         return 0;
-    // A part for every block of the first kernel and every slot, one of which begins or ends with each.
-    return (size_t)(plan_slots(rows, adapters) + (int64_t)d.sms * kMostBlocks) * kSlotRows * padded_rank(rank) *
-           (dtype == FPEMU_DT_F64 ? 8 : 4);
+    return workspace_size(d, dtype, rows, rank, adapters);
 }
 
 int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters,
-                         const void* x, int64_t x_row, const void* w1, int64_t w1_adapter, int64_t w1_row,
-                         const void* w2, int64_t w2_adapter, int64_t w2_row, int transposed, const void* base,
-                         int64_t base_row, void* y, int64_t y_row, const double* scales, double scale,
-                         const void* index, int index_bytes, const void* plan, void* u, void* workspace,
-                         size_t workspace_bytes, void* stream) {
+                         const void* x, int64_t x_row, const void* A, int64_t A_adapter, int64_t A_row,
+                         const void* B, int64_t B_adapter, int64_t B_row, const void* base, int64_t base_row, void* y,
+                         int64_t y_row, const double* scales, double scale, const void* index, int index_bytes,
+                         const void* plan, void* u, void* workspace, size_t workspace_bytes, void* stream) {
     DevInfo d;
     FPEMU_TRY(check_sizes("adapter_matmul", dtype, rows, k, n, rank, adapters));
     if (rows == 0) return FPEMU_OK;
-    if ((k > 0 && (x == nullptr || w1 == nullptr)) || (n > 0 && (w2 == nullptr || y == nullptr)))
+    if ((k > 0 && (x == nullptr || A == nullptr)) || (n > 0 && (B == nullptr || y == nullptr)))
         return fail(FPEMU_ERR_INVALID, "adapter_matmul: null matrix pointer");
-    if (x_row < 0 || base_row < 0 || w1_adapter < 0 || w2_adapter < 0 || w1_row < 0 || w2_row < 0 ||
-        (y_row < n && rows > 1))
+    if (x_row < 0 || base_row < 0 || A_adapter < 0 || B_adapter < 0 || A_row < 0 || B_row < 0 || (y_row < n && rows > 1))
         return fail(FPEMU_ERR_INVALID, "adapter_matmul: negative stride or output rows that overlap");
-    if (plan == nullptr && (rows > FPEMU_ADAPTER_FEW_ROWS || transposed || index == nullptr || (index_bytes != 4 && index_bytes != 8)))
-        return fail(FPEMU_ERR_INVALID, "adapter_matmul: %lld rows%s need a plan, few rows an index of 4 or 8 bytes",
-                    (long long)rows, transposed ? ", transposed," : "");
+    if (plan == nullptr && (rows > FPEMU_ADAPTER_FEW_ROWS || index == nullptr || (index_bytes != 4 && index_bytes != 8)))
+        return fail(FPEMU_ERR_INVALID, "adapter_matmul: %lld rows need a plan, few rows an index of 4 or 8 bytes",
+                    (long long)rows);
     FPEMU_TRY(device_info(&d));
-    if (plan != nullptr && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
-                            workspace_bytes < fpemu_adapter_workspace_size(dtype, rows, rank, adapters)))
-        return fail(FPEMU_ERR_WORKSPACE, "adapter_matmul: need %zu bytes of 16-byte aligned workspace, got %zu",
-                    fpemu_adapter_workspace_size(dtype, rows, rank, adapters), workspace_bytes);
+    if (plan != nullptr) FPEMU_TRY(check_workspace("adapter_matmul", dtype, rows, rank, adapters, workspace, workspace_bytes));
     AdapterParams P = {};
     P.rows = rows, P.k = k, P.n = n, P.r = (int)rank, P.adapters = (int)adapters;
     P.x = x, P.x_row = x_row;
-    P.w1 = w1, P.w1_adapter = w1_adapter, P.w1_row = w1_row;
-    P.w2 = w2, P.w2_adapter = w2_adapter, P.w2_row = w2_row;
+    P.w1 = A, P.w1_adapter = A_adapter, P.w1_row = A_row;
+    P.w2 = B, P.w2_adapter = B_adapter, P.w2_row = B_row;
     P.base = base, P.base_row = base_row, P.y = y, P.y_row = y_row;
     P.scales = scales, P.scale = scale;
     P.index = index, P.index_wide = index_bytes == 8, P.plan = static_cast<const int32_t*>(plan);
@@ -294,30 +303,49 @@ int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t 
     return with_type(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
-        if (P.plan) return transposed ? launch_tiles<T, true>(P, d, st) : launch_tiles<T, false>(P, d, st);
-        return launch_few<T>(P, d, st);
+        return P.plan ? launch_tiles<T, false>(P, d, st) : launch_few<T>(P, d, st);
     });
 }
 
-int fpemu_adapter_grads(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters,
-                        const void* x, int64_t x_row, const void* dy, int64_t dy_row, const void* u, const void* v,
-                        const void* plan, void* dA, void* dB, void* stream) {
+int fpemu_adapter_backward(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters,
+                           const void* x, int64_t x_row, const void* A, int64_t A_adapter, int64_t A_row,
+                           const void* B, int64_t B_adapter, int64_t B_row, const void* dy, int64_t dy_row,
+                           const double* scales, double scale, const void* plan, const void* u, void* v, void* dx,
+                           void* dA, void* dB, void* workspace, size_t workspace_bytes, void* stream) {
     DevInfo d;
-    FPEMU_TRY(check_sizes("adapter_grads", dtype, rows, k, n, rank, adapters));
-    if (plan == nullptr || (dA && (!x || !v) && rows * k > 0) || (dB && (!dy || !u) && rows * n > 0))
-        return fail(FPEMU_ERR_INVALID, "adapter_grads: null pointer");
+    FPEMU_TRY(check_sizes("adapter_backward", dtype, rows, k, n, rank, adapters));
+    if (plan == nullptr || (rows > 0 && ((k > 0 && dA && !x) || (n > 0 && !dy) || (k > 0 && dx && !A) ||
+                                         (n > 0 && (dx || dA) && !B) || (dB && !u) || ((dx || dA) && !v))))
+        return fail(FPEMU_ERR_INVALID, "adapter_backward: null pointer");
     if ((reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(v)) % 16 != 0)
-        return fail(FPEMU_ERR_INVALID, "adapter_grads: u and v start on a 16-byte boundary");
-    if (x_row < 0 || dy_row < 0) return fail(FPEMU_ERR_INVALID, "adapter_grads: negative stride");
+        return fail(FPEMU_ERR_INVALID, "adapter_backward: u and v start on a 16-byte boundary");
+    if (x_row < 0 || dy_row < 0 || A_adapter < 0 || B_adapter < 0 || A_row < 0 || B_row < 0)
+        return fail(FPEMU_ERR_INVALID, "adapter_backward: negative stride");
     FPEMU_TRY(device_info(&d));
+    if (dx || dA) FPEMU_TRY(check_workspace("adapter_backward", dtype, rows, rank, adapters, workspace, workspace_bytes));
     return with_type(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        AdapterGradParams P = {};
-        P.rows = rows, P.r = (int)rank, P.p_row = middle_row((int)rank), P.adapters = (int)adapters;
-        P.plan = static_cast<const int32_t*>(plan);
-        P.side[0] = AdapterGradSide{v, x, x_row, k, dA, 0};
-        P.side[1] = AdapterGradSide{u, dy, dy_row, n, dB, 1};
-        return launch_grad<T>(P, d, static_cast<cudaStream_t>(stream));
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (rows > 0 && (dx || dA)) {  // v = s dy B, dx = v A: the forward product with the factors' roles exchanged
+            AdapterParams P = {};
+            P.rows = rows, P.k = n, P.n = dx ? k : 0, P.r = (int)rank, P.adapters = (int)adapters;
+            P.x = dy, P.x_row = dy_row;
+            P.w1 = B, P.w1_adapter = B_adapter, P.w1_row = B_row;
+            P.w2 = A, P.w2_adapter = A_adapter, P.w2_row = A_row;
+            P.y = dx, P.y_row = k;
+            P.scales = scales, P.scale = scale;
+            P.plan = static_cast<const int32_t*>(plan);
+            P.u = v, P.u_row = middle_row((int)rank), P.parts = workspace;
+            FPEMU_TRY(error_sink(&P.sink));
+            const int status = launch_tiles<T, true>(P, d, st);
+            if (status != FPEMU_OK) return status;
+        }
+        AdapterGradParams G = {};
+        G.rows = rows, G.r = (int)rank, G.p_row = middle_row((int)rank), G.adapters = (int)adapters;
+        G.plan = static_cast<const int32_t*>(plan);
+        G.side[0] = AdapterGradSide{v, x, x_row, k, dA, 0};
+        G.side[1] = AdapterGradSide{u, dy, dy_row, n, dB, 1};
+        return launch_grad<T>(G, d, st);
     });
 }
 

@@ -61,10 +61,10 @@ SIGNATURES = {
     "fpemu_adapter_plan_size": (_i64, [_i64, _i64]),
     "fpemu_adapter_plan": (_int, [_vp, _int, _i64, _i64, _vp, _sz, _vp]),
     "fpemu_adapter_matmul": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
-                                    _int, _vp, _i64, _vp, _i64, _vp, _dp, _vp, _int, _vp, _vp, _vp, _sz, _vp]),
+                                    _vp, _i64, _vp, _i64, _vp, _dp, _vp, _int, _vp, _vp, _vp, _sz, _vp]),
     "fpemu_adapter_workspace_size": (_sz, [_int, _i64, _i64, _i64]),
-    "fpemu_adapter_grads": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
-                                   _vp]),
+    "fpemu_adapter_backward": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                                      _vp, _i64, _vp, _dp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "fpemu_clip_workspace_size": (_sz, [_i64]),
     "fpemu_clip_grads": (_int, [_i64, _vp, _vp, _vp, _vp, _int, _dp, _vp, _int, _vp, _sz, _vp]),
     "fpemu_device_error": (_int, [_IP, _IP, _IP, _IP, _int]),

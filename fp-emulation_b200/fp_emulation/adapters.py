@@ -18,7 +18,6 @@ import math
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from fp_emulation import _lib
 from fp_emulation.ozaki import _after_call, _dtype_bits, _on, _raw_stream, _require_cuda, _stream
@@ -80,83 +79,90 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _launch(x, w1, w2, transposed, base, y, scale, index, plan, adapters, rank, k, n, u):
+def _launch(x, A, B, base, y, scale, rows, index, u):
     """One fpemu_adapter_matmul on the current stream of x's device (2-D x, base and y)."""
     dev = x.device
     d = dev.index
     lib = _lib.load()
-    code, rows = _DTYPE_CODE[x.dtype], x.shape[0]
+    code, count = _DTYPE_CODE[x.dtype], x.shape[0]
+    adapters, rank, k = A.shape
+    plan = work = None  # few rows are grouped inside the kernel; more go by the plan
+    size = 0
     with _on(d):
-        size = 0
-        if plan is not None:
-            size = lib.fpemu_adapter_workspace_size(code, rows, rank, adapters)
-            workspace = torch.empty((size,), dtype=torch.uint8, device=dev)
+        if count > _lib.FPEMU_ADAPTER_FEW_ROWS:
+            plan = rows.plan.data_ptr()
+            size = lib.fpemu_adapter_workspace_size(code, count, rank, adapters)
+            work = torch.empty((size,), dtype=torch.uint8, device=dev)
         st = lib.fpemu_adapter_matmul(
-            code, rows, k, n, rank, adapters, x.data_ptr(), _row_stride(x),
-            w1.data_ptr(), w1.stride(0), w1.stride(1), w2.data_ptr(), w2.stride(0), w2.stride(1), transposed,
-            None if base is None else base.data_ptr(), 0 if base is None else base.stride(0),
-            None if y is None else y.data_ptr(), n if y is None else _row_stride(y),
+            code, count, k, B.shape[1], rank, adapters, x.data_ptr(), _row_stride(x), A.data_ptr(), A.stride(0),
+            A.stride(1), B.data_ptr(), B.stride(0), B.stride(1), None if base is None else base.data_ptr(),
+            0 if base is None else base.stride(0), y.data_ptr(), _row_stride(y),
             None if scale.__class__ is float else scale.data_ptr(), scale if scale.__class__ is float else 0.0,
-            None if plan is not None else index.data_ptr(), 0 if plan is not None else index.element_size(),
-            None if plan is None else plan.data_ptr(), None if u is None else u.data_ptr(),
-            workspace.data_ptr() if size else None, size, _raw_stream(d))
+            index.data_ptr(), index.element_size(), plan, None if u is None else u.data_ptr(),
+            None if work is None else work.data_ptr(), size, _raw_stream(d))
     if st:
         _lib.check(st, "adapter_matmul")
     _after_call("adapter_matmul", dev)
 
 
-def _sum_dtype(dtype):
-    return torch.float64 if dtype == torch.float64 else torch.float32
-
-
 class _AdapterMatmul(torch.autograd.Function):
     """The operator and its gradients.  Products of the first factor (u) are kept
-    in the sums' type for dB; the backward pass makes v = scale * dy B the same
-    way while it makes dx, and sums dA and dB over the rows of each adapter."""
+    for dB; the backward pass makes v = scale * dy B the same way while it makes
+    dx, and sums dA and dB over the rows of each adapter."""
 
     @staticmethod
     def forward(ctx, x, A, B, base, rows, scale):
         y = torch.empty((x.shape[0], B.shape[1]), dtype=x.dtype, device=x.device)
-        u = torch.empty((x.shape[0], (A.shape[1] + 3) // 4 * 4), dtype=_sum_dtype(x.dtype), device=x.device)
-        _launch(x, A, B, 0, base, y, scale, rows.index, _plan_of(rows), rows.adapters, A.shape[1], A.shape[2],
-                B.shape[1], u)
+        u = torch.empty((x.shape[0], (A.shape[1] + 3) // 4 * 4),
+                        dtype=torch.float64 if x.dtype == torch.float64 else torch.float32, device=x.device)
+        _launch(x, A, B, base, y, scale, rows, rows.index, u)
         ctx.save_for_backward(x, A, B, u)
         ctx.rows, ctx.scale = rows, scale
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        if torch.is_grad_enabled():  # create_graph: the gradients below are computed outside autograd
+            with torch.no_grad():
+                grads = _AdapterMatmul._backward(ctx, dy)
+            return tuple(g if g is None else torch._C._functions.DelayedError(
+                "adapter_matmul is differentiable once, not twice", 1)(g.requires_grad_(True)) for g in grads)
+        return _AdapterMatmul._backward(ctx, dy)
+
+    @staticmethod
+    def _backward(ctx, dy):
         x, A, B, u = ctx.saved_tensors
-        rows, scale = ctx.rows, ctx.scale
+        scale = ctx.scale
         need_x, need_A, need_B, need_base = ctx.needs_input_grad[:4]
-        n_ad, rank, k = A.shape
+        dev = x.device
+        d = dev.index
+        count = x.shape[0]
+        adapters, rank, k = A.shape
         n = B.shape[1]
         dyc = _last_contiguous(dy)
-        dx = dA = dB = v = None
-        if need_x or need_A:
-            v = torch.empty_like(u)
-            if need_x:
-                dx = torch.empty((x.shape[0], k), dtype=x.dtype, device=x.device)
-            _launch(dyc, B, A, 1, None, dx, scale, rows.index, rows.plan, n_ad, rank, n, k if need_x else 0, v)
-        if need_A or need_B:
-            dA = torch.empty((n_ad, rank, k), dtype=A.dtype, device=A.device) if need_A else None
-            dB = torch.empty((n_ad, n, rank), dtype=B.dtype, device=B.device) if need_B else None
-            dev = x.device
-            with _on(dev.index):
-                st = _lib.load().fpemu_adapter_grads(
-                    _DTYPE_CODE[x.dtype], x.shape[0], k, n, rank, n_ad, x.data_ptr(), _row_stride(x),
-                    dyc.data_ptr(), _row_stride(dyc), u.data_ptr(), None if v is None else v.data_ptr(),
-                    rows.plan.data_ptr(), None if dA is None else dA.data_ptr(),
-                    None if dB is None else dB.data_ptr(), _stream(dev))
+        lib = _lib.load()
+        code = _DTYPE_CODE[x.dtype]
+        with _on(d):
+            dx = torch.empty((count, k), dtype=x.dtype, device=dev) if need_x else None
+            dA = torch.empty((adapters, rank, k), dtype=x.dtype, device=dev) if need_A else None
+            dB = torch.empty((adapters, n, rank), dtype=x.dtype, device=dev) if need_B else None
+            size = v = work = None
+            if need_x or need_A:  # v, then the workspace
+                size = lib.fpemu_adapter_workspace_size(code, count, rank, adapters)
+                v_bytes = u.numel() * u.element_size()  # of rows of 16 bytes or more
+                work = torch.empty((size + v_bytes,), dtype=torch.uint8, device=dev)
+                v = work.data_ptr()
+            st = lib.fpemu_adapter_backward(
+                code, count, k, n, rank, adapters, x.data_ptr(), _row_stride(x), A.data_ptr(), A.stride(0), A.stride(1),
+                B.data_ptr(), B.stride(0), B.stride(1), dyc.data_ptr(), _row_stride(dyc),
+                None if scale.__class__ is float else scale.data_ptr(), scale if scale.__class__ is float else 0.0,
+                ctx.rows.plan.data_ptr(), u.data_ptr(), v, None if dx is None else dx.data_ptr(),
+                None if dA is None else dA.data_ptr(), None if dB is None else dB.data_ptr(),
+                None if v is None else v + v_bytes, size or 0, _raw_stream(d))
+        if st:
             _lib.check(st, "adapter_matmul backward")
-            _after_call("adapter_matmul backward", dev)
+        _after_call("adapter_matmul backward", dev)
         return dx, dA, dB, dy if need_base else None, None, None
-
-
-def _plan_of(rows):
-    """Few rows are grouped inside the kernel; more go by the plan."""
-    return None if rows.index.shape[0] <= _lib.FPEMU_ADAPTER_FEW_ROWS else rows.plan
 
 
 def _span(t):
@@ -271,7 +277,7 @@ def adapter_matmul(x, A, B, rows, base=None, scale=1.0, out=None):
         y = torch.empty((count, n), dtype=dtype, device=x.device)
     else:
         y = _check_out(out, shape, x, base, (x2, A, B))
-    _launch(x2, A, B, 0, base2, y, scale, index, None if rows is None else _plan_of(rows), adapters, rank, k, n, None)
+    _launch(x2, A, B, base2, y, scale, rows, index, None)
     if out is None:
         return y if flat else y.view(shape)
     torch.autograd.graph.increment_version(out)

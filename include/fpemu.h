@@ -211,44 +211,44 @@ size_t fpemu_gemm_workspace_size(int64_t m, int64_t n, int n_mod);
  * row (index_bytes 4 or 8): 0 .. adapters - 1, or -1 for a row without an
  * adapter.  Any other id is recorded as a device error (FPEMU_ERR_INVALID) and
  * that row's output becomes NaN.  A plan serves every fpemu_adapter_matmul and
- * fpemu_adapter_grads of the batch; it is a snapshot of the index. */
+ * fpemu_adapter_backward of the batch; it is a snapshot of the index. */
 int64_t fpemu_adapter_plan_size(int64_t rows, int64_t adapters); /* bytes; 0 when out of range */
 int fpemu_adapter_plan(const void *index, int index_bytes, int64_t rows, int64_t adapters,
                        void *plan, size_t plan_bytes, void *stream);
 
-/* y[t] = base[t] + W2_i (s_i W1_i x[t]) for every row t with adapter i;
- * base[t] (0 when base is NULL) for a row without one.  x is rows x k, y and
- * base rows x n; strides are in elements and the last dimension is contiguous.
- *   transposed 0: w1 is [adapters][rank][k], w2 is [adapters][n][rank]
- *                 (the forward product, w1 = A, w2 = B);
- *   transposed 1: w1 is [adapters][k][rank], w2 is [adapters][rank][n]
- *                 (its gradient by x: x = dy, w1 = B, w2 = A).
+/* y[t] = base[t] + B_i (s_i A_i x[t]) for every row t with adapter i; base[t] (0
+ * when base is NULL) for a row without one.  x is rows x k, A [adapters][rank][k],
+ * B [adapters][n][rank], y and base rows x n; strides are in elements and the last
+ * dimension is contiguous.
  * scales: one double per adapter, or NULL for `scale` everywhere.
- * u (or NULL): rows of `rank` values s_i W1_i x[t], each row rank rounded up to a
- * multiple of 4 apart, for fpemu_adapter_grads -- doubles for FPEMU_DT_F64, floats,
- * or for FPEMU_DT_BF16 the float cut into two bfloat16 parts; rows without an adapter
- * are not written.
+ * u (or NULL): what fpemu_adapter_backward needs, rows of `rank` values s_i A_i x[t],
+ * each row rank rounded up to a multiple of 4 apart -- doubles for FPEMU_DT_F64,
+ * else 4 bytes a value; rows without an adapter are not written.
  * y may be base itself; otherwise it overlaps no input.
- * plan NULL: rows <= FPEMU_ADAPTER_FEW_ROWS and not transposed, grouped by the
- * kernel from index; no workspace.  With a plan: fpemu_adapter_workspace_size
- * bytes, 16-byte aligned, for this call alone. */
+ * plan NULL: rows <= FPEMU_ADAPTER_FEW_ROWS, grouped by the kernel from index; no
+ * workspace.  With a plan: fpemu_adapter_workspace_size bytes, 16-byte aligned, for
+ * this call alone. */
 int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank,
-                         int64_t adapters, const void *x, int64_t x_row, const void *w1,
-                         int64_t w1_adapter, int64_t w1_row, const void *w2, int64_t w2_adapter,
-                         int64_t w2_row, int transposed, const void *base, int64_t base_row,
-                         void *y, int64_t y_row, const double *scales, double scale,
-                         const void *index, int index_bytes, const void *plan, void *u,
-                         void *workspace, size_t workspace_bytes, void *stream);
+                         int64_t adapters, const void *x, int64_t x_row, const void *A,
+                         int64_t A_adapter, int64_t A_row, const void *B, int64_t B_adapter,
+                         int64_t B_row, const void *base, int64_t base_row, void *y, int64_t y_row,
+                         const double *scales, double scale, const void *index, int index_bytes,
+                         const void *plan, void *u, void *workspace, size_t workspace_bytes,
+                         void *stream);
 size_t fpemu_adapter_workspace_size(int dtype, int64_t rows, int64_t rank, int64_t adapters);
 
-/* Gradients of the factors, each [adapters][...] packed, zero for an adapter
- * without rows: dA[i] = sum_t v[t]^T x[t] (rank x k) and dB[i] = sum_t dy[t]^T u[t]
- * (n x rank) over the rows t of adapter i, in the rows' order.  u and v are what
- * fpemu_adapter_matmul left (forward, and transposed on dy).  dA or dB may be NULL. */
-int fpemu_adapter_grads(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank,
-                        int64_t adapters, const void *x, int64_t x_row, const void *dy,
-                        int64_t dy_row, const void *u, const void *v, const void *plan, void *dA,
-                        void *dB, void *stream);
+/* The gradients of that product for dy (rows x n): dx (packed, rows x k), and
+ * dA[i] = sum_t v[t]^T x[t], dB[i] = sum_t dy[t]^T u[t] over the rows t of adapter i
+ * (packed, [adapters][rank][k] and [adapters][n][rank], zero for an adapter without
+ * rows), where v[t] = s_i dy[t] B_i; v is scratch like u, 16-byte aligned.  dx, dA and
+ * dB may each be NULL.  plan, scales, strides and workspace as above. */
+int fpemu_adapter_backward(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank,
+                           int64_t adapters, const void *x, int64_t x_row, const void *A,
+                           int64_t A_adapter, int64_t A_row, const void *B, int64_t B_adapter,
+                           int64_t B_row, const void *dy, int64_t dy_row, const double *scales,
+                           double scale, const void *plan, const void *u, void *v, void *dx,
+                           void *dA, void *dB, void *workspace, size_t workspace_bytes,
+                           void *stream);
 
 /* The norm over every element of `count` tensors of any types (arrays of
  * pointers, sizes and FPEMU_DT_ codes in host memory), norm_type 1, 2, or 0 for

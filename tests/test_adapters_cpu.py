@@ -100,7 +100,7 @@ def test_plan_size_and_c_refusals():
     assert lib.fpemu_adapter_plan(None, 2, 1, 1, None, 0, None) == _lib.FPEMU_ERR_INVALID
 
     def matmul(dtype=0, rows=4, k=8, n=8, rank=2, adapters=2, x=16, y=16, x_row=8, y_row=8, index=16, nbytes=4, plan=None):
-        return lib.fpemu_adapter_matmul(dtype, rows, k, n, rank, adapters, x, x_row, 16, 16, 8, 16, 16, 2, 0, None, 0,
+        return lib.fpemu_adapter_matmul(dtype, rows, k, n, rank, adapters, x, x_row, 16, 16, 8, 16, 16, 2, None, 0,
                                         y, y_row, None, 1.0, index, nbytes, plan, None, None, 0, None)
 
     bad, unsupported = _lib.FPEMU_ERR_INVALID, _lib.FPEMU_ERR_UNSUPPORTED
@@ -109,7 +109,13 @@ def test_plan_size_and_c_refusals():
     assert matmul(index=None) == bad and matmul(nbytes=2) == bad and matmul(rows=257) == bad
     assert matmul(rank=0) == unsupported and matmul(rank=129) == unsupported and matmul(adapters=0) == unsupported
     assert matmul(rows=0) == 0
-    assert lib.fpemu_adapter_grads(0, 4, 8, 8, 2, 2, 16, 8, 16, 8, 16, 16, None, 16, 16, None) == bad
+
+    def backward(rows=4, plan=16, v=16, dx=16, x=16, stride=8):
+        return lib.fpemu_adapter_backward(0, rows, 8, 8, 2, 2, x, stride, 16, 16, 8, 16, 16, 2, 16, 8, None, 1.0, plan, 16, v,
+                                          dx, 16, 16, None, 0, None)
+
+    assert backward(plan=None) == bad and backward(v=None) == bad and backward(v=8) == bad
+    assert backward(x=None) == bad and backward(stride=-1) == bad
 
 
 def test_clip_c_refusals():
