@@ -48,7 +48,7 @@ int launch_few_rank(const AdapterParams& P, const DevInfo& d, cudaStream_t st) {
     // Groups of eight rows of one adapter, of none, or with a bad id: never more than this.
     const int64_t units = std::min<int64_t>(P.rows, P.rows / kGroupRows + P.adapters + 2);
     int cluster = 8;
-    while (cluster > 2 && units * cluster > d.sms * 4) cluster /= 2;
+    while (cluster > 2 && units * cluster > (P.r > 32 ? d.sms * 4 : d.sms * Tile::kBlocks)) cluster /= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(units * cluster));
     cfg.blockDim = dim3(kFewThreads);

@@ -63,15 +63,19 @@ struct FewTile {
     static constexpr int E = sizeof(T), V = 16 / E, KS = 4 * V;     // elements of k a warp takes at a step
     static constexpr int MR = E == 8 ? 8 : 16;                      // ranks of an instruction
     static constexpr int RT = RP / MR, PA = E == 8 ? 2 : 4;         // rank tiles; sums a thread holds of one
-    static constexpr int UN = RP <= 16 ? 4 : RP <= 32 ? 2 : 1;      // steps with their loads in flight together
+    static constexpr int UN = RP <= 16 ? (E == 8 ? 3 : 4) : RP <= 32 ? 2 : 1;  // steps with their loads in flight together
     static constexpr int JS = (RP + KS - 1) / KS;                   // 16-byte steps along the rank
-    static constexpr int UG = JS * V >= 16 ? 1 : JS * V >= 8 ? 2 : 4;  // column groups, likewise
+    static constexpr int UG = JS * V >= 16 ? 1 : JS * V >= 8 ? 2 : E == 8 ? 3 : 4;  // column groups, likewise
     static constexpr int kWarps = kFewThreads / 32;
     static constexpr int kSmem = (kWarps + 2) * RP * kGroupRows * (int)sizeof(Acc);
+    static constexpr int kBlocks = RP <= 16 && E != 4 ? 3 : RP <= 64 ? 2 : 1;  // an SM, by registers
+    // Whether the second product's first loads start before the blocks exchange the middle (for float64
+    // the registers they hold cost more: 200 rows, 24 adapters, 4096 x 4096: 27 us against 24).
+    static constexpr bool kEarly = E != 8;
 };
 
 template <typename T, int RP>
-__global__ void __launch_bounds__(kFewThreads) adapter_few_kernel(const __grid_constant__ AdapterParams P) {
+__global__ void __launch_bounds__(kFewThreads, FewTile<T, RP>::kBlocks) adapter_few_kernel(const __grid_constant__ AdapterParams P) {
     using Tile = FewTile<T, RP>;
     using Acc = typename Tile::Acc;
     constexpr int E = Tile::E, V = Tile::V, KS = Tile::KS, RT = Tile::RT, MR = Tile::MR, UN = Tile::UN, JS = Tile::JS;
@@ -196,6 +200,27 @@ __global__ void __launch_bounds__(kFewThreads) adapter_few_kernel(const __grid_c
             }
         }
     }
+    // The second product's loads: UG groups of KS columns of this warp, their weights and base.
+    constexpr int NT = V / 2;  // 8-column tiles of a group; a thread's results are 16 bytes of neighbours
+    constexpr int UG = Tile::UG;
+    uint4 w2v[UG][NT][JS], held[UG];
+    auto load_groups = [&](int first) {
+#pragma unroll
+        for (int u = 0; u < UG; ++u) {
+            const int c0 = first + u * W * KS;
+#pragma unroll
+            for (int p = 0; p < NT; ++p)
+#pragma unroll
+                for (int t = 0; t < JS; ++t) {
+                    const int c = c0 + g / 2 * V + 2 * p + g % 2, j = t * KS + q * V;
+                    w2v[u][p][t] = c < n1 && j < P.r ? load16(w2 + c * P.w2_row + j, P.r - j, vec_w2) : uint4{0, 0, 0, 0};
+                }
+            const int avail = g < count ? n1 - c0 - q * V : 0;
+            held[u] = base && avail > 0 ? load16(base + c0 + q * V, avail, vec_base) : uint4{0, 0, 0, 0};
+        }
+    };
+    if (Tile::kEarly) load_groups(n0 + warp * KS);
+
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -250,23 +275,8 @@ __global__ void __launch_bounds__(kFewThreads) adapter_few_kernel(const __grid_c
                 split16<T>(at(2 * i) * down, at(2 * i + 1) * down, ua[t][2 * i], ua[t][2 * i + 1]);
         }
     }
-    constexpr int NT = V / 2;  // 8-column tiles of a group of KS columns; a thread's results are 16 bytes of neighbours
-    constexpr int UG = Tile::UG;
     for (int first = n0 + warp * KS; first < n1; first += W * KS * UG) {
-        uint4 wv[UG][NT][JS], held[UG];
-#pragma unroll
-        for (int u = 0; u < UG; ++u) {
-            const int c0 = first + u * W * KS;
-#pragma unroll
-            for (int p = 0; p < NT; ++p)
-#pragma unroll
-                for (int t = 0; t < JS; ++t) {
-                    const int c = c0 + g / 2 * V + 2 * p + g % 2, j = t * KS + q * V;
-                    wv[u][p][t] = c < n1 && j < P.r ? load16(w2 + c * P.w2_row + j, P.r - j, vec_w2) : uint4{0, 0, 0, 0};
-                }
-            const int avail = g < count ? n1 - c0 - q * V : 0;
-            held[u] = base && avail > 0 ? load16(base + c0 + q * V, avail, vec_base) : uint4{0, 0, 0, 0};
-        }
+        if (!Tile::kEarly || first != n0 + warp * KS) load_groups(first);
 #pragma unroll
         for (int u = 0; u < UG; ++u) {
             const int col = first + u * W * KS + q * V, avail = g < count ? n1 - col : 0;
@@ -278,7 +288,7 @@ __global__ void __launch_bounds__(kFewThreads) adapter_few_kernel(const __grid_c
                     double c[2] = {};
 #pragma unroll
                     for (int t = 0; t < JS; ++t) {
-                        const double* wd = reinterpret_cast<const double*>(&wv[u][p][t]);
+                        const double* wd = reinterpret_cast<const double*>(&w2v[u][p][t]);
                         mma_f64_8(c, ua[t][0], wd[0]);
                         mma_f64_8(c, ua[t][1], wd[1]);
                     }
@@ -287,7 +297,7 @@ __global__ void __launch_bounds__(kFewThreads) adapter_few_kernel(const __grid_c
                     float c[4] = {};
 #pragma unroll
                     for (int t = 0; t < JS; ++t) {
-                        const uint32_t* wr = reinterpret_cast<const uint32_t*>(&wv[u][p][t]);
+                        const uint32_t* wr = reinterpret_cast<const uint32_t*>(&w2v[u][p][t]);
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
                             const uint32_t a[4] = {ua[t][4 * m], ua[t][4 * m + 1], ua[t][4 * m + 2], ua[t][4 * m + 3]};
