@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "adapter_few.cuh"
@@ -39,12 +40,25 @@ int check_sizes(const char* what, int dtype, int64_t rows, int64_t k, int64_t n,
     return FPEMU_OK;
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory, once per kernel and device.
+template <auto* KERNEL>
+int allow_shared(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    FPEMU_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(done.load(std::memory_order_relaxed) & bit)) {
+        FPEMU_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        done.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return FPEMU_OK;
+}
+
 template <typename T, int RP>
 int launch_few_rank(const AdapterParams& P, const DevInfo& d, cudaStream_t st) {
     auto kern = adapter_few_kernel<T, RP>;
     using Tile = FewTile<T, RP>;
-    if (Tile::kSmem > 48 * 1024)
-        FPEMU_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem));
+    if (Tile::kSmem > 48 * 1024) FPEMU_TRY((allow_shared<adapter_few_kernel<T, RP>>(Tile::kSmem)));
     // Groups of eight rows of one adapter, of none, or with a bad id: never more than this.
     const int64_t units = std::min<int64_t>(P.rows, P.rows / kGroupRows + P.adapters + 2);
     int cluster = 8;
@@ -126,8 +140,8 @@ int launch_tiles_rank(AdapterParams& P, const DevInfo& d, cudaStream_t st) {
     static_assert(Tile::kBlocks <= kMostBlocks, "the workspace holds a part of every block");
     auto shrink = adapter_shrink_kernel<T, TR, RP>;
     auto expand = adapter_expand_kernel<T, TR, RP>;
-    FPEMU_CUDA(cudaFuncSetAttribute(shrink, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem));
-    FPEMU_CUDA(cudaFuncSetAttribute(expand, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem));
+    FPEMU_TRY((allow_shared<adapter_shrink_kernel<T, TR, RP>>(Tile::kSmem)));
+    FPEMU_TRY((allow_shared<adapter_expand_kernel<T, TR, RP>>(Tile::kSmem)));
     const int64_t slots = plan_slots(P.rows, P.adapters);
     auto grid = [&](int64_t length) {
         const int64_t chunks = std::max<int64_t>((length + Tile::KC - 1) / Tile::KC, 1);
@@ -175,7 +189,7 @@ template <typename T, int RP>
 int launch_grad_rank(AdapterGradParams& P, const DevInfo& d, cudaStream_t st) {
     using Tile = AdapterGradTile<T, RP>;
     auto kern = adapter_grad_kernel<T, RP>;
-    FPEMU_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem));
+    FPEMU_TRY((allow_shared<adapter_grad_kernel<T, RP>>(Tile::kSmem)));
     int64_t blocks[2];
     for (int i = 0; i < 2; ++i) blocks[i] = P.side[i].grad ? (P.side[i].cols + Tile::COLS - 1) / Tile::COLS : 0;
     if (blocks[0] + blocks[1] == 0) return FPEMU_OK;
