@@ -154,6 +154,8 @@ int launch_tiles_rank(AdapterParams& P, const DevInfo& d, cudaStream_t st) {
         return by_long ? make_weight_map<T>(map, w, row, adapter, P.r, length, P.adapters, turns, inner, Tile::KC / turns)
                        : make_weight_map<T>(map, w, row, adapter, length, P.r, P.adapters, 1, Tile::KC, RP);
     };
+    P.budget_ns = wait_budget_ns();
+    P.stall = test_stall_idx();
     P.tma1 = P.tma2 = 0;
     if (P.k > 0 && make_row_map<T>(&maps[0], P.x, P.x_row, P.k, P.rows)) P.tma1 |= kTmaRows;
     if (P.k > 0 && weights(&maps[1], P.w1, P.w1_row, P.w1_adapter, P.k, TR, 1)) P.tma1 |= kTmaWeights;

@@ -214,6 +214,8 @@ struct AdapterParams {
     int u_row;
     void* parts;          // with a plan: the first product's partial sums
     int shrink_grid;      // blocks that leave them
+    uint64_t budget_ns;   // of a wait
+    int stall;            // chunk at which the first block's copying warps stop (failure tests), or -1
     int tma1, tma2;       // which maps there are for the first and the second product
     ErrorSink sink;
 };

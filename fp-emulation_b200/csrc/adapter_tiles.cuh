@@ -161,7 +161,6 @@ struct MiddleOf<__nv_bfloat16> {
 
 constexpr int kTileThreads = 256;      // eight warps that compute
 constexpr int kCopyThreads = 64;       // and two that copy
-constexpr uint64_t kTileWaitNs = 2000000000ull;
 
 // Tiles in shared memory, as TMA writes them with 128-byte swizzle: rows of 128
 // bytes whose 16-byte units change places by the row.  "Rank-major" weights have a
@@ -312,8 +311,10 @@ constexpr int kCopyBarrier = 1, kWorkBarrier = 2;
 template <int S>
 struct ChunkRing {
     uint64_t full[S], empty[S];
+    volatile int failed;  // a computing warp's wait ran out
     __device__ __forceinline__ void init() {
         if (threadIdx.x == 0) {
+            failed = 0;
 #pragma unroll
             for (int i = 0; i < S; ++i)
                 mbar_init(&full[i], 2 * kCopyThreads), mbar_init(&empty[i], kTileThreads / 32);
@@ -381,6 +382,8 @@ struct StreamParams {
     int length, rank;
     const CUtensorMap *row_map, *w_map;
     int tma;  // kTmaRows, kTmaWeights: which maps there are
+    uint64_t budget_ns;
+    int stall;
 };
 
 // The copying warps of a block: its chunks from `at` of slot `slot` on.  Weights,
@@ -407,7 +410,8 @@ __device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<T
     uint32_t round = 1;
     bool box = false;
     for (; c < chunks; ++c) {
-        if (c >= S && !mbar_wait(&ring.empty[stage], round, kTileWaitNs)) {
+        if (blockIdx.x == 0 && c == q.stall) break;
+        if (c >= S && !mbar_wait(&ring.empty[stage], round, q.budget_ns)) {
             report_error(sink.dev, sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterEmpty, c);
             break;
         }
@@ -442,7 +446,7 @@ __device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<T
     copy_wait<0>();
     // Given up: what TMA has under way has to land before the block may end.
     if (c < chunks)
-        for (int i = c < S ? 0 : c - S; i < c; ++i) mbar_wait(&ring.full[i % S], i / S & 1, kTileWaitNs);
+        for (int i = c < S ? 0 : c - S; i < c; ++i) mbar_wait(&ring.full[i % S], i / S & 1, q.budget_ns);
 }
 
 // Block b of `blocks` takes chunks [total b / blocks, total (b + 1) / blocks).  A
@@ -490,7 +494,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     const int chunks = (int)(share.first(blockIdx.x + 1) - begin);
     ring.init();
     if (tid >= kTileThreads) {
-        const StreamParams q{P.x, P.w1, P.x_row, P.w1_adapter, P.w1_row, k, P.r, &row_map, &w_map, P.tma1};
+        const StreamParams q{P.x, P.w1, P.x_row, P.w1_adapter, P.w1_row, k, P.r, &row_map, &w_map, P.tma1, P.budget_ns, P.stall};
         stream_chunks<T, Tile, RP, TR, false>(q, ring, smem, list, rec, plan_busy(P), plan_perm(P), busy,
                                               (int)(begin / per), (int)(begin % per), per, chunks, P.sink);
         return;
@@ -594,18 +598,19 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
             named_barrier<kWorkBarrier, kTileThreads>();
         }
         Acc* out = static_cast<Acc*>(P.parts) + part * (kSlotRows * RP);
-        for (int i = tid; i < kSlotRows * RP; i += kTileThreads) out[i] = red[i / RP * Tile::kPitchU + i % RP];
+        const bool ok = !ring.failed;  // else some warp's part is missing: the rows become NaN
+        for (int i = tid; i < kSlotRows * RP; i += kTileThreads)
+            out[i] = ok ? red[i / RP * Tile::kPitchU + i % RP] : (Acc)__longlong_as_double(0x7ff8000000000000ll);
     };
 
     int at = (int)(begin % per), slot = (int)(begin / per), stage = 0;
     uint32_t round = 0;
     bool ok = true;
     for (int c = 0; c < chunks; ++c) {
-        if (ok && !mbar_wait(&ring.full[stage], round, kTileWaitNs)) {
+        if (ok && !mbar_wait(&ring.full[stage], round, P.budget_ns)) {
             report_error(P.sink.dev, P.sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterFull, c);
-            ok = false;  // what is left becomes NaN
-#pragma unroll
-            for (int m = 0; m < MT; ++m) acc[m][0][0] = (Acc)__longlong_as_double(0x7ff8000000000000ll);
+            ring.failed = 1;
+            ok = false;
         }
         if (ok && rows0 < rec[slot % SlotFeed::kRing].count) shrink(smem + stage * Tile::kStage);
         ring.left(stage);
@@ -649,7 +654,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     constexpr int kParts = 8;
     const int width = (n + kParts * V - 1) / (kParts * V) * V;
     if (tid >= kTileThreads) {
-        const StreamParams q{P.base, P.w2, P.base_row, P.w2_adapter, P.w2_row, n, P.r, &row_map, &w_map, P.tma2};
+        const StreamParams q{P.base, P.w2, P.base_row, P.w2_adapter, P.w2_row, n, P.r, &row_map, &w_map, P.tma2, P.budget_ns, P.stall};
         stream_chunks<T, Tile, RP, !TR, !TR>(q, ring, smem, list, rec, plan_busy(P), plan_perm(P), busy,
                                              (int)(begin / per), (int)(begin % per), per, chunks, P.sink);
         cudaGridDependencySynchronize();
@@ -870,9 +875,15 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     int at = (int)(begin % per), slot = (int)(begin / per), stage = 0;
     uint32_t round = 0;
     for (int c = 0; c < chunks; ++c) {
-        if (ok && !mbar_wait(&ring.full[stage], round, kTileWaitNs)) {
+        if (ok && !mbar_wait(&ring.full[stage], round, P.budget_ns)) {
             report_error(P.sink.dev, P.sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterFull, c);
+            ring.failed = 1;
             ok = false;
+        }
+        if (c == 0 || at == 0) {  // a warp that has given up still meets the others
+            if (ok) take_slot(slot, at);
+            else named_barrier<kWorkBarrier, kTileThreads>();
+            ok = ok && !ring.failed;  // else a warp's share of the middle is missing
         }
         if (!ok) {  // what is left becomes NaN
             const AdapterSlot s = plan_busy(P)[slot];
@@ -884,7 +895,6 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
             if (++at == per) at = 0, ++slot;
             continue;
         }
-        if (c == 0 || at == 0) take_slot(slot, at);
         const int count = rec[slot % SlotFeed::kRing].count;
         if (rows0 < count) expand(smem + stage * Tile::kStage, n - at * KC, list[slot % SlotFeed::kRing], count);
         ring.left(stage);

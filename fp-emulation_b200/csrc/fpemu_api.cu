@@ -89,16 +89,18 @@ int split_rows_ctas_per_sm() {
     return v < 1 ? 1 : (v > 64 ? 64 : v);
 }
 
+}  // namespace
+
 // Test hook of the failure-detection tests (FPEMU_TEST_STALL_UNIT=i): the TMA
 // producers of the GEMM's first unit stop delivering at their unit i, so the
 // consumers' bounded waits run out exactly as they would behind a stalled
 // producer.  Read on every call; -1 (unset) disables it.
-int test_stall_idx() {
+int fpemu::test_stall_idx() {
     const char* s = getenv("FPEMU_TEST_STALL_UNIT");
     return s && *s ? atoi(s) : -1;
 }
 
-uint64_t wait_budget_ns() {
+uint64_t fpemu::wait_budget_ns() {
     static uint64_t v = [] {
         const char* s = getenv("FPEMU_WAIT_BUDGET_MS");
         long long ms = s ? atoll(s) : 2000;
@@ -107,8 +109,6 @@ uint64_t wait_budget_ns() {
     }();
     return v;
 }
-
-}  // namespace
 
 PFN_cuTensorMapEncodeTiled_v12000 fpemu::tensor_map_encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {

@@ -28,6 +28,11 @@ int device_info(DevInfo* out);
 // The driver's encoder of TMA tensor maps (null if the driver has none).
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
+// How long a kernel's wait may take (FPEMU_WAIT_BUDGET_MS), and the unit at which
+// the failure tests' producers stop (FPEMU_TEST_STALL_UNIT; -1: none).
+uint64_t wait_budget_ns();
+int test_stall_idx();
+
 // Device address of the record that fpemu_device_error() reads, and of its
 // host-visible copy (null until fpemu_watch_errors), for the current device.
 // Kernels of other translation units get both as arguments.
