@@ -109,7 +109,8 @@ __device__ __forceinline__ int row_class(const void* index, int wide, int64_t t,
 // One block per class.  Each warp counts the class's rows, and those of smaller
 // classes, in its own stretch of the index; a scan over the warps' counts gives
 // every warp its first position, and a second walk writes the rows in order.
-// No atomics: the order is that of the rows.
+// No atomics: the order is that of the rows.  Every block reads the whole index, which
+// stays in the L2: a few microseconds for the batches here, once for all layers.
 __global__ void __launch_bounds__(1024) adapter_plan_kernel(const void* index, int wide, int64_t rows, int adapters,
                                                             int32_t* plan, ErrorSink sink) {
     __shared__ int own_count[32], below_count[32];

@@ -9,10 +9,17 @@
 // workspace, which the second kernel adds in the blocks' order.  x, base and y
 // pass through one block once; u and its parts are a rank wide and stay in the L2.
 //
-// What a chunk costs: the rank is small, so both products are bound by the
-// bytes of x, base and y for float64 up to rank 16 and for 16-bit data up to
-// rank 64; mma.sync reaches 37 TFLOP/s for f64 (the device's whole rate), 545
-// for 16-bit and 273 for tf32 data, which is enough there.
+// What bounds them: the bytes of x, base and y, as long as the rank is small --
+// float64 up to rank 16 or so (mma.sync f64 reaches 37 TFLOP/s, the device's whole
+// rate), 16-bit data up to rank 64 (545 TFLOP/s; tf32, for floats, 273).  Measured:
+//   float64, 16384 x 4096 -> 4096, rank 16, 8 adapters in runs: 300 us, 5.4 TB/s of
+//     algorithmic bytes, 0.83 of the measured copy rate (107 us for u, 5.0 TB/s);
+//   half, 16384 x 4096 -> 8192, rank 64, 16 adapters: 207 us, 3.4 TB/s.  There the
+//     second kernel (170 us) is bound by what a computing warp does for a chunk:
+//     without its matrix instructions it takes 119 us, its copies alone 80.
+// One kernel for both products, in clusters that exchanged the middle through
+// distributed shared memory, took 330 and 199 us: its blocks' shares came in whole
+// slots, and 256 of them on 148 SMs left a seventh of the device idle.
 #pragma once
 
 #include <cuda.h>
@@ -306,8 +313,10 @@ constexpr int kCopyBarrier = 1, kWorkBarrier = 2;
 
 // The ring of chunks: a buffer is full when TMA's bytes and every copying thread's
 // copies have arrived (and what they wrote themselves is visible), and free again
-// when each of the eight computing warps has left it.  So a warp runs ahead of another by as many
-// chunks as there are buffers, and loads, products and stores overlap.
+// when each of the eight computing warps has left it.  So a warp runs ahead of
+// another by as many chunks as there are buffers, and loads, products and stores
+// overlap.  Waits are bounded (FPEMU_WAIT_BUDGET_MS): when one runs out, the error
+// is recorded and what could not be finished becomes NaN.
 template <int S>
 struct ChunkRing {
     uint64_t full[S], empty[S];
@@ -918,10 +927,17 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
 // the adapter's rows, so q is read once and p (rank values a row) by every block
 // of columns.  Where that gives too few blocks, a cluster splits the rows into
 // consecutive parts, whose sums meet in the blocks' order.
+//
+// Bound by the bytes of x and dy on paper; measured, 16384 x 4096 bfloat16, rank 32,
+// four adapters: 116 us for the 268 MB of both, 2.3 TB/s, with the warps waiting for
+// their loads from shared memory and for one another in turn.  The ring of the
+// products, with two copying warps, was no faster here (117 us) and slower for rows
+// in any order (3333 x 1024 bfloat16 rank 20: 35 us against 18), whose copies two
+// warps cannot issue fast enough.
 constexpr int kGradThreads = 128;
 
 struct AdapterGradSide {
-    const void* p;  // [rows, p_row] of the sums' type
+    const void* p;  // [rows, p_row], as the products left it
     const void* q;  // [rows, cols]
     int64_t q_row, cols;
     void* grad;     // [adapters, r, cols] or, by_column, [adapters, cols, r]
