@@ -9,9 +9,9 @@
 // instruction; in the second product the sixteen rows of its wide side hold the
 // eight rows twice, as the high and the low part of the middle.
 //
-// Measured (kernel alone): 32 rows with an adapter each, 4096 -> 4096 bfloat16, rank
-// 16: 10.5 us (its 9 MB take 1.4 at the copy rate); 200 rows of 24 adapters, float64:
-// 18 us (44 MB, 6.8).  What is left is latency, a few microseconds each for finding
+// Measured (kernel alone, cold L2), 4096 -> 4096, rank 16: 32 rows with an adapter
+// each, bfloat16, 9.7 us (its 9 MB take 1.4 at the copy rate), float64 15.8 (5.6);
+// 200 rows of 24 adapters, 10.6 (1.7) and 19.4 (6.9); 7 us for any tiny call.  What is left is latency, a few microseconds each for finding
 // the rows, the two streams of loads and the two meetings of the cluster; the call's
 // host side takes 15 us.  Fetching the weights ahead into the L2 changed nothing.
 #pragma once
@@ -28,12 +28,21 @@ __device__ __forceinline__ void mma_f64_8(double (&c)[2], double a, double b) {
                  : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
 }
 
-// 16 bytes of a row: `avail` elements, zeros after them.  (Not through the read-only
-// path: base may be y itself.)
-template <typename T>
-__device__ __forceinline__ uint4 load16(const T* p, int avail, bool vec) {
+// 16 bytes of a row: `avail` elements, zeros after them.  Vec: the row is aligned and
+// `avail` is a whole 16 bytes or none; the load is predicated, not branched around, so
+// that a thread's loads leave together.  (Not through the read-only path: base may be
+// y itself.)
+template <bool Vec, typename T>
+__device__ __forceinline__ uint4 load16(const T* p, int avail) {
     constexpr int V = 16 / sizeof(T);
-    if (vec && avail >= V) return *reinterpret_cast<const uint4*>(p);
+    if constexpr (Vec) {
+        uint4 v;
+        asm("{\n.reg .pred p;\nsetp.gt.s32 p, %5, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\nmov.b32 %2, 0;\nmov.b32 %3, 0;\n"
+            "@p ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n}"
+            : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+            : "l"(p), "r"(avail));
+        return v;
+    }
     alignas(16) T v[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = i < avail ? p[i] : T(0.0f);
@@ -71,15 +80,13 @@ struct FewTile {
     static constexpr int E = sizeof(T), V = 16 / E, KS = 4 * V;     // elements of k a warp takes at a step
     static constexpr int MR = E == 8 ? 8 : 16;                      // ranks of an instruction
     static constexpr int RT = RP / MR, PA = E == 8 ? 2 : 4;         // rank tiles; sums a thread holds of one
-    static constexpr int UN = RP <= 16 ? (E == 8 ? 3 : 4) : RP <= 32 ? 2 : 1;  // steps with their loads in flight together
+    static constexpr int UN = RP <= 16 ? 4 : RP <= 32 ? 2 : 1;  // steps with their loads in flight together
     static constexpr int JS = (RP + KS - 1) / KS;                   // 16-byte steps along the rank
-    static constexpr int UG = JS * V >= 16 ? 1 : JS * V >= 8 ? 2 : E == 8 ? 3 : 4;  // column groups, likewise
+    static constexpr int UG = E == 8 && RP <= 16 ? 4 : JS * V >= 16 ? 1 : JS * V >= 8 ? 2 : 4;  // column groups, likewise
     static constexpr int kWarps = kFewThreads / 32;
     static constexpr int kSmem = (kWarps + 2) * RP * kGroupRows * (int)sizeof(Acc);
-    static constexpr int kBlocks = RP <= 16 && E != 4 ? 3 : RP <= 64 ? 2 : 1;  // an SM, by registers
-    // Whether the second product's first loads start before the blocks exchange the middle (for float64
-    // the registers they hold cost more: 200 rows, 24 adapters, 4096 x 4096: 27 us against 24).
-    static constexpr bool kEarly = E != 8;
+    // An SM's blocks, by registers (three with 80 registers each spill: 32 rows, bfloat16, 10.4 us for 9.7).
+    static constexpr int kBlocks = RP <= 64 ? 2 : 1;
 };
 
 template <typename T, int RP>
@@ -159,60 +166,66 @@ __global__ void __launch_bounds__(kFewThreads, FewTile<T, RP>::kBlocks) adapter_
     }
 
     Acc acc[RT][Tile::PA] = {};
-    for (int c = k0 + warp * KS; c < k1; c += W * KS * UN) {
-        uint4 xv[UN], wv[UN][RT][MR / 8];
+    auto add_up = [&](auto vec) {
+        for (int c = k0 + warp * KS; c < k1; c += W * KS * UN) {
+            uint4 xv[UN], wv[UN][RT][MR / 8];
 #pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            const int at = c + u * W * KS + q * V, avail = k1 - at;
-            xv[u] = load16(xp + at, avail, vec_x);
+            for (int u = 0; u < UN; ++u) {
+                const int at = c + u * W * KS + q * V, avail = k1 - at;
+                xv[u] = load16<vec>(xp + at, avail);
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
+                for (int t = 0; t < RT; ++t)
 #pragma unroll
-                for (int h = 0; h < MR / 8; ++h) {
-                    const int j = t * MR + h * 8 + g;
-                    wv[u][t][h] = load16(w1 + (j < P.r ? j : 0) * P.w1_row + at, avail, vec_w1);
-                }
-        }
+                    for (int h = 0; h < MR / 8; ++h) {
+                        const int j = t * MR + h * 8 + g;
+                        wv[u][t][h] = load16<vec>(w1 + j * P.w1_row + at, j < P.r ? avail : 0);
+                    }
+            }
 #pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            const uint32_t* xr = reinterpret_cast<const uint32_t*>(&xv[u]);
+            for (int u = 0; u < UN; ++u) {
+                const uint32_t* xr = reinterpret_cast<const uint32_t*>(&xv[u]);
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                if constexpr (E == 8) {
-                    const double* xd = reinterpret_cast<const double*>(&xv[u]);
-                    const double* wd = reinterpret_cast<const double*>(&wv[u][t][0]);
-                    mma_f64_8(acc[t], wd[0], xd[0]);
-                    mma_f64_8(acc[t], wd[1], xd[1]);
-                } else {
-                    const uint32_t* wa = reinterpret_cast<const uint32_t*>(&wv[u][t][0]);
-                    const uint32_t* wb = reinterpret_cast<const uint32_t*>(&wv[u][t][MR / 8 - 1]);
+                for (int t = 0; t < RT; ++t) {
+                    if constexpr (E == 8) {
+                        const double* xd = reinterpret_cast<const double*>(&xv[u]);
+                        const double* wd = reinterpret_cast<const double*>(&wv[u][t][0]);
+                        mma_f64_8(acc[t], wd[0], xd[0]);
+                        mma_f64_8(acc[t], wd[1], xd[1]);
+                    } else {
+                        const uint32_t* wa = reinterpret_cast<const uint32_t*>(&wv[u][t][0]);
+                        const uint32_t* wb = reinterpret_cast<const uint32_t*>(&wv[u][t][MR / 8 - 1]);
 #pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        if constexpr (E == 2) {
-                            const uint32_t a[4] = {wa[2 * m], wb[2 * m], wa[2 * m + 1], wb[2 * m + 1]};
-                            mma16<T>(acc[t], a, xr[2 * m], xr[2 * m + 1]);
-                        } else {
-                            const Tf32Pair p0 = tf32_split(__uint_as_float(wa[2 * m]));
-                            const Tf32Pair p1 = tf32_split(__uint_as_float(wb[2 * m]));
-                            const Tf32Pair p2 = tf32_split(__uint_as_float(wa[2 * m + 1]));
-                            const Tf32Pair p3 = tf32_split(__uint_as_float(wb[2 * m + 1]));
-                            const Tf32Pair b0 = tf32_split(__uint_as_float(xr[2 * m]));
-                            const Tf32Pair b1 = tf32_split(__uint_as_float(xr[2 * m + 1]));
-                            const uint32_t hi[4] = {p0.hi, p1.hi, p2.hi, p3.hi}, lo[4] = {p0.lo, p1.lo, p2.lo, p3.lo};
-                            mma_tf32(acc[t], hi, b0.lo, b1.lo);
-                            mma_tf32(acc[t], lo, b0.hi, b1.hi);
-                            mma_tf32(acc[t], hi, b0.hi, b1.hi);
+                        for (int m = 0; m < 2; ++m) {
+                            if constexpr (E == 2) {
+                                const uint32_t a[4] = {wa[2 * m], wb[2 * m], wa[2 * m + 1], wb[2 * m + 1]};
+                                mma16<T>(acc[t], a, xr[2 * m], xr[2 * m + 1]);
+                            } else {
+                                const Tf32Pair p0 = tf32_split(__uint_as_float(wa[2 * m]));
+                                const Tf32Pair p1 = tf32_split(__uint_as_float(wb[2 * m]));
+                                const Tf32Pair p2 = tf32_split(__uint_as_float(wa[2 * m + 1]));
+                                const Tf32Pair p3 = tf32_split(__uint_as_float(wb[2 * m + 1]));
+                                const Tf32Pair b0 = tf32_split(__uint_as_float(xr[2 * m]));
+                                const Tf32Pair b1 = tf32_split(__uint_as_float(xr[2 * m + 1]));
+                                const uint32_t hi[4] = {p0.hi, p1.hi, p2.hi, p3.hi}, lo[4] = {p0.lo, p1.lo, p2.lo, p3.lo};
+                                mma_tf32(acc[t], hi, b0.lo, b1.lo);
+                                mma_tf32(acc[t], lo, b0.hi, b1.hi);
+                                mma_tf32(acc[t], hi, b0.hi, b1.hi);
+                            }
                         }
                     }
                 }
             }
         }
-    }
+    };
+    if (vec_x && vec_w1 && k % V == 0)
+        add_up(std::true_type{});
+    else
+        add_up(std::false_type{});
     // The second product's loads: UG groups of KS columns of this warp, their weights and base.
     constexpr int NT = V / 2;  // 8-column tiles of a group; a thread's results are 16 bytes of neighbours
     constexpr int UG = Tile::UG;
     uint4 w2v[UG][NT][JS], held[UG];
-    auto load_groups = [&](int first) {
+    auto load_groups = [&](int first, auto vec) {
 #pragma unroll
         for (int u = 0; u < UG; ++u) {
             const int c0 = first + u * W * KS;
@@ -221,13 +234,20 @@ __global__ void __launch_bounds__(kFewThreads, FewTile<T, RP>::kBlocks) adapter_
 #pragma unroll
                 for (int t = 0; t < JS; ++t) {
                     const int c = c0 + g / 2 * V + 2 * p + g % 2, j = t * KS + q * V;
-                    w2v[u][p][t] = c < n1 && j < P.r ? load16(w2 + c * P.w2_row + j, P.r - j, vec_w2) : uint4{0, 0, 0, 0};
+                    w2v[u][p][t] = load16<vec>(w2 + c * P.w2_row + j, c < n1 ? P.r - j : 0);
                 }
             const int avail = g < count ? n1 - c0 - q * V : 0;
-            held[u] = base && avail > 0 ? load16(base + c0 + q * V, avail, vec_base) : uint4{0, 0, 0, 0};
+            held[u] = load16<vec>(base + c0 + q * V, base ? avail : 0);
         }
     };
-    if (Tile::kEarly) load_groups(n0 + warp * KS);
+    const bool vec2 = vec_w2 && vec_base && P.r % V == 0 && n % V == 0;
+    auto load_second = [&](int first) {
+        if (vec2)
+            load_groups(first, std::true_type{});
+        else
+            load_groups(first, std::false_type{});
+    };
+    load_second(n0 + warp * KS);  // its first loads cross the exchange of the middle
 
 #pragma unroll
     for (int t = 0; t < RT; ++t)
@@ -284,7 +304,7 @@ __global__ void __launch_bounds__(kFewThreads, FewTile<T, RP>::kBlocks) adapter_
         }
     }
     for (int first = n0 + warp * KS; first < n1; first += W * KS * UG) {
-        if (!Tile::kEarly || first != n0 + warp * KS) load_groups(first);
+        if (first != n0 + warp * KS) load_second(first);
 #pragma unroll
         for (int u = 0; u < UG; ++u) {
             const int col = first + u * W * KS + q * V, avail = g < count ? n1 - col : 0;
