@@ -58,8 +58,10 @@ def prepare_rows(index, adapters, shape=None):
     0 .. adapters - 1, or -1 for none; ``shape`` gives it the leading shape of the
     layers' inputs where it has fewer dimensions (one id for each request of a
     [requests, length, features] batch).  Later changes of ``index`` do not
-    change the result.  An id that is no adapter makes its rows NaN and raises
-    ``FpemuError`` in the first call that ends after the kernel has seen it."""
+    change the result.  On another stream than the one it was made on, wait for that
+    one first, and keep the result until its uses have finished.  An id that is no
+    adapter makes its rows NaN and raises ``FpemuError`` in the first call that ends
+    after the kernel has seen it."""
     return PreparedRows(index, adapters, shape)
 
 
@@ -331,14 +333,21 @@ class _ActiveRows:
 def use_adapters(model, index):
     """Within the block, the model's layers that have adapters (``add_adapters``)
     apply row t's adapter ``index[t]`` (-1: none).  ``index`` has the leading shape
-    of the layers' inputs, or the first dimensions of it."""
+    of the layers' inputs, or the first dimensions of it, and is copied as the block
+    begins: later changes of it take no effect (a CUDA graph that is to follow them
+    captures the whole block).  The block holds for the model, in every thread; a
+    backward pass that computes the layers again (activation checkpointing) has to
+    run inside it."""
     from fp_emulation.nn import Linear
+
+    if not isinstance(index, torch.Tensor) or index.dtype not in (torch.int32, torch.int64):
+        raise TypeError("adapter ids are an int32 or int64 tensor")
 
     layers = [m for m in model.modules() if isinstance(m, Linear) and m._modules.get("adapters") is not None]
     if not layers:
         raise RuntimeError("use_adapters: the model has no Linear with adapters (add_adapters)")
     before = [m.active_rows for m in layers]
-    active = _ActiveRows(index)
+    active = _ActiveRows(index.clone())
     for m in layers:
         m.active_rows = active
     try:
