@@ -191,20 +191,32 @@ int launch_tiles(AdapterParams& P, const DevInfo& d, cudaStream_t st) {
 }
 
 template <typename T, int RP>
-int launch_grad_rank(AdapterGradParams& P, const DevInfo& d, cudaStream_t st) {
+int launch_grad_rank(AdapterGradParams& P, size_t parts_bytes, const DevInfo& d, cudaStream_t st) {
     using Tile = AdapterGradTile<T, RP>;
     auto kern = adapter_grad_kernel<T, RP>;
     FPEMU_TRY((allow_shared<adapter_grad_kernel<T, RP>>(Tile::kSmem)));
     int64_t blocks[2];
     for (int i = 0; i < 2; ++i) blocks[i] = P.side[i].grad ? (P.side[i].cols + Tile::COLS - 1) / Tile::COLS : 0;
     if (blocks[0] + blocks[1] == 0) return FPEMU_OK;
+    // The most parts of an adapter's rows with which the blocks are on the device together, five an SM
+    // (16384 rows of 4 adapters, 4096 x 4096 bfloat16, rank 32: 96 us in 512 blocks, 117 in 1024); twice
+    // that while a part is long enough for its start not to count, since an SM's last blocks weigh less
+    // then (the same in float64: 315 us in 1024 blocks, 377 in 512).
+    const int64_t all = (blocks[0] + blocks[1]) * P.adapters, each = P.rows / P.adapters;
     int cluster = 1;
-    while (cluster < 8 && (blocks[0] + blocks[1]) * P.adapters * cluster < d.sms * 4 &&
-           P.rows / P.adapters > cluster * 4 * Tile::KT)
+    while (cluster < kGradCluster && each > cluster * 4 * Tile::KT &&
+           all * cluster * 2 <= d.sms * (each >= cluster * 128 * Tile::KT ? 10 : 5))
         cluster *= 2;
+    // Segments of 8 chunks a block or more, as many as the device holds and the workspace has room for
+    // (bfloat16, one adapter, with the second kernel and without segments: 20000 rows, 512 -> 512, rank 16,
+    // 22 us and 62; a million rows, 32 -> 32, rank 8, 118 and 2670).
+    int64_t segments = 1;
+    if (cluster == kGradCluster && P.parts != nullptr)
+        segments = std::max<int64_t>(1, std::min({d.sms * 5 / (all * cluster), each / (cluster * 8 * Tile::KT),
+                                                  (int64_t)(parts_bytes / (grad_values(P, 2) * sizeof(typename Tile::Acc)))}));
     P.first_blocks = blocks[0] * cluster;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((blocks[0] + blocks[1]) * cluster), (unsigned)P.adapters);
+    cfg.gridDim = dim3((unsigned)((blocks[0] + blocks[1]) * cluster), (unsigned)P.adapters, (unsigned)segments);
     cfg.blockDim = dim3(kGradThreads);
     cfg.dynamicSmemBytes = Tile::kSmem;
     cfg.stream = st;
@@ -216,15 +228,20 @@ int launch_grad_rank(AdapterGradParams& P, const DevInfo& d, cudaStream_t st) {
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     FPEMU_CUDA(cudaLaunchKernelEx(&cfg, kern, P));
+    if (segments > 1) {
+        const int64_t grid = std::min<int64_t>((grad_values(P, 2) + 255) / 256, d.sms * 8);
+        adapter_grad_join_kernel<T><<<(unsigned)grid, 256, 0, st>>>(P, (int)segments);
+        FPEMU_CUDA(cudaGetLastError());
+    }
     return FPEMU_OK;
 }
 
 template <typename T>
-int launch_grad(AdapterGradParams& P, const DevInfo& d, cudaStream_t st) {
-    if (P.r <= 16) return launch_grad_rank<T, 16>(P, d, st);
-    if (P.r <= 32) return launch_grad_rank<T, 32>(P, d, st);
-    if (P.r <= 64) return launch_grad_rank<T, 64>(P, d, st);
-    return launch_grad_rank<T, 128>(P, d, st);
+int launch_grad(AdapterGradParams& P, size_t parts_bytes, const DevInfo& d, cudaStream_t st) {
+    if (P.r <= 16) return launch_grad_rank<T, 16>(P, parts_bytes, d, st);
+    if (P.r <= 32) return launch_grad_rank<T, 32>(P, parts_bytes, d, st);
+    if (P.r <= 64) return launch_grad_rank<T, 64>(P, parts_bytes, d, st);
+    return launch_grad_rank<T, 128>(P, parts_bytes, d, st);
 }
 
 size_t workspace_size(const DevInfo& d, int dtype, int64_t rows, int64_t rank, int64_t adapters) {
@@ -364,7 +381,8 @@ int fpemu_adapter_backward(int dtype, int64_t rows, int64_t k, int64_t n, int64_
         G.plan = static_cast<const int32_t*>(plan);
         G.side[0] = AdapterGradSide{v, x, x_row, k, dA, 0};
         G.side[1] = AdapterGradSide{u, dy, dy_row, n, dB, 1};
-        return launch_grad<T>(G, d, st);
+        if (dx || dA) G.parts = workspace;  // the products before have been through with it
+        return launch_grad<T>(G, workspace_bytes, d, st);
     });
 }
 

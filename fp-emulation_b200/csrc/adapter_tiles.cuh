@@ -926,15 +926,18 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
 // A block holds a stretch of columns and all of the rank in registers and walks
 // the adapter's rows, so q is read once and p (rank values a row) by every block
 // of columns.  Where that gives too few blocks, a cluster splits the rows into
-// consecutive parts, whose sums meet in the blocks' order.
+// consecutive parts, whose sums meet in the blocks' order; where a cluster of eight is
+// still too little, the rows come in segments, a cluster each, whose sums meet in the
+// forward pass's workspace.
 //
 // Bound by the bytes of x and dy on paper; measured, 16384 x 4096 bfloat16, rank 32,
-// four adapters: 116 us for the 268 MB of both, 2.3 TB/s, with the warps waiting for
-// their loads from shared memory and for one another in turn.  The ring of the
-// products, with two copying warps, was no faster here (117 us) and slower for rows
-// in any order (3333 x 1024 bfloat16 rank 20: 35 us against 18), whose copies two
-// warps cannot issue fast enough.
+// four adapters: 96 us for the 268 MB of both, 2.8 TB/s, with the warps waiting for
+// their loads from shared memory and for one another in turn; a million rows, 32
+// columns to 32, rank 8, one adapter: 118 us for 192 MB.  The ring of the products, with two
+// copying warps, was no faster here and slower for rows in any order (3333 x 1024
+// bfloat16 rank 20: 35 us against 18), whose copies two warps cannot issue fast enough.
 constexpr int kGradThreads = 128;
+constexpr int kGradCluster = 8;  // the most blocks whose sums meet in a cluster
 
 struct AdapterGradSide {
     const void* p;  // [rows, p_row], as the products left it
@@ -949,7 +952,15 @@ struct AdapterGradParams {
     int64_t rows;
     int r, p_row, adapters;
     const int32_t* plan;
+    void* parts;  // with several segments of the rows: their sums, laid out like the gradients
 };
+
+// The values of the first `sides` gradients that are wanted.
+__host__ __device__ inline int64_t grad_values(const AdapterGradParams& P, int sides) {
+    int64_t v = 0;
+    for (int i = 0; i < sides; ++i) v += P.side[i].grad ? (int64_t)P.adapters * P.r * P.side[i].cols : 0;
+    return v;
+}
 
 template <typename T, int RP>
 struct AdapterGradTile {
@@ -961,7 +972,7 @@ struct AdapterGradTile {
     static constexpr int kPitchQ = COLS * E + (E == 2 ? 16 : 32);
     static constexpr int kPitchP = (RP + (E == 4 ? 8 : 4)) * (int)sizeof(Acc);
     static constexpr int kStage = KT * (kPitchQ + kPitchP);
-    static constexpr int kStages = RP <= 64 ? 4 : 3;
+    static constexpr int kStages = 3;  // a fourth leaves room for fewer blocks: 3333 x 1023 -> 515 floats, 24 us for 20
     static constexpr int kPitchD = RP + 1;                    // the block's sums, after the rows
     static constexpr int kJoin = COLS * kPitchD * (int)sizeof(Acc);
     static constexpr int kSmem = kStages * kStage > kJoin ? kStages * kStage : kJoin;
@@ -983,8 +994,9 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
     const int cls = blockIdx.y;
     const int start = P.plan[cls], rows = P.plan[cls + 1] - start;
     const int32_t* perm = P.plan + plan_perm_word(P.rows, P.adapters) + start;
-    const int share = (rows + KT * cs - 1) / (KT * cs) * KT;
-    const int t0 = cr * share < rows ? cr * share : rows, t1 = t0 + share < rows ? t0 + share : rows;
+    const int ways = cs * (int)gridDim.z, way = (int)blockIdx.z * cs + cr;
+    const int share = (int)(((int64_t)rows + KT * ways - 1) / (KT * ways) * KT);
+    const int t0 = (int64_t)way * share < rows ? way * share : rows, t1 = t0 + share < rows ? t0 + share : rows;
     const int chunks = (t1 - t0 + KT - 1) / KT;
     const T* qs = static_cast<const T*>(side.q);
     const Acc* ps = static_cast<const Acc*>(side.p);
@@ -1153,23 +1165,45 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
                 mine[((warp * MT + m) * 16 + g + (e >> 1) * 8) * Tile::kPitchD +
                      (E == 2 ? t / 2 * 16 + 2 * (2 * q + (e & 1)) + t % 2 : t * 8 + 2 * q + (e & 1))] = acc[m][t][e];
     cluster.sync();
-    const Acc* parts[8];
+    const Acc* parts[kGradCluster];
 #pragma unroll
-    for (int b = 0; b < 8; ++b) parts[b] = b < cs ? cluster.map_shared_rank(mine, b) : nullptr;
+    for (int b = 0; b < kGradCluster; ++b) parts[b] = b < cs ? cluster.map_shared_rank(mine, b) : nullptr;
     const int cols = side.cols - c0 < COLS ? (int)(side.cols - c0) : COLS, own = COLS / cs;
     const int first = cr * own, last = first + own < cols ? first + own : cols;
-    T* grad = static_cast<T*>(side.grad) + (int64_t)cls * P.r * side.cols;
+    const int64_t at = (int64_t)cls * P.r * side.cols;
+    T* grad = static_cast<T*>(side.grad) + at;
+    Acc* part = nullptr;
+    if (gridDim.z > 1)
+        part = static_cast<Acc*>(P.parts) + grad_values(P, 2) * blockIdx.z + (second ? grad_values(P, 1) : 0) + at;
     const int many = last > first ? (last - first) * P.r : 0;
     for (int i = tid; i < many; i += kGradThreads) {
         const int c = first + (side.by_column ? i / P.r : i % (last - first));
         const int j = side.by_column ? i % P.r : i / (last - first);
         Acc v = 0;
 #pragma unroll
-        for (int b = 0; b < 8; ++b)
+        for (int b = 0; b < kGradCluster; ++b)
             if (b < cs) v += parts[b][c * Tile::kPitchD + j];
-        grad[side.by_column ? (c0 + c) * P.r + j : j * side.cols + c0 + c] = narrow<T>(v);
+        const int64_t o = side.by_column ? (c0 + c) * P.r + j : j * side.cols + c0 + c;
+        if (part)
+            part[o] = v;
+        else
+            grad[o] = narrow<T>(v);
     }
     cluster.sync();
+}
+
+// Adds the segments' sums in their order.
+template <typename T>
+__global__ void __launch_bounds__(256) adapter_grad_join_kernel(const __grid_constant__ AdapterGradParams P, int segments) {
+    using Acc = typename AccOf<T>::type;
+    const int64_t first = grad_values(P, 1), all = grad_values(P, 2);
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
+        const Acc* p = static_cast<const Acc*>(P.parts) + i;
+        Acc v = 0;
+#pragma unroll 8
+        for (int s = 0; s < segments; ++s) v += p[s * all];
+        static_cast<T*>(P.side[i >= first].grad)[i >= first ? i - first : i] = narrow<T>(v);
+    }
 }
 
 }  // namespace fpemu

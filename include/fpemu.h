@@ -241,7 +241,7 @@ size_t fpemu_adapter_workspace_size(int dtype, int64_t rows, int64_t rank, int64
  * dA[i] = sum_t v[t]^T x[t], dB[i] = sum_t dy[t]^T u[t] over the rows t of adapter i
  * (packed, [adapters][rank][k] and [adapters][n][rank], zero for an adapter without
  * rows), where v[t] = s_i dy[t] B_i; v is scratch like u, 16-byte aligned.  dx, dA and
- * dB may each be NULL.  plan, scales, strides and workspace as above. */
+ * dB may each be NULL.  plan, scales, strides and workspace (for dx or dA) as above. */
 int fpemu_adapter_backward(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank,
                            int64_t adapters, const void *x, int64_t x_row, const void *A,
                            int64_t A_adapter, int64_t A_row, const void *B, int64_t B_adapter,

@@ -220,3 +220,33 @@ def test_block_of_linear_layers():
         ids.copy_(source)
         graph.replay()
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("adapters", [1, 3])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_long_batches_of_narrow_layers(dtype, adapters):
+    """Few columns and many rows: the gradients' sums come in several parts."""
+    rows, k, m, r = 30011, 40, 24, 5
+    x, A, B, base, dy, scale, index = _data(rows, adapters, k, m, r, dtype, "mixed", 8)
+    index[-7000:] = adapters - 1
+    for t in (x, A, B):
+        t.requires_grad_(True)
+
+    def grads(*wanted):
+        y = fp.adapter_matmul(x, A, B, index, base=base, scale=scale)
+        return torch.autograd.grad(y, wanted, dy)
+
+    dx, dA, dB = grads(x, A, B)
+    assert all(torch.equal(a, b) for a, b in zip(grads(x, A, B), (dx, dA, dB)))
+    only_A, = grads(A)
+    only_B, = grads(B)
+    with torch.no_grad():
+        _, _, u, ua = _formula(x, A, B, base, scale, index)
+        dxw, dxm, v, va = _formula(dy, B.transpose(1, 2), A.transpose(1, 2), None, scale, index)
+        _close(dx, dxw, dxm, m + r, dtype)
+        for i in range(adapters):
+            t = index == i
+            for got in (dA[i], only_A[i]):
+                _close(got, v[t].T @ x[t].double(), va[t].T @ x[t].double().abs(), m + rows, dtype)
+            for got in (dB[i], only_B[i]):
+                _close(got, dy[t].double().T @ u[t], dy[t].double().abs().T @ ua[t], k + rows, dtype)
