@@ -81,6 +81,11 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _packed_like(t, shape):
+    """A new packed tensor of t's type (the cheapest way there is to make one)."""
+    return torch.empty_like(t) if t.shape == shape and t.is_contiguous() else t.new_empty(shape)
+
+
 def _launch(x, A, B, base, y, scale, rows, index, u):
     """One fpemu_adapter_matmul on the current stream of x's device (2-D x, base and y)."""
     dev = x.device
@@ -94,7 +99,7 @@ def _launch(x, A, B, base, y, scale, rows, index, u):
         if count > _lib.FPEMU_ADAPTER_FEW_ROWS:
             plan = rows.plan.data_ptr()
             size = lib.fpemu_adapter_workspace_size(code, count, rank, adapters)
-            work = torch.empty((size,), dtype=torch.uint8, device=dev)
+            work = x.new_empty((size // x.element_size(),))
         st = lib.fpemu_adapter_matmul(
             code, count, k, B.shape[1], rank, adapters, x.data_ptr(), _row_stride(x), A.data_ptr(), A.stride(0),
             A.stride(1), B.data_ptr(), B.stride(0), B.stride(1), None if base is None else base.data_ptr(),
@@ -114,7 +119,7 @@ class _AdapterMatmul(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, A, B, base, rows, scale):
-        y = torch.empty((x.shape[0], B.shape[1]), dtype=x.dtype, device=x.device)
+        y = _packed_like(x if base is None else base, (x.shape[0], B.shape[1]))
         u = torch.empty((x.shape[0], (A.shape[1] + 3) // 4 * 4),
                         dtype=torch.float64 if x.dtype == torch.float64 else torch.float32, device=x.device)
         _launch(x, A, B, base, y, scale, rows, rows.index, u)
@@ -145,14 +150,14 @@ class _AdapterMatmul(torch.autograd.Function):
         lib = _lib.load()
         code = _DTYPE_CODE[x.dtype]
         with _on(d):
-            dx = torch.empty((count, k), dtype=x.dtype, device=dev) if need_x else None
-            dA = torch.empty((adapters, rank, k), dtype=x.dtype, device=dev) if need_A else None
-            dB = torch.empty((adapters, n, rank), dtype=x.dtype, device=dev) if need_B else None
+            dx = _packed_like(x, (count, k)) if need_x else None
+            dA = _packed_like(A, (adapters, rank, k)) if need_A else None
+            dB = _packed_like(B, (adapters, n, rank)) if need_B else None
             size = v = work = None
             if need_x or need_A:  # v, then the workspace
                 size = lib.fpemu_adapter_workspace_size(code, count, rank, adapters)
                 v_bytes = u.numel() * u.element_size()  # of rows of 16 bytes or more
-                work = torch.empty((size + v_bytes,), dtype=torch.uint8, device=dev)
+                work = x.new_empty(((size + v_bytes) // x.element_size(),))
                 v = work.data_ptr()
             st = lib.fpemu_adapter_backward(
                 code, count, k, n, rank, adapters, x.data_ptr(), _row_stride(x), A.data_ptr(), A.stride(0), A.stride(1),
@@ -276,7 +281,7 @@ def adapter_matmul(x, A, B, rows, base=None, scale=1.0, out=None):
         y = _AdapterMatmul.apply(x2, A, B, base2, rows, scale)
         return y if flat else y.view(shape)
     if out is None:
-        y = torch.empty((count, n), dtype=dtype, device=x.device)
+        y = _packed_like(x2 if base2 is None else base2, (count, n))
     else:
         y = _check_out(out, shape, x, base, (x2, A, B))
     _launch(x2, A, B, base2, y, scale, rows, index, None)
