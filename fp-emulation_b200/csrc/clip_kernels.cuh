@@ -10,8 +10,8 @@
 //
 // Bound by the bytes: the norm reads every element once, the scaling reads and
 // writes it (what the norm read last from the L2).  Measured, 285 M bfloat16 values
-// in 38 tensors: norm 108 us, 5.3 TB/s (the conversions to double, 16 a clock and SM,
-// would take 63); scaling 181 us, 6.3 TB/s.  219 MB of mixed types in bounds: 41 us
+// in 38 tensors: norm 110 us, 5.2 TB/s (doubles made from the bits instead of by
+// conversions, 16 a clock and SM: no faster); scaling 181 us, 6.3 TB/s.  219 MB of mixed types in bounds: 41 us
 // for the norm, and 5 us to see that nothing is to be scaled.  Eight small tensors:
 // 3 us each, of a call that takes 25-40 on the host.
 #pragma once
