@@ -11,6 +11,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <limits.h>
 #include <stdint.h>
 
 #include <type_traits>
@@ -117,11 +118,34 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const void* index, i
     const int cls = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t stretch = ((rows + 31) / 32 + 31) / 32 * 32;
     const int64_t t0 = warp * stretch, t1 = t0 + stretch < rows ? t0 + stretch : rows;
+    constexpr int U = 8;  // ids a thread has in flight
+    auto ids = [&](int64_t b, int (&c)[U]) {
+        if (b + 32 * U <= t1) {  // all loads before the first use (a million rows: 222 us against 362; 16384: 6.5, 7.6)
+            auto load = [&](const auto* p) {
+                std::remove_cv_t<std::remove_pointer_t<decltype(p)>> v[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u] = p[b + u * 32 + lane];
+#pragma unroll
+                for (int u = 0; u < U; ++u) c[u] = v[u] >= 0 && v[u] < adapters ? (int)v[u] : adapters + (v[u] != -1);
+            };
+            if (wide)
+                load(static_cast<const int64_t*>(index));
+            else
+                load(static_cast<const int32_t*>(index));
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t t = b + u * 32 + lane;
+                c[u] = t < t1 ? row_class(index, wide, t, adapters) : INT_MAX;
+            }
+        }
+    };
     int own = 0, below = 0;
-    for (int64_t t = t0 + lane; t < t1; t += 32) {
-        const int c = row_class(index, wide, t, adapters);
-        own += c == cls;
-        below += c < cls;
+    for (int64_t b = t0; b < t1; b += 32 * U) {
+        int c[U];
+        ids(b, c);
+#pragma unroll
+        for (int u = 0; u < U; ++u) own += c[u] == cls, below += c[u] < cls;
     }
     own = __reduce_add_sync(0xffffffffu, own);
     below = __reduce_add_sync(0xffffffffu, below);
@@ -135,12 +159,15 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const void* index, i
     }
     int32_t* perm = plan + plan_perm_word(rows, adapters);
     at += start;
-    for (int64_t b = t0; b < t1; b += 32) {
-        const int64_t t = b + lane;
-        const bool mine = t < t1 && row_class(index, wide, t, adapters) == cls;
-        const unsigned m = __ballot_sync(0xffffffffu, mine);
-        if (mine) perm[at + __popc(m & ((1u << lane) - 1))] = (int32_t)t;
-        at += __popc(m);
+    for (int64_t b = t0; b < t1; b += 32 * U) {
+        int c[U];
+        ids(b, c);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const unsigned m = __ballot_sync(0xffffffffu, c[u] == cls);
+            if (c[u] == cls) perm[at + __popc(m & ((1u << lane) - 1))] = (int32_t)(b + u * 32 + lane);
+            at += __popc(m);
+        }
     }
     const int64_t s0 = start / kSlotRows + cls, s1 = (start + total) / kSlotRows + cls + 1;
     AdapterSlot* slots = reinterpret_cast<AdapterSlot*>(plan + plan_slot_word(adapters));
