@@ -148,6 +148,21 @@ __device__ __forceinline__ void split16(float x, float y, uint32_t& hi, uint32_t
     }
 }
 
+// Two neighbouring floats as three bfloat16 parts each, largest first, which hold all of their 24
+// bits: every part is cut, not rounded, so that a finite value stays finite and the rest is exact.
+// The parts have one sign; those after an infinite one are finite.
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&p)[3]) {
+    constexpr uint32_t keep = 0xffff0000u;
+    auto rest = [](float v) {  // of an infinite v the difference is NaN
+        const float r = fabsf(v - __uint_as_float(__float_as_uint(v) & keep));
+        return copysignf(fminf(r, 1e38f), v);
+    };
+    const float x1 = rest(x), y1 = rest(y);
+    const float x2 = x1 - __uint_as_float(__float_as_uint(x1) & keep), y2 = y1 - __uint_as_float(__float_as_uint(y1) & keep);
+    auto pack = [](float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); };
+    p[0] = pack(x, y), p[1] = pack(x1, y1), p[2] = pack(x2, y2);
+}
+
 // How u and v are kept for the gradients: as they are, or, for bfloat16 data, as
 // the two parts that the products use (high in the upper half of the word), which
 // saves every block of the gradient kernel the splitting.

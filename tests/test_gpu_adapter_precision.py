@@ -1,0 +1,46 @@
+"""What the adapter products keep of the rank-long intermediate u = s A x, shown
+where its leading bits cancel.
+
+Every number below is a sum of few powers of two, chosen so that each product and
+each partial sum is exact in 24 bits: an evaluation that holds u as a float gives
+the expected value itself, with no rounding anywhere."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import fp_emulation as fp
+
+pytestmark = pytest.mark.gpu
+
+FEW = [1, 9, 200]
+
+
+def _cancelling(rows, p, k, m):
+    """u = (1 + 2^-8 + 2^-p, -(1 + 2^-8)); with B = (1, 1) only 2^-p is left."""
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    x[:, :3] = 1
+    A = torch.zeros(1, 2, k, dtype=torch.bfloat16, device="cuda")
+    A[0, 0, :3] = torch.tensor([1.0, 2.0 ** -8, 2.0 ** -p])
+    A[0, 1, :2] = torch.tensor([-1.0, -(2.0 ** -8)])
+    B = torch.ones(1, m, 2, dtype=torch.bfloat16, device="cuda")
+    return x, A, B, torch.zeros(rows, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("p", [12, 16, 18, 20])
+@pytest.mark.parametrize("rows", FEW)
+def test_bfloat16_middle_has_the_bits_of_a_float(rows, p):
+    x, A, B, index = _cancelling(rows, p, 40, 24)
+    y = fp.adapter_matmul(x, A, B, index)
+    assert torch.equal(y, torch.full_like(y, 2.0 ** -p))
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("rows", FEW)
+def test_infinite_bfloat16_row_keeps_its_sign(rows, sign):
+    """Weights of 8: no part of the infinite u may overflow to the other sign."""
+    x = torch.full((rows, 1), sign * float("inf"), dtype=torch.bfloat16, device="cuda")
+    A = torch.ones(1, 1, 1, dtype=torch.bfloat16, device="cuda")
+    B = torch.full((1, 20, 1), 8.0, dtype=torch.bfloat16, device="cuda")
+    y = fp.adapter_matmul(x, A, B, torch.zeros(rows, dtype=torch.int32, device="cuda"))
+    assert torch.equal(y, torch.full_like(y, sign * float("inf")))
