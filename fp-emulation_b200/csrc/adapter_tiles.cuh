@@ -606,6 +606,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     Acc* red = reinterpret_cast<Acc*>(smem + S * Tile::kStage);
     auto leave = [&](int64_t part) {
         flush();
+        named_barrier<kWorkBarrier, kTileThreads>();  // every warp has read the last slot's sums
         for (int p = 0; p < KW; ++p) {
             if (kw == p) {
 #pragma unroll
@@ -702,6 +703,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
         const int b0 = kper ? kshare.owner((int64_t)slot * kper) : 0;
         const int b1 = kper ? kshare.owner((int64_t)(slot + 1) * kper - 1) : -1;
         const Acc* parts = static_cast<const Acc*>(P.parts) + (int64_t)(b0 + slot) * (kSlotRows * RP);
+        named_barrier<kWorkBarrier, kTileThreads>();  // every warp has read the last slot's middle
 #pragma unroll 4
         for (int i = tid; i < kSlotRows * RP; i += kTileThreads) {
             Acc v = 0;
@@ -904,9 +906,13 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
             ring.failed = 1;
             ok = false;
         }
-        if (c == 0 || at == 0) {  // a warp that has given up still meets the others
-            if (ok) take_slot(slot, at);
-            else named_barrier<kWorkBarrier, kTileThreads>();
+        if (c == 0 || at == 0) {
+            if (ok) {
+                take_slot(slot, at);
+            } else {  // a warp that has given up still meets the others, as often as in take_slot
+                named_barrier<kWorkBarrier, kTileThreads>();
+                named_barrier<kWorkBarrier, kTileThreads>();
+            }
             ok = ok && !ring.failed;  // else a warp's share of the middle is missing
         }
         if (!ok) {  // what is left becomes NaN
