@@ -897,6 +897,14 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
         if (!Tile::kDirect || !whole) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     };
 
+    // This thread's share of a middle that take_slot did not get to.
+    auto lose_middle = [&](const AdapterSlot& s) {
+        for (int i = tid; i < kSlotRows * RP; i += kTileThreads)
+            if (i / RP < s.count && i % RP < P.r)
+                static_cast<typename MiddleOf<T>::type*>(P.u)[(int64_t)plan_perm(P)[s.start + i / RP] * P.u_row + i % RP] =
+                    MiddleOf<T>::pack((Acc)__longlong_as_double(0x7ff8000000000000ll));
+    };
+
     cudaGridDependencySynchronize();  // the parts of u are there
     int at = (int)(begin % per), slot = (int)(begin / per), stage = 0;
     uint32_t round = 0;
@@ -912,6 +920,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
             } else {  // a warp that has given up still meets the others, as often as in take_slot
                 named_barrier<kWorkBarrier, kTileThreads>();
                 named_barrier<kWorkBarrier, kTileThreads>();
+                if (P.u && at == 0) lose_middle(plan_busy(P)[slot]);
             }
             ok = ok && !ring.failed;  // else a warp's share of the middle is missing
         }
