@@ -661,6 +661,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     __shared__ int list[SlotFeed::kRing][kSlotRows];
     __shared__ AdapterSlot rec[SlotFeed::kRing];
     __shared__ ChunkRing<S> ring;
+    __shared__ int plain[kSlotRows];  // rows without an adapter, apart from the copying warps' lists
     const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, q = lane & 3;
     const int rows0 = (tid >> 5 & 3) * 16, half = tid >> 7;
     const int32_t* header = P.plan + plan_header_word(P.rows, P.adapters);
@@ -944,9 +945,9 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     for (int i = blockIdx.x; i < idle * kParts; i += gridDim.x) {
         const AdapterSlot s = last[-(i / kParts)];
         named_barrier<kWorkBarrier, kTileThreads>();
-        if (tid < s.count) list[0][tid] = plan_perm(P)[s.start + tid];
+        if (tid < s.count) plain[tid] = plan_perm(P)[s.start + tid];
         named_barrier<kWorkBarrier, kTileThreads>();
-        plain_rows<T>(P, list[0], s.count, s.cls != P.adapters, min(i % kParts * width, n), min((i % kParts + 1) * width, n));
+        plain_rows<T>(P, plain, s.count, s.cls != P.adapters, min(i % kParts * width, n), min((i % kParts + 1) * width, n));
     }
 }
 
