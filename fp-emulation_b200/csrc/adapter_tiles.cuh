@@ -324,14 +324,30 @@ template <int ID, int N>
 __device__ __forceinline__ void named_barrier() {
     asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
 }
+// Meets the N threads of barrier ID and says whether every one of them came with `yes`.
+template <int ID, int N>
+__device__ __forceinline__ bool agreed_barrier(bool yes) {
+    uint32_t all;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.and.pred q, %2, %3, p;\nselp.u32 %0, 1, 0, q;\n}"
+                 : "=r"(all) : "r"((uint32_t)yes), "n"(ID), "n"(N) : "memory");
+    return all != 0;
+}
 constexpr int kCopyBarrier = 1, kWorkBarrier = 2;
+
+// A warp's wait: it runs out for all lanes or for none (each has a clock of its own, and
+// what follows a wait takes the whole warp).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint64_t budget_ns) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, budget_ns));
+}
 
 // The ring of chunks: a buffer is full when TMA's bytes and every copying thread's
 // copies have arrived (and what they wrote themselves is visible), and free again
 // when each of the eight computing warps has left it.  So a warp runs ahead of
 // another by as many chunks as there are buffers, and loads, products and stores
 // overlap.  Waits are bounded (FPEMU_WAIT_BUDGET_MS): when one runs out, the error
-// is recorded and what could not be finished becomes NaN.
+// is recorded and what could not be finished becomes NaN.  A warp gives up as a whole;
+// the others find out at their own next wait, so until then it still meets them at
+// every barrier that they pass.
 template <int S>
 struct ChunkRing {
     uint64_t full[S], empty[S];
@@ -384,18 +400,19 @@ struct SlotFeed {
         next = load(first), after = load(first + 1);
         id = load_id(next);
     }
-    // All copying threads; returns the slot whose rows are now in list[(slot - 1) % kRing].
-    __device__ __forceinline__ AdapterSlot enter() {
+    // All copying threads; `now` becomes the slot whose rows are in list[(slot - 1) % kRing].  False,
+    // for both warps, if one of them comes without `ok`.
+    __device__ __forceinline__ bool enter(bool ok, AdapterSlot& now) {
         const int at = slot % kRing;
         list[at][t] = id;
         if (t == 0) rec[at] = next;
-        named_barrier<kCopyBarrier, kCopyThreads>();
-        const AdapterSlot now = next;
+        if (!agreed_barrier<kCopyBarrier, kCopyThreads>(ok)) return false;
+        now = next;
         next = after;
         id = load_id(next);
         ++slot;
         after = load(slot + 1);
-        return now;
+        return true;
     }
 };
 
@@ -430,17 +447,18 @@ __device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<T
     const int unit_rows = copy_unit<T>(rows, q.row_stride), unit_w = copy_unit2<T>(w, q.w_row, q.w_adapter);
     SlotFeed feed{list, rec, slots, perm, busy, t};
     if (chunks > 0) feed.begin(slot);
-    int stage = 0, cls = 0, first = 0, c = 0;
+    int stage = 0, cls = 0, first = 0, asked = 0;  // chunks whose copies this warp has asked for
     uint32_t round = 1;
-    bool box = false;
-    for (; c < chunks; ++c) {
-        if (blockIdx.x == 0 && c == q.stall) break;
-        if (c >= S && !mbar_wait(&ring.empty[stage], round, q.budget_ns)) {
+    bool box = false, ok = true;
+    for (int c = 0; c < chunks; ++c) {
+        if (ok && blockIdx.x == 0 && c == q.stall) ok = false;
+        if (ok && c >= S && !warp_wait(&ring.empty[stage], round, q.budget_ns)) {
             report_error(sink.dev, sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterEmpty, c);
-            break;
+            ok = false;
         }
         if (c == 0 || at == 0) {
-            const AdapterSlot s = feed.enter();
+            AdapterSlot s;
+            if (!feed.enter(ok, s)) break;
             const int* ids = list[(feed.slot - 1) % SlotFeed::kRing];
             cls = s.cls, first = ids[0];
             box = (q.tma & kTmaRows) && ids[s.count - 1] - first == s.count - 1;
@@ -448,7 +466,7 @@ __device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<T
             if (!tma_w) wt.aim(t, w + s.cls * q.w_adapter, q.w_row, (int64_t)at * KC);
         }
         uint8_t* st = smem + stage * Tile::kStage;
-        ring.copied_after(stage, t, (rows && box ? Tile::kStageX : 0) + (tma_w ? RP * 128 : 0), [&]() {
+        if (ok) ring.copied_after(stage, t, (rows && box ? Tile::kStageX : 0) + (tma_w ? RP * 128 : 0), [&]() {
             if (rows && !box) xt.fetch(t, st, q.length - at * KC, unit_rows);
             if (!tma_w) wt.fetch(t, st + Tile::kStageX, q.w_row, q.rank, q.length - at * KC, unit_w);
         }, [&]() {
@@ -463,14 +481,17 @@ __device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<T
                 else tma_box4(to + Tile::kStageX, q.w_map, &ring.full[stage], at * KC, 0, cls);
             }
         });
+        asked += ok;
         if (++at == per) at = 0;
         if (++stage == S) stage = 0, round ^= 1;
     }
     copy_commit();
     copy_wait<0>();
-    // Given up: what TMA has under way has to land before the block may end.
-    if (c < chunks)
-        for (int i = c < S ? 0 : c - S; i < c; ++i) mbar_wait(&ring.full[i % S], i / S & 1, q.budget_ns);
+    // Given up: what TMA has under way has to land before the block may end.  (A chunk that the other
+    // warp gave up never becomes full; its wait is the time that the copies have.)
+    if (asked < chunks)
+        for (int i = asked < S ? 0 : asked - S; i < asked; ++i)
+            if (!warp_wait(&ring.full[i % S], i / S & 1, q.budget_ns)) break;
 }
 
 // Block b of `blocks` takes chunks [total b / blocks, total (b + 1) / blocks).  A
@@ -632,7 +653,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     uint32_t round = 0;
     bool ok = true;
     for (int c = 0; c < chunks; ++c) {
-        if (ok && !mbar_wait(&ring.full[stage], round, P.budget_ns)) {
+        if (ok && !warp_wait(&ring.full[stage], round, P.budget_ns)) {
             report_error(P.sink.dev, P.sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterFull, c);
             ring.failed = 1;
             ok = false;
@@ -910,7 +931,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     int at = (int)(begin % per), slot = (int)(begin / per), stage = 0;
     uint32_t round = 0;
     for (int c = 0; c < chunks; ++c) {
-        if (ok && !mbar_wait(&ring.full[stage], round, P.budget_ns)) {
+        if (ok && !warp_wait(&ring.full[stage], round, P.budget_ns)) {
             report_error(P.sink.dev, P.sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterFull, c);
             ring.failed = 1;
             ok = false;
@@ -923,7 +944,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
                 named_barrier<kWorkBarrier, kTileThreads>();
                 if (P.u && at == 0) lose_middle(plan_busy(P)[slot]);
             }
-            ok = ok && !ring.failed;  // else a warp's share of the middle is missing
+            ok = __all_sync(0xffffffffu, ok && !ring.failed);  // else a warp's share of the middle is missing
         }
         if (!ok) {  // what is left becomes NaN
             const AdapterSlot s = plan_busy(P)[slot];

@@ -62,7 +62,7 @@ def _child(dtype, q):
         q.put(("error", traceback.format_exc()))
 
 
-@pytest.mark.parametrize("dtype", ["float64", "float32", "bfloat16"])
+@pytest.mark.parametrize("dtype", ["float64", "float32", "float16", "bfloat16"])
 def test_every_value_is_right_or_nan(dtype):
     import torch.multiprocessing as mp
 
