@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kFewThreads, FewTile<T, RP>::kBlocks) adapter_
     join_parts<RP * kGroupRows>(cluster, cr, cs, part, us, [](int e) { return e; }, [&](int e, Acc v) {
         const int j = e / kGroupRows, r = e % kGroupRows;
         v = j < P.r ? v * s : Acc(0);
-        if (P.u && j < P.r && r < count) static_cast<typename MiddleOf<T>::type*>(P.u)[(int64_t)list[r] * P.u_row + j] = MiddleOf<T>::pack(v);
+        if (P.u && j < P.r && r < count) static_cast<Acc*>(P.u)[(int64_t)list[r] * P.u_row + j] = v;
         return v;
     });
     cluster.sync();
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kFewThreads, FewTile<T, RP>::kBlocks) adapter_
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                split16<T>(at(2 * i) * down, at(2 * i + 1) * down, ua[t][2 * i], ua[t][2 * i + 1]);
+                split_half(at(2 * i) * down, at(2 * i + 1) * down, ua[t][2 * i], ua[t][2 * i + 1]);
         }
     }
     for (int first = n0 + warp * KS; first < n1; first += W * KS * UG) {

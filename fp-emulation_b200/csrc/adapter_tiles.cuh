@@ -130,22 +130,13 @@ __device__ __forceinline__ Tf32Pair tf32_split(float x) {
     return p;
 }
 
-// The same for two neighbouring values as pairs of 16-bit parts (16 bits of bfloat16, 22 of halves).
-template <typename T>
-__device__ __forceinline__ void split16(float x, float y, uint32_t& hi, uint32_t& lo) {
-    if constexpr (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(x, y);
-        const float2 f = __half22float2(h);
-        const __half2 l = __floats2half2_rn(fminf(x - f.x, 65504.f), fminf(y - f.y, 65504.f));
-        hi = *reinterpret_cast<const uint32_t*>(&h);
-        lo = *reinterpret_cast<const uint32_t*>(&l);
-    } else {  // cut, not rounded: a finite value stays finite
-        const uint32_t a = __float_as_uint(x) & 0xffff0000u, b = __float_as_uint(y) & 0xffff0000u;
-        const __nv_bfloat162 l = __floats2bfloat162_rn(fminf(x - __uint_as_float(a), 1e38f),
-                                                       fminf(y - __uint_as_float(b), 1e38f));
-        hi = (a >> 16) | b;
-        lo = *reinterpret_cast<const uint32_t*>(&l);
-    }
+// Two neighbouring floats as two halves each, 22 bits of them.
+__device__ __forceinline__ void split_half(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(fminf(x - f.x, 65504.f), fminf(y - f.y, 65504.f));
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
 // Two neighbouring floats as three bfloat16 parts each, largest first, which hold all of their 24
@@ -162,24 +153,6 @@ __device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&p)[3]) {
     auto pack = [](float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); };
     p[0] = pack(x, y), p[1] = pack(x1, y1), p[2] = pack(x2, y2);
 }
-
-// How u and v are kept for the gradients: as they are, or, for bfloat16 data, as
-// the two parts that the products use (high in the upper half of the word), which
-// saves every block of the gradient kernel the splitting.
-template <typename T>
-struct MiddleOf {
-    using type = typename AccOf<T>::type;
-    static __device__ __forceinline__ type pack(type v) { return v; }
-};
-template <>
-struct MiddleOf<__nv_bfloat16> {
-    using type = uint32_t;
-    static __device__ __forceinline__ uint32_t pack(float v) {
-        uint32_t hi, lo;
-        split16<__nv_bfloat16>(v, 0.f, hi, lo);
-        return hi << 16 | (lo & 0xffffu);
-    }
-};
 
 constexpr int kTileThreads = 256;      // eight warps that compute
 constexpr int kCopyThreads = 64;       // and two that copy
@@ -711,9 +684,10 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     // f64: the rank that step t of this thread stands for (any order will do; this one spreads the banks).
     auto rank_of = [&](int t) { return t / 4 * 16 + (q >> 1) * 8 + t % 4 * 2 + (q & 1); };
     Acc* us = reinterpret_cast<Acc*>(smem + S * Tile::kStage);
-    // The middle as this thread's part of the left operand: 16-bit data split in
-    // two and, for halves, scaled by a power of two per row; f32 and f64 plain.
-    uint32_t uh[E == 2 ? RP / 16 : 1][4], ul[E == 2 ? RP / 16 : 1][4];
+    // The middle as this thread's part of the left operand: halves in two parts,
+    // scaled by a power of two per row; bfloat16 in three; f32 and f64 plain.
+    constexpr bool kThird = std::is_same<T, __nv_bfloat16>::value;
+    uint32_t uh[E == 2 ? RP / 16 : 1][4], ul[E == 2 ? RP / 16 : 1][4], um[kThird ? RP / 16 : 1][4];
     Acc uf[E == 2 ? 1 : RP / (E == 4 ? 8 : 4)][E == 4 ? 4 : 2];
     float back[2];
     T* yp[2];
@@ -734,7 +708,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
             v = r < P.r ? v * s : Acc(0);  // past the rank, an infinite x met a zero: NaN
             us[row * Tile::kPitchU + r] = v;
             if (P.u && at == 0 && r < P.r && row < now.count)
-                static_cast<typename MiddleOf<T>::type*>(P.u)[(int64_t)rows[row] * P.u_row + r] = MiddleOf<T>::pack(v);
+                static_cast<Acc*>(P.u)[(int64_t)rows[row] * P.u_row + r] = v;
         }
         named_barrier<kWorkBarrier, kTileThreads>();
         const Acc* from = us + (rows0 + g) * Tile::kPitchU;
@@ -770,8 +744,15 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
 #pragma unroll
             for (int t = 0; t < RP / 16; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    split16<T>(v[t][2 * e] * down[e & 1], v[t][2 * e + 1] * down[e & 1], uh[t][e], ul[t][e]);
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (kThird) {
+                        uint32_t part[3];
+                        split_bf16(v[t][2 * e], v[t][2 * e + 1], part);
+                        uh[t][e] = part[0], um[t][e] = part[1], ul[t][e] = part[2];
+                    } else {
+                        split_half(v[t][2 * e] * down[e & 1], v[t][2 * e + 1] * down[e & 1], uh[t][e], ul[t][e]);
+                    }
+                }
         } else {
             constexpr int step = E == 4 ? 8 : 4;  // a0, a1 of rows g, g + 8; f32 two more, four columns on
 #pragma unroll
@@ -814,6 +795,9 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
                 }
 #pragma unroll
                 for (int p = 0; p < 4; ++p) mma16<T>(c[p], ul[t], b[p / 2][p % 2 * 2], b[p / 2][p % 2 * 2 + 1]);
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+                    if constexpr (kThird) mma16<T>(c[p], um[t], b[p / 2][p % 2 * 2], b[p / 2][p % 2 * 2 + 1]);
 #pragma unroll
                 for (int p = 0; p < 4; ++p) mma16<T>(c[p], uh[t], b[p / 2][p % 2 * 2], b[p / 2][p % 2 * 2 + 1]);
             }
@@ -923,8 +907,8 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     auto lose_middle = [&](const AdapterSlot& s) {
         for (int i = tid; i < kSlotRows * RP; i += kTileThreads)
             if (i / RP < s.count && i % RP < P.r)
-                static_cast<typename MiddleOf<T>::type*>(P.u)[(int64_t)plan_perm(P)[s.start + i / RP] * P.u_row + i % RP] =
-                    MiddleOf<T>::pack((Acc)__longlong_as_double(0x7ff8000000000000ll));
+                static_cast<Acc*>(P.u)[(int64_t)plan_perm(P)[s.start + i / RP] * P.u_row + i % RP] =
+                    (Acc)__longlong_as_double(0x7ff8000000000000ll);
     };
 
     cudaGridDependencySynchronize();  // the parts of u are there
@@ -1119,17 +1103,14 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
                     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            uint32_t hi[2], lo[2];
+                            uint32_t p0[3], p1[3];
+                            auto value = [&](int e, int i) { return __uint_as_float(h ? w[e][i].y : w[e][i].x); };
+                            split_bf16(value(0, 0), value(0, 1), p0);
+                            split_bf16(value(1, 0), value(1, 1), p1);
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const uint32_t a = h ? w[e][0].y : w[e][0].x, b = h ? w[e][1].y : w[e][1].x;
-                                hi[e] = __byte_perm(a, b, 0x7632), lo[e] = __byte_perm(a, b, 0x5410);
-                            }
+                            for (int i = 2; i >= 0; --i)
 #pragma unroll
-                            for (int m = 0; m < MT; ++m) {
-                                mma16<T>(sum[m][2 * t + h], a[m], lo[0], lo[1]);
-                                mma16<T>(sum[m][2 * t + h], a[m], hi[0], hi[1]);
-                            }
+                                for (int m = 0; m < MT; ++m) mma16<T>(sum[m][2 * t + h], a[m], p0[i], p1[i]);
                         }
                     } else {
                         // A half is a tf32 value as it is; the middle, whose range is a float's, is split in two.

@@ -13,7 +13,7 @@ import fp_emulation as fp
 
 pytestmark = pytest.mark.gpu
 
-FEW = [1, 9, 200]
+ROWS = [1, 9, 200, 257, 3000]
 
 
 def _cancelling(rows, p, k, m):
@@ -28,7 +28,7 @@ def _cancelling(rows, p, k, m):
 
 
 @pytest.mark.parametrize("p", [12, 16, 18, 20])
-@pytest.mark.parametrize("rows", FEW)
+@pytest.mark.parametrize("rows", ROWS)
 def test_bfloat16_middle_has_the_bits_of_a_float(rows, p):
     x, A, B, index = _cancelling(rows, p, 40, 24)
     y = fp.adapter_matmul(x, A, B, index)
@@ -36,7 +36,7 @@ def test_bfloat16_middle_has_the_bits_of_a_float(rows, p):
 
 
 @pytest.mark.parametrize("sign", [1, -1])
-@pytest.mark.parametrize("rows", FEW)
+@pytest.mark.parametrize("rows", ROWS)
 def test_infinite_bfloat16_row_keeps_its_sign(rows, sign):
     """Weights of 8: no part of the infinite u may overflow to the other sign."""
     x = torch.full((rows, 1), sign * float("inf"), dtype=torch.bfloat16, device="cuda")
@@ -44,3 +44,28 @@ def test_infinite_bfloat16_row_keeps_its_sign(rows, sign):
     B = torch.full((1, 20, 1), 8.0, dtype=torch.bfloat16, device="cuda")
     y = fp.adapter_matmul(x, A, B, torch.zeros(rows, dtype=torch.int32, device="cuda"))
     assert torch.equal(y, torch.full_like(y, sign * float("inf")))
+
+
+@pytest.mark.parametrize("p", [16, 20])
+@pytest.mark.parametrize("rows", [2, 64, 512, 2048])
+def test_bfloat16_gradients_have_the_bits_of_a_float(rows, p):
+    """Rows in pairs whose u, and whose v = B^T dy, are 1 + 2^-8 + 2^-p and -(1 + 2^-8); the
+    gradients' sums over a pair are 2^-p.  dx is the product of test_bfloat16_middle."""
+    power = torch.tensor([1.0, 2.0 ** -8, 2.0 ** -p], dtype=torch.bfloat16, device="cuda")
+    pair = torch.stack([power, torch.cat([-power[:2], power.new_zeros(1)])])
+    x = pair.repeat(rows // 2, 1)
+    dy = x.clone()
+    A = torch.ones(1, 1, 3, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    B = torch.ones(1, 3, 1, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    index = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    ones = torch.ones(rows, 1, dtype=torch.bfloat16, device="cuda")
+    want = rows // 2 * 2.0 ** -p
+    dB, = torch.autograd.grad(fp.adapter_matmul(x, A, B[:, :1], index), B, ones)
+    assert torch.equal(dB[:, :1], torch.full_like(dB[:, :1], want))
+    dA, = torch.autograd.grad(fp.adapter_matmul(ones, A[..., :1], B, index), A, dy)
+    assert torch.equal(dA[..., :1], torch.full_like(dA[..., :1], want))
+    A2 = torch.ones(1, 2, 1, dtype=torch.bfloat16, device="cuda")
+    B2 = torch.stack([torch.ones(3), torch.tensor([-1.0, -1.0, 0.0])], 1)[None].to(A2)
+    ones.requires_grad_(True)
+    dx, = torch.autograd.grad(fp.adapter_matmul(ones, A2, B2, index), ones, power.expand(rows, 3))
+    assert torch.equal(dx, torch.full_like(dx, 2.0 ** -p))
