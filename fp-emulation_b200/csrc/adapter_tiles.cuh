@@ -967,8 +967,9 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
 // forward pass's workspace.
 //
 // Bound by the bytes of x and dy on paper; measured, 16384 x 4096 bfloat16, rank 32,
-// four adapters: 96 us for the 268 MB of both, 2.8 TB/s, with the warps waiting for
-// their loads from shared memory and for one another in turn; a million rows, 32
+// four adapters: 126 us for the 268 MB of both, 2.1 TB/s, with the warps waiting for
+// their loads from shared memory and for one another in turn (with p in two parts, 16
+// bits of it, 96 us); a million rows, 32
 // columns to 32, rank 8, one adapter: 118 us for 192 MB.  The ring of the products, with two
 // copying warps, was no faster here and slower for rows in any order (3333 x 1024
 // bfloat16 rank 20: 35 us against 18), whose copies two warps cannot issue fast enough.
@@ -1011,7 +1012,13 @@ struct AdapterGradTile {
     static constexpr int kStages = 3;  // a fourth leaves room for fewer blocks: 3333 x 1023 -> 515 floats, 24 us for 20
     static constexpr int kPitchD = RP + 1;                    // the block's sums, after the rows
     static constexpr int kJoin = COLS * kPitchD * (int)sizeof(Acc);
-    static constexpr int kSmem = kStages * kStage > kJoin ? kStages * kStage : kJoin;
+    // bfloat16: p as three parts, split where it was copied to, a pair of rows to a word.  The first
+    // parts of rows 2 j and 2 j + 1 take row 2 j's place, the second ones row 2 j + 1's; the third
+    // ones have a place of their own, for two chunks.
+    static constexpr bool kPairs = std::is_same<T, __nv_bfloat16>::value;
+    static constexpr int kPitchL = (RP + 8) * 4, kThird = kPairs ? KT / 2 * kPitchL : 0;
+    static constexpr int kRing = kStages * kStage + 2 * kThird;
+    static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
     static constexpr int kFlush = E == 2 ? 8 : 1;             // chunks that the tensor cores sum by themselves
 };
 
@@ -1041,7 +1048,10 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
     // A thread's copies of a chunk: 16 bytes of QI rows of q, 16 of PI rows of p, each at one place along
     // the row.  Every warp reads the chunk's row ids, one chunk ahead of the copies that need them.
     constexpr int QU = COLS / V, QI = KT * QU / kGradThreads, QS = kGradThreads / QU;
-    constexpr int PV = 16 / (int)sizeof(Acc), PU = RP / PV, PI = KT * PU / kGradThreads, PS = kGradThreads / PU;
+    constexpr int PV = 16 / (int)sizeof(Acc), PU = RP / PV, PS = kGradThreads / PU;
+    constexpr int PI = KT * PU <= kGradThreads && Tile::kPairs ? 2 : KT * PU / kGradThreads;
+    // The row of p of a thread's copy i; in pairs, of the first half of the threads alone for the smallest rank.
+    auto p_row_of = [&](int i) { return Tile::kPairs ? tid / PU * 2 + i % 2 + i / 2 * 2 * PS : tid / PU + i * PS; };
     const int64_t col = c0 + tid % QU * V, cols_left = side.cols - col;
     const int q_avail = cols_left < 0 ? 0 : cols_left > V ? V : (int)cols_left;
     const int p_bytes = tid % PU * PV < P.p_row ? 16 : 0;  // p_row is a multiple of PV
@@ -1061,9 +1071,35 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
         }
 #pragma unroll
         for (int i = 0; i < PI; ++i) {
-            const int r = __shfl_sync(0xffffffffu, id, tid / PU + i * PS);
-            copy16(shared_address(st + KT * Tile::kPitchQ + (tid / PU + i * PS) * Tile::kPitchP + tid % PU * 16),
-                   pc + (int64_t)r * P.p_row, r < 0 ? 0 : p_bytes);
+            const int row = p_row_of(i), r = __shfl_sync(0xffffffffu, id, row & 31);
+            if (row < KT)
+                copy16(shared_address(st + KT * Tile::kPitchQ + row * Tile::kPitchP + tid % PU * 16),
+                       pc + (int64_t)r * P.p_row, r < 0 ? 0 : p_bytes);
+        }
+    };
+    // A chunk's p in parts: each thread what it copied itself, before the others look at it.  (Every
+    // warp splitting the operands that it loads: 147 us in the training case above for 126.)
+    auto split = [&](int c) {
+        if constexpr (Tile::kPairs) {
+            uint8_t* pt = smem + c % S * Tile::kStage + KT * Tile::kPitchQ + tid % PU * 16;
+            uint8_t* third = smem + S * Tile::kStage + (c & 1) * Tile::kThird + tid % PU * 16;
+#pragma unroll
+            for (int i = 0; i < PI; i += 2) {
+                const int row = p_row_of(i);
+                if (row >= KT) break;
+                float a[4], b[4];
+                uint32_t part[4][3];
+                *reinterpret_cast<float4*>(a) = *reinterpret_cast<const float4*>(pt + row * Tile::kPitchP);
+                *reinterpret_cast<float4*>(b) = *reinterpret_cast<const float4*>(pt + (row + 1) * Tile::kPitchP);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) split_bf16(a[e], b[e], part[e]);
+                auto store = [&](uint8_t* to, int k) {
+                    *reinterpret_cast<uint4*>(to) = make_uint4(part[0][k], part[1][k], part[2][k], part[3][k]);
+                };
+                store(pt + row * Tile::kPitchP, 0);
+                store(pt + (row + 1) * Tile::kPitchP, 1);
+                store(third + row / 2 * Tile::kPitchL, 2);
+            }
         }
     };
 
@@ -1078,8 +1114,9 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
                     for (int e = 0; e < 4; ++e) acc[m][t][e] += sum[m][t][e], sum[m][t][e] = 0;
         }
     };
-    auto compute = [&](const uint8_t* st) {
-        const uint8_t* pt = st + KT * Tile::kPitchQ;
+    auto compute = [&](int chunk) {
+        const uint8_t *st = smem + chunk % S * Tile::kStage, *pt = st + KT * Tile::kPitchQ;
+        const uint8_t* third = smem + S * Tile::kStage + (chunk & 1) * Tile::kThird;
         auto p_at = [&](int row, int j) {
             return *reinterpret_cast<const Acc*>(pt + row * Tile::kPitchP + j * (int)sizeof(Acc));
         };
@@ -1095,24 +1132,28 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
                 // tile t, so that one 8-byte load serves both.
 #pragma unroll
                 for (int t = 0; t < RP / 16; ++t) {
-                    uint2 w[2][2];  // rows 2 q, 2 q + 1, then 8 on; .x for tile 2 t, .y for 2 t + 1
+                    if constexpr (Tile::kPairs) {
+                        uint2 w[3][2];  // part; rows 2 q and 2 q + 1, then 8 on; .x for tile 2 t, .y for 2 t + 1
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        w[e >> 1][e & 1] = *reinterpret_cast<const uint2*>(
-                            pt + (ks * 16 + 2 * q + (e >> 1) * 8 + (e & 1)) * Tile::kPitchP + (t * 16 + 2 * g) * 4);
-                    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            uint32_t p0[3], p1[3];
-                            auto value = [&](int e, int i) { return __uint_as_float(h ? w[e][i].y : w[e][i].x); };
-                            split_bf16(value(0, 0), value(0, 1), p0);
-                            split_bf16(value(1, 0), value(1, 1), p1);
-#pragma unroll
-                            for (int i = 2; i >= 0; --i)
-#pragma unroll
-                                for (int m = 0; m < MT; ++m) mma16<T>(sum[m][2 * t + h], a[m], p0[i], p1[i]);
+                        for (int i = 0; i < 2; ++i) {
+                            const int pair = ks * 8 + i * 4 + q, at = (t * 16 + 2 * g) * 4;
+                            w[0][i] = *reinterpret_cast<const uint2*>(pt + 2 * pair * Tile::kPitchP + at);
+                            w[1][i] = *reinterpret_cast<const uint2*>(pt + (2 * pair + 1) * Tile::kPitchP + at);
+                            w[2][i] = *reinterpret_cast<const uint2*>(third + pair * Tile::kPitchL + at);
                         }
+#pragma unroll
+                        for (int i = 2; i >= 0; --i)
+#pragma unroll
+                            for (int m = 0; m < MT; ++m) {
+                                mma16<T>(sum[m][2 * t], a[m], w[i][0].x, w[i][1].x);
+                                mma16<T>(sum[m][2 * t + 1], a[m], w[i][0].y, w[i][1].y);
+                            }
                     } else {
+                        uint2 w[2][2];  // rows 2 q, 2 q + 1, then 8 on; .x for tile 2 t, .y for 2 t + 1
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e >> 1][e & 1] = *reinterpret_cast<const uint2*>(
+                                pt + (ks * 16 + 2 * q + (e >> 1) * 8 + (e & 1)) * Tile::kPitchP + (t * 16 + 2 * g) * 4);
                         // A half is a tf32 value as it is; the middle, whose range is a float's, is split in two.
                         // The order of rows within the sum is free: rows 2q and 2q + 1 stand where the
                         // instruction has q and q + 4.
@@ -1176,13 +1217,14 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
     }
     for (int c = 0; c < chunks; ++c) {
         copy_wait<S - 2>();
+        split(c);
         __syncthreads();
         if (c + S - 1 < chunks) {
             fetch(c + S - 1);
             ids(c + S);
         }
         copy_commit();
-        compute(smem + c % S * Tile::kStage);
+        compute(c);
         if (c % Tile::kFlush == Tile::kFlush - 1) flush();
     }
     flush();
