@@ -343,6 +343,15 @@ int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t 
     });
 }
 
+int fpemu_capture_id(void* stream, uint64_t* id) {
+    if (id == nullptr) return fail(FPEMU_ERR_INVALID, "capture_id: id is null");
+    cudaStreamCaptureStatus status;
+    unsigned long long number = 0;
+    FPEMU_CUDA(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &number));
+    *id = status == cudaStreamCaptureStatusNone ? 0 : number;
+    return FPEMU_OK;
+}
+
 int fpemu_adapter_backward(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters,
                            const void* x, int64_t x_row, const void* A, int64_t A_adapter, int64_t A_row,
                            const void* B, int64_t B_adapter, int64_t B_row, const void* dy, int64_t dy_row,

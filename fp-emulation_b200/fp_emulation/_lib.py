@@ -63,6 +63,7 @@ SIGNATURES = {
     "fpemu_adapter_matmul": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
                                     _vp, _i64, _vp, _i64, _vp, _dp, _vp, _int, _vp, _vp, _vp, _sz, _vp]),
     "fpemu_adapter_workspace_size": (_sz, [_int, _i64, _i64, _i64]),
+    "fpemu_capture_id": (_int, [_vp, _vp]),
     "fpemu_adapter_backward": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
                                       _vp, _i64, _vp, _dp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "fpemu_clip_workspace_size": (_sz, [_i64]),

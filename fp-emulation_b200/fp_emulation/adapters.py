@@ -14,7 +14,10 @@ counterpart in the reference.
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import math
+import threading
+import weakref
 
 import torch
 from torch import nn
@@ -24,6 +27,14 @@ from fp_emulation.ozaki import _after_call, _dtype_bits, _on, _raw_stream, _requ
 
 _DTYPE_CODE = {torch.float64: _lib.FPEMU_DT_F64, torch.float32: _lib.FPEMU_DT_F32,
                torch.float16: _lib.FPEMU_DT_F16, torch.bfloat16: _lib.FPEMU_DT_BF16}
+
+
+def _capture_id(device_index):
+    """The graph capture that the current stream of a device belongs to, or 0."""
+    number = ctypes.c_uint64(0)
+    with _on(device_index):
+        _lib.check(_lib.load().fpemu_capture_id(_raw_stream(device_index), ctypes.byref(number)), "capture")
+    return number.value
 
 
 class PreparedRows:
@@ -50,6 +61,12 @@ class PreparedRows:
                                         self.plan.data_ptr(), self.plan.numel() * 4, _stream(dev))
         _lib.check(st, "prepare_rows")
         _after_call("prepare_rows", dev)
+        self.capture = _capture_id(dev.index)
+
+    def check_capture(self):
+        """A plan made in a capture is memory that nothing has written before the graph's first replay."""
+        if self.capture and self.capture != _capture_id(self.index.get_device()):
+            raise RuntimeError("rows prepared in the capture of a CUDA graph serve that capture alone")
 
 
 def prepare_rows(index, adapters, shape=None):
@@ -59,9 +76,10 @@ def prepare_rows(index, adapters, shape=None):
     layers' inputs where it has fewer dimensions (one id for each request of a
     [requests, length, features] batch).  Later changes of ``index`` do not
     change the result.  On another stream than the one it was made on, wait for that
-    one first, and keep the result until its uses have finished.  An id that is no
-    adapter makes its rows NaN and raises ``FpemuError`` in the first call that ends
-    after the kernel has seen it."""
+    one first, and keep the result until its uses have finished.  Made while a CUDA
+    graph is captured, it serves that capture alone.  An id that is no adapter makes its
+    rows NaN and raises ``FpemuError`` in the first call that ends after the kernel has
+    seen it."""
     return PreparedRows(index, adapters, shape)
 
 
@@ -140,6 +158,8 @@ class _AdapterMatmul(torch.autograd.Function):
     def _backward(ctx, dy):
         x, A, B, u = ctx.saved_tensors
         scale = ctx.scale
+        if ctx.rows.capture:
+            ctx.rows.check_capture()
         need_x, need_A, need_B, need_base = ctx.needs_input_grad[:4]
         dev = x.device
         d = dev.index
@@ -256,6 +276,8 @@ def adapter_matmul(x, A, B, rows, base=None, scale=1.0, out=None):
             raise RuntimeError(f"adapter_matmul: {index.shape[0]} prepared rows for {count} rows of x")
         if index.get_device() != d:
             raise RuntimeError(f"operands on different devices: {x.device} and {index.device}")
+        if rows.capture:
+            rows.check_capture()
     elif isinstance(rows, torch.Tensor):
         if rows.dtype not in (torch.int32, torch.int64):
             raise TypeError("adapter ids are an int32 or int64 tensor")
@@ -319,19 +341,45 @@ class Adapters(nn.Module):
         return adapter_matmul(x, self.A, self.B, rows, base=base, scale=self.scale, out=out)
 
 
+_captured_ids = weakref.WeakKeyDictionary()  # model -> the ids that graphs captured in its blocks read
+
+
 class _ActiveRows:
     """The ids of the batch inside a ``use_adapters`` block; grouped once for each
-    leading shape that the layers meet."""
+    leading shape that the layers meet on a stream.  Streams are not ordered among
+    each other, and what a capture makes is there after a replay alone: each stream,
+    and each capture, has plans of its own."""
 
-    def __init__(self, index):
-        self.index = index
+    def __init__(self, index, model):
+        self.index = index.clone()
         self.prepared = {}
+        self.lock = threading.Lock()
+        self.kept = _captured_ids.setdefault(model, [])
+        d = index.get_device()
+        if d >= 0:  # else the first layer refuses it
+            self.stream, self.capture = _raw_stream(d), _capture_id(d)
+            self.copied = torch.cuda.Event()
+            self.copied.record(torch.cuda.current_stream(d))
 
     def prepare(self, lead, adapters):
-        key = (tuple(lead), adapters)
-        if key not in self.prepared:
-            self.prepared[key] = PreparedRows(self.index, adapters, lead)
-        return self.prepared[key]
+        d = self.index.get_device()
+        if d < 0:
+            return PreparedRows(self.index, adapters, lead)
+        stream, capture = _raw_stream(d), _capture_id(d)
+        if self.capture and capture != self.capture:
+            raise RuntimeError("a use_adapters block that began in the capture of a CUDA graph serves that capture alone")
+        key = (tuple(lead), adapters, stream, capture)
+        with self.lock:
+            if key not in self.prepared:
+                if stream != self.stream:
+                    current = torch.cuda.current_stream(d)
+                    if capture == self.capture:  # a capture cannot wait for what was issued before it
+                        current.wait_event(self.copied)
+                    self.index.record_stream(current)
+                if capture != self.capture:  # the graph copies the ids at every replay, after the block too
+                    self.kept.append(self.index)
+                self.prepared[key] = PreparedRows(self.index, adapters, lead)
+            return self.prepared[key]
 
 
 @contextlib.contextmanager
@@ -340,9 +388,10 @@ def use_adapters(model, index):
     apply row t's adapter ``index[t]`` (-1: none).  ``index`` has the leading shape
     of the layers' inputs, or the first dimensions of it, and is copied as the block
     begins: later changes of it take no effect (a CUDA graph that is to follow them
-    captures the whole block).  The block holds for the model, in every thread; a
-    backward pass that computes the layers again (activation checkpointing) has to
-    run inside it."""
+    captures the whole block; one captured inside keeps the block's ids).  The block
+    holds for the model, in every thread and on every stream, but one that begins in a
+    capture serves that capture alone.  A backward pass that computes the layers again
+    (activation checkpointing) has to run inside it."""
     from fp_emulation.nn import Linear
 
     if not isinstance(index, torch.Tensor) or index.dtype not in (torch.int32, torch.int64):
@@ -352,7 +401,7 @@ def use_adapters(model, index):
     if not layers:
         raise RuntimeError("use_adapters: the model has no Linear with adapters (add_adapters)")
     before = [m.active_rows for m in layers]
-    active = _ActiveRows(index.clone())
+    active = _ActiveRows(index, model)
     for m in layers:
         m.active_rows = active
     try:

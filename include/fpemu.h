@@ -237,6 +237,11 @@ int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t 
                          void *stream);
 size_t fpemu_adapter_workspace_size(int dtype, int64_t rows, int64_t rank, int64_t adapters);
 
+/* Which graph capture `stream` belongs to (each has its own number), or 0.  What a call
+ * makes in a capture is there after a replay alone, so a plan that is kept for later calls
+ * belongs to the capture that it was made in. */
+int fpemu_capture_id(void *stream, uint64_t *id);
+
 /* The gradients of that product for dy (rows x n): dx (packed, rows x k), and
  * dA[i] = sum_t v[t]^T x[t], dB[i] = sum_t dy[t]^T u[t] over the rows t of adapter i
  * (packed, [adapters][rank][k] and [adapters][n][rank], zero for an adapter without
