@@ -421,7 +421,7 @@ __device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<T
     SlotFeed feed{list, rec, slots, perm, busy, t};
     if (chunks > 0) feed.begin(slot);
     int stage = 0, cls = 0, first = 0, asked = 0;  // chunks whose copies this warp has asked for
-    uint32_t round = 1;
+    uint32_t round = 1, by_threads = 0;  // a bit for each buffer whose rows the threads copied last
     bool box = false, ok = true;
     for (int c = 0; c < chunks; ++c) {
         if (ok && blockIdx.x == 0 && c == q.stall) ok = false;
@@ -444,6 +444,8 @@ __device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<T
             if (!tma_w) wt.fetch(t, st + Tile::kStageX, q.w_row, q.rank, q.length - at * KC, unit_w);
         }, [&]() {
             const uint32_t to = shared_address(st);
+            // The threads' copies were ordinary writes; TMA's to the same place come after them.
+            if (box && (by_threads >> stage & 1)) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             if (rows && box) tma_box2(to, q.row_map, &ring.full[stage], at * KC, first);
             if (tma_w) {
                 if (LONG)
@@ -455,6 +457,7 @@ __device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<T
             }
         });
         asked += ok;
+        by_threads = box ? by_threads & ~(1u << stage) : by_threads | 1u << stage;
         if (++at == per) at = 0;
         if (++stage == S) stage = 0, round ^= 1;
     }

@@ -69,3 +69,26 @@ def test_one_slot_does_not_reach_the_next(dtype, r):
                 assert torch.equal(fp.adapter_matmul(x, A, B, plan, base=base, scale=scale), first[0])
         for _ in range(5):
             assert all(torch.equal(a, b) for a, b in zip(step(), first))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_rows_in_runs_beside_rows_in_any_order(dtype):
+    """Slots whose rows follow one another (copied in one box) and slots whose rows do not (copied
+    one by one) share the buffers in turn; x and base of odd strides, never copied in boxes, give
+    the same bits."""
+    n, rows, k, m, r = 60, 9000, 256, 320, 16
+    x, A, B, base, dy, scale, _ = _data(rows, n, k, m, r, dtype)
+    index = torch.arange(rows, device="cuda") * n // rows
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    loose = torch.nonzero(index % 2).flatten()  # every other adapter's rows change places among themselves
+    index[loose] = index[loose[torch.randperm(len(loose), generator=gen, device="cuda")]]
+
+    def odd(t):
+        view = torch.zeros((rows, t.shape[1] + 1), dtype=dtype, device="cuda")[:, :t.shape[1]]
+        view.copy_(t)
+        return view
+
+    plan = fp.prepare_rows(index, n)
+    want = fp.adapter_matmul(odd(x), A, B, plan, base=odd(base), scale=scale)
+    for _ in range(20):
+        assert torch.equal(fp.adapter_matmul(x, A, B, plan, base=base, scale=scale), want)
