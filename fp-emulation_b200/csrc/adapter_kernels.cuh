@@ -176,6 +176,7 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const void* index, i
         const int64_t left = total - first;
         slots[s] = AdapterSlot{cls, (int)(start + first), (int)(left < 0 ? 0 : left < kSlotRows ? left : kSlotRows), 0};
     }
+    __syncthreads();  // perm is written: the first bad row may be another warp's
     if (threadIdx.x == 0) {
         plan[cls] = start;
         if (cls == adapters + 1) {
