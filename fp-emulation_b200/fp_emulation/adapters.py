@@ -141,8 +141,9 @@ class _AdapterMatmul(torch.autograd.Function):
         u = torch.empty((x.shape[0], (A.shape[1] + 3) // 4 * 4),
                         dtype=torch.float64 if x.dtype == torch.float64 else torch.float32, device=x.device)
         _launch(x, A, B, base, y, scale, rows, rows.index, u)
-        ctx.save_for_backward(x, A, B, u)
-        ctx.rows, ctx.scale = rows, scale
+        # A tensor of scales is guarded like the others: u holds the values of now.
+        ctx.save_for_backward(x, A, B, u, scale if isinstance(scale, torch.Tensor) else None)
+        ctx.rows, ctx.scale = rows, scale if scale.__class__ is float else None
         return y
 
     @staticmethod
@@ -156,8 +157,9 @@ class _AdapterMatmul(torch.autograd.Function):
 
     @staticmethod
     def _backward(ctx, dy):
-        x, A, B, u = ctx.saved_tensors
-        scale = ctx.scale
+        x, A, B, u, scale = ctx.saved_tensors
+        if scale is None:
+            scale = ctx.scale
         if ctx.rows.capture:
             ctx.rows.check_capture()
         need_x, need_A, need_B, need_base = ctx.needs_input_grad[:4]
@@ -227,7 +229,8 @@ def adapter_matmul(x, A, B, rows, base=None, scale=1.0, out=None):
     the batch, or an int32/int64 tensor of ids whose shape is x's leading shape or
     the first dimensions of it (-1: no adapter; such a row returns ``base``).
     base: broadcastable to [..., n], or None for zero.  scale: one number, or a
-    tensor with one value for each adapter (no gradient).  out: where to write the
+    tensor with one value for each adapter (no gradient; like the other operands it
+    must not change in place before the backward pass).  out: where to write the
     result when autograd does not record; it may be ``base`` itself.
 
     Sums are held in float64 for float64 and in float32 otherwise, and the result

@@ -26,3 +26,17 @@ def test_the_error_names_the_first_bad_row(rows, monkeypatch):
             torch.cuda.synchronize()
             code, where, _, detail = _lib.device_error(clear=True)
             assert (code, where, detail) == (_lib.FPEMU_ERR_INVALID, _lib.WHERE_ADAPTER_INDEX, bad)
+
+
+@pytest.mark.parametrize("rows", [20, 400])
+def test_scales_changed_before_the_backward_pass(rows):
+    x, A, B, base, dy, scale, index = _data(rows, 3, 16, 24, 4, torch.float64)
+    x.requires_grad_(True)
+    y = fp.adapter_matmul(x, A, B, index, base=base, scale=scale)
+    want, = torch.autograd.grad(y, x, dy, retain_graph=True)
+    scale.mul_(2)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y, x, dy)
+    scale.mul_(0.5)
+    again, = torch.autograd.grad(fp.adapter_matmul(x, A, B, index, base=base, scale=scale), x, dy)
+    assert torch.equal(again, want)
