@@ -21,6 +21,7 @@ import weakref
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from fp_emulation import _lib
 from fp_emulation.ozaki import _after_call, _dtype_bits, _on, _raw_stream, _require_cuda, _stream
@@ -89,6 +90,14 @@ def _spread_index(index, shape):
     if index.dim() > len(shape) or index.shape != shape[:index.dim()]:
         raise RuntimeError(f"adapter ids of shape {tuple(index.shape)} do not match rows of shape {tuple(shape)}")
     return index.reshape(index.shape + (1,) * (len(shape) - index.dim())).expand(shape)
+
+
+def _no_tangents(what, *tensors):
+    """Refuses forward-mode differentiation, which the kernels would drop in silence."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 def _last_contiguous(t):
@@ -234,10 +243,11 @@ def adapter_matmul(x, A, B, rows, base=None, scale=1.0, out=None):
     result when autograd does not record; it may be ``base`` itself.
 
     Sums are held in float64 for float64 and in float32 otherwise, and the result
-    is rounded once.  x, A, B and base have gradients (once; not twice
-    differentiable); repeated calls give the same bits."""
+    is rounded once.  x, A, B and base have gradients (once; not twice differentiable,
+    and not in forward mode); repeated calls give the same bits."""
     dtype = x.dtype
     _dtype_bits(dtype)
+    _no_tangents("adapter_matmul", x, A, B, base, scale)
     d = x.get_device()
     if d < 0 or A.get_device() != d or B.get_device() != d or (base is not None and base.get_device() != d) \
             or d not in _lib._watched:

@@ -15,7 +15,7 @@ from array import array
 import torch
 
 from fp_emulation import _lib
-from fp_emulation.adapters import _DTYPE_CODE
+from fp_emulation.adapters import _DTYPE_CODE, _no_tangents
 from fp_emulation.ozaki import _after_call, _dtype_bits, _on, _raw_stream, _require_cuda
 
 _NORMS = {1.0: 1, 2.0: 2, math.inf: 0}
@@ -45,6 +45,7 @@ _layout, _dtype, _grad = map(operator.attrgetter, ("layout", "dtype", "grad"))
 
 def _check_list(tensors, what):
     """The tensors' dtype codes; refuses what the kernels do not take."""
+    _no_tangents(what, *tensors)
     try:
         devices = set(map(torch.Tensor.get_device, tensors))
         codes = list(map(_DTYPE_CODE.__getitem__, map(_dtype, tensors)))
@@ -104,7 +105,7 @@ def grad_norm(tensors, norm_type=2.0):
     """The norm (1, 2 or inf) over every element of every tensor, as a 0-d tensor
     on their device: float64 if one of them is float64, else float32.  Sums are
     held in float64, and squares neither overflow nor vanish before the norm does.
-    No tensors: 0 on the CPU."""
+    The result has no gradient.  No tensors: 0 on the CPU."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     code = _norm_code(norm_type)
     if not tensors:
@@ -117,7 +118,8 @@ def grad_norm(tensors, norm_type=2.0):
 def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     """``(clipped, norm)``: new tensors, the gradients times
     ``min(1, max_norm / (norm + 1e-6))``, and their global norm before.  The
-    gradients stay as they are (those of ``torch.autograd.grad``, say).  out: tensors
+    gradients stay as they are (those of ``torch.autograd.grad``, say); the results have
+    none of their own.  out: tensors
     to write to, of the gradients' shapes and dtypes; none may overlap another
     tensor, but each may be its own gradient."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)

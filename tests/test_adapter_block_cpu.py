@@ -128,3 +128,14 @@ def test_threads_on_one_stream_share_one_plan(monkeypatch):
     for t in threads:
         t.join()
     assert len(gpu.made) == 1 and all(g is got[0] for g in got)
+
+
+def test_forward_mode_tangents_are_seen():
+    import torch.autograd.forward_ad as fwd
+
+    t = torch.ones(3)
+    adapters._no_tangents("call", t, None, 2.0)
+    with fwd.dual_level():
+        adapters._no_tangents("call", t, None, 2.0)
+        with pytest.raises(RuntimeError, match="call has no forward-mode"):
+            adapters._no_tangents("call", t, fwd.make_dual(t, t))

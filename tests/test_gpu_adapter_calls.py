@@ -40,3 +40,23 @@ def test_scales_changed_before_the_backward_pass(rows):
     scale.mul_(0.5)
     again, = torch.autograd.grad(fp.adapter_matmul(x, A, B, index, base=base, scale=scale), x, dy)
     assert torch.equal(again, want)
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+
+    x, A, B, base, dy, scale, index = _data(20, 3, 16, 24, 4, torch.float64)
+    with fwd.dual_level():
+        operands = [x, A, B, base, scale]
+        for i, t in enumerate(operands):
+            dual = operands[:i] + [fwd.make_dual(t, torch.ones_like(t))] + operands[i + 1:]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                fp.adapter_matmul(*dual[:3], index, base=dual[3], scale=dual[4])
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            fp.grad_norm([x, fwd.make_dual(dy, torch.ones_like(dy))])
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            fp.clip_grads([fwd.make_dual(dy, torch.ones_like(dy))], 1.0)
+        plain = fp.adapter_matmul(x, A, B, index, base=base, scale=scale)
+    assert torch.equal(plain, fp.adapter_matmul(x, A, B, index, base=base, scale=scale))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: fp.adapter_matmul(t, A, B, index), (x,), (x,))
