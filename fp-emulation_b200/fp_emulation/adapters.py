@@ -235,8 +235,9 @@ def adapter_matmul(x, A, B, rows, base=None, scale=1.0, out=None):
 
     x: [..., k]; A: [adapters, rank, k]; B: [adapters, n, rank], all of one float
     dtype (float64, float32, float16, bfloat16).  rows: ``prepare_rows(...)`` of
-    the batch, or an int32/int64 tensor of ids whose shape is x's leading shape or
-    the first dimensions of it (-1: no adapter; such a row returns ``base``).
+    the batch (of x's leading shape, unless one of the two is flat), or an int32/int64
+    tensor of ids whose shape is x's leading shape or the first dimensions of it (-1: no
+    adapter; such a row returns ``base``).
     base: broadcastable to [..., n], or None for zero.  scale: one number, or a
     tensor with one value for each adapter (no gradient; like the other operands it
     must not change in place before the backward pass).  out: where to write the
@@ -287,6 +288,8 @@ def adapter_matmul(x, A, B, rows, base=None, scale=1.0, out=None):
         index = rows.index
         if index.shape[0] != count:
             raise RuntimeError(f"adapter_matmul: {index.shape[0]} prepared rows for {count} rows of x")
+        if rows.shape != lead and len(rows.shape) > 1 and not flat:
+            raise RuntimeError(f"adapter_matmul: rows prepared for {tuple(rows.shape)}, x has rows of {tuple(lead)}")
         if index.get_device() != d:
             raise RuntimeError(f"operands on different devices: {x.device} and {index.device}")
         if rows.capture:

@@ -60,3 +60,16 @@ def test_forward_mode_is_refused():
     assert torch.equal(plain, fp.adapter_matmul(x, A, B, index, base=base, scale=scale))
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda t: fp.adapter_matmul(t, A, B, index), (x,), (x,))
+
+
+def test_prepared_rows_of_another_shape():
+    x, A, B, base, _, scale, index = _data(12, 3, 16, 24, 4, torch.float64)
+    want = fp.adapter_matmul(x, A, B, index)
+    square = fp.prepare_rows(index.view(4, 3), 3)
+    with pytest.raises(RuntimeError, match="prepared for"):
+        fp.adapter_matmul(x.view(3, 4, 16), A, B, square)
+    with pytest.raises(RuntimeError, match="prepared for"):
+        fp.adapter_matmul(x.view(3, 4, 16), A, B, fp.prepare_rows(index[:4], 3, (4, 3)))
+    assert torch.equal(fp.adapter_matmul(x.view(4, 3, 16), A, B, square).view(12, 24), want)
+    assert torch.equal(fp.adapter_matmul(x, A, B, square), want)  # rows in their order
+    assert torch.equal(fp.adapter_matmul(x.view(2, 6, 16), A, B, fp.prepare_rows(index, 3)).view(12, 24), want)
