@@ -159,9 +159,9 @@ class _AdapterMatmul(torch.autograd.Function):
     def backward(ctx, dy):
         if torch.is_grad_enabled():  # create_graph: the gradients below are computed outside autograd
             with torch.no_grad():
-                grads = _AdapterMatmul._backward(ctx, dy)
-            return tuple(g if g is None else torch._C._functions.DelayedError(
-                "adapter_matmul is differentiable once, not twice", 1)(g.requires_grad_(True)) for g in grads)
+                *grads, dbase, _, _ = _AdapterMatmul._backward(ctx, dy)
+            error = torch._C._functions.DelayedError("adapter_matmul is differentiable once, not twice", 1)
+            return *(g if g is None else error(g.requires_grad_(True)) for g in grads), dbase, None, None
         return _AdapterMatmul._backward(ctx, dy)
 
     @staticmethod

@@ -73,3 +73,19 @@ def test_prepared_rows_of_another_shape():
     assert torch.equal(fp.adapter_matmul(x.view(4, 3, 16), A, B, square).view(12, 24), want)
     assert torch.equal(fp.adapter_matmul(x, A, B, square), want)  # rows in their order
     assert torch.equal(fp.adapter_matmul(x.view(2, 6, 16), A, B, fp.prepare_rows(index, 3)).view(12, 24), want)
+
+
+def test_the_callers_gradient_stays_as_it_was():
+    """create_graph: base's gradient is dy itself, which is not the operator's to change."""
+    x, A, B, base, dy, scale, index = _data(12, 3, 16, 24, 4, torch.float64)
+    for t in (x, A, B, base):
+        t.requires_grad_(True)
+    y = fp.adapter_matmul(x, A, B, index, base=base, scale=scale)
+    dx, dbase = torch.autograd.grad(y, (x, base), dy, create_graph=True)
+    assert not dy.requires_grad and torch.equal(dbase, dy)
+    with pytest.raises(RuntimeError, match="once"):
+        dx.sum().backward()
+    weight = torch.ones_like(dy).requires_grad_(True)
+    y = fp.adapter_matmul(x, A, B, index, base=base, scale=scale)
+    dbase, = torch.autograd.grad((y * weight).sum(), base, create_graph=True)
+    assert torch.equal(torch.autograd.grad(dbase.sum(), weight)[0], torch.ones_like(dy))  # linear in dy
