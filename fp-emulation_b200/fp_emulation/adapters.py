@@ -211,7 +211,7 @@ def _span(t):
 def _check_out(out, shape, x, base, others):
     if out.shape != shape or out.dtype != x.dtype or out.device != x.device:
         raise RuntimeError(f"out must be a {x.dtype} tensor of shape {tuple(shape)} on {x.device}")
-    o2 = out.view(-1, shape[-1]) if out.numel() else out.reshape(-1, shape[-1])
+    o2 = out.view(-1, shape[-1]) if out.numel() else out.reshape(math.prod(shape[:-1]), shape[-1])
     if out.numel() == 0:
         return o2
     if o2.stride(-1) != 1 and o2.shape[-1] > 1 or o2.shape[0] > 1 and o2.stride(0) < o2.shape[1]:

@@ -3,6 +3,7 @@ streams, captures and plans are stand-ins that record what was asked of them."""
 from __future__ import annotations
 
 import contextlib
+import math
 import threading
 
 import pytest
@@ -139,3 +140,9 @@ def test_forward_mode_tangents_are_seen():
         adapters._no_tangents("call", t, None, 2.0)
         with pytest.raises(RuntimeError, match="call has no forward-mode"):
             adapters._no_tangents("call", t, fwd.make_dual(t, t))
+
+
+def test_out_without_rows_or_columns():
+    for shape in ((3, 0), (0, 3), (2, 0, 3), (2, 3, 0)):
+        out = torch.empty(shape)
+        assert adapters._check_out(out, out.shape, out, None, ()).shape == (math.prod(shape[:-1]), shape[-1])

@@ -89,3 +89,12 @@ def test_the_callers_gradient_stays_as_it_was():
     y = fp.adapter_matmul(x, A, B, index, base=base, scale=scale)
     dbase, = torch.autograd.grad((y * weight).sum(), base, create_graph=True)
     assert torch.equal(torch.autograd.grad(dbase.sum(), weight)[0], torch.ones_like(dy))  # linear in dy
+
+
+def test_out_without_columns():
+    x, A, B, base, _, scale, index = _data(12, 3, 16, 0, 4, torch.float64)
+    out = torch.empty(12, 0, dtype=torch.float64, device="cuda")
+    assert fp.adapter_matmul(x, A, B, index, base=base, out=out) is out
+    layer = fp.add_adapters(fp.Linear(16, 0, device="cuda"), 3, rank=4)
+    with torch.no_grad(), fp.use_adapters(layer, index):
+        assert layer(x).shape == (12, 0)
