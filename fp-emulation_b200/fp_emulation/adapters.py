@@ -321,7 +321,9 @@ def adapter_matmul(x, A, B, rows, base=None, scale=1.0, out=None):
     if out is None:
         y = _packed_like(x2 if base2 is None else base2, (count, n))
     else:
-        y = _check_out(out, shape, x, base, (x2, A, B))
+        if out.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("adapter_matmul: out requires a gradient, which would not include this call")
+        y = _check_out(out, shape, x, base, (x2, A, B, index) + ((scale,) if scale.__class__ is not float else ()))
     _launch(x2, A, B, base2, y, scale, rows, index, None)
     if out is None:
         return y if flat else y.view(shape)

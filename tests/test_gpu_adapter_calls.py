@@ -98,3 +98,23 @@ def test_out_without_columns():
     layer = fp.add_adapters(fp.Linear(16, 0, device="cuda"), 3, rank=4)
     with torch.no_grad(), fp.use_adapters(layer, index):
         assert layer(x).shape == (12, 0)
+
+
+@pytest.mark.parametrize("rows", [12, 300])
+def test_out_over_the_ids_or_the_scales(rows):
+    x, A, B, base, _, scale, index = _data(rows, 3, 16, 4, 4, torch.float64)
+    out = torch.zeros(rows, 4, dtype=torch.float64, device="cuda")
+    ids = out.view(torch.int64).flatten()[:rows]
+    ids.copy_(index)
+    if rows <= _lib.FPEMU_ADAPTER_FEW_ROWS:  # more are copied as they are grouped
+        with pytest.raises(RuntimeError, match="overlaps"):
+            fp.adapter_matmul(x, A, B, ids, out=out)
+    want = fp.adapter_matmul(x, A, B, index)
+    assert torch.equal(fp.adapter_matmul(x, A, B, fp.prepare_rows(ids, 3), out=out), want)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        fp.adapter_matmul(x, A, B, index, scale=out.flatten()[4:7], out=out)
+    leaf = torch.zeros_like(out).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="requires a gradient"):
+        fp.adapter_matmul(x, A, B, index, out=leaf)
+    with torch.no_grad():
+        assert torch.equal(fp.adapter_matmul(x, A, B, index, out=leaf), want)
