@@ -95,19 +95,27 @@ __device__ __forceinline__ double clip_widen(double v) { return v; }
 __device__ __forceinline__ float clip_widen(__half v) { return __half2float(v); }
 __device__ __forceinline__ float clip_widen(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// The factor as one double, and as two floats whose sum it is.
+// The factor as one double, and as two floats whose sum it is: but for 2^-48 of it, as long as it is
+// above 2^-100.  TINY: below that a float loses digits and then all of them, and the product is one
+// of doubles.
 struct ClipFactor {
     double c;
     float hi, lo;
 };
+template <bool TINY>
 __device__ __forceinline__ double clip_scale(double v, const ClipFactor& f) { return v * f.c; }
 // The product with the float pair rounds once (but for 2^-48), as the product with the double would.
-__device__ __forceinline__ float clip_scale(float v, const ClipFactor& f) { return fmaf(v, f.hi, v * f.lo); }
-__device__ __forceinline__ __half clip_scale(__half v, const ClipFactor& f) {
-    return __float2half_rn(__half2float(v) * f.hi);
+template <bool TINY>
+__device__ __forceinline__ float clip_scale(float v, const ClipFactor& f) {
+    return TINY ? (float)((double)v * f.c) : fmaf(v, f.hi, v * f.lo);
 }
+template <bool TINY>
+__device__ __forceinline__ __half clip_scale(__half v, const ClipFactor& f) {
+    return TINY ? __double2half((double)__half2float(v) * f.c) : __float2half_rn(__half2float(v) * f.hi);
+}
+template <bool TINY>
 __device__ __forceinline__ __nv_bfloat16 clip_scale(__nv_bfloat16 v, const ClipFactor& f) {
-    return __float2bfloat16_rn(__bfloat162float(v) * f.hi);
+    return TINY ? __double2bfloat16((double)__bfloat162float(v) * f.c) : __float2bfloat16_rn(__bfloat162float(v) * f.hi);
 }
 
 // Block-wide join of the threads' sums, in a fixed order; thread 0 has the result.
@@ -165,7 +173,7 @@ __device__ void chunk_norm(const T* p, int n, NormSum& sum) {
     sum.join<P>(s[1].mid, s[1].big, s[1].small);
 }
 
-template <typename T>
+template <bool TINY, typename T>
 __device__ void chunk_scale(const T* p, T* o, int n, const ClipFactor& f) {
     constexpr int V = 16 / sizeof(T), U = 4;
     const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(o)) & 15) == 0;
@@ -175,7 +183,7 @@ __device__ void chunk_scale(const T* p, T* o, int n, const ClipFactor& f) {
     auto scaled = [&](uint4 raw) {
         T* v = reinterpret_cast<T*>(&raw);
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = clip_scale(v[e], f);
+        for (int e = 0; e < V; ++e) v[e] = clip_scale<TINY>(v[e], f);
         return raw;
     };
     int i = threadIdx.x;
@@ -187,8 +195,8 @@ __device__ void chunk_scale(const T* p, T* o, int n, const ClipFactor& f) {
         for (int u = 0; u < U; ++u) __stcs(w + i + u * kClipThreads, scaled(raw[u]));
     }
     for (; i < vecs; i += kClipThreads) __stcs(w + i, scaled(__ldcs(q + i)));
-    if (threadIdx.x < head) o[threadIdx.x] = clip_scale(p[threadIdx.x], f);
-    for (int t = head + vecs * V + threadIdx.x; t < n; t += kClipThreads) o[t] = clip_scale(p[t], f);
+    if (threadIdx.x < head) o[threadIdx.x] = clip_scale<TINY>(p[threadIdx.x], f);
+    for (int t = head + vecs * V + threadIdx.x; t < n; t += kClipThreads) o[t] = clip_scale<TINY>(p[t], f);
 }
 
 // Calls f(tensor, first element, elements) for this block's share of the chunks,
@@ -268,21 +276,21 @@ __global__ void __launch_bounds__(kClipThreads) clip_scale_kernel(const __grid_c
     f.c = c > 1.0 ? 1.0 : c;  // NaN stays
     f.hi = (float)f.c;
     f.lo = (float)(f.c - (double)f.hi);
+    const bool tiny = f.c < 0x1p-100 && f.c > 0;
     for_chunks<true>(t, [&](int i, int64_t at, int n) {
         if (t.src[i] == t.dst[i] && f.c == 1.0) return;
+        auto scale = [&](auto type) {
+            using T = decltype(type);
+            const T* p = static_cast<const T*>(t.src[i]) + at;
+            T* o = static_cast<T*>(t.dst[i]) + at;
+            if (tiny && sizeof(T) < 8) chunk_scale<true>(p, o, n, f);
+            else chunk_scale<false>(p, o, n, f);
+        };
         switch (t.dtype[i]) {
-            case FPEMU_DT_F64:
-                chunk_scale(static_cast<const double*>(t.src[i]) + at, static_cast<double*>(t.dst[i]) + at, n, f);
-                break;
-            case FPEMU_DT_F32:
-                chunk_scale(static_cast<const float*>(t.src[i]) + at, static_cast<float*>(t.dst[i]) + at, n, f);
-                break;
-            case FPEMU_DT_F16:
-                chunk_scale(static_cast<const __half*>(t.src[i]) + at, static_cast<__half*>(t.dst[i]) + at, n, f);
-                break;
-            default:
-                chunk_scale(static_cast<const __nv_bfloat16*>(t.src[i]) + at,
-                            static_cast<__nv_bfloat16*>(t.dst[i]) + at, n, f);
+            case FPEMU_DT_F64: scale(double()); break;
+            case FPEMU_DT_F32: scale(float()); break;
+            case FPEMU_DT_F16: scale(__half()); break;
+            default: scale(__nv_bfloat16());
         }
     });
 }
