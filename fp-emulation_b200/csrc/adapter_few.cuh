@@ -168,7 +168,27 @@ __global__ void __launch_bounds__(kFewThreads, FewTile<T, RP>::kBlocks) adapter_
     }
 
     Acc acc[RT][Tile::PA] = {};
+    // The tensor cores' adders truncate: after some instructions (FL rounds of loads) their sums of
+    // floats go to this thread's places in `red`, rounded there (65536 values of one sign, one block,
+    // float32: 9e-5 off without).
+    constexpr int FL = E == 4 ? 1 : 32 / UN;
+    bool more = false;
+    auto flush = [&]() {
+        if constexpr (E != 8) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float2* o = reinterpret_cast<float2*>(&red[(warp * RP + t * MR + h * 8 + g) * kGroupRows + 2 * q]);
+                    const float2 old = more ? *o : make_float2(0.f, 0.f);
+                    *o = make_float2(old.x + acc[t][2 * h], old.y + acc[t][2 * h + 1]);
+                    acc[t][2 * h] = acc[t][2 * h + 1] = 0;
+                }
+            more = true;
+        }
+    };
     auto add_up = [&](auto vec) {
+        int rounds = 0;
         for (int c = k0 + warp * KS; c < k1; c += W * KS * UN) {
             uint4 xv[UN], wv[UN][RT][MR / 8];
 #pragma unroll
@@ -217,6 +237,7 @@ __global__ void __launch_bounds__(kFewThreads, FewTile<T, RP>::kBlocks) adapter_
                     }
                 }
             }
+            if (E != 8 && ++rounds % FL == 0) flush();
         }
     };
     if (vec_x && vec_w1 && k % V == 0)
@@ -251,11 +272,14 @@ __global__ void __launch_bounds__(kFewThreads, FewTile<T, RP>::kBlocks) adapter_
     };
     load_second(n0 + warp * KS);  // its first loads cross the exchange of the middle
 
+    if constexpr (E == 8) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
+        for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int e = 0; e < Tile::PA; ++e)
-            red[(warp * RP + t * MR + (e >> 1) * 8 + g) * kGroupRows + 2 * q + (e & 1)] = acc[t][e];
+            for (int e = 0; e < 2; ++e) red[(warp * RP + t * MR + g) * kGroupRows + 2 * q + e] = acc[t][e];
+    } else {
+        flush();
+    }
     __syncthreads();
     for (int i = tid; i < RP * kGroupRows; i += kFewThreads) {
         Acc v = red[i];

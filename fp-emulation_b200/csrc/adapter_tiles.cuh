@@ -497,7 +497,10 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     using Acc = typename Tile::Acc;
     constexpr int E = Tile::E, KC = Tile::KC, S = Tile::kStages;
     constexpr int MT = RP < (E == 4 ? 32 : 128) ? 2 : 1, RG = 4 / MT, KW = 8 / RG, NT = RP / 8;
-    constexpr int FLUSH = 4;  // chunks that the tensor cores sum by themselves, for floats
+    // Chunks that the tensor cores sum by themselves.  Their adders truncate, which moves a sum of one
+    // sign by some 2^-25 an instruction: floats are flushed into registers, and 16-bit data, for
+    // which there are none left, into the slot's part in the workspace.
+    constexpr int FLUSH = 4, HOLD = E == 2 ? 64 : INT_MAX;
     extern __shared__ uint8_t raw[];
     uint8_t* smem = raw + ((1024 - (shared_address(raw) & 1023)) & 1023);  // the swizzles repeat every 1024 bytes
     __shared__ int list[SlotFeed::kRing][kSlotRows];
@@ -601,7 +604,7 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
     };
     // The block's sums of a slot to the workspace: the parts of k one after the other.
     Acc* red = reinterpret_cast<Acc*>(smem + S * Tile::kStage);
-    auto leave = [&](int64_t part) {
+    auto leave = [&](int64_t part, bool more) {  // `more`: adds to what the block left there before
         flush();
         named_barrier<kWorkBarrier, kTileThreads>();  // every warp has read the last slot's sums
         for (int p = 0; p < KW; ++p) {
@@ -621,13 +624,15 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
         }
         Acc* out = static_cast<Acc*>(P.parts) + part * (kSlotRows * RP);
         const bool ok = !ring.failed;  // else some warp's part is missing: the rows become NaN
-        for (int i = tid; i < kSlotRows * RP; i += kTileThreads)
-            out[i] = ok ? red[i / RP * Tile::kPitchU + i % RP] : (Acc)__longlong_as_double(0x7ff8000000000000ll);
+        for (int i = tid; i < kSlotRows * RP; i += kTileThreads) {
+            const Acc v = red[i / RP * Tile::kPitchU + i % RP];
+            out[i] = !ok ? (Acc)__longlong_as_double(0x7ff8000000000000ll) : more ? out[i] + v : v;
+        }
     };
 
-    int at = (int)(begin % per), slot = (int)(begin / per), stage = 0;
+    int at = (int)(begin % per), slot = (int)(begin / per), stage = 0, held = 0;
     uint32_t round = 0;
-    bool ok = true;
+    bool ok = true, more = false;
     for (int c = 0; c < chunks; ++c) {
         if (ok && !warp_wait(&ring.full[stage], round, P.budget_ns)) {
             report_error(P.sink.dev, P.sink.host, FPEMU_ERR_TIMEOUT, kWaitAdapterFull, c);
@@ -638,9 +643,11 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
         ring.left(stage);
         if (++stage == S) stage = 0, round ^= 1;
         if (c % FLUSH == FLUSH - 1) flush();
-        if (++at == per || c + 1 == chunks) {
-            leave((int64_t)blockIdx.x + slot);
-            at = 0, ++slot;
+        ++at, ++held;
+        if (at == per || c + 1 == chunks || held == HOLD) {
+            leave((int64_t)blockIdx.x + slot, more);
+            held = 0, more = at < per;
+            if (at == per) at = 0, ++slot;
         }
     }
 }

@@ -69,3 +69,34 @@ def test_bfloat16_gradients_have_the_bits_of_a_float(rows, p):
     ones.requires_grad_(True)
     dx, = torch.autograd.grad(fp.adapter_matmul(ones, A2, B2, index), ones, power.expand(rows, 3))
     assert torch.equal(dx, torch.full_like(dx, 2.0 ** -p))
+
+
+@pytest.mark.parametrize("long", [False, True], ids=["few", "many"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+def test_long_sums_of_one_sign(dtype, long):
+    """u_0 adds 65536 positive products, u_1 subtracts their exact sum S in up to four pieces, and y is
+    what u_0 is off by.  Tolerance: the tensor cores' adders keep 22 bits or more, and a block joins
+    their sums after 64 of their instructions at most (24 for floats), into a float that is rounded
+    to nearest (at most 128 times); a float's product is off by 2^-21 of it."""
+    k, m = 65536, 8
+    n, rows = (1, 64 * 300) if long else (200, 200)  # whole sums in one block
+    gen = torch.Generator(device="cuda").manual_seed(1)
+
+    def ones(*shape):
+        return (torch.rand(shape, generator=gen, device="cuda", dtype=torch.float64) + 1).to(dtype)
+
+    x = ones(1, k)
+    x[:, :4] = 1
+    A = torch.zeros(n, 2, k, dtype=dtype, device="cuda")
+    A[:, 0] = ones(n, k) * 2.0 ** -6
+    rest = (x.double() * A[:, 0].double()).sum(1)
+    total = rest.clone()
+    for j in range(4):
+        A[:, 1, j] = -rest.to(dtype)
+        rest = rest + A[:, 1, j].double()
+    assert (rest.abs() <= 2.0 ** -23 * total).all()
+    index = torch.arange(rows, dtype=torch.int32, device="cuda") % n
+    y = fp.adapter_matmul(x.expand(rows, k), A, torch.ones(n, m, 2, dtype=dtype, device="cuda"), index)
+    off = (y.double() / total[index.long()][:, None]).abs().max().item()
+    adds = 24 if dtype == torch.float32 else 64
+    assert off <= adds * 2.0 ** -22 + 128 * 2.0 ** -24 + 2.0 ** -21
