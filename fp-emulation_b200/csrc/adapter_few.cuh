@@ -303,16 +303,15 @@ __global__ void __launch_bounds__(kFewThreads, FewTile<T, RP>::kBlocks) adapter_
     constexpr bool kThird = std::is_same<T, __nv_bfloat16>::value;
     Part ua[JS][UA];
     uint32_t third[kThird ? JS : 1][4];
-    float back = 1.f;
+    float down = 1.f, back = 1.f;
     if constexpr (E == 2 && std::is_same<T, __half>::value) {
         float top = 0.f;
-        for (int j = q; j < RP; j += 4) top = fmaxf(top, fabsf((float)us[j * kGroupRows + g]));
+        for (int j = q; j < RP; j += 4) top = HalfScale::larger(top, us[j * kGroupRows + g]);
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = (int)(__float_as_uint(top) >> 23);
-        if (e > 0 && e < 254) back = __uint_as_float(e << 23);
+        const HalfScale s(top);
+        down = s.down, back = s.back;
     }
-    const float down = back == 1.f ? 1.f : __uint_as_float((254u << 23) - __float_as_uint(back));
 #pragma unroll
     for (int t = 0; t < JS; ++t) {
         const int j0 = t * KS + q * V;

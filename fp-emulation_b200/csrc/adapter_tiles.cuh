@@ -130,6 +130,22 @@ __device__ __forceinline__ Tf32Pair tf32_split(float x) {
     return p;
 }
 
+// What a row of the middle is multiplied by for halves, and its reciprocal: powers of two that put
+// the row's largest finite magnitude `top` between 2^14 and 2^15.  The values down to 2^-17 of it then
+// keep 22 bits, those down to 2^-28 at least 11, as many as a half (below 2^-112 nothing of
+// a row is left in a half).
+struct HalfScale {
+    float down = 1.f, back = 1.f;
+    __device__ __forceinline__ explicit HalfScale(float top) {
+        const uint32_t e = __float_as_uint(top) >> 23;
+        if (e >= 15) down = __uint_as_float((268 - e) << 23), back = __uint_as_float((e - 14) << 23);
+    }
+    // The largest finite magnitude so far.
+    static __device__ __forceinline__ float larger(float top, float v) {
+        return fabsf(v) < __int_as_float(0x7f800000) ? fmaxf(top, fabsf(v)) : top;
+    }
+};
+
 // Two neighbouring floats as two halves each, 22 bits of them.
 __device__ __forceinline__ void split_half(float x, float y, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -735,20 +751,16 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
             float down[2] = {1.f, 1.f};
             if constexpr (std::is_same<T, __half>::value) {
                 float top[2] = {0.f, 0.f};
-                back[0] = back[1] = 1.f;
 #pragma unroll
                 for (int t = 0; t < RP / 16; ++t)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) top[e >> 1 & 1] = fmaxf(top[e >> 1 & 1], fabsf(v[t][e]));
+                    for (int e = 0; e < 8; ++e) top[e >> 1 & 1] = HalfScale::larger(top[e >> 1 & 1], v[t][e]);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-                    const int e = (int)(__float_as_uint(top[h]) >> 23);  // 0 and 255 stay unscaled
-                    if (e > 0 && e < 254) {
-                        down[h] = __uint_as_float((254 - e) << 23);
-                        back[h] = __uint_as_float(e << 23);
-                    }
+                    const HalfScale s(top[h]);
+                    down[h] = s.down, back[h] = s.back;
                 }
             }
 #pragma unroll

@@ -100,3 +100,25 @@ def test_long_sums_of_one_sign(dtype, long):
     off = (y.double() / total[index.long()][:, None]).abs().max().item()
     adds = 24 if dtype == torch.float32 else 64
     assert off <= adds * 2.0 ** -22 + 128 * 2.0 ** -24 + 2.0 ** -21
+
+
+@pytest.mark.parametrize("apart", [4, 12, 16, 18, 24, 28])
+@pytest.mark.parametrize("rows", ROWS)
+def test_half_middle_of_far_magnitudes(rows, apart):
+    """u = (2^a, 2^-b (1 + 2^-9)), b + a = apart; B takes the second alone, which a half holds."""
+    b = min(apart, 14)
+    x = torch.tensor([1.0, 1 + 2.0 ** -9], dtype=torch.float16, device="cuda").expand(rows, 2)
+    A = torch.tensor([[[2.0 ** (apart - b), 0], [0, 2.0 ** -b]]], dtype=torch.float16, device="cuda")
+    B = torch.tensor([0, 2.0 ** 10], dtype=torch.float16, device="cuda").expand(1, 20, 2)
+    y = fp.adapter_matmul(x, A, B, torch.zeros(rows, dtype=torch.int32, device="cuda"))
+    assert torch.equal(y, torch.full_like(y, 2.0 ** (10 - b) * (1 + 2.0 ** -9)))
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_half_middle_beside_an_infinity(rows):
+    """u = (inf, 3.6e9): the second is finite, and takes nothing from the first."""
+    x = torch.tensor([1.0, 60000.0], dtype=torch.float16, device="cuda").expand(rows, 2)
+    A = torch.tensor([[[float("inf"), 0], [0, 60000.0]]], dtype=torch.float16, device="cuda")
+    B = torch.tensor([1.0, -1.0], dtype=torch.float16, device="cuda").expand(1, 20, 2)
+    y = fp.adapter_matmul(x, A, B, torch.zeros(rows, dtype=torch.int32, device="cuda"))
+    assert torch.equal(y, torch.full_like(y, float("inf")))
