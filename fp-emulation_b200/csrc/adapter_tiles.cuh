@@ -326,7 +326,13 @@ constexpr int kCopyBarrier = 1, kWorkBarrier = 2;
 // A warp's wait: it runs out for all lanes or for none (each has a clock of its own, and
 // what follows a wait takes the whole warp).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint64_t budget_ns) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, budget_ns));
+    const uint32_t a = smem_u32(bar);
+    if (__all_sync(0xffffffffu, mbar_try_wait(a, parity))) return true;
+    const uint64_t t0 = global_ns();
+    for (uint32_t i = 1;; ++i) {
+        if (__all_sync(0xffffffffu, mbar_try_wait(a, parity))) return true;
+        if ((i & 255u) == 0u && __any_sync(0xffffffffu, global_ns() - t0 > budget_ns)) return false;
+    }
 }
 
 // The ring of chunks: a buffer is full when TMA's bytes and every copying thread's
@@ -437,8 +443,9 @@ __device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<T
     SlotFeed feed{list, rec, slots, perm, busy, t};
     if (chunks > 0) feed.begin(slot);
     int stage = 0, cls = 0, first = 0, asked = 0;  // chunks whose copies this warp has asked for
-    uint32_t round = 1, by_threads = 0;  // a bit for each buffer whose rows the threads copied last
-    bool box = false, ok = true;
+    uint32_t round = 1;
+    bool box = true, ok = true;
+    int fenced = 0;  // up to this chunk, buffers may hold rows that the threads copied
     for (int c = 0; c < chunks; ++c) {
         if (ok && blockIdx.x == 0 && c == q.stall) ok = false;
         if (ok && c >= S && !warp_wait(&ring.empty[stage], round, q.budget_ns)) {
@@ -450,7 +457,9 @@ __device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<T
             if (!feed.enter(ok, s)) break;
             const int* ids = list[(feed.slot - 1) % SlotFeed::kRing];
             cls = s.cls, first = ids[0];
+            const bool before = box;
             box = (q.tma & kTmaRows) && ids[s.count - 1] - first == s.count - 1;
+            if (box && !before) fenced = c + S;
             if (rows && !box) xt.aim(t, rows, q.row_stride, ids, s.count, (int64_t)at * KC);
             if (!tma_w) wt.aim(t, w + s.cls * q.w_adapter, q.w_row, (int64_t)at * KC);
         }
@@ -461,7 +470,7 @@ __device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<T
         }, [&]() {
             const uint32_t to = shared_address(st);
             // The threads' copies were ordinary writes; TMA's to the same place come after them.
-            if (box && (by_threads >> stage & 1)) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            if (c < fenced) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             if (rows && box) tma_box2(to, q.row_map, &ring.full[stage], at * KC, first);
             if (tma_w) {
                 if (LONG)
@@ -473,7 +482,6 @@ __device__ __forceinline__ void stream_chunks(const StreamParams& q, ChunkRing<T
             }
         });
         asked += ok;
-        by_threads = box ? by_threads & ~(1u << stage) : by_threads | 1u << stage;
         if (++at == per) at = 0;
         if (++stage == S) stage = 0, round ^= 1;
     }
@@ -640,10 +648,11 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
         }
         Acc* out = static_cast<Acc*>(P.parts) + part * (kSlotRows * RP);
         const bool ok = !ring.failed;  // else some warp's part is missing: the rows become NaN
-        for (int i = tid; i < kSlotRows * RP; i += kTileThreads) {
-            const Acc v = red[i / RP * Tile::kPitchU + i % RP];
-            out[i] = !ok ? (Acc)__longlong_as_double(0x7ff8000000000000ll) : more ? out[i] + v : v;
+        if (more) {
+            for (int i = tid; i < kSlotRows * RP; i += kTileThreads) red[i / RP * Tile::kPitchU + i % RP] += out[i];
         }
+        for (int i = tid; i < kSlotRows * RP; i += kTileThreads)
+            out[i] = ok ? red[i / RP * Tile::kPitchU + i % RP] : (Acc)__longlong_as_double(0x7ff8000000000000ll);
     };
 
     int at = (int)(begin % per), slot = (int)(begin / per), stage = 0, held = 0;
