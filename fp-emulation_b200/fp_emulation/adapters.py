@@ -368,16 +368,20 @@ class _ActiveRows:
     each other, and what a capture makes is there after a replay alone: each stream,
     and each capture, has plans of its own."""
 
-    def __init__(self, index, model):
+    def __init__(self, index, model=None):
         self.index = index.clone()
         self.prepared = {}
         self.lock = threading.Lock()
-        self.kept = _captured_ids.setdefault(model, [])
+        self.kept = [] if model is None else _captured_ids.setdefault(model, [])
         d = index.get_device()
         if d >= 0:  # else the first layer refuses it
             self.stream, self.capture = _raw_stream(d), _capture_id(d)
             self.copied = torch.cuda.Event()
             self.copied.record(torch.cuda.current_stream(d))
+
+    def __reduce__(self):
+        """A copy of a model (or a pickled one) inside the block has the block's ids, and groups them anew."""
+        return _ActiveRows, (self.index,)
 
     def prepare(self, lead, adapters):
         d = self.index.get_device()

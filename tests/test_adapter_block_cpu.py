@@ -146,3 +146,18 @@ def test_out_without_rows_or_columns():
     for shape in ((3, 0), (0, 3), (2, 0, 3), (2, 3, 0)):
         out = torch.empty(shape)
         assert adapters._check_out(out, out.shape, out, None, ()).shape == (math.prod(shape[:-1]), shape[-1])
+
+
+def test_a_model_is_copied_inside_a_block():
+    import copy
+    import pickle
+
+    import fp_emulation as fp
+
+    model = fp.add_adapters(torch.nn.Sequential(fp.Linear(2, 3)), 4, rank=1)
+    ids = torch.tensor([1, -1, 3])
+    with fp.use_adapters(model, ids):
+        for twin in (copy.deepcopy(model), pickle.loads(pickle.dumps(model))):
+            assert torch.equal(twin[0].active_rows.index, ids) and twin[0].active_rows is not model[0].active_rows
+            assert torch.equal(twin[0].adapters.A, model[0].adapters.A)
+    assert model[0].active_rows is None
