@@ -152,12 +152,12 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
 
 
 @torch.no_grad()
-def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, foreach=None):
     """Scale the gradients of ``parameters`` in place to a global norm of at most
     ``max_norm`` and return the norm before (see ``grad_norm``); parameters without
     a gradient are passed over.  With ``error_if_nonfinite`` the norm is read back
     first, and a RuntimeError leaves the gradients as they were.  Each gradient may
-    appear once."""
+    appear once.  ``foreach`` is there for callers of the other: all tensors go at once."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     code, max_norm = _norm_code(norm_type), _max_norm(max_norm)
     grads = [g for g in map(_grad, parameters) if g is not None]

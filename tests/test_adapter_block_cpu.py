@@ -161,3 +161,15 @@ def test_a_model_is_copied_inside_a_block():
             assert torch.equal(twin[0].active_rows.index, ids) and twin[0].active_rows is not model[0].active_rows
             assert torch.equal(twin[0].adapters.A, model[0].adapters.A)
     assert model[0].active_rows is None
+
+
+def test_clipping_has_the_signature_it_names():
+    import inspect
+
+    import fp_emulation as fp
+
+    ours, theirs = (inspect.signature(f).parameters for f in (fp.clip_grad_norm_, torch.nn.utils.clip_grad_norm_))
+    assert list(ours) == list(theirs) and all(ours[n].default == p.default for n, p in theirs.items())
+    p = torch.nn.Parameter(torch.ones(3))
+    for foreach in (None, True, False):
+        assert fp.clip_grad_norm_([p], 1.0, foreach=foreach) == 0
