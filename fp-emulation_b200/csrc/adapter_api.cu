@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
 #include <type_traits>
 
 #include "adapter_few.cuh"
@@ -38,6 +39,13 @@ int check_sizes(const char* what, int dtype, int64_t rows, int64_t k, int64_t n,
         return fail(FPEMU_ERR_UNSUPPORTED, "%s: %lld adapters outside [1, %d]", what, (long long)adapters,
                     FPEMU_ADAPTER_MAX_COUNT);
     return FPEMU_OK;
+}
+
+// Whether one of the addresses is no multiple of `size` (a power of two).
+bool misplaced(int size, std::initializer_list<const void*> pointers) {
+    uintptr_t all = 0;
+    for (const void* p : pointers) all |= reinterpret_cast<uintptr_t>(p);
+    return all % size != 0;
 }
 
 // Lets a kernel use `bytes` of dynamic shared memory, once per kernel and device.
@@ -290,6 +298,7 @@ int fpemu_adapter_plan(const void* index, int index_bytes, int64_t rows, int64_t
         return fail(FPEMU_ERR_WORKSPACE, "adapter_plan: need %lld bytes, 16-byte aligned",
                     (long long)plan_words(rows, adapters) * 4);
     if (rows > 0 && index == nullptr) return fail(FPEMU_ERR_INVALID, "adapter_plan: null index");
+    if (misplaced(index_bytes, {index})) return fail(FPEMU_ERR_INVALID, "adapter_plan: misaligned index");
     FPEMU_TRY(device_info(&d));
     ErrorSink sink;
     FPEMU_TRY(error_sink(&sink));
@@ -324,6 +333,10 @@ int fpemu_adapter_matmul(int dtype, int64_t rows, int64_t k, int64_t n, int64_t 
     if (plan == nullptr && (rows > FPEMU_ADAPTER_FEW_ROWS || index == nullptr || (index_bytes != 4 && index_bytes != 8)))
         return fail(FPEMU_ERR_INVALID, "adapter_matmul: %lld rows need a plan, few rows an index of 4 or 8 bytes",
                     (long long)rows);
+    const int size = element_size(dtype);
+    if (misplaced(size, {x, A, B, base, y}) || misplaced(8, {scales}) || misplaced(size == 8 ? 8 : 4, {u}) ||
+        misplaced(16, {plan}) || (plan == nullptr && misplaced(index_bytes, {index})))
+        return fail(FPEMU_ERR_INVALID, "adapter_matmul: a pointer is not aligned to its elements (the plan to 16 bytes)");
     FPEMU_TRY(device_info(&d));
     if (plan != nullptr) FPEMU_TRY(check_workspace("adapter_matmul", dtype, rows, rank, adapters, workspace, workspace_bytes));
     AdapterParams P = {};
@@ -366,6 +379,8 @@ int fpemu_adapter_backward(int dtype, int64_t rows, int64_t k, int64_t n, int64_
         return fail(FPEMU_ERR_INVALID, "adapter_backward: u and v start on a 16-byte boundary");
     if (x_row < 0 || dy_row < 0 || A_adapter < 0 || B_adapter < 0 || A_row < 0 || B_row < 0)
         return fail(FPEMU_ERR_INVALID, "adapter_backward: negative stride");
+    if (misplaced(element_size(dtype), {x, A, B, dy, dx, dA, dB}) || misplaced(8, {scales}) || misplaced(16, {plan}))
+        return fail(FPEMU_ERR_INVALID, "adapter_backward: a pointer is not aligned to its elements (the plan to 16 bytes)");
     FPEMU_TRY(device_info(&d));
     if (dx || dA) FPEMU_TRY(check_workspace("adapter_backward", dtype, rows, rank, adapters, workspace, workspace_bytes));
     return with_type(dtype, [&](auto* t) {

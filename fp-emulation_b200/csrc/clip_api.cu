@@ -26,6 +26,8 @@ int chunk_size(const DevInfo& d, int64_t count, const int64_t* numel) {
     return size;
 }
 
+constexpr int64_t kTypeSize[4] = {8, 4, 2, 2};  // by FPEMU_DT_ code
+
 // The scaling kernel's blocks read and write in any order, so no output may meet
 // another output, or an input that is not its own.
 int clip_check_overlap(int64_t count, const void* const* src, void* const* dst, const int64_t* numel,
@@ -35,14 +37,13 @@ int clip_check_overlap(int64_t count, const void* const* src, void* const* dst, 
         int64_t tensor;
         bool output;
     };
-    static const int64_t size[4] = {8, 4, 2, 2};
     try {
         std::vector<Range> r;
         r.reserve((size_t)count * 2);
         for (int64_t i = 0; i < count; ++i) {
             if (numel[i] == 0) continue;
             const uintptr_t s = reinterpret_cast<uintptr_t>(src[i]), o = reinterpret_cast<uintptr_t>(dst[i]);
-            const uintptr_t bytes = (uintptr_t)(numel[i] * size[dtype[i]]);
+            const uintptr_t bytes = (uintptr_t)(numel[i] * kTypeSize[dtype[i]]);
             r.push_back({o, o + bytes, i, true});
             if (s != o) r.push_back({s, s + bytes, i, false});
         }
@@ -70,6 +71,9 @@ int clip_check(int64_t count, const void* const* src, void* const* dst, const in
             return fail(FPEMU_ERR_INVALID, "clip_grads: tensor %lld has a null pointer or a negative size", (long long)i);
         if (dtype[i] < FPEMU_DT_F64 || dtype[i] > FPEMU_DT_BF16)
             return fail(FPEMU_ERR_INVALID, "clip_grads: tensor %lld has unknown dtype code %d", (long long)i, dtype[i]);
+        const uintptr_t at = reinterpret_cast<uintptr_t>(src[i]) | (dst ? reinterpret_cast<uintptr_t>(dst[i]) : 0);
+        if (numel[i] > 0 && at % kTypeSize[dtype[i]] != 0)
+            return fail(FPEMU_ERR_INVALID, "clip_grads: tensor %lld is not aligned to its elements", (long long)i);
     }
     return dst == nullptr ? FPEMU_OK : clip_check_overlap(count, src, dst, numel, dtype);
 }
@@ -144,7 +148,8 @@ int fpemu_clip_grads(int64_t count, const void* const* src, void* const* dst, co
     if (norm_type < 0 || norm_type > 2)
         return fail(FPEMU_ERR_INVALID, "clip_grads: norm_type %d (1, 2, or 0 for the largest magnitude)", norm_type);
     if (dst != nullptr && !(max_norm >= 0)) return fail(FPEMU_ERR_INVALID, "clip_grads: max_norm %g", max_norm);
-    if (norm == nullptr) return fail(FPEMU_ERR_INVALID, "clip_grads: null norm");
+    if (norm == nullptr || reinterpret_cast<uintptr_t>(norm) % (norm_f64 ? 8 : 4) != 0)
+        return fail(FPEMU_ERR_INVALID, "clip_grads: null or misaligned norm");
     FPEMU_TRY(device_info(&d));
     if (workspace == nullptr || workspace_bytes < fpemu_clip_workspace_size(count) ||
         reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
