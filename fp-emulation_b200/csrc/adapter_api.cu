@@ -70,10 +70,11 @@ int launch_few_rank(const AdapterParams& P, const DevInfo& d, cudaStream_t st) {
     // Groups of eight rows of one adapter, of none, or with a bad id: never more than this.
     const int64_t units = std::min<int64_t>(P.rows, P.rows / kGroupRows + P.adapters + 2);
     // The largest cluster with which all blocks are on the device at once (200 rows of 24 adapters,
-    // 4096 x 4096 bfloat16: 10.6 us with 4 blocks, 16.7 with 8 that are not; 250 rows with an adapter
-    // each: 24.5 with 1, 29.5 with 2).
+    // 4096 x 4096 bfloat16, rank 16: 10.6 us with 4 blocks, 16.7 with 8 that are not; 250 rows with an
+    // adapter each: 24.5 with 1, 29.5 with 2.  100 rows with one each, rank 64 and 128: 32 and 59 us so, 39
+    // and 82 with twice and four times the blocks; float64 101 and 219, 113 and 251).
     int cluster = 8;
-    while (cluster > 1 && units * cluster > (P.r > 32 ? d.sms * 4 : d.sms * Tile::kBlocks)) cluster /= 2;
+    while (cluster > 1 && units * cluster > d.sms * Tile::kBlocks) cluster /= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(units * cluster));
     cfg.blockDim = dim3(kFewThreads);
