@@ -207,18 +207,20 @@ int launch_grad_rank(AdapterGradParams& P, size_t parts_bytes, const DevInfo& d,
     int64_t blocks[2];
     for (int i = 0; i < 2; ++i) blocks[i] = P.side[i].grad ? (P.side[i].cols + Tile::COLS - 1) / Tile::COLS : 0;
     if (blocks[0] + blocks[1] == 0) return FPEMU_OK;
-    // The most parts of an adapter's rows with which the blocks are on the device together, five an SM
-    // (16384 rows of 4 adapters, 4096 x 4096 bfloat16, rank 32: 96 us in 512 blocks, 117 in 1024); twice
-    // that while a part is long enough for its start not to count, since an SM's last blocks weigh less
-    // then (the same in float64: 315 us in 1024 blocks, 377 in 512).
+    // Parts of an adapter's rows, by the average adapter (an uneven batch waits for its longest): as many as
+    // make five blocks an SM (two to six fit, by type and rank; 16384 rows of 4 adapters, 4096 x 4096
+    // bfloat16, rank 32, middle in two parts: 96 us in 512 blocks, 117 in 1024); twice that while a part
+    // is long enough for its start not to count, since an SM's last blocks weigh less then (the same in
+    // float64: 315 us in 1024 blocks, 377 in 512).
     const int64_t all = (blocks[0] + blocks[1]) * P.adapters, each = P.rows / P.adapters;
     int cluster = 1;
     while (cluster < kGradCluster && each > cluster * 4 * Tile::KT &&
            all * cluster * 2 <= d.sms * (each >= cluster * 128 * Tile::KT ? 10 : 5))
         cluster *= 2;
     // Segments of 8 chunks a block or more, as many as the device holds and the workspace has room for
-    // (bfloat16, one adapter, with the second kernel and without segments: 20000 rows, 512 -> 512, rank 16,
-    // 22 us and 62; a million rows, 32 -> 32, rank 8, 118 and 2670).
+    // (bfloat16, one adapter, middle in two parts, with the second kernel and without segments: 20000 rows,
+    // 512 -> 512, rank 16, 22 us and 62; a million rows, 32 -> 32, rank 8, 118 and 2670; in three parts with
+    // segments 25 and 163).
     int64_t segments = 1;
     if (cluster == kGradCluster && P.parts != nullptr)
         segments = std::max<int64_t>(1, std::min({d.sms * 5 / (all * cluster), each / (cluster * 8 * Tile::KT),

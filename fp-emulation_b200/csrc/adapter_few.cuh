@@ -12,8 +12,8 @@
 // bits, which moved three results in a thousand to a neighbouring bfloat16.
 //
 // Measured (kernel alone, cold L2), 4096 -> 4096, rank 16: 32 rows with an adapter
-// each, bfloat16, 9.7 us (its 9 MB take 1.4 at the copy rate), float64 15.8 (5.6);
-// 200 rows of 24 adapters, 10.6 (1.7) and 19.4 (6.9); 7 us for any tiny call.  What is left is latency, a few microseconds each for finding
+// each, bfloat16, 10.1 us (its 9 MB take 1.4 at the copy rate), float64 15.4 (5.6);
+// 200 rows of 24 adapters, 11.3 (1.7) and 19.0 (6.9); 7 us for any tiny call.  What is left is latency, a few microseconds each for finding
 // the rows, the two streams of loads and the two meetings of the cluster; the call's
 // host side takes 15 us.  Fetching the weights ahead into the L2 changed nothing.
 #pragma once

@@ -111,7 +111,8 @@ __device__ __forceinline__ int row_class(const void* index, int wide, int64_t t,
 // classes, in its own stretch of the index; a scan over the warps' counts gives
 // every warp its first position, and a second walk writes the rows in order.
 // No atomics: the order is that of the rows.  Every block reads the whole index, which
-// stays in the L2: a few microseconds for the batches here, once for all layers.
+// stays in the L2: rows x adapters, once for all layers (16384 rows of 64 adapters 7 us, of
+// 1000 41 us, of 65000 2.4 ms; a million rows of 64 224 us).
 __global__ void __launch_bounds__(1024) adapter_plan_kernel(const void* index, int wide, int64_t rows, int adapters,
                                                             int32_t* plan, ErrorSink sink) {
     __shared__ int own_count[32], below_count[32];

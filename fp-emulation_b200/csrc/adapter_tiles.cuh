@@ -12,14 +12,14 @@
 // What bounds them: the bytes of x, base and y, as long as the rank is small --
 // float64 up to rank 16 or so (mma.sync f64 reaches 37 TFLOP/s, the device's whole
 // rate), 16-bit data up to rank 64 (545 TFLOP/s; tf32, for floats, 273).  Measured:
-//   float64, 16384 x 4096 -> 4096, rank 16, 8 adapters in runs: 300 us, 5.4 TB/s of
-//     algorithmic bytes, 0.83 of the measured copy rate (107 us for u, 5.0 TB/s);
-//   half, 16384 x 4096 -> 8192, rank 64, 16 adapters: 207 us, 3.4 TB/s.  There the
-//     second kernel (170 us) is bound by what a computing warp does for a chunk:
+//   float64, 16384 x 4096 -> 4096, rank 16, 8 adapters in runs: 307 us, 5.3 TB/s of
+//     algorithmic bytes, 0.81 of the measured copy rate (107 us for u, 5.0 TB/s);
+//   half, 16384 x 4096 -> 8192, rank 64, 16 adapters: 215 us, 3.2 TB/s.  There the
+//     second kernel (172 us) is bound by what a computing warp does for a chunk:
 //     without its matrix instructions it takes 119 us, its copies alone 80.
 // One kernel for both products, in clusters that exchanged the middle through
-// distributed shared memory, took 330 and 199 us: its blocks' shares came in whole
-// slots, and 256 of them on 148 SMs left a seventh of the device idle.
+// distributed shared memory, was no faster (330 us for the float64 case): its blocks'
+// shares came in whole slots, and 256 of them on 148 SMs left a seventh of the device idle.
 #pragma once
 
 #include <cuda.h>
@@ -117,7 +117,8 @@ __device__ __forceinline__ void mma_f64(double (&c)[4], double a0, double a1, do
 
 // A float as two tf32 parts: hi is x rounded to 10 bits after the point, lo the
 // first bits of the rest.  A product of two floats takes three of the four partial
-// products; what it loses is 2^-20 of it at most.  An infinite or NaN x is in lo,
+// products; what it loses is 2^-21 of it at most (lo x lo, and the last bit of a lo that
+// has twelve).  An infinite or NaN x is in lo,
 // with a finite hi, so that a zero lo of the other factor meets no infinity.
 struct Tf32Pair {
     uint32_t hi, lo;
@@ -1001,9 +1002,9 @@ __global__ void __launch_bounds__(kTileThreads + kCopyThreads, AdapterTile<T, TR
 // four adapters: 126 us for the 268 MB of both, 2.1 TB/s, with the warps waiting for
 // their loads from shared memory and for one another in turn (with p in two parts, 16
 // bits of it, 96 us); a million rows, 32
-// columns to 32, rank 8, one adapter: 118 us for 192 MB.  The ring of the products, with two
+// columns to 32, rank 8, one adapter: 157 us for 192 MB.  The ring of the products, with two
 // copying warps, was no faster here and slower for rows in any order (3333 x 1024
-// bfloat16 rank 20: 35 us against 18), whose copies two warps cannot issue fast enough.
+// bfloat16 rank 20, p in two parts: 35 us against 18), whose copies two warps cannot issue fast enough.
 constexpr int kGradThreads = 128;
 constexpr int kGradCluster = 8;  // the most blocks whose sums meet in a cluster
 
