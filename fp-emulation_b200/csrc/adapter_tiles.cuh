@@ -1051,8 +1051,8 @@ struct AdapterGradTile {
     static constexpr int kPitchL = (RP + 8) * 4, kThird = kPairs ? KT / 2 * kPitchL : 0;
     static constexpr int kRing = kStages * kStage + 2 * kThird;
     static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
-    // Chunks that the (truncating) tensor cores sum by themselves: of 16-bit data 4, of which 8 moved
-    // twice as many results to a neighbour and took 125 us for 126.
+    // Chunks that the (truncating) tensor cores sum by themselves: of 16-bit data 4 (8 moved a fifth
+    // more results to a neighbouring bfloat16, in 125 us for 126).
     static constexpr int kFlush = E == 2 ? 4 : 1;
 };
 
@@ -1121,7 +1121,7 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
             for (int i = 0; i < PI; i += 2) {
                 const int row = p_row_of(i);
                 if (row >= KT) break;
-                float a[4], b[4];
+                alignas(16) float a[4], b[4];
                 uint32_t part[4][3];
                 *reinterpret_cast<float4*>(a) = *reinterpret_cast<const float4*>(pt + row * Tile::kPitchP);
                 *reinterpret_cast<float4*>(b) = *reinterpret_cast<const float4*>(pt + (row + 1) * Tile::kPitchP);

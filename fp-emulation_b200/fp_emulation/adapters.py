@@ -248,8 +248,9 @@ def adapter_matmul(x, A, B, rows, base=None, scale=1.0, out=None):
     and off by 2^-21 of it at most; sums of up to 64 tensor-core instructions are
     truncated, not rounded (5e-6 of a long sum of one sign; 7e-7 for float32); with
     float16 the intermediate ``x @ A[i].T`` enters the second product with 22 bits
-    (values below 2^-17 of their row's largest with fewer), with bfloat16 with all 24.  x, A, B and base have gradients (once; not twice differentiable,
-    and not in forward mode); repeated calls give the same bits."""
+    (values below 2^-17 of their row's largest with fewer), with bfloat16 with all 24.
+    x, A, B and base have gradients (once; not twice differentiable, and not in forward
+    mode); repeated calls give the same bits."""
     dtype = x.dtype
     _dtype_bits(dtype)
     _no_tangents("adapter_matmul", x, A, B, base, scale)
